@@ -121,6 +121,9 @@ SIGNATURES = {
     "cubert_bias_res_ln_slices_split_pairs_f32": (ci, [vp, vp, ci, ci, cll, vp, vp, vp, vp, ci, ci, cf, vp, vp, vp]),
     "cubert_dense_large_f16": (ci, [vp, ci, ci, ci, vp, vp, vp, ci, vp, ci]),
     "cubert_dense_large_plan": (ci, [ci, ci, ci, ci, ci, ctypes.POINTER(ci), ctypes.POINTER(ci), ctypes.POINTER(ci)]),
+    "cubert_w4_packed_bytes": (ctypes.c_size_t, [ci, ci, ci]),
+    "cubert_w4_pack": (ci, [vp, vp, ci, ci, ci, vp, vp]),
+    "cubert_attention_window_partials": (ctypes.c_size_t, [ci, ci, ci, ci, ci, ci, ci, ci, ci, ci]),
     "cubert_blas_create": (vp, []),
     "cubert_blas_destroy": (ci, [vp]),
     "cubert_blas_set_stream": (ci, [vp, vp]),
@@ -152,6 +155,13 @@ for _t in ("f32", "f16"):
         "cubert_dense_" + _t: (ci, [vp, ci, ci, ci, vp, ci, vp, ci, vp, ci, vp, ci]),
         "cubert_dense_slices_" + _t: (ci, [vp, ci, ci, ci, vp, ci, vp, ci, vp, ctypes.c_size_t, ctypes.POINTER(ci)]),
         "cubert_bias_res_ln_slices_" + _t: (ci, [vp, vp, ci, ci, cll, vp, vp, vp, vp, ci, ci, vp]),
+        "cubert_res_rms_norm_" + _t: (ci, [vp, vp, vp, cf, vp, vp, ci, ci, vp]),
+        "cubert_res_rms_norm_i8_" + _t: (ci, [vp, vp, vp, cf, vp, vp, vp, ci, ci, vp]),
+        "cubert_w4_quantize_" + _t: (ci, [vp, ci, ci, ci, vp, vp, vp, vp]),
+        "cubert_dense_w4_" + _t: (ci, [vp, ci, ci, ci, vp, ci, vp, ci, vp, ci, vp, ci]),
+        "cubert_dense_w4_i8_" + _t: (ci, [vp, ci, ci, ci, vp, ci, vp, vp, ci, vp, ci, vp, ci]),
+        "cubert_attention_window_" + _t: (ci, [vp, ci, vp, vp, ci, vp, vp, vp, vp, ci, cf, ci, ci, ci, ci, ci, ci, ci, ci, ci, vp,
+                                               ctypes.c_size_t, vp]),
         "cubert_gemm_strided_batch_" + _t: (ci, [vp, ci, ci, ci, ci, ci, cf, vp, ci, cll, vp, ci, cll, cf, vp, ci, cll, ci]),
         "cubert_gemm_batch_" + _t: (ci, [vp, ci, ci, ci, ci, ci, cf, vp, ci, vp, ci, cf, vp, ci, ci]),
     })

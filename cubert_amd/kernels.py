@@ -389,6 +389,186 @@ def bias_res_ln_slices(partials, residual, bias, beta, gamma):
     return out
 
 
+# ---- layers of pre-norm models, few tokens
+
+
+def _device(t, *others):
+    """The device that the call's tensors are on: one and the same."""
+    if not t.is_cuda:
+        raise ValueError("CUDA tensors expected")
+    for o in others:
+        if o is not None and o.device != t.device:
+            raise ValueError("tensors on different devices: %s and %s" % (t.device, o.device))
+    return t.device
+
+
+def _run_on(device, name, args, declines=False):
+    """The entry point `name` on `device` and its current stream (the last of args, or the first, is None for it);
+    True, or False where it declines."""
+    fn = getattr(lib(), name)
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args(torch.cuda.current_stream().cuda_stream))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args(torch.cuda.current_stream().cuda_stream))
+    if rc == -2 and declines:
+        return False
+    _check(rc, name)
+    return True
+
+
+def _like(t, ref, shape, what):
+    if t is not None and (t.dtype != ref.dtype or tuple(t.shape) != tuple(shape)):
+        raise ValueError("%s: %s %s expected, got %s %s" % (what, ref.dtype, tuple(shape), t.dtype, tuple(t.shape)))
+
+
+def _rms_norm(name, x, residual, gamma, eps, codes):
+    device = _device(x, residual, gamma)
+    hidden = x.shape[-1]
+    rows = x.numel() // hidden if hidden else 0
+    suffix = _suffix(x)
+    if hidden == 0 or rows >= 1 << 31:
+        raise ValueError("rows expected, got %s" % (tuple(x.shape),))
+    _like(residual, x, x.shape, "residual")
+    _like(gamma, x, (hidden,), "gamma")
+    total = torch.empty_like(x) if residual is not None else None
+    outs = (torch.empty_like(x, dtype=torch.int8), torch.empty(x.shape[:-1], dtype=torch.float32, device=device)) if codes \
+        else (torch.empty_like(x),)
+    pointers = tuple(_ptr(t) for t in (x, residual, gamma))
+    if not _run_on(device, name + suffix, lambda stream: pointers + (float(eps), _ptr(total)) + tuple(_ptr(t) for t in outs) +
+                   (rows, hidden, stream), declines=True):
+        return None
+    return outs + (total,)
+
+
+def res_rms_norm(x, residual, gamma, eps=1e-6):
+    """(gamma * s / sqrt(mean(s^2) + eps), s) of s = x + residual over the last axis; without a residual s is x and the second
+    result None.  None when the rows are too long."""
+    return _rms_norm("cubert_res_rms_norm_", x, residual, gamma, eps, False)
+
+
+def res_rms_norm_i8(x, residual, gamma, eps=1e-6):
+    """res_rms_norm in 8 bits: (int8 codes, fp32 scale per row, s), where codes * scales is the norm's result."""
+    return _rms_norm("cubert_res_rms_norm_i8_", x, residual, gamma, eps, True)
+
+
+class W4Weights(object):
+    """Weights [features, width] of 4 bits in the order of the Dense kernel, as w4_pack makes them."""
+
+    def __init__(self, packed, features, width, group):
+        self.packed, self.features, self.width, self.group = packed, features, width, group
+
+
+def w4_quantize(w, group=128, overflow=None):
+    """(codes uint8 [features, width / 2], scales fp16 [features, width / group]) of weights [features, width]; overflow: an int32
+    that becomes 1 where a group has a weight that is not finite or a scale beyond fp16."""
+    device = _device(w, overflow)
+    features, width = w.shape
+    if group not in (32, 64, 128) or width % group:
+        raise ValueError("groups of 32, 64 or 128 columns that divide %d expected, got %d" % (width, group))
+    codes = torch.empty((features, width // 2), dtype=torch.uint8, device=device)
+    scales = torch.empty((features, width // group), dtype=torch.float16, device=device)
+    _run_on(device, "cubert_w4_quantize_" + _suffix(w), lambda stream: (
+        _ptr(w), features, width, group, _ptr(codes), _ptr(scales), _ptr(overflow), stream))
+    return codes, scales
+
+
+def w4_pack(codes, scales, group=128):
+    """W4Weights of codes and scales as w4_quantize gives them (two's complement, two to a byte, the even column low)."""
+    device = _device(codes, scales)
+    features, width = codes.shape[0], 2 * codes.shape[1]
+    size = lib().cubert_w4_packed_bytes(features, width, group)
+    if size == 0:
+        raise ValueError("groups of 32, 64 or 128 columns that divide %d expected, got %d" % (width, group))
+    if codes.dtype != torch.uint8 or scales.dtype != torch.float16 or tuple(scales.shape) != (features, width // group):
+        raise ValueError("uint8 codes and float16 scales %s expected, got %s, %s %s" % ((features, width // group), codes.dtype,
+                                                                                       scales.dtype, tuple(scales.shape)))
+    packed = torch.empty(size, dtype=torch.uint8, device=device)
+    _run_on(device, "cubert_w4_pack", lambda stream: (_ptr(codes), _ptr(scales), features, width, group, _ptr(packed), stream))
+    return W4Weights(packed, features, width, group)
+
+
+def _dense_w4(name, x, x_scales, w, bias, gelu, dtype, out):
+    device = _device(x, x_scales, w.packed, bias, out)
+    tokens, width = x.shape
+    if width != w.width:
+        raise ValueError("rows of %d expected, got %d" % (w.width, width))
+    if out is None:
+        out = torch.empty((tokens, w.features), dtype=dtype, device=device)
+    elif out.dtype != dtype or tuple(out.shape) != (tokens, w.features):
+        raise ValueError("out: %s %s expected" % (dtype, (tokens, w.features)))
+    _like(bias, out, (w.features,), "bias")
+    rows = (_rows_ptr(x), x.stride(0) if tokens > 1 else width)
+    if x_scales is not None:
+        rows += (_ptr(x_scales),)
+    ldo = out.stride(0) if tokens > 1 else w.features
+    if not _run_on(device, name + _suffix(out), lambda stream: (stream, tokens, w.features, width) + rows + (
+            _ptr(w.packed), w.group, _ptr(bias), int(gelu), _rows_ptr(out), ldo), declines=True):
+        return None
+    return out
+
+
+def dense_w4(x, w, bias=None, gelu=False, out=None):
+    """[gelu](x w^T + bias) of fp32 or fp16 rows and W4Weights; rows of x and out may be wider than they are long.  None where
+    rows of x are not whole 16-byte pieces."""
+    _suffix(x)
+    return _dense_w4("cubert_dense_w4_", x, None, w, bias, gelu, x.dtype, out)
+
+
+def dense_w4_i8(x, x_scales, w, bias=None, gelu=False, dtype=torch.float16, out=None):
+    """dense_w4 of int8 rows with an fp32 scale per row (res_rms_norm_i8), the result in `dtype`."""
+    if x.dtype != torch.int8 or x_scales.dtype != torch.float32 or x_scales.numel() != x.shape[0]:
+        raise ValueError("int8 rows and a float32 scale for each expected")
+    return _dense_w4("cubert_dense_w4_i8_", x, x_scales, w, bias, gelu, dtype, out)
+
+
+def _heads_ptr(t, what):
+    """Of a [batch, rows, heads, size] tensor whose rows are a fixed pitch apart, in rows of contiguous heads; and that pitch."""
+    batch, rows, heads, size = t.shape
+    b, r, h, d = t.stride()
+    pitch = r if rows > 1 else b if batch > 1 else heads * size
+    if t.numel() == 0:
+        return t.data_ptr(), heads * size
+    if not heads * size <= pitch < 1 << 31 or (size > 1 and d != 1) or (heads > 1 and h != size) or (batch > 1 and b != rows * pitch):
+        raise ValueError("%s: heads side by side in rows of one pitch expected, got strides %s of %s" % (what, t.stride(), tuple(t.shape)))
+    return t.data_ptr(), pitch
+
+
+def attention_window(q, k, v, left=-1, right=-1, sinks=0, first=None, lengths=None, mask=None, alpha=None):
+    """softmax(alpha q k^T) v over the keys that each query sees, [batch, q_rows, heads, size]: query i of a sequence stands at
+    p = first + i and sees key j < length that the mask keeps with j <= p + right and (j >= p - left or j < sinks); a negative
+    left or right is no bound.  q [batch, q_rows, heads, size], k and v [batch, kv_rows, kv_heads, size] (views of a packed
+    projection or of a cache), first and lengths int32 [batch], mask int8 [batch, kv_rows].  Queries that see nothing, or
+    stand outside their sequence, give zeros.  None when the head size or the alignment does not fit."""
+    device = _device(q, k, v, first, lengths, mask)
+    batch, q_rows, heads, size = q.shape
+    kv_rows, kv_heads = k.shape[1], k.shape[2]
+    if k.dtype != q.dtype or v.dtype != q.dtype or k.shape != v.shape or k.shape[0] != batch or k.shape[3] != size:
+        raise ValueError("k and v like q expected, got %s, %s and %s" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    if kv_heads < 1 or heads % kv_heads:
+        raise ValueError("%d heads cannot share %d" % (heads, kv_heads))
+    for t, kind, shape, what in ((first, torch.int32, (batch,), "first"), (lengths, torch.int32, (batch,), "lengths"),
+                                 (mask, torch.int8, (batch, kv_rows), "mask")):
+        if t is not None and (t.dtype != kind or tuple(t.shape) != shape):
+            raise ValueError("%s: %s %s expected, got %s %s" % (what, kind, shape, t.dtype, tuple(t.shape)))
+    left, right, sinks = (min(n, 1 << 30) for n in (left, right, sinks))
+    left, right = max(left, -1), max(right, -1)
+    suffix = _suffix(q)
+    (qp, ldq), (kp, ldkv), (vp, ldv) = _heads_ptr(q, "q"), _heads_ptr(k, "k"), _heads_ptr(v, "v")
+    if ldkv != ldv:
+        raise ValueError("k and v at one row pitch expected, got %d and %d" % (ldkv, ldv))
+    ctx = torch.empty((batch, q_rows, heads, size), dtype=q.dtype, device=device)
+    floats = lib().cubert_attention_window_partials(int(suffix == "f16"), batch, heads, kv_heads, q_rows, kv_rows, size, left, right,
+                                                    sinks)
+    partials = torch.empty(floats, dtype=torch.float32, device=device) if floats else None
+    if not _run_on(device, "cubert_attention_window_" + suffix, lambda stream: (
+            qp, ldq, kp, vp, ldkv, _ptr(first), _ptr(lengths), _ptr(mask), _ptr(ctx), heads * size,
+            size ** -0.5 if alpha is None else float(alpha), batch, heads, kv_heads, q_rows, kv_rows, size, left, right, sinks,
+            _ptr(partials), floats, stream), declines=True):
+        return None
+    return ctx
+
+
 class Blas(object):
     """A BLAS context of the runtime bound to torch's current stream."""
 

@@ -220,6 +220,86 @@ int cubert_classifier_head_f16(cubert_half *pooled, const cubert_half *pooler_bi
 int cubert_transpose_f32(const float *in, int rows, int cols, float *out, void *stream);
 int cubert_transpose_f16(const cubert_half *in, int rows, int cols, cubert_half *out, void *stream);
 
+/* ------------------------------------------- layers of pre-norm models, few tokens
+ * The pieces of a layer that a pre-norm model runs a few tokens at a time: residual + RMS norm, Dense layers on weights of
+ * 4 bits, attention over a cache.  The reference, which serves post-norm encoders of at most 512 positions from 32- and
+ * 16-bit weights, has no counterpart of any of them; they stand beside the kernels named at each. */
+
+/* residual + root-mean-square norm (beside cubert_bias_res_ln_*):
+ *   s = in[r] + residual[r];   out[r] = gamma * s / sqrt(mean(s^2) + eps)
+ * `residual` may be NULL (s = in[r]).  s goes to sum_out, rounded to the storage type, as the residual of the next layer
+ * (NULL = not wanted); sum_out may be `in` or `residual` itself, `out` may be neither of the three.  The norm is taken of the unrounded fp32 s, whose
+ * squares have to stay within fp32's range.  hidden up to 32768 (more: CUBERT_UNSUPPORTED), eps >= 0. */
+int cubert_res_rms_norm_f32(const float *in, const float *residual, const float *gamma, float eps, float *sum_out, float *out,
+                            int rows, int hidden, void *stream);
+int cubert_res_rms_norm_f16(const cubert_half *in, const cubert_half *residual, const cubert_half *gamma, float eps,
+                            cubert_half *sum_out, cubert_half *out, int rows, int hidden, void *stream);
+/* The same in 8 bits, as cubert_dense_w4_i8_* takes its rows: the result is out[r, c] * scales[r] with
+ *   t = gamma * s,  m = max |t|,  out = rint(t * (127 / m)),  scales[r] = m / (127 sqrt(mean(s^2) + eps)),
+ * in fp32.  A row of zeros has scale 0 and codes 0; a row with a value (or a sum of squares) that is not finite has
+ * scale NaN and codes 0, so that whatever is made of it is NaN. */
+int cubert_res_rms_norm_i8_f32(const float *in, const float *residual, const float *gamma, float eps, float *sum_out, int8_t *out,
+                               float *scales, int rows, int hidden, void *stream);
+int cubert_res_rms_norm_i8_f16(const cubert_half *in, const cubert_half *residual, const cubert_half *gamma, float eps,
+                               cubert_half *sum_out, int8_t *out, float *scales, int rows, int hidden, void *stream);
+
+/* Weights of 4 bits with a scale per group: w[f, k] = code[f, k] * scale[f, k / group], codes -8..7, fp16 scales
+ * [features, in / group], group 32, 64 or 128 and a divisor of `in` (otherwise CUBERT_UNSUPPORTED).  Codes stand two to a
+ * byte, codes[f, k / 2], the even column in the low half, as two's complement.
+ * cubert_w4_quantize_* makes them from weights [features, in]: scale = fp16(max |w| / 7) over the group,
+ * code = rint(w / scale) within -8..7.  A group with a weight that is not finite, or whose scale fp16 cannot hold,
+ * gets scale NaN and stores 1 to *overflow (device memory, or page-locked host memory from cubert_malloc_host; NULL = not
+ * wanted; never written otherwise).  Weights of less than about 4e-4 have scales among fp16's subnormals, which are
+ * coarser.
+ * cubert_w4_pack lays codes and scales out in the order the kernel below takes them, cubert_w4_packed_bytes of them
+ * (0 for sizes it does not take) at a 16-byte aligned address; both once per model. */
+int cubert_w4_quantize_f32(const float *w, int features, int in, int group, uint8_t *codes, cubert_half *scales, int *overflow,
+                           void *stream);
+int cubert_w4_quantize_f16(const cubert_half *w, int features, int in, int group, uint8_t *codes, cubert_half *scales,
+                           int *overflow, void *stream);
+size_t cubert_w4_packed_bytes(int features, int in, int group);
+int cubert_w4_pack(const uint8_t *codes, const cubert_half *scales, int features, int in, int group, void *packed, void *stream);
+
+/* A Dense layer on such weights (beside cubert_gemm_skinny_* and cubert_dense_*):
+ *   out[t, f] = act(sum_k x[t, k] w[f, k] + bias[f]),  act = identity (0) or the erf-form GELU (1)
+ * with fp32 sums and no rounding of a weight.  x [tokens, in] at ldx elements per row, 16-byte aligned with rows of whole
+ * 16-byte pieces (otherwise CUBERT_UNSUPPORTED); `bias` may be NULL; out rows are ldo apart.  The _i8_ forms take rows of 8
+ * bits and a scale per row, x[t, k] * x_scales[t].  Any number of tokens is right, few (up to 64) are what it is made for.
+ * Asynchronous on `stream`; needs no handle and no workspace, and the same call gives the same bits. */
+int cubert_dense_w4_f32(void *stream, int tokens, int features, int in, const float *x, int ldx, const void *packed, int group,
+                        const float *bias, int activation, float *out, int ldo);
+int cubert_dense_w4_f16(void *stream, int tokens, int features, int in, const cubert_half *x, int ldx, const void *packed, int group,
+                        const cubert_half *bias, int activation, cubert_half *out, int ldo);
+int cubert_dense_w4_i8_f32(void *stream, int tokens, int features, int in, const int8_t *x, int ldx, const float *x_scales,
+                           const void *packed, int group, const float *bias, int activation, float *out, int ldo);
+int cubert_dense_w4_i8_f16(void *stream, int tokens, int features, int in, const int8_t *x, int ldx, const float *x_scales,
+                           const void *packed, int group, const cubert_half *bias, int activation, cubert_half *out, int ldo);
+
+/* Attention with a sliding window and first tokens that stay visible (beside cubert_attention_fused_*, which sees all of at most
+ * 512 keys): whole sequences, pieces of a prompt behind what a cache holds, or single tokens.
+ *   query i of sequence b stands at p = first[b] + i and sees key j if
+ *       j < lengths[b],  mask[b, j] != 0,  j <= p + right  and  (j >= p - left  or  j < sinks);
+ *   ctx[b, i, a, :] = sum_j softmax_j(alpha Q[b, i, a, :] . K[b, j, a', :]) V[b, j, a', :],  a' = a / (heads / kv_heads)
+ * over the keys it sees.  A query that sees none, or that stands outside its sequence (p < 0 or p >= lengths[b]), gets
+ * zeros; unlike in cubert_attention_fused_* a masked key is no key at all.  Scores and sums are held in fp32.
+ * q is [batch * q_rows, heads * head_size] at ldq elements per row, k and v [batch * kv_rows, kv_heads * head_size] at ldkv
+ * (kv_rows: the rows a sequence has in the cache, whatever its length), ctx like q at ld_ctx.  `first` (NULL: 0) and
+ * `lengths` (NULL: kv_rows; larger ones count as kv_rows) are device arrays of `batch` ints, `mask` (NULL: all kept) is
+ * int8 [batch, kv_rows].  K and V behind a sequence's length, and where the mask is 0, may hold anything.  A negative left or right is no bound; a right of 0 is causal.
+ * head_size 32, 64 or 128, pointers and rows of whole 16-byte pieces; otherwise CUBERT_UNSUPPORTED.
+ * Few rows over a long axis are cut along it, into `partials`: cubert_attention_window_partials floats of device memory,
+ * 16-byte aligned, that no other call uses before this one is done.  With less (or NULL) the same call runs uncut. */
+size_t cubert_attention_window_partials(int half_precision, int batch, int heads, int kv_heads, int q_rows, int kv_rows,
+                                        int head_size, int left, int right, int sinks);
+int cubert_attention_window_f32(const float *q, int ldq, const float *k, const float *v, int ldkv, const int *first,
+                                const int *lengths, const int8_t *mask, float *ctx, int ld_ctx, float alpha, int batch, int heads,
+                                int kv_heads, int q_rows, int kv_rows, int head_size, int left, int right, int sinks,
+                                float *partials, size_t partial_floats, void *stream);
+int cubert_attention_window_f16(const cubert_half *q, int ldq, const cubert_half *k, const cubert_half *v, int ldkv, const int *first,
+                                const int *lengths, const int8_t *mask, cubert_half *ctx, int ld_ctx, float alpha, int batch,
+                                int heads, int kv_heads, int q_rows, int kv_rows, int head_size, int left, int right, int sinks,
+                                float *partials, size_t partial_floats, void *stream);
+
 /* ------------------------------------------------------------------ runtime
  * replaces: reference src/cuBERT/common.h:17-92 (cudart + cuBLAS side). */
 

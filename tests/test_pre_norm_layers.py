@@ -1,0 +1,110 @@
+"""What the kernels of pre-norm layers refuse, and the sizes that callers ask for: no device call is made."""
+import pytest
+
+torch = pytest.importorskip("torch")  # before the library: both bring a HIP runtime
+
+BAD_ARGUMENT, UNSUPPORTED = -1, -2
+P = 4096  # an aligned address that nothing may read
+
+
+@pytest.fixture(scope="module")
+def L():
+    from cubert_amd._lib import lib
+    return lib()
+
+
+def norm(L, t, codes, rows=4, hidden=64, eps=1e-6, x=P, gamma=P, out=P, scales=P):
+    if codes:
+        return getattr(L, "cubert_res_rms_norm_i8_" + t)(x, P, gamma, eps, P, out, scales, rows, hidden, None)
+    return getattr(L, "cubert_res_rms_norm_" + t)(x, P, gamma, eps, P, out, rows, hidden, None)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("codes", [False, True])
+def test_rms_norm_refuses(L, t, codes):
+    for wrong in (dict(rows=-1), dict(hidden=0), dict(eps=-1.0), dict(eps=float("nan")), dict(eps=float("inf")), dict(x=None),
+                  dict(gamma=None), dict(out=None)):
+        assert norm(L, t, codes, **wrong) == BAD_ARGUMENT, wrong
+    if codes:
+        assert norm(L, t, codes, scales=None) == BAD_ARGUMENT
+    assert norm(L, t, codes, hidden=32769) == UNSUPPORTED
+    assert norm(L, t, codes, rows=0, x=None, out=None) == 0
+
+
+def dense(L, name, tokens=3, features=40, width=256, x=P, ldx=None, packed=P, group=64, activation=0, out=P, ldo=None, scales=P):
+    rows = (x, width if ldx is None else ldx) + ((scales,) if "i8" in name else ())
+    return getattr(L, "cubert_dense_w4_" + name)(None, tokens, features, width, *rows, packed, group, None, activation, out,
+                                                 features if ldo is None else ldo)
+
+
+@pytest.mark.parametrize("name", ["f32", "f16", "i8_f32", "i8_f16"])
+def test_dense_w4_refuses(L, name):
+    for wrong in (dict(tokens=-1), dict(features=0), dict(width=0), dict(x=None), dict(packed=None), dict(out=None), dict(ldx=255),
+                  dict(ldo=39), dict(activation=2)) + ((dict(scales=None),) if "i8" in name else ()):
+        assert dense(L, name, **wrong) == BAD_ARGUMENT, wrong
+    for other in (dict(group=16), dict(group=96), dict(width=96, group=64), dict(x=P + 8), dict(ldx=258), dict(packed=P + 4)):
+        assert dense(L, name, **other) == UNSUPPORTED, other
+    assert dense(L, name, tokens=0, x=None, out=None) == 0
+
+
+def test_w4_sizes_and_refusals(L):
+    # 16 features and 128 columns are 1024 bytes of codes, and 32 bytes of scales for each of their groups
+    assert L.cubert_w4_packed_bytes(16, 128, 128) == 1024 + 32
+    assert L.cubert_w4_packed_bytes(17, 160, 32) == 4 * (1024 + 4 * 32)
+    assert L.cubert_w4_packed_bytes(1, 64, 64) == 1024 + 2 * 32
+    assert L.cubert_w4_packed_bytes(32768, 65536, 128) == 2048 * 512 * (1024 + 32)
+    for sizes in ((0, 128, 128), (16, 0, 128), (16, 128, 16), (16, 96, 64)):
+        assert L.cubert_w4_packed_bytes(*sizes) == 0
+    for t in ("f32", "f16"):
+        quantize = getattr(L, "cubert_w4_quantize_" + t)
+        assert quantize(None, 16, 128, 64, P, P, None, None) == BAD_ARGUMENT
+        assert quantize(P, 16, 128, 64, None, P, None, None) == BAD_ARGUMENT
+        assert quantize(P, 0, 128, 64, P, P, None, None) == BAD_ARGUMENT
+        assert quantize(P, 16, 100, 64, P, P, None, None) == UNSUPPORTED
+    assert L.cubert_w4_pack(P, None, 16, 128, 64, P, None) == BAD_ARGUMENT
+    assert L.cubert_w4_pack(P, P, 16, 128, 48, P, None) == UNSUPPORTED
+    assert L.cubert_w4_pack(P, P, 16, 128, 64, P + 8, None) == UNSUPPORTED
+
+
+def attention(L, t, q=P, ldq=None, k=P, v=P, ldkv=None, ctx=P, ld_ctx=None, batch=2, heads=4, kv_heads=2, q_rows=3, kv_rows=50, size=64,
+              left=-1, right=0, sinks=0):
+    return getattr(L, "cubert_attention_window_" + t)(
+        q, heads * size if ldq is None else ldq, k, v, kv_heads * size if ldkv is None else ldkv, None, None, None, ctx,
+        heads * size if ld_ctx is None else ld_ctx, 1.0, batch, heads, kv_heads, q_rows, kv_rows, size, left, right, sinks, None, 0, None)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+def test_attention_window_refuses(L, t):
+    for wrong in (dict(q=None), dict(k=None), dict(v=None), dict(ctx=None), dict(batch=-1), dict(heads=0), dict(kv_heads=0), dict(kv_heads=3),
+                  dict(q_rows=-1), dict(kv_rows=-1), dict(size=0), dict(sinks=-1), dict(ldq=255), dict(ldkv=127), dict(ld_ctx=255),
+                  dict(kv_rows=(1 << 30) + 1)):
+        assert attention(L, t, **wrong) == BAD_ARGUMENT, wrong
+    for other in (dict(size=48), dict(size=256), dict(q=P + 8), dict(k=P + 8), dict(v=P + 8), dict(ctx=P + 8), dict(ldq=258), dict(ldkv=130),
+                  dict(ld_ctx=258)):
+        assert attention(L, t, **other) == UNSUPPORTED, other
+    assert attention(L, t, batch=0, q=None) == 0
+    assert attention(L, t, q_rows=0, q=None) == 0
+
+
+def test_wrappers_refuse_host_tensors():
+    from cubert_amd import kernels
+    x, g = torch.zeros(2, 64), torch.ones(64)
+    with pytest.raises(ValueError):
+        kernels.res_rms_norm(x, None, g)
+    with pytest.raises(ValueError):
+        kernels.w4_quantize(x)
+    q = torch.zeros(1, 2, 2, 64)
+    with pytest.raises(ValueError):
+        kernels.attention_window(q, q, q)
+
+
+def test_strided_heads_are_recognised():
+    from cubert_amd.kernels import _heads_ptr
+    packed = torch.zeros(3, 5, 8, 64)
+    assert _heads_ptr(packed[:, :, 2:4], "k")[1] == 8 * 64
+    assert _heads_ptr(packed[:1, :, :4], "q")[1] == 8 * 64
+    assert _heads_ptr(packed[:, :1].contiguous()[:, :, 4:], "q")[1] == 8 * 64
+    for wrong in (packed[:, :, ::2], packed[..., ::2], packed.transpose(1, 2), packed[:, 1:4], packed[::2],
+                  packed[:, :1].expand(3, 5, 8, 64)):
+        with pytest.raises(ValueError):
+            _heads_ptr(wrong, "k")
