@@ -7,6 +7,8 @@
 // A query that sees nothing, or that stands outside its sequence (p < 0 or p >= length[b]), gets zeros.  Heads share keys
 // and values in groups of heads / kv_heads.
 
+#include <atomic>
+
 #include "cubert_kernels.h"
 #include "device_common.h"
 
@@ -25,65 +27,538 @@ struct WindowArgs {
     int ldq, ldkv, ld_ctx;
     int batch, heads, kv_heads, q_rows, kv_rows;
     int left, right, sinks;
+    bool negate;  // alpha is negative: q changes its sign, so that the largest score is that of the largest product
 };
 
 __device__ __forceinline__ int clamp_to(int x, int low, int high) { return x < low ? low : x > high ? high : x; }
 
-// One wavefront per query and head, 64 keys at a time: a lane scores one key, then sums D / 64 columns over the keys.
+typedef _Float16 v8f16 __attribute__((ext_vector_type(8)));
+typedef _Float16 v4f16 __attribute__((ext_vector_type(4)));
+typedef _Float16 v2f16 __attribute__((ext_vector_type(2)));
+typedef float v4f32 __attribute__((ext_vector_type(4)));
+typedef float v2f32 __attribute__((ext_vector_type(2)));
+typedef float v16f32 __attribute__((ext_vector_type(16)));
+
+constexpr float kNone = -3e38f;  // the maximum of no scores: finite, so that differences to it are numbers
+constexpr float kSlack = 8.f;    // how far a maximum may rise, in powers of two, before sums are scaled anew
+
+// 32 rows (queries and heads of one key head) meet 32 keys in one matrix product with the keys as its rows: lane l has row
+// l % 32 and, in accumulator i, key 8 (i / 4) + 4 (l / 32) + i % 4.  The probabilities are then the second operand of the
+// product with V transposed, whose reduction may take its keys in any order that both operands keep, so they never
+// leave their lane, and neither does what belongs to a row: maximum, sum and the D / 2 results that a lane holds.
 template <typename T, int D>
-__global__ __launch_bounds__(kBlock) void attention_window_kernel(WindowArgs a) {
-    __shared__ float probs[kBlock / kWave][kWave];
-    const int wave = wave_in_block(), lane = threadIdx.x & (kWave - 1);
-    const size_t at = (size_t) blockIdx.x * (kBlock / kWave) + wave;
-    if (at >= (size_t) a.batch * a.heads * a.q_rows) return;
-    const int i = (int) (at % a.q_rows), head = (int) (at / a.q_rows % a.heads), b = (int) (at / a.q_rows / a.heads);
-    const int length = a.lengths != nullptr ? clamp_to(a.lengths[b], 0, a.kv_rows) : a.kv_rows;
-    const int p = (a.first != nullptr ? clamp_to(a.first[b], -kFar, kFar) : 0) + i;
-    const T *q = (const T *) a.q + ((size_t) b * a.q_rows + i) * a.ldq + head * D;
-    const int kv_head = head / (a.heads / a.kv_heads);
-    const T *k = (const T *) a.k + (size_t) b * a.kv_rows * a.ldkv + kv_head * D;
-    const T *v = (const T *) a.v + (size_t) b * a.kv_rows * a.ldkv + kv_head * D;
-    const int8_t *mask = a.mask != nullptr ? a.mask + (size_t) b * a.kv_rows : nullptr;
-    constexpr int kCols = (D + kWave - 1) / kWave;
-    float acc[kCols] = {};
-    float top = -INFINITY, sum = 0.f;
-    const bool there = p >= 0 && p < length;
-    const int end = there ? (p < length - a.right ? p + a.right + 1 : length) : 0;  // (p + right does not overflow here)
-    const int begin = p > a.left ? p - a.left : 0;
-    for (int base = 0; base < end; base += kWave) {
-        if (base >= a.sinks && base + kWave <= begin) base = begin / kWave * kWave;  // nothing between the sinks and the window
-        const int j = base + lane;
-        const bool seen = j < end && (j >= begin || j < a.sinks) && (mask == nullptr || mask[j] != 0);
-        float score = -INFINITY;
-        if (seen) {
-            score = 0.f;
-            for (int d = 0; d < D; ++d) score = fmaf(to_f32(q[d]), to_f32(k[(size_t) j * a.ldkv + d]), score);
-            score *= a.scale;
-        }
-        const float high = fmaxf(top, wave_max(score));
-        if (high == -INFINITY) continue;  // (the same in every lane)
-        const float shrink = exp2f(top - high), prob = seen ? exp2f(score - high) : 0.f;
-        sum = sum * shrink + wave_sum(prob);
-        top = high;
-        probs[wave][lane] = prob;
-        __builtin_amdgcn_wave_barrier();
+struct Rows {
+    static constexpr int kSteps = D * (int) sizeof(T) / 32;  // 16-byte pieces of an operand row in a half wavefront
+    static constexpr int kRowBytes = D * (int) sizeof(T);
+    static constexpr int kPieces = kRowBytes / 16;
+
+    v4f32 q[kSteps];  // pieces 2 s + l / 32 of the row
+    v16f32 ctx[D / 32];
+    float top, sum;
+
+    __device__ __forceinline__ void load(const T *row, int half_wave, bool negate) {
 #pragma unroll
-        for (int c = 0; c < kCols; ++c) {
-            const int d = c * kWave + lane;
-            acc[c] *= shrink;
-            for (int n = 0; n < kWave && base + n < end; ++n) {
-                const float pn = probs[wave][n];
-                if (pn != 0.f && d < D) acc[c] = fmaf(pn, to_f32(v[(size_t) (base + n) * a.ldkv + d]), acc[c]);
+        for (int s = 0; s < kSteps; ++s) {
+            q[s] = *reinterpret_cast<const v4f32 *>(reinterpret_cast<const char *>(row) + (2 * s + half_wave) * 16);
+            if (negate) {
+                if constexpr (sizeof(T) == 2) q[s] = __builtin_bit_cast(v4f32, -__builtin_bit_cast(v8f16, q[s]));
+                else q[s] = -q[s];
             }
         }
-        __builtin_amdgcn_wave_barrier();
-    }
-    T *ctx = (T *) a.ctx + ((size_t) b * a.q_rows + i) * a.ld_ctx + head * D;
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) {
-        const int d = c * kWave + lane;
-        if (d < D) ctx[d] = from_f32<T>(sum > 0.f ? acc[c] / sum : 0.f);
+        for (int d = 0; d < D / 32; ++d) ctx[d] = v16f32{};
+        top = kNone, sum = 0.f;
     }
+};
+
+// Which of its 16-byte pieces a row of K or V keeps its piece `at` in, so that the lanes that read together find their
+// pieces on different banks (64 of 4 bytes): of K 16 lanes read one piece of as many rows; of V in 16 bits a half wavefront reads
+// 64 bytes of four rows, in 32 bits either half 128 bytes of rows that are four apart.
+template <int ROW_BYTES>
+__device__ __forceinline__ int k_piece(int key, int at) {
+    constexpr int kShift = ROW_BYTES >= 256 ? 0 : ROW_BYTES == 128 ? 1 : 2, kMask = ROW_BYTES >= 256 ? 15 : ROW_BYTES / 16 - 1;
+    return at ^ ((key >> kShift) & kMask);
+}
+template <typename T, int ROW_BYTES>
+__device__ __forceinline__ int v_piece(int key, int at) {
+    if constexpr (sizeof(T) == 2) return ROW_BYTES == 256 ? at ^ ((key & 3) << 2) : ROW_BYTES == 128 ? at ^ ((key & 2) << 1) : at;
+    return ROW_BYTES >= 256 ? at ^ ((key & 4) << 1) : at;
+}
+
+__device__ __forceinline__ v4f16 read_transposed(const unsigned char *p) {
+    typedef short v4i16 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) v4i16 lds_v4i16;
+    return __builtin_bit_cast(v4f16, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16 *) p));
+}
+
+// 32 N keys of K and V in LDS, keys of bits 0 in `visible` left out where not all of them are seen
+template <typename T, int D, int N>
+__device__ __forceinline__ void attend(Rows<T, D> &r, const unsigned char *k, const unsigned char *v, float scale, bool all,
+                                       unsigned long long visible, int lane) {
+    typedef Rows<T, D> R;
+    const int col = lane & 31, half_wave = lane >> 5;
+    v16f32 s[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        s[n] = v16f32{};
+        const int key = 32 * n + col;
+#pragma unroll
+        for (int t = 0; t < R::kSteps; ++t) {
+            const v4f32 piece = *reinterpret_cast<const v4f32 *>(k + key * R::kRowBytes + k_piece<R::kRowBytes>(key, 2 * t + half_wave) * 16);
+            if constexpr (sizeof(T) == 2) {
+                s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8f16, piece), __builtin_bit_cast(v8f16, r.q[t]), s[n], 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(piece[e], r.q[t][e], s[n], 0, 0, 0);
+            }
+        }
+    }
+    if (!all) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const unsigned word = (unsigned) (visible >> (32 * n)) >> (4 * half_wave);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[n][i] = word >> (8 * (i / 4) + i % 4) & 1u ? s[n][i] : -INFINITY;
+        }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[n][i]);
+    top *= scale;
+    // Sums are scaled anew only when some maximum has risen by a factor of 2^8, which a probability and the sums bear.
+    if (__any(top > r.top + kSlack)) {
+        const float high = fmaxf(r.top, fmaxf(top, __shfl_xor(top, 32, kWave)));
+        const float shrink = __builtin_amdgcn_exp2f(r.top - high);
+        r.top = high;
+        r.sum *= shrink;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) r.ctx[d][i] *= shrink;
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[n][i] = __builtin_amdgcn_exp2f(fmaf(s[n][i], scale, -r.top));
+    }
+    if constexpr (sizeof(T) == 2) {
+        const int patch = lane & 15, side = (lane >> 4) & 1;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                v8f16 p;
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const v2f16 pair = __builtin_convertvector((v2f32{s[n][8 * ks + e], s[n][8 * ks + e + 1]}), v2f16);
+                    p[e] = pair[0], p[e + 1] = pair[1];
+                    // the sum is one of the probabilities as the product takes them
+                    r.sum = __builtin_amdgcn_fdot2(pair, v2f16{(half_t) 1.f, (half_t) 1.f}, r.sum, false);
+                }
+#pragma unroll
+                for (int d = 0; d < D / 32; ++d) {
+                    v4f16 part[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int key = 32 * n + 16 * ks + 8 * h + 4 * half_wave + patch / 4, at = 4 * d + 2 * side + (patch & 3) / 2;
+                        part[h] = read_transposed(v + key * R::kRowBytes + v_piece<T, R::kRowBytes>(key, at) * 16 + (patch & 1) * 8);
+                    }
+                    const v8f16 a = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
+                    r.ctx[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, p, r.ctx[d], 0, 0, 0);
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                r.sum += s[n][i];
+                const int key = 32 * n + 8 * (i / 4) + 4 * half_wave + i % 4;
+#pragma unroll
+                for (int d = 0; d < D / 32; ++d) {
+                    const float a = *reinterpret_cast<const float *>(v + key * R::kRowBytes + v_piece<T, R::kRowBytes>(key, 8 * d + col / 4) * 16 +
+                                                                     (col & 3) * 4);
+                    r.ctx[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, s[n][i], r.ctx[d], 0, 0, 0);
+                }
+            }
+    }
+}
+
+__device__ __forceinline__ unsigned long long bits_below(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; }
+
+// The keys that queries at the positions low..high of a sequence see between them, and those that each of them sees.
+struct Reach {
+    int first_begin, last_begin, first_end, last_end;  // of the window's bounds; sinks come on top
+    bool any;
+
+    __device__ __forceinline__ Reach(const WindowArgs &a, int low, int high, int length) {
+        low = low < 0 ? 0 : low, high = high < length ? high : length - 1;
+        any = low <= high;
+        first_begin = low > a.left ? low - a.left : 0, last_begin = high > a.left ? high - a.left : 0;
+        first_end = low < length - a.right ? low + a.right + 1 : length;  // (position + right may leave 32 bits)
+        last_end = high < length - a.right ? high + a.right + 1 : length;
+    }
+    // of the keys base .. base + 63: what some query may see, leaving the mask aside
+    __device__ __forceinline__ unsigned long long of(int base, int sinks) const {
+        return bits_below(last_end - base) & (~bits_below(first_begin - base) | bits_below(sinks - base));
+    }
+    __device__ __forceinline__ bool all(int base, int keys, int sinks) const {
+        return base + keys <= first_end && (base >= last_begin || base + keys <= sinks);
+    }
+};
+
+// Tiles of KEYS keys that a reach takes: those of the sinks, then those of the window.
+template <int KEYS>
+struct Tiles {
+    int of_sinks, first, count;
+
+    __device__ __forceinline__ Tiles(const Reach &reach, int sinks) {
+        first = reach.first_begin / KEYS;
+        const int end = (reach.last_end + KEYS - 1) / KEYS, far = sinks > reach.last_end ? reach.last_end : sinks;
+        of_sinks = (far + KEYS - 1) / KEYS;
+        of_sinks = of_sinks < first ? of_sinks : first;
+        count = reach.any ? of_sinks + end - first : 0;
+    }
+    __device__ __forceinline__ int base(int tile) const { return (tile < of_sinks ? tile : tile - of_sinks + first) * KEYS; }
+};
+
+// Whole 16-byte pieces of KEYS rows from row `base` on, brought to LDS by WAVES wavefronts; rows past the last are read from it.
+template <typename T, int D, int KEYS, int WAVES, bool IS_V>
+__device__ __forceinline__ void request(const T *from, int base, int rows, size_t pitch, unsigned char *to, int wave, int lane) {
+    constexpr int kRowBytes = D * (int) sizeof(T), kPieces = kRowBytes / 16, kRequests = KEYS * kPieces / (kWave * WAVES);
+    static_assert(KEYS * kPieces % (kWave * WAVES) == 0, "whole requests");
+    const char *tile = reinterpret_cast<const char *>(from + (size_t) base * pitch);
+    const int last = rows - 1 - base;
+#pragma unroll
+    for (int i = 0; i < kRequests; ++i) {
+        const int at = (i * WAVES + wave) * kWave + lane, key = at / kPieces, place = at % kPieces;
+        const int piece = IS_V ? v_piece<T, kRowBytes>(key, place) : k_piece<kRowBytes>(key, place);  // (its own inverse)
+        load_to_lds(tile + (size_t) (key < last ? key : last) * (pitch * sizeof(T)) + piece * 16, to + (i * WAVES + wave) * 1024);
+    }
+}
+
+// A key that nobody sees has probability 0, but 0 times what its row of V may hold need not be 0.
+template <typename T, int D, int KEYS, int THREADS>
+__device__ __forceinline__ void clear_rows(unsigned char *v, unsigned long long seen, int thread) {
+    constexpr int kPieces = D * (int) sizeof(T) / 16;
+#pragma unroll
+    for (int i = 0; i < KEYS * kPieces / THREADS; ++i) {
+        const int at = i * THREADS + thread;
+        if (!(seen >> (at / kPieces) & 1ull)) *reinterpret_cast<v4f32 *>(v + at * 16) = v4f32{};
+    }
+}
+
+struct Problem {
+    int b, kv_head, length, first;
+
+    __device__ __forceinline__ Problem(const WindowArgs &a, int problem) {
+        b = problem / a.kv_heads, kv_head = problem - b * a.kv_heads;
+        length = a.lengths != nullptr ? clamp_to(a.lengths[b], 0, a.kv_rows) : a.kv_rows;
+        first = a.first != nullptr ? clamp_to(a.first[b], -kFar, kFar) : 0;
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ void store4(T *to, float a, float b, float c, float d) {
+    store_vec<T, 4>(to, Vec<T, 4>{from_f32<T>(a), from_f32<T>(b), from_f32<T>(c), from_f32<T>(d)});
+}
+
+__device__ __forceinline__ void landed() {  // what this wavefront requested is in LDS
+    wait_loads<0>();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+}
+
+// Four wavefronts of 32 rows each share every tile of K and V, the next one on its way while they work on this one.
+template <typename T, int D>
+__global__ __launch_bounds__(kBlock) void attention_window_shared_kernel(WindowArgs a, int row_tiles) {
+    constexpr int kKeys = sizeof(T) == 2 ? 64 : 32, kTileBytes = kKeys * D * (int) sizeof(T);
+    extern __shared__ __align__(16) unsigned char smem[];  // two buffers of K and V
+    const int wave = wave_in_block(), lane = threadIdx.x & (kWave - 1);
+    const int problem = blockIdx.x / row_tiles, row0 = (blockIdx.x - problem * row_tiles) * 128;
+    const Problem at(a, problem);
+    const int share = a.heads / a.kv_heads, rows = a.q_rows * share;
+    const int row = row0 + 32 * wave + (lane & 31), my_row = row < rows ? row : rows - 1;
+    const int query = my_row / share, head = at.kv_head * share + my_row - query * share;
+    const int p = at.first + query;
+    const bool there = row < rows && p >= 0 && p < at.length;
+    const int begin = p > a.left ? p - a.left : 0, end = p < at.length - a.right ? p + a.right + 1 : at.length;
+
+    const T *k = (const T *) a.k + (size_t) at.b * a.kv_rows * a.ldkv + at.kv_head * D;
+    const T *v = (const T *) a.v + (size_t) at.b * a.kv_rows * a.ldkv + at.kv_head * D;
+    const int8_t *mask = a.mask != nullptr ? a.mask + (size_t) at.b * a.kv_rows : nullptr;
+    const int last_row = (row0 + 128 < rows ? row0 + 128 : rows) - 1;
+    const Reach reach(a, at.first + row0 / share, at.first + last_row / share, at.length);
+    const Tiles<kKeys> tiles(reach, a.sinks);
+    const int wave_row = row0 + 32 * wave, wave_last = wave_row + 31 < rows ? wave_row + 31 : rows - 1;
+    Reach mine(a, at.first + wave_row / share, at.first + wave_last / share, at.length);
+    mine.any = mine.any && wave_row < rows;
+
+    Rows<T, D> r;
+    r.load((const T *) a.q + ((size_t) at.b * a.q_rows + query) * a.ldq + (size_t) head * D, lane >> 5, a.negate);
+    auto bring = [&](int tile, int buffer) {
+        unsigned char *to = smem + buffer * 2 * kTileBytes;
+        request<T, D, kKeys, 4, false>(k, tiles.base(tile), a.kv_rows, a.ldkv, to, wave, lane);
+        request<T, D, kKeys, 4, true>(v, tiles.base(tile), a.kv_rows, a.ldkv, to + kTileBytes, wave, lane);
+    };
+    auto mask_byte = [&](int tile) -> int {
+        const int j = tiles.base(tile) + lane;
+        return mask != nullptr && lane < kKeys && j < a.kv_rows ? mask[j] : 1;
+    };
+    int kept = 1;
+    if (tiles.count > 0) {
+        bring(0, 0);
+        kept = mask_byte(0);
+    }
+    for (int tile = 0; tile < tiles.count; ++tile) {
+        landed();
+        const unsigned long long kept_bits = __ballot(kept != 0);
+        __syncthreads();  // everybody's; and nobody reads the other buffer any more
+        if (tile + 1 < tiles.count) {
+            bring(tile + 1, (tile + 1) & 1);
+            kept = mask_byte(tile + 1);
+        }
+        unsigned char *kt = smem + (tile & 1) * 2 * kTileBytes, *vt = kt + kTileBytes;
+        const int base = tiles.base(tile);
+        const unsigned long long seen = reach.of(base, a.sinks) & kept_bits, whole = bits_below(kKeys);
+        if ((seen & whole) != whole) {
+            clear_rows<T, D, kKeys, kBlock>(vt, seen, threadIdx.x);
+            __syncthreads();
+        }
+        if (mine.any && (mine.of(base, a.sinks) & kept_bits & whole) != 0) {
+            const bool all = mine.all(base, kKeys, a.sinks) && (kept_bits & whole) == whole;
+            const unsigned long long visible =
+                    all ? ~0ull : bits_below(end - base) & (~bits_below(begin - base) | bits_below(a.sinks - base)) & kept_bits;
+            attend<T, D, kKeys / 32>(r, kt, vt, a.scale, all, visible, lane);
+        }
+    }
+    if (row >= rows) return;
+    const float sum = r.sum + __shfl_xor(r.sum, 32, kWave);
+    const float by = there && sum > 0.f ? 1.f / sum : 0.f;
+    T *ctx = (T *) a.ctx + ((size_t) at.b * a.q_rows + query) * a.ld_ctx + (size_t) head * D + 4 * (lane >> 5);
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            if (by != 0.f) store4(ctx + 32 * d + 2 * i, r.ctx[d][i] * by, r.ctx[d][i + 1] * by, r.ctx[d][i + 2] * by, r.ctx[d][i + 3] * by);
+            else store4(ctx + 32 * d + 2 * i, 0.f, 0.f, 0.f, 0.f);
+        }
+}
+
+template <typename T, int D>
+struct Spread {
+    static constexpr int kTileBytes = 32 * D * (int) sizeof(T);                // of K, and of V
+    static constexpr int kBuffers = kTileBytes * 2 * 2 * 4 <= 128 * 1024 ? 2 : 1;
+    static constexpr int kWaveBytes = kBuffers * 2 * kTileBytes;
+    static constexpr int kPitch = D + 4;                                       // floats between rows of a wavefront's results
+    static constexpr int kMergeBytes = 4 * 32 * kPitch * 4;
+    static constexpr int kLds = 4 * kWaveBytes > kMergeBytes ? 4 * kWaveBytes : kMergeBytes;
+};
+
+// 32 rows per workgroup, whose four wavefronts take every fourth tile of 32 keys of this workgroup's piece of the axis; their
+// sums meet in LDS, in wavefront order, and go out as results or, where the axis is cut, as sums for the kernel below.
+template <typename T, int D>
+__global__ __launch_bounds__(kBlock) void attention_window_spread_kernel(WindowArgs a, int row_tiles, int pieces) {
+    typedef Spread<T, D> S;
+    extern __shared__ __align__(16) unsigned char smem[];
+    const int wave = wave_in_block(), lane = threadIdx.x & (kWave - 1);
+    const int piece = blockIdx.x % pieces, tile_at = blockIdx.x / pieces;
+    const int problem = tile_at / row_tiles, row0 = (tile_at - problem * row_tiles) * 32;
+    const Problem at(a, problem);
+    const int share = a.heads / a.kv_heads, rows = a.q_rows * share;
+    const int row = row0 + (lane & 31), my_row = row < rows ? row : rows - 1;
+    const int query = my_row / share, head = at.kv_head * share + my_row - query * share;
+    const int p = at.first + query;
+    const int begin = p > a.left ? p - a.left : 0, end = p < at.length - a.right ? p + a.right + 1 : at.length;
+
+    const T *k = (const T *) a.k + (size_t) at.b * a.kv_rows * a.ldkv + at.kv_head * D;
+    const T *v = (const T *) a.v + (size_t) at.b * a.kv_rows * a.ldkv + at.kv_head * D;
+    const int8_t *mask = a.mask != nullptr ? a.mask + (size_t) at.b * a.kv_rows : nullptr;
+    const int last_row = (row0 + 32 < rows ? row0 + 32 : rows) - 1;
+    const Reach reach(a, at.first + row0 / share, at.first + last_row / share, at.length);
+    const Tiles<32> tiles(reach, a.sinks);
+
+    Rows<T, D> r;
+    r.load((const T *) a.q + ((size_t) at.b * a.q_rows + query) * a.ldq + (size_t) head * D, lane >> 5, a.negate);
+    unsigned char *buffers = smem + wave * S::kWaveBytes;
+    // pieces of the axis: whole tiles, the first ones one more where they do not divide
+    const int each = tiles.count / pieces, more = tiles.count - each * pieces;
+    const int until = piece * each + (piece < more ? piece : more) + each + (piece < more ? 1 : 0);
+    int tile = piece * each + (piece < more ? piece : more) + wave;
+    auto bring = [&](int t, int buffer) {
+        unsigned char *to = buffers + buffer * 2 * S::kTileBytes;
+        request<T, D, 32, 1, false>(k, tiles.base(t), a.kv_rows, a.ldkv, to, 0, lane);
+        request<T, D, 32, 1, true>(v, tiles.base(t), a.kv_rows, a.ldkv, to + S::kTileBytes, 0, lane);
+    };
+    auto mask_byte = [&](int t) -> int {
+        const int j = tiles.base(t) + lane;
+        return mask != nullptr && lane < 32 && j < a.kv_rows ? mask[j] : 1;
+    };
+    int kept = 1, buffer = 0;
+    if (tile < until) {
+        bring(tile, 0);
+        kept = mask_byte(tile);
+    }
+    for (; tile < until; tile += 4) {
+        constexpr int kRequests = 2 * S::kTileBytes / 1024;
+        unsigned long long kept_bits;
+        if (S::kBuffers == 2 && tile + 4 < until) {
+            const int now = kept;
+            bring(tile + 4, buffer ^ 1);
+            kept = mask_byte(tile + 4);
+            wait_loads<kRequests>();  // (one more where a mask was read: its request is the youngest)
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("" ::: "memory");
+            kept_bits = __ballot(now != 0);
+        } else {
+            landed();
+            kept_bits = __ballot(kept != 0);
+        }
+        unsigned char *kt = buffers + buffer * 2 * S::kTileBytes, *vt = kt + S::kTileBytes;
+        const int base = tiles.base(tile);
+        const unsigned long long seen = reach.of(base, a.sinks) & kept_bits, whole = bits_below(32);
+        if ((seen & whole) != whole) {
+            clear_rows<T, D, 32, kWave>(vt, seen, lane);
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_wave_barrier();
+        }
+        if ((seen & whole) != 0) {
+            const bool all = reach.all(base, 32, a.sinks) && (kept_bits & whole) == whole;
+            const unsigned long long visible =
+                    all ? ~0ull : bits_below(end - base) & (~bits_below(begin - base) | bits_below(a.sinks - base)) & kept_bits;
+            attend<T, D, 1>(r, kt, vt, a.scale, all, visible, lane);
+        }
+        if (S::kBuffers == 2) {
+            buffer ^= 1;
+            __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): this tile has been read, its buffer is free
+            __builtin_amdgcn_sched_barrier(0);
+        } else {
+            __builtin_amdgcn_s_waitcnt(0xc07f);
+            __builtin_amdgcn_sched_barrier(0);
+            if (tile + 4 < until) {
+                bring(tile + 4, 0);
+                kept = mask_byte(tile + 4);
+            }
+        }
+    }
+    // the four wavefronts' sums, 32 rows of D + 4 floats each: results, maximum, sum
+    __syncthreads();
+    float *merge = reinterpret_cast<float *>(smem);
+    const float sum = r.sum + __shfl_xor(r.sum, 32, kWave);
+    float *to = merge + (wave * 32 + (lane & 31)) * S::kPitch;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<v4f32 *>(to + 32 * d + 2 * i + 4 * (lane >> 5)) = v4f32{r.ctx[d][i], r.ctx[d][i + 1], r.ctx[d][i + 2], r.ctx[d][i + 3]};
+    if (lane < 32) to[D] = r.top, to[D + 1] = sum;
+    __syncthreads();
+    constexpr int kQuads = D / 4;  // a thread has four columns of a row
+    for (int i = threadIdx.x; i < (last_row - row0 + 1) * kQuads; i += kBlock) {
+        const int m = i / kQuads, d = (i - m * kQuads) * 4;
+        float top = kNone;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top = fmaxf(top, merge[(w * 32 + m) * S::kPitch + D]);
+        v4f32 x = v4f32{};
+        float total = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float *from = merge + (w * 32 + m) * S::kPitch;
+            const float f = __builtin_amdgcn_exp2f(from[D] - top);
+            total += from[D + 1] * f;
+            x += *reinterpret_cast<const v4f32 *>(from + d) * f;
+        }
+        const int out_row = row0 + m, out_query = out_row / share, out_head = at.kv_head * share + out_row - out_query * share;
+        const int out_p = at.first + out_query;
+        const bool out_there = out_p >= 0 && out_p < at.length;
+        if (pieces > 1) {
+            float *out = a.partials + ((size_t) blockIdx.x * 32 + m) * S::kPitch;
+            *reinterpret_cast<v4f32 *>(out + d) = out_there ? x : v4f32{};
+            if (d == 0) out[D] = top, out[D + 1] = out_there ? total : 0.f;
+        } else {
+            const float by = out_there && total > 0.f ? 1.f / total : 0.f;
+            T *ctx = (T *) a.ctx + ((size_t) at.b * a.q_rows + out_query) * a.ld_ctx + (size_t) out_head * D + d;
+            if (by != 0.f) store4(ctx, x[0] * by, x[1] * by, x[2] * by, x[3] * by);
+            else store4(ctx, 0.f, 0.f, 0.f, 0.f);
+        }
+    }
+}
+
+// The pieces' sums of a row joined, in the order of the axis; D / 4 lanes to a row.
+template <typename T, int D>
+__global__ __launch_bounds__(kBlock) void attention_window_join_kernel(WindowArgs a, int row_tiles, int pieces, int total_rows) {
+    constexpr int kPitch = Spread<T, D>::kPitch, kQuads = D / 4;
+    const int i = blockIdx.x * (kBlock / kQuads) + threadIdx.x / kQuads, d = threadIdx.x % kQuads * 4;
+    if (i >= total_rows) return;
+    const int share = a.heads / a.kv_heads, rows = a.q_rows * share;
+    const int problem = i / rows, row = i - problem * rows, b = problem / a.kv_heads, kv_head = problem - b * a.kv_heads;
+    const float *from = a.partials + ((size_t) (problem * row_tiles + row / 32) * pieces * 32 + row % 32) * kPitch;
+    const size_t step = (size_t) 32 * kPitch;
+    float top = kNone;
+    for (int n = 0; n < pieces; ++n) top = fmaxf(top, from[n * step + D]);
+    v4f32 x = v4f32{};
+    float sum = 0.f;
+    for (int n = 0; n < pieces; ++n) {
+        const float f = __builtin_amdgcn_exp2f(from[n * step + D] - top);
+        sum += from[n * step + D + 1] * f;
+        x += *reinterpret_cast<const v4f32 *>(from + n * step + d) * f;
+    }
+    const int query = row / share, head = kv_head * share + row - query * share;
+    T *ctx = (T *) a.ctx + ((size_t) b * a.q_rows + query) * a.ld_ctx + (size_t) head * D + d;
+    const float by = sum > 0.f ? 1.f / sum : 0.f;
+    if (by != 0.f) store4(ctx, x[0] * by, x[1] * by, x[2] * by, x[3] * by);
+    else store4(ctx, 0.f, 0.f, 0.f, 0.f);
+}
+
+// How a call is run: rows of a workgroup, and into how many pieces the axis is cut.
+struct WindowPlan {
+    bool shared;
+    int row_tiles, pieces;
+    size_t floats;
+};
+
+WindowPlan plan_window(int batch, int heads, int kv_heads, int q_rows, int kv_rows, int head_size, int left, int right, int sinks) {
+    WindowPlan plan;
+    const long long rows = (long long) q_rows * (heads / kv_heads), problems = (long long) batch * kv_heads;
+    const long long shared_tiles = (rows + 127) / 128 * problems;
+    plan.shared = rows > 32 && shared_tiles >= 192;
+    plan.pieces = 1, plan.floats = 0;
+    if (plan.shared) {
+        plan.row_tiles = (int) ((rows + 127) / 128);
+        return plan;
+    }
+    plan.row_tiles = (int) ((rows + 31) / 32);
+    // the most keys that 32 rows reach
+    long long reach = kv_rows;
+    if (left >= 0 && right >= 0) reach = (long long) left + right + 33 + sinks < reach ? (long long) left + right + 33 + sinks : reach;
+    const long long tiles = (reach + 31) / 32, blocks = problems * plan.row_tiles;
+    long long pieces = blocks > 0 ? (1024 + blocks - 1) / blocks : 1;
+    pieces = pieces < (tiles + 7) / 8 ? pieces : (tiles + 7) / 8;  // two tiles to a wavefront at least
+    plan.pieces = (int) (pieces < 1 ? 1 : pieces > 256 ? 256 : pieces);
+    if (plan.pieces > 1) plan.floats = (size_t) blocks * plan.pieces * 32 * (head_size + 4);
+    return plan;
+}
+
+template <typename T, int D>
+int run_window(const WindowArgs &a, WindowPlan plan, hipStream_t stream) {
+    const int problems = a.batch * a.kv_heads;
+    if (plan.shared) {
+        constexpr int kLds = 4 * (sizeof(T) == 2 ? 64 : 32) * D * (int) sizeof(T);
+        static std::atomic<unsigned long long> done{0};
+        if (kLds > 48 * 1024 && !allow_large_lds(attention_window_shared_kernel<T, D>, done)) return CUBERT_UNSUPPORTED;
+        return launch_lds(attention_window_shared_kernel<T, D>, dim3(problems * plan.row_tiles), dim3(kBlock), kLds, stream, a, plan.row_tiles);
+    }
+    static std::atomic<unsigned long long> done{0};
+    if (Spread<T, D>::kLds > 48 * 1024 && !allow_large_lds(attention_window_spread_kernel<T, D>, done)) return CUBERT_UNSUPPORTED;
+    const int rc = launch_lds(attention_window_spread_kernel<T, D>, dim3(problems * plan.row_tiles * plan.pieces), dim3(kBlock),
+                              Spread<T, D>::kLds, stream, a, plan.row_tiles, plan.pieces);
+    if (rc != 0 || plan.pieces == 1) return rc;
+    const int total = problems * a.q_rows * (a.heads / a.kv_heads), per_block = kBlock / (D / 4);
+    return launch(attention_window_join_kernel<T, D>, dim3((total + per_block - 1) / per_block), dim3(kBlock), stream, a, plan.row_tiles,
+                  plan.pieces, total);
 }
 
 template <typename T>
@@ -91,7 +566,7 @@ int attention_window(const T *q, int ldq, const T *k, const T *v, int ldkv, cons
                      T *ctx, int ld_ctx, float alpha, int batch, int heads, int kv_heads, int q_rows, int kv_rows, int head_size,
                      int left, int right, int sinks, float *partials, size_t partial_floats, void *stream) {
     if (batch < 0 || heads < 1 || kv_heads < 1 ||
-        heads % kv_heads != 0 || q_rows < 0 || kv_rows < 0 || head_size < 1 || sinks < 0 || kv_rows > kFar || q_rows > kFar)
+        heads % kv_heads != 0 || !(alpha > -INFINITY && alpha < INFINITY) || q_rows < 0 || kv_rows < 0 || head_size < 1 || sinks < 0 || kv_rows > kFar || q_rows > kFar)
         return CUBERT_BAD_ARGUMENT;
     const long long width = (long long) heads * head_size, kv_width = (long long) kv_heads * head_size;
     if (ldq < width || ldkv < kv_width || ld_ctx < width) return CUBERT_BAD_ARGUMENT;
@@ -107,16 +582,19 @@ int attention_window(const T *q, int ldq, const T *k, const T *v, int ldkv, cons
     WindowArgs a;
     a.q = q, a.k = k, a.v = v, a.ctx = ctx, a.first = first, a.lengths = lengths, a.mask = mask;
     a.partials = partials;
-    a.scale = alpha * 1.44269504089f;
+    a.negate = alpha < 0.f;
+    // (a factor of 0 would make numbers of the infinities that stand for keys left out)
+    a.scale = fmaxf(fabsf(alpha) * 1.44269504089f, 1e-30f);
     a.ldq = ldq, a.ldkv = ldkv, a.ld_ctx = ld_ctx;
     a.batch = batch, a.heads = heads, a.kv_heads = kv_heads, a.q_rows = q_rows, a.kv_rows = kv_rows;
     a.left = left < 0 || left > kFar ? kFar : left, a.right = right < 0 || right > kFar ? kFar : right;
     a.sinks = sinks;
-    (void) partial_floats;
-    const dim3 grid((unsigned) ((rows + 3) / 4));
-    if (head_size == 32) return launch(attention_window_kernel<T, 32>, grid, dim3(kBlock), (hipStream_t) stream, a);
-    if (head_size == 64) return launch(attention_window_kernel<T, 64>, grid, dim3(kBlock), (hipStream_t) stream, a);
-    return launch(attention_window_kernel<T, 128>, grid, dim3(kBlock), (hipStream_t) stream, a);
+    WindowPlan plan = plan_window(batch, heads, kv_heads, q_rows, kv_rows, head_size, left, right, sinks);
+    if ((unsigned long long) batch * kv_heads * plan.row_tiles * plan.pieces >= 1u << 24) return CUBERT_UNSUPPORTED;
+    if (plan.pieces > 1 && (partials == nullptr || partial_floats < plan.floats || !is_aligned(partials, 16))) plan.pieces = 1;
+    if (head_size == 32) return run_window<T, 32>(a, plan, (hipStream_t) stream);
+    if (head_size == 64) return run_window<T, 64>(a, plan, (hipStream_t) stream);
+    return run_window<T, 128>(a, plan, (hipStream_t) stream);
 }
 
 }  // namespace
@@ -128,9 +606,9 @@ extern "C" {
 
 size_t cubert_attention_window_partials(int half_precision, int batch, int heads, int kv_heads, int q_rows, int kv_rows,
                                         int head_size, int left, int right, int sinks) {
-    (void) half_precision, (void) batch, (void) heads, (void) kv_heads, (void) q_rows, (void) kv_rows, (void) head_size;
-    (void) left, (void) right, (void) sinks;
-    return 0;
+    (void) half_precision;
+    if (batch < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || q_rows < 1 || kv_rows < 1 || head_size < 1) return 0;
+    return cubert::plan_window(batch, heads, kv_heads, q_rows, kv_rows, head_size, left, right, sinks).floats;
 }
 
 int cubert_attention_window_f32(const float *q, int ldq, const float *k, const float *v, int ldkv, const int *first,
