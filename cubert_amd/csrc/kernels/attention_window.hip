@@ -15,6 +15,7 @@
 namespace cubert {
 namespace {
 
+constexpr int kMaxPieces = 128;  // of an axis that is cut
 constexpr int kFar = 1 << 30;  // a bound, position or length that no sequence reaches
 
 struct WindowArgs {
@@ -487,25 +488,42 @@ __global__ __launch_bounds__(kBlock) void attention_window_spread_kernel(WindowA
     }
 }
 
-// The pieces' sums of a row joined, in the order of the axis; D / 4 lanes to a row.
+// The pieces' sums of a row joined: a workgroup per row, D / 4 threads to a piece's results, the pieces' weights in LDS.
 template <typename T, int D>
-__global__ __launch_bounds__(kBlock) void attention_window_join_kernel(WindowArgs a, int row_tiles, int pieces, int total_rows) {
-    constexpr int kPitch = Spread<T, D>::kPitch, kQuads = D / 4;
-    const int i = blockIdx.x * (kBlock / kQuads) + threadIdx.x / kQuads, d = threadIdx.x % kQuads * 4;
-    if (i >= total_rows) return;
-    const int share = a.heads / a.kv_heads, rows = a.q_rows * share;
-    const int problem = i / rows, row = i - problem * rows, b = problem / a.kv_heads, kv_head = problem - b * a.kv_heads;
+__global__ __launch_bounds__(kBlock) void attention_window_join_kernel(WindowArgs a, int row_tiles, int pieces) {
+    constexpr int kPitch = Spread<T, D>::kPitch, kQuads = D / 4, kAtOnce = kBlock / kQuads;
+    __shared__ float weights[kMaxPieces], tops[kBlock / kWave], sums[kBlock / kWave];
+    __shared__ v4f32 parts[kAtOnce][kQuads];
+    const int share = a.heads / a.kv_heads, rows = a.q_rows * share, thread = threadIdx.x;
+    const int problem = blockIdx.x / rows, row = blockIdx.x - problem * rows, b = problem / a.kv_heads, kv_head = problem - b * a.kv_heads;
     const float *from = a.partials + ((size_t) (problem * row_tiles + row / 32) * pieces * 32 + row % 32) * kPitch;
     const size_t step = (size_t) 32 * kPitch;
-    float top = kNone;
-    for (int n = 0; n < pieces; ++n) top = fmaxf(top, from[n * step + D]);
+    const int at = thread / kQuads, d = thread % kQuads * 4;
+    static_assert(kMaxPieces <= kBlock, "a thread per piece");
+    const bool mine = thread < pieces;
+    const float my_top = mine ? from[thread * step + D] : kNone, my_sum = mine ? from[thread * step + D + 1] : 0.f;
+    const float wave_top = wave_max(my_top);
+    if ((thread & (kWave - 1)) == 0) tops[thread / kWave] = wave_top;
+    __syncthreads();
+    float top = tops[0];
+#pragma unroll
+    for (int w = 1; w < kBlock / kWave; ++w) top = fmaxf(top, tops[w]);
+    const float weight = __builtin_amdgcn_exp2f(my_top - top);
+    if (mine) weights[thread] = weight;
+    const float wave_total = wave_sum(weight * my_sum);
+    if ((thread & (kWave - 1)) == 0) sums[thread / kWave] = wave_total;
+    __syncthreads();
     v4f32 x = v4f32{};
+#pragma unroll 4
+    for (int n = at; n < pieces; n += kAtOnce) x += *reinterpret_cast<const v4f32 *>(from + n * step + d) * weights[n];
+    parts[at][thread % kQuads] = x;
+    __syncthreads();
+    if (at != 0) return;
     float sum = 0.f;
-    for (int n = 0; n < pieces; ++n) {
-        const float f = __builtin_amdgcn_exp2f(from[n * step + D] - top);
-        sum += from[n * step + D + 1] * f;
-        x += *reinterpret_cast<const v4f32 *>(from + n * step + d) * f;
-    }
+#pragma unroll
+    for (int w = 0; w < kBlock / kWave; ++w) sum += sums[w];
+#pragma unroll
+    for (int n = 1; n < kAtOnce; ++n) x += parts[n][thread];
     const int query = row / share, head = kv_head * share + row - query * share;
     T *ctx = (T *) a.ctx + ((size_t) b * a.q_rows + query) * a.ld_ctx + (size_t) head * D + d;
     const float by = sum > 0.f ? 1.f / sum : 0.f;
@@ -537,7 +555,7 @@ WindowPlan plan_window(int batch, int heads, int kv_heads, int q_rows, int kv_ro
     const long long tiles = (reach + 31) / 32, blocks = problems * plan.row_tiles;
     long long pieces = blocks > 0 ? (1024 + blocks - 1) / blocks : 1;
     pieces = pieces < (tiles + 7) / 8 ? pieces : (tiles + 7) / 8;  // two tiles to a wavefront at least
-    plan.pieces = (int) (pieces < 1 ? 1 : pieces > 256 ? 256 : pieces);
+    plan.pieces = (int) (pieces < 1 ? 1 : pieces > kMaxPieces ? kMaxPieces : pieces);
     if (plan.pieces > 1) plan.floats = (size_t) blocks * plan.pieces * 32 * (head_size + 4);
     return plan;
 }
@@ -556,9 +574,8 @@ int run_window(const WindowArgs &a, WindowPlan plan, hipStream_t stream) {
     const int rc = launch_lds(attention_window_spread_kernel<T, D>, dim3(problems * plan.row_tiles * plan.pieces), dim3(kBlock),
                               Spread<T, D>::kLds, stream, a, plan.row_tiles, plan.pieces);
     if (rc != 0 || plan.pieces == 1) return rc;
-    const int total = problems * a.q_rows * (a.heads / a.kv_heads), per_block = kBlock / (D / 4);
-    return launch(attention_window_join_kernel<T, D>, dim3((total + per_block - 1) / per_block), dim3(kBlock), stream, a, plan.row_tiles,
-                  plan.pieces, total);
+    return launch(attention_window_join_kernel<T, D>, dim3(problems * a.q_rows * (a.heads / a.kv_heads)), dim3(kBlock), stream, a,
+                  plan.row_tiles, plan.pieces);
 }
 
 template <typename T>
@@ -578,7 +595,7 @@ int attention_window(const T *q, int ldq, const T *k, const T *v, int ldkv, cons
         return CUBERT_UNSUPPORTED;
     if (head_size != 32 && head_size != 64 && head_size != 128) return CUBERT_UNSUPPORTED;
     const unsigned long long rows = (unsigned long long) batch * q_rows * heads;
-    if (rows >= 1u << 26) return CUBERT_UNSUPPORTED;  // a launch holds less than 2^32 threads
+    if (rows >= 1u << 24) return CUBERT_UNSUPPORTED;  // a launch holds less than 2^32 threads
     WindowArgs a;
     a.q = q, a.k = k, a.v = v, a.ctx = ctx, a.first = first, a.lengths = lengths, a.mask = mask;
     a.partials = partials;

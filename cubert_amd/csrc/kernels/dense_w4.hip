@@ -9,7 +9,7 @@
 // bytes to a lane of a wavefront.  Lane l has feature l % 16 and, in its word s, the 8 columns 32 s + 8 (l / 16) + e: the
 // even e in the low four nibbles and the odd ones in the high four, as code + 8, so that
 // ((word >> 4 j) & 0x000f000f) | 0x64006400 is a pair of the fp16 numbers 1032 + code.  Features are filled up to 16 and
-// columns to 128 with code 0 and scale 0.  Behind the codes stand the scales, per 16 features and group the 16 of them.
+// columns to 128 with code 0 and scale 0.  Behind the codes stand the scales, of each block feature by feature, groups in order.
 
 #include "activations.h"
 #include "cubert_kernels.h"
@@ -76,9 +76,9 @@ __global__ void w4_pack_kernel(const uint8_t *__restrict__ codes, const half_t *
         }
         packed[at] = word;
     }
-    const size_t groups = blocks * (kColumns / group), real = width / group;
-    if (at < tiles * groups * kTile) {
-        const size_t f = at / (groups * kTile) * kTile + at % kTile, g = at / kTile % groups;
+    const size_t each = kColumns / group, real = width / group;
+    if (at < tiles * blocks * kTile * each) {
+        const size_t block = at / (kTile * each), f = block / blocks * kTile + at / each % kTile, g = block % blocks * each + at % each;
         half_t *to = reinterpret_cast<half_t *>(packed + words);
         to[at] = f < (size_t) features && g < real ? scales[f * real + g] : (half_t) 0.f;
     }
@@ -86,35 +86,218 @@ __global__ void w4_pack_kernel(const uint8_t *__restrict__ codes, const half_t *
 
 // ---- the product ----------------------------------------------------------
 
-// One wavefront per feature and token: a lane takes every 64th run of 8 columns.
-template <typename X, typename T>
-__global__ __launch_bounds__(kBlock) void dense_w4_kernel(int tokens, int features, int width, const X *__restrict__ x, int ldx,
-                                                          const float *__restrict__ x_scales, const uint32_t *__restrict__ packed,
-                                                          int group, const T *__restrict__ bias, int activation,
-                                                          T *__restrict__ out, int ldo) {
-    const size_t at = (size_t) blockIdx.x * (kBlock / kWave) + wave_in_block();
-    if (at >= (size_t) tokens * features) return;
-    const int lane = threadIdx.x & (kWave - 1);
-    const int t = (int) (at / features), f = (int) (at % features);
-    const size_t blocks = packed_blocks(width), tiles = packed_tiles(features), groups = blocks * (kColumns / group);
-    const half_t *scales = reinterpret_cast<const half_t *>(packed + blocks * tiles * (kBlockBytes / 4));
-    x += (size_t) t * ldx;
-    float sum = 0.f;
-    for (int k = 8 * lane; k < width; k += 8 * kWave) {
-        const size_t block = (f / kTile) * blocks + k / kColumns;
-        const int s = k % kColumns / 32, g = k % 32 / 8;
-        const uint32_t word = packed[block * (kBlockBytes / 4) + (size_t) (16 * g + f % kTile) * 4 + s];
-        float part = 0.f;
+typedef _Float16 v8f16 __attribute__((ext_vector_type(8)));
+typedef _Float16 v2f16 __attribute__((ext_vector_type(2)));
+typedef __bf16 v8bf16 __attribute__((ext_vector_type(8)));
+typedef float v4f32 __attribute__((ext_vector_type(4)));
+typedef int v4i32 __attribute__((ext_vector_type(4)));
+typedef unsigned v4u32 __attribute__((ext_vector_type(4)));
+typedef unsigned v2u32 __attribute__((ext_vector_type(2)));
+
+// What 8 columns are as operands of v_mfma_*_16x16x32, of a token (from memory) and of a feature (from a word of codes), and
+// how a group's products become a number: sums[i] * kUnit * scale.
+template <typename X>
+struct Operand;
+
+template <>
+struct Operand<half_t> {
+    typedef v4f32 Raw;
+    typedef v4f32 Sums;
+    static constexpr float kUnit = 1.f;
+    v8f16 w;
+    __device__ __forceinline__ void weights(uint32_t word) {
+        uint32_t pair[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) part = fmaf((float) ((int) (word >> (4 * (e / 2 + 4 * (e & 1))) & 15u) - 8), (float) x[k + e], part);
-        sum = fmaf((float) scales[((f / kTile) * groups + k / group) * kTile + f % kTile], part, sum);
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t biased = (word >> (4 * j) & 0x000f000fu) | 0x64006400u;  // 1024 + 8 + code
+            pair[j] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2f16, biased) - v2f16{(half_t) 1032.f, (half_t) 1032.f});
+        }
+        w = __builtin_bit_cast(v8f16, v4u32{pair[0], pair[1], pair[2], pair[3]});
     }
-    sum = wave_sum(sum);
-    if (lane == 0) {
-        if (x_scales != nullptr) sum *= x_scales[t];
-        if (bias != nullptr) sum += to_f32(bias[f]);
-        if (activation != 0) sum = GeluOp<float>()(sum);
-        out[(size_t) t * ldo + f] = from_f32<T>(sum);
+    __device__ __forceinline__ static Sums add(const Raw &x, const Operand &o, Sums sums) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8f16, x), o.w, sums, 0, 0, 0);
+    }
+};
+
+// A code in the high half of a byte is 16 times the code; the columns of a word stand in the order 0 4 1 5 2 6 3 7.
+template <>
+struct Operand<int8_t> {
+    typedef v2u32 Raw;
+    typedef v4i32 Sums;
+    static constexpr float kUnit = 1.f / 16.f;
+    long w;
+    __device__ __forceinline__ void weights(uint32_t word) {
+        word ^= 0x88888888u;
+        w = __builtin_bit_cast(long, v2u32{word << 4 & 0xf0f0f0f0u, word & 0xf0f0f0f0u});
+    }
+    __device__ __forceinline__ static Sums add(const Raw &x, const Operand &o, Sums sums) {
+        const v2u32 turned = {__builtin_amdgcn_perm(x[1], x[0], 0x05010400u), __builtin_amdgcn_perm(x[1], x[0], 0x07030602u)};
+        return __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, turned), o.w, sums, 0, 0, 0);
+    }
+};
+
+// An fp32 value is the sum of three bf16 numbers, its leading, middle and last 8 bits, and codes are bf16 numbers: every
+// product is exact, anywhere in fp32's range.
+template <>
+struct Operand<float> {
+    struct Raw {
+        v4f32 part[2];
+    };
+    typedef v4f32 Sums;
+    static constexpr float kUnit = 1.f;
+    v8bf16 w;
+    __device__ __forceinline__ void weights(uint32_t word) {
+        const uint32_t low = word & 0x0f0f0f0fu, high = word >> 4 & 0x0f0f0f0fu;  // columns 0 4 1 5 and 2 6 3 7
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int nibble = e / 2 + 4 * (e & 1);
+            f[e] = (float) ((nibble & 1 ? high : low) >> (8 * (nibble / 2)) & 0xffu) - 8.f;
+        }
+        w = top_halves(f);
+    }
+    __device__ __forceinline__ static v8bf16 top_halves(const float (&f)[8]) {
+        v4u32 r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            r[i] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, f[2 * i + 1]), __builtin_bit_cast(uint32_t, f[2 * i]), 0x07060302u);
+        return __builtin_bit_cast(v8bf16, r);
+    }
+    __device__ __forceinline__ static float top(float x) {
+        return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & 0xffff0000u);
+    }
+    struct Terms {
+        v8bf16 t[3];
+    };
+    __device__ __forceinline__ static Terms terms(const Raw &x) {
+        float a[8], b[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            a[e] = x.part[e / 4][e % 4];
+            const float lead = top(a[e]);
+            b[e] = a[e] == lead ? 0.f : a[e] - lead;  // (an infinity is its own first term; a NaN stays one in the second)
+        }
+        Terms r;
+        r.t[0] = top_halves(a);
+        r.t[1] = top_halves(b);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) b[e] -= top(b[e]);
+        r.t[2] = top_halves(b);
+        return r;
+    }
+    __device__ __forceinline__ static Sums add(const Terms &x, const Operand &o, Sums sums) {
+        sums = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.t[2], o.w, sums, 0, 0, 0);
+        sums = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.t[1], o.w, sums, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.t[0], o.w, sums, 0, 0, 0);
+    }
+};
+
+__device__ __forceinline__ v4f32 prepared(const v4f32 &x) { return x; }
+__device__ __forceinline__ v2u32 prepared(const v2u32 &x) { return x; }
+__device__ __forceinline__ Operand<float>::Terms prepared(const Operand<float>::Raw &x) { return Operand<float>::terms(x); }
+
+// The scales of a lane's feature in a block, 128 / group of them, as the low halves of one number.
+__device__ __forceinline__ unsigned long long load_scales(const half_t *scales, size_t row, int each) {
+    if (each == 4) return *reinterpret_cast<const unsigned long long *>(scales + row * 4);
+    if (each == 2) return *reinterpret_cast<const unsigned *>(scales + row * 2);
+    return *reinterpret_cast<const unsigned short *>(scales + row);
+}
+
+// A workgroup has 16 FT features and 16 TT tokens; its W wavefronts take every W-th block of 128 columns, so that all of a weight
+// row that fits is on its way at once, and their sums meet in LDS, in wavefront order.  The matrix product has tokens as rows
+// and features as columns: a lane keeps one feature per 16, whose scale it multiplies each group's sums with.
+template <typename X, typename T, int TT, int FT, int W>
+__global__ __launch_bounds__(W * kWave) void dense_w4_kernel(int tokens, int features, int width, const X *__restrict__ x, size_t ldx,
+                                                             const float *__restrict__ x_scales, const v4u32 *__restrict__ packed,
+                                                             int group, const T *__restrict__ bias, int activation,
+                                                             T *__restrict__ out, size_t ldo) {
+    typedef Operand<X> Op;
+    __shared__ float traded[W][TT * 16][17];
+    const int wave = wave_in_block(), lane = threadIdx.x & (kWave - 1), col = lane & 15, quarter = lane >> 4;
+    const int tile0 = blockIdx.x * FT, token0 = blockIdx.y * (16 * TT);
+    const int blocks = (int) packed_blocks(width), tiles = (int) packed_tiles(features), each = kColumns / group;
+    const half_t *scales = reinterpret_cast<const half_t *>(packed + (size_t) blocks * tiles * kWave);
+    const X *rows[TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+        const int token = token0 + 16 * t + col;
+        rows[t] = x + (size_t) (token < tokens ? token : tokens - 1) * ldx + 8 * quarter;  // (rows past the last are not stored)
+    }
+    size_t first[FT];  // block of a feature tile; tiles past the last repeat it and are not stored
+#pragma unroll
+    for (int f = 0; f < FT; ++f) first[f] = (size_t) (tile0 + f < tiles ? tile0 + f : tiles - 1) * blocks;
+
+    v4f32 acc[TT][FT] = {};
+    v4u32 codes[FT];
+    unsigned long long by[FT];
+    auto bring = [&](int block) {
+#pragma unroll
+        for (int f = 0; f < FT; ++f) {
+            codes[f] = packed[(first[f] + block) * kWave + lane];
+            by[f] = load_scales(scales, (first[f] + block) * kTile + col, each);
+        }
+    };
+    if (wave < blocks) bring(wave);
+    for (int block = wave; block < blocks; block += W) {
+        v4u32 now[FT];
+        unsigned long long scale[FT];
+#pragma unroll
+        for (int f = 0; f < FT; ++f) now[f] = codes[f], scale[f] = by[f];
+        typename Op::Raw piece[TT][4];
+        const int steps = (width - block * kColumns) / 32;  // of this block, 4 but in the last one
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int t = 0; t < TT; ++t)  // (steps past the end read the last one again)
+                piece[t][s] = *reinterpret_cast<const typename Op::Raw *>(rows[t] + block * kColumns + 32 * (s < steps ? s : steps - 1));
+        if (block + W < blocks) bring(block + W);
+        typename Op::Sums sums[TT][FT] = {};
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            if (s < steps) {
+                Op o[FT];
+#pragma unroll
+                for (int f = 0; f < FT; ++f) o[f].weights(now[f][s]);
+#pragma unroll
+                for (int t = 0; t < TT; ++t) {
+                    const auto ready = prepared(piece[t][s]);
+#pragma unroll
+                    for (int f = 0; f < FT; ++f) sums[t][f] = Op::add(ready, o[f], sums[t][f]);
+                }
+                if ((s + 1) * 32 % group == 0) {
+#pragma unroll
+                    for (int f = 0; f < FT; ++f) {
+                        const float by_now = (float) __builtin_bit_cast(half_t, (unsigned short) (scale[f] >> (s * 32 / group * 16))) * Op::kUnit;
+#pragma unroll
+                        for (int t = 0; t < TT; ++t) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) acc[t][f][i] = fmaf((float) sums[t][f][i], by_now, acc[t][f][i]);
+                            sums[t][f] = typename Op::Sums{};
+                        }
+                    }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int f = 0; f < FT; ++f) {
+        if (f > 0) __syncthreads();
+#pragma unroll
+        for (int t = 0; t < TT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) traded[wave][16 * t + 4 * quarter + i][col] = acc[t][f][i];
+        __syncthreads();
+        for (int i = threadIdx.x; i < TT * 256; i += W * kWave) {
+            const int token = token0 + i / 16, feature = (tile0 + f) * kTile + i % 16;
+            if (token >= tokens || feature >= features) continue;
+            float sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) sum += traded[w][i / 16][i % 16];
+            if (sizeof(X) == 1) sum *= x_scales[token];
+            if (bias != nullptr) sum += to_f32(bias[feature]);
+            if (activation != 0) sum = GeluOp<float>()(sum);
+            out[token * ldo + feature] = from_f32<T>(sum);
+        }
     }
 }
 
@@ -127,10 +310,31 @@ int dense_w4(void *stream, int tokens, int features, int in, const X *x, int ldx
     if (x == nullptr || packed == nullptr || out == nullptr || (sizeof(X) == 1 && x_scales == nullptr)) return CUBERT_BAD_ARGUMENT;
     if (!good_group(group) || in % group != 0 || !is_aligned(x, 16) || (size_t) ldx * sizeof(X) % 16 != 0 || !is_aligned(packed, 16))
         return CUBERT_UNSUPPORTED;
-    const size_t waves = (size_t) tokens * features;
-    if (waves >= (size_t) 1 << 26) return CUBERT_UNSUPPORTED;  // a launch holds less than 2^32 threads
-    return launch(dense_w4_kernel<X, T>, dim3((unsigned) ((waves + 3) / 4)), dim3(kBlock), (hipStream_t) stream, tokens, features, in,
-                  x, ldx, x_scales, (const uint32_t *) packed, group, bias, activation, out, ldo);
+    const int tiles = (int) packed_tiles(features), blocks = (int) packed_blocks(in);
+    const int token_tiles = tokens <= 16 ? 1 : tokens <= 32 ? 2 : 4;
+    const int strips = (tokens + 16 * token_tiles - 1) / (16 * token_tiles);
+    if (strips > 65535) return CUBERT_UNSUPPORTED;
+    const bool wide = tiles >= 2048, deep = blocks >= 16;
+    const hipStream_t s = (hipStream_t) stream;
+#define RUN(TT, FT, W)                                                                                                        \
+    return launch(dense_w4_kernel<X, T, TT, FT, W>, dim3((tiles + FT - 1) / FT, strips), dim3(W * kWave), s, tokens, features, in, x, \
+                  ldx, x_scales, (const v4u32 *) packed, group, bias, activation, out, ldo);
+    // (with 64 tokens, fewer features or wavefronts keep the sums and the rows of x in registers)
+    constexpr int kWide4 = sizeof(X) == 4 ? 1 : sizeof(X) == 2 ? 2 : 4, kDeep4 = sizeof(X) == 4 ? 8 : 16;
+    if (wide) {
+        if (token_tiles == 1) RUN(1, 4, 8)
+        if (token_tiles == 2) RUN(2, 4, 8)
+        RUN(4, kWide4, 8)
+    }
+    if (deep) {
+        if (token_tiles == 1) RUN(1, 1, 16)
+        if (token_tiles == 2) RUN(2, 1, 16)
+        RUN(4, 1, kDeep4)
+    }
+    if (token_tiles == 1) RUN(1, 1, 8)
+    if (token_tiles == 2) RUN(2, 1, 8)
+    RUN(4, 1, 8)
+#undef RUN
 }
 
 template <typename T>

@@ -343,6 +343,21 @@ ATTENTION = {
     "behind all keys": (2, 4, 100, 2, 1, 20, 5, 2, (98, 200), (100, 100), "no"),
 }
 
+# the same kinds of calls with so many rows that 128 of them share their tiles of keys
+WIDE = {
+    "wide encoder": (3, 257, 257, 70, 70, 40, 40, 1, None, (257, 100, 1), "no"),
+    "wide masked encoder": (2, 200, 200, 100, 50, 33, 33, 3, None, None, "padding"),
+    "wide piece": (3, 137, 500, 96, 48, 64, 0, 5, "end", (500, 200, 137), "holes"),
+    "wide piece of seven heads to one": (8, 65, 333, 56, 8, 100, 0, 70, "end", (320, 65, 333, 100, 200, 300, 66, 67), "holes"),
+    "wide causal": (1, 400, 400, 50, 50, -1, 0, 0, None, None, "no"),
+    "wide and all": (4, 150, 150, 24, 24, -1, -1, 0, None, (150, 149, 64, 65), "no"),
+    "wide and nothing left": (2, 140, 140, 48, 48, 5, 5, 0, None, None, "nothing"),
+    "wide before the sequence": (3, 150, 164, 40, 40, 10, 0, 1, "end", (164, 7, 120), "no"),
+    "wide window of one": (2, 129, 129, 49, 49, 0, 0, 0, None, None, "no"),
+    "wide sinks alone": (5, 40, 900, 80, 20, 3, 0, 40, "end", (900, 100, 800, 40, 41), "no"),
+}
+ATTENTION.update(WIDE)
+
 
 def attention_inputs(name, t, size, seed=0):
     batch, q_rows, kv_rows, heads, kv_heads, left, right, sinks, first, lengths, masked = ATTENTION[name]
@@ -427,7 +442,8 @@ def test_attention_window(K, name, t, size):
     assert bool((got[blind] == 0).all())
 
 
-@pytest.mark.parametrize("name", ["one query", "masked encoder", "piece", "few tokens", "long", "encoder", "nothing left"])
+@pytest.mark.parametrize("name", ["one query", "masked encoder", "piece", "few tokens", "long", "encoder", "nothing left", "wide encoder",
+                                  "wide masked encoder", "wide piece", "wide and nothing left"])
 @pytest.mark.parametrize("t", ["f32", "f16"])
 @pytest.mark.parametrize("filler", [math.nan, math.inf])
 def test_attention_window_past_what_it_sees(K, name, t, filler):
