@@ -488,7 +488,34 @@ __global__ __launch_bounds__(kBlock) void attention_window_spread_kernel(WindowA
     }
 }
 
-// The pieces' sums of a row joined: a workgroup per row, D / 4 threads to a piece's results, the pieces' weights in LDS.
+// The pieces' sums of a row joined, where they are few: D / 4 lanes to a row.
+template <typename T, int D>
+__global__ __launch_bounds__(kBlock) void attention_window_join_few_kernel(WindowArgs a, int row_tiles, int pieces, int total_rows) {
+    constexpr int kPitch = Spread<T, D>::kPitch, kQuads = D / 4;
+    const int i = blockIdx.x * (kBlock / kQuads) + threadIdx.x / kQuads, d = threadIdx.x % kQuads * 4;
+    if (i >= total_rows) return;
+    const int share = a.heads / a.kv_heads, rows = a.q_rows * share;
+    const int problem = i / rows, row = i - problem * rows, b = problem / a.kv_heads, kv_head = problem - b * a.kv_heads;
+    const float *from = a.partials + ((size_t) (problem * row_tiles + row / 32) * pieces * 32 + row % 32) * kPitch;
+    const size_t step = (size_t) 32 * kPitch;
+    float top = kNone;
+    for (int n = 0; n < pieces; ++n) top = fmaxf(top, from[n * step + D]);
+    v4f32 x = v4f32{};
+    float sum = 0.f;
+#pragma unroll 4
+    for (int n = 0; n < pieces; ++n) {
+        const float f = __builtin_amdgcn_exp2f(from[n * step + D] - top);
+        sum += from[n * step + D + 1] * f;
+        x += *reinterpret_cast<const v4f32 *>(from + n * step + d) * f;
+    }
+    const int query = row / share, head = kv_head * share + row - query * share;
+    T *ctx = (T *) a.ctx + ((size_t) b * a.q_rows + query) * a.ld_ctx + (size_t) head * D + d;
+    const float by = sum > 0.f ? 1.f / sum : 0.f;
+    if (by != 0.f) store4(ctx, x[0] * by, x[1] * by, x[2] * by, x[3] * by);
+    else store4(ctx, 0.f, 0.f, 0.f, 0.f);
+}
+
+// The same for many pieces: a workgroup per row, D / 4 threads to a piece's results, the pieces' weights in LDS.
 template <typename T, int D>
 __global__ __launch_bounds__(kBlock) void attention_window_join_kernel(WindowArgs a, int row_tiles, int pieces) {
     constexpr int kPitch = Spread<T, D>::kPitch, kQuads = D / 4, kAtOnce = kBlock / kQuads;
@@ -574,7 +601,12 @@ int run_window(const WindowArgs &a, WindowPlan plan, hipStream_t stream) {
     const int rc = launch_lds(attention_window_spread_kernel<T, D>, dim3(problems * plan.row_tiles * plan.pieces), dim3(kBlock),
                               Spread<T, D>::kLds, stream, a, plan.row_tiles, plan.pieces);
     if (rc != 0 || plan.pieces == 1) return rc;
-    return launch(attention_window_join_kernel<T, D>, dim3(problems * a.q_rows * (a.heads / a.kv_heads)), dim3(kBlock), stream, a,
+    const int total = problems * a.q_rows * (a.heads / a.kv_heads), per_block = kBlock / (D / 4);
+    // (18612 rows of 2 pieces: 5 us so, 22 us with a workgroup per row; 16 rows of 128: 4.4 us with one)
+    if (plan.pieces <= 8)
+        return launch(attention_window_join_few_kernel<T, D>, dim3((total + per_block - 1) / per_block), dim3(kBlock), stream, a,
+                      plan.row_tiles, plan.pieces, total);
+    return launch(attention_window_join_kernel<T, D>, dim3(total), dim3(kBlock), stream, a,
                   plan.row_tiles, plan.pieces);
 }
 

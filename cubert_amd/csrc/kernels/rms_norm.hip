@@ -20,41 +20,63 @@ namespace {
 constexpr int kMaxHidden = 32768;
 constexpr int kMaxRows = 1 << 21;  // a launch holds less than 2^32 threads
 
-// One workgroup of WAVES wavefronts per row, PER elements to a lane, WAVES * 64 apart.
-template <typename T, int WAVES, int PER, bool CODES>
-__global__ __launch_bounds__(WAVES * kWave) void rms_norm_kernel(const T *x, const T *residual, const T *__restrict__ gamma, float eps,
-                                                                T *sum_out, T *__restrict__ out, int8_t *__restrict__ codes,
-                                                                float *__restrict__ scales, int hidden) {
+// WAVES wavefronts per row, ROWS rows to a workgroup; a lane has CHUNKS runs of VEC elements, WAVES * 64 runs apart.
+template <typename T, int VEC, int CHUNKS, int WAVES, int ROWS, bool CODES>
+__global__ __launch_bounds__(WAVES * ROWS * kWave) void rms_norm_kernel(const T *x, const T *residual, const T *__restrict__ gamma, float eps,
+                                                                        T *sum_out, T *__restrict__ out, int8_t *__restrict__ codes,
+                                                                        float *__restrict__ scales, int rows, int hidden) {
+    static_assert(WAVES == 1 || ROWS == 1, "a row of several wavefronts has the workgroup to itself");
     __shared__ float traded[2][WAVES];
-    const size_t row = blockIdx.x;
-    const int thread = threadIdx.x, wave = wave_in_block();
-    x += row * hidden;
-    if (residual != nullptr) residual += row * hidden;
-    float s[PER];
+    const int wave = wave_in_block(), row = blockIdx.x * ROWS + (WAVES == 1 ? wave : 0);
+    if (row >= rows) return;  // (with several wavefronts to a row, never)
+    const int run = WAVES == 1 ? threadIdx.x & (kWave - 1) : threadIdx.x;
+    const size_t at = (size_t) row * hidden;
+    Vec<T, VEC> a[CHUNKS], r[CHUNKS], g[CHUNKS];
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+        const int col = (c * WAVES * kWave + run) * VEC;
+        if (col < hidden) a[c] = load_vec<T, VEC>(x + at + col);
+    }
+    if (residual != nullptr) {
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            const int col = (c * WAVES * kWave + run) * VEC;
+            if (col < hidden) r[c] = load_vec<T, VEC>(residual + at + col);
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+        const int col = (c * WAVES * kWave + run) * VEC;
+        if (col < hidden) g[c] = load_vec<T, VEC>(gamma + col);
+    }
+    float s[CHUNKS][VEC];
     float squares = 0.f, top = 0.f;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int col = i * WAVES * kWave + thread;
-        s[i] = 0.f;
-        if (col < hidden) {
-            s[i] = to_f32(x[col]);
-            if (residual != nullptr) s[i] += to_f32(residual[col]);
-            squares = fmaf(s[i], s[i], squares);
-            if (CODES) top = fmaxf(top, fabsf(to_f32(gamma[col]) * s[i]));
+    for (int c = 0; c < CHUNKS; ++c) {
+        if ((c * WAVES * kWave + run) * VEC < hidden) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                s[c][i] = to_f32(a[c].v[i]);
+                if (residual != nullptr) s[c][i] += to_f32(r[c].v[i]);
+                squares = fmaf(s[c][i], s[c][i], squares);
+                if (CODES) top = fmaxf(top, fabsf(to_f32(g[c].v[i]) * s[c][i]));
+            }
         }
     }
     squares = wave_sum(squares);
     if (CODES) top = wave_max(top);
-    if ((thread & (kWave - 1)) == 0) {
-        traded[0][wave] = squares;
-        traded[1][wave] = top;
-    }
-    __syncthreads();
-    squares = 0.f;
+    if constexpr (WAVES > 1) {
+        if ((threadIdx.x & (kWave - 1)) == 0) {
+            traded[0][wave] = squares;
+            traded[1][wave] = top;
+        }
+        __syncthreads();
+        squares = 0.f;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-        squares += traded[0][w];
-        top = fmaxf(top, traded[1][w]);
+        for (int w = 0; w < WAVES; ++w) {
+            squares += traded[0][w];
+            if (CODES) top = fmaxf(top, traded[1][w]);
+        }
     }
     const float rstd = 1.f / sqrtf(squares / (float) hidden + eps);
     // A NaN is lost in a maximum and an infinity leaves no finite factor: such a row's scale is NaN and its codes are 0.
@@ -62,15 +84,23 @@ __global__ __launch_bounds__(WAVES * kWave) void rms_norm_kernel(const T *x, con
     // 127 / m leaves fp32's range for m below 2^-121: rows that small are raised by a power of two first, which is exact.
     const float raise = top < 0x1p-60f ? 0x1p80f : 1.f;
     const float inverse = top > 0.f && finite ? 127.f / (top * raise) : 0.f;
-    if (CODES && thread == 0) scales[row] = finite ? top * rstd / 127.f : NAN;
+    if (CODES && run == 0) scales[row] = finite ? top * rstd / 127.f : NAN;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int col = i * WAVES * kWave + thread;
+    for (int c = 0; c < CHUNKS; ++c) {
+        const int col = (c * WAVES * kWave + run) * VEC;
         if (col < hidden) {
-            const float g = to_f32(gamma[col]);
-            if (sum_out != nullptr) sum_out[row * hidden + col] = from_f32<T>(s[i]);
-            if (CODES) codes[row * hidden + col] = finite ? (int8_t) rintf(((g * s[i]) * raise) * inverse) : (int8_t) 0;
-            else out[row * hidden + col] = from_f32<T>(g * (s[i] * rstd));
+            Vec<T, VEC> total, y;
+            Vec<int8_t, VEC> code;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const float gain = to_f32(g[c].v[i]);
+                total.v[i] = from_f32<T>(s[c][i]);
+                if (CODES) code.v[i] = finite ? (int8_t) rintf(((gain * s[c][i]) * raise) * inverse) : (int8_t) 0;
+                else y.v[i] = from_f32<T>(gain * (s[c][i] * rstd));
+            }
+            if (sum_out != nullptr) store_vec<T, VEC>(sum_out + at + col, total);
+            if (CODES) store_vec<int8_t, VEC>(codes + at + col, code);
+            else store_vec<T, VEC>(out + at + col, y);
         }
     }
 }
@@ -83,11 +113,21 @@ int rms_norm(const T *x, const T *residual, const T *gamma, float eps, T *sum_ou
     if (rows == 0) return 0;
     if (x == nullptr || gamma == nullptr || (CODES ? codes == nullptr || scales == nullptr : out == nullptr)) return CUBERT_BAD_ARGUMENT;
     const hipStream_t s = (hipStream_t) stream;
-#define RUN(WAVES, PER)                                                                                                     \
-    if (hidden <= WAVES * kWave * PER)                                                                                      \
-        return launch(rms_norm_kernel<T, WAVES, PER, CODES>, dim3(rows), dim3(WAVES * kWave), s, x, residual, gamma, eps, sum_out, \
-                      out, codes, scales, hidden);
-    RUN(4, 4) RUN(4, 16) RUN(16, 8) RUN(16, 32)
+    constexpr int kVec = 16 / (int) sizeof(T);
+    const bool whole = hidden % kVec == 0 && is_aligned(x, 16) && is_aligned(gamma, 16) && (residual == nullptr || is_aligned(residual, 16)) &&
+                       (sum_out == nullptr || is_aligned(sum_out, 16)) && (CODES ? is_aligned(codes, kVec) : is_aligned(out, 16));
+#define RUN(VEC, CHUNKS, WAVES, ROWS)                                                                                         \
+    if (hidden <= VEC * CHUNKS * WAVES * kWave)                                                                               \
+        return launch(rms_norm_kernel<T, VEC, CHUNKS, WAVES, ROWS, CODES>, dim3((rows + ROWS - 1) / ROWS), dim3(WAVES * ROWS * kWave), s, \
+                      x, residual, gamma, eps, sum_out, out, codes, scales, rows, hidden);
+    if (whole && rows >= 1024) {
+        RUN(kVec, 1, 1, 4) RUN(kVec, 2, 1, 4) RUN(kVec, 4, 1, 4)
+    }
+    if (whole) {
+        RUN(kVec, 1, 4, 1) RUN(kVec, 2, 4, 1) RUN(kVec, 1, 16, 1) RUN(kVec, 4, 16, 1)
+        if (sizeof(T) == 4) RUN(kVec, 8, 16, 1)
+    }
+    RUN(1, 4, 4, 1) RUN(1, 4, 16, 1) RUN(1, 32, 16, 1)
 #undef RUN
     return CUBERT_UNSUPPORTED;
 }
