@@ -392,64 +392,82 @@ def bias_res_ln_slices(partials, residual, bias, beta, gamma):
 # ---- layers of pre-norm models, few tokens
 
 
+_SUFFIXES = {torch.float32: "f32", torch.float16: "f16"}
+# a few tokens take a few microseconds, so the host's share of a call counts: the stream's handle without a Stream around it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
 def _device(t, *others):
-    """The device that the call's tensors are on: one and the same."""
-    if not t.is_cuda:
+    """The number of the device that the call's tensors are on: one and the same."""
+    device = t.get_device()
+    if device < 0:
         raise ValueError("CUDA tensors expected")
     for o in others:
-        if o is not None and o.device != t.device:
+        if o is not None and o.get_device() != device:
             raise ValueError("tensors on different devices: %s and %s" % (t.device, o.device))
-    return t.device
+    return device
 
 
-def _run_on(device, name, args, declines=False):
-    """The entry point `name` on `device` and its current stream (the last of args, or the first, is None for it);
-    True, or False where it declines."""
+def _run_on(device, name, args, declines=True):
+    """The entry point `name`, with `device` the current one; True, or False where it declines."""
     fn = getattr(lib(), name)
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args(torch.cuda.current_stream().cuda_stream))
+    if device == torch.cuda.current_device():
+        rc = fn(*args)
     else:
         with torch.cuda.device(device):
-            rc = fn(*args(torch.cuda.current_stream().cuda_stream))
+            rc = fn(*args)
+    if rc == 0:
+        return True
     if rc == -2 and declines:
         return False
     _check(rc, name)
-    return True
 
 
 def _like(t, ref, shape, what):
-    if t is not None and (t.dtype != ref.dtype or tuple(t.shape) != tuple(shape)):
+    if t.dtype != ref.dtype or t.shape != shape:
         raise ValueError("%s: %s %s expected, got %s %s" % (what, ref.dtype, tuple(shape), t.dtype, tuple(t.shape)))
 
 
-def _rms_norm(name, x, residual, gamma, eps, codes):
+def _whole_ptr(t):
+    if not t.is_contiguous():
+        raise ValueError("contiguous CUDA tensor expected")
+    return t.data_ptr()
+
+
+def _rms_norm(x, residual, gamma, eps, codes):
     device = _device(x, residual, gamma)
+    suffix = _SUFFIXES.get(x.dtype) or _suffix(x)
     hidden = x.shape[-1]
     rows = x.numel() // hidden if hidden else 0
-    suffix = _suffix(x)
     if hidden == 0 or rows >= 1 << 31:
         raise ValueError("rows expected, got %s" % (tuple(x.shape),))
-    _like(residual, x, x.shape, "residual")
     _like(gamma, x, (hidden,), "gamma")
-    total = torch.empty_like(x) if residual is not None else None
-    outs = (torch.empty_like(x, dtype=torch.int8), torch.empty(x.shape[:-1], dtype=torch.float32, device=device)) if codes \
-        else (torch.empty_like(x),)
-    pointers = tuple(_ptr(t) for t in (x, residual, gamma))
-    if not _run_on(device, name + suffix, lambda stream: pointers + (float(eps), _ptr(total)) + tuple(_ptr(t) for t in outs) +
-                   (rows, hidden, stream), declines=True):
-        return None
-    return outs + (total,)
+    args = (_whole_ptr(x),)
+    total = None
+    if residual is not None:
+        _like(residual, x, x.shape, "residual")
+        total = torch.empty_like(x)
+        args += (_whole_ptr(residual), _whole_ptr(gamma), float(eps), total.data_ptr())
+    else:
+        args += (None, _whole_ptr(gamma), float(eps), None)
+    if codes:
+        out, scales = torch.empty_like(x, dtype=torch.int8), torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        args += (out.data_ptr(), scales.data_ptr(), rows, hidden, _raw_stream(device))
+        return (out, scales, total) if _run_on(device, "cubert_res_rms_norm_i8_" + suffix, args) else None
+    out = torch.empty_like(x)
+    args += (out.data_ptr(), rows, hidden, _raw_stream(device))
+    return (out, total) if _run_on(device, "cubert_res_rms_norm_" + suffix, args) else None
 
 
 def res_rms_norm(x, residual, gamma, eps=1e-6):
     """(gamma * s / sqrt(mean(s^2) + eps), s) of s = x + residual over the last axis; without a residual s is x and the second
     result None.  None when the rows are too long."""
-    return _rms_norm("cubert_res_rms_norm_", x, residual, gamma, eps, False)
+    return _rms_norm(x, residual, gamma, eps, False)
 
 
 def res_rms_norm_i8(x, residual, gamma, eps=1e-6):
     """res_rms_norm in 8 bits: (int8 codes, fp32 scale per row, s), where codes * scales is the norm's result."""
-    return _rms_norm("cubert_res_rms_norm_i8_", x, residual, gamma, eps, True)
+    return _rms_norm(x, residual, gamma, eps, True)
 
 
 class W4Weights(object):
@@ -466,10 +484,10 @@ def w4_quantize(w, group=128, overflow=None):
     features, width = w.shape
     if group not in (32, 64, 128) or width % group:
         raise ValueError("groups of 32, 64 or 128 columns that divide %d expected, got %d" % (width, group))
-    codes = torch.empty((features, width // 2), dtype=torch.uint8, device=device)
-    scales = torch.empty((features, width // group), dtype=torch.float16, device=device)
-    _run_on(device, "cubert_w4_quantize_" + _suffix(w), lambda stream: (
-        _ptr(w), features, width, group, _ptr(codes), _ptr(scales), _ptr(overflow), stream))
+    codes = torch.empty((features, width // 2), dtype=torch.uint8, device=w.device)
+    scales = torch.empty((features, width // group), dtype=torch.float16, device=w.device)
+    _run_on(device, "cubert_w4_quantize_" + _suffix(w), (_ptr(w), features, width, group, _ptr(codes), _ptr(scales), _ptr(overflow),
+                                                         _raw_stream(device)), declines=False)
     return codes, scales
 
 
@@ -483,43 +501,49 @@ def w4_pack(codes, scales, group=128):
     if codes.dtype != torch.uint8 or scales.dtype != torch.float16 or tuple(scales.shape) != (features, width // group):
         raise ValueError("uint8 codes and float16 scales %s expected, got %s, %s %s" % ((features, width // group), codes.dtype,
                                                                                        scales.dtype, tuple(scales.shape)))
-    packed = torch.empty(size, dtype=torch.uint8, device=device)
-    _run_on(device, "cubert_w4_pack", lambda stream: (_ptr(codes), _ptr(scales), features, width, group, _ptr(packed), stream))
+    packed = torch.empty(size, dtype=torch.uint8, device=codes.device)
+    _run_on(device, "cubert_w4_pack", (_ptr(codes), _ptr(scales), features, width, group, _ptr(packed), _raw_stream(device)),
+            declines=False)
     return W4Weights(packed, features, width, group)
 
 
-def _dense_w4(name, x, x_scales, w, bias, gelu, dtype, out):
+def _dense_w4(x, x_scales, w, bias, gelu, dtype, out):
     device = _device(x, x_scales, w.packed, bias, out)
+    suffix = _SUFFIXES.get(dtype)
+    if suffix is None:
+        raise TypeError("float32 or float16 expected, got %s" % dtype)
     tokens, width = x.shape
+    features = w.features
     if width != w.width:
         raise ValueError("rows of %d expected, got %d" % (w.width, width))
     if out is None:
-        out = torch.empty((tokens, w.features), dtype=dtype, device=device)
-    elif out.dtype != dtype or tuple(out.shape) != (tokens, w.features):
-        raise ValueError("out: %s %s expected" % (dtype, (tokens, w.features)))
-    _like(bias, out, (w.features,), "bias")
-    rows = (_rows_ptr(x), x.stride(0) if tokens > 1 else width)
+        out = torch.empty((tokens, features), dtype=dtype, device=x.device)
+        to, ldo = out.data_ptr(), features
+    else:
+        if out.dtype != dtype or out.shape != (tokens, features):
+            raise ValueError("out: %s %s expected" % (dtype, (tokens, features)))
+        to, ldo = _rows_ptr(out), out.stride(0) if tokens > 1 else features
+    if bias is not None:
+        _like(bias, out, (features,), "bias")
+        bias = _whole_ptr(bias)
+    args = (_raw_stream(device), tokens, features, width, _rows_ptr(x), x.stride(0) if tokens > 1 else width)
     if x_scales is not None:
-        rows += (_ptr(x_scales),)
-    ldo = out.stride(0) if tokens > 1 else w.features
-    if not _run_on(device, name + _suffix(out), lambda stream: (stream, tokens, w.features, width) + rows + (
-            _ptr(w.packed), w.group, _ptr(bias), int(gelu), _rows_ptr(out), ldo), declines=True):
-        return None
-    return out
+        args += (_whole_ptr(x_scales),)
+        suffix = "i8_" + suffix
+    return out if _run_on(device, "cubert_dense_w4_" + suffix, args + (w.packed.data_ptr(), w.group, bias, int(gelu), to, ldo)) else None
 
 
 def dense_w4(x, w, bias=None, gelu=False, out=None):
     """[gelu](x w^T + bias) of fp32 or fp16 rows and W4Weights; rows of x and out may be wider than they are long.  None where
     rows of x are not whole 16-byte pieces."""
-    _suffix(x)
-    return _dense_w4("cubert_dense_w4_", x, None, w, bias, gelu, x.dtype, out)
+    return _dense_w4(x, None, w, bias, gelu, x.dtype, out)
 
 
 def dense_w4_i8(x, x_scales, w, bias=None, gelu=False, dtype=torch.float16, out=None):
     """dense_w4 of int8 rows with an fp32 scale per row (res_rms_norm_i8), the result in `dtype`."""
     if x.dtype != torch.int8 or x_scales.dtype != torch.float32 or x_scales.numel() != x.shape[0]:
         raise ValueError("int8 rows and a float32 scale for each expected")
-    return _dense_w4("cubert_dense_w4_i8_", x, x_scales, w, bias, gelu, dtype, out)
+    return _dense_w4(x, x_scales, w, bias, gelu, dtype, out)
 
 
 def _heads_ptr(t, what):
@@ -547,26 +571,25 @@ def attention_window(q, k, v, left=-1, right=-1, sinks=0, first=None, lengths=No
         raise ValueError("k and v like q expected, got %s, %s and %s" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
     if kv_heads < 1 or heads % kv_heads:
         raise ValueError("%d heads cannot share %d" % (heads, kv_heads))
-    for t, kind, shape, what in ((first, torch.int32, (batch,), "first"), (lengths, torch.int32, (batch,), "lengths"),
-                                 (mask, torch.int8, (batch, kv_rows), "mask")):
-        if t is not None and (t.dtype != kind or tuple(t.shape) != shape):
-            raise ValueError("%s: %s %s expected, got %s %s" % (what, kind, shape, t.dtype, tuple(t.shape)))
-    left, right, sinks = (min(n, 1 << 30) for n in (left, right, sinks))
-    left, right = max(left, -1), max(right, -1)
-    suffix = _suffix(q)
+    if first is not None and (first.dtype != torch.int32 or first.shape != (batch,)):
+        raise ValueError("first: int32 (%d,) expected, got %s %s" % (batch, first.dtype, tuple(first.shape)))
+    if lengths is not None and (lengths.dtype != torch.int32 or lengths.shape != (batch,)):
+        raise ValueError("lengths: int32 (%d,) expected, got %s %s" % (batch, lengths.dtype, tuple(lengths.shape)))
+    if mask is not None and (mask.dtype != torch.int8 or mask.shape != (batch, kv_rows)):
+        raise ValueError("mask: int8 (%d, %d) expected, got %s %s" % (batch, kv_rows, mask.dtype, tuple(mask.shape)))
+    left, right, sinks = max(min(left, 1 << 30), -1), max(min(right, 1 << 30), -1), min(sinks, 1 << 30)
+    suffix = _SUFFIXES.get(q.dtype) or _suffix(q)
     (qp, ldq), (kp, ldkv), (vp, ldv) = _heads_ptr(q, "q"), _heads_ptr(k, "k"), _heads_ptr(v, "v")
     if ldkv != ldv:
         raise ValueError("k and v at one row pitch expected, got %d and %d" % (ldkv, ldv))
-    ctx = torch.empty((batch, q_rows, heads, size), dtype=q.dtype, device=device)
-    floats = lib().cubert_attention_window_partials(int(suffix == "f16"), batch, heads, kv_heads, q_rows, kv_rows, size, left, right,
-                                                    sinks)
-    partials = torch.empty(floats, dtype=torch.float32, device=device) if floats else None
-    if not _run_on(device, "cubert_attention_window_" + suffix, lambda stream: (
-            qp, ldq, kp, vp, ldkv, _ptr(first), _ptr(lengths), _ptr(mask), _ptr(ctx), heads * size,
-            size ** -0.5 if alpha is None else float(alpha), batch, heads, kv_heads, q_rows, kv_rows, size, left, right, sinks,
-            _ptr(partials), floats, stream), declines=True):
-        return None
-    return ctx
+    ctx = torch.empty((batch, q_rows, heads, size), dtype=q.dtype, device=q.device)
+    floats = lib().cubert_attention_window_partials(suffix == "f16", batch, heads, kv_heads, q_rows, kv_rows, size, left, right, sinks)
+    partials = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
+    args = (qp, ldq, kp, vp, ldkv, None if first is None else _whole_ptr(first), None if lengths is None else _whole_ptr(lengths),
+            None if mask is None else _whole_ptr(mask), ctx.data_ptr(), heads * size, size ** -0.5 if alpha is None else float(alpha),
+            batch, heads, kv_heads, q_rows, kv_rows, size, left, right, sinks, partials.data_ptr() if floats else None, floats,
+            _raw_stream(device))
+    return ctx if _run_on(device, "cubert_attention_window_" + suffix, args) else None
 
 
 class Blas(object):
