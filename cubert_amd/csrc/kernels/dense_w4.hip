@@ -8,7 +8,7 @@
 // cubert_w4_pack lays the weights out once in the order the kernel takes them: 16 features and 128 columns are 1 KB, 16
 // bytes to a lane of a wavefront.  Lane l has feature l % 16 and, in its word s, the 8 columns 32 s + 8 (l / 16) + e: the
 // even e in the low four nibbles and the odd ones in the high four, as code + 8, so that
-// ((word >> 4 j) & 0x000f000f) | 0x64006400 is a pair of the fp16 numbers 1032 + code.  Features are filled up to 16 and
+// (word & 0x000f000f) | 0x64006400 is a pair of the fp16 numbers 1032 + code.  Features are filled up to 16 and
 // columns to 128 with code 0 and scale 0.  Behind the codes stand the scales, of each block feature by feature, groups in order.
 
 #include "activations.h"
@@ -94,6 +94,13 @@ typedef int v4i32 __attribute__((ext_vector_type(4)));
 typedef unsigned v4u32 __attribute__((ext_vector_type(4)));
 typedef unsigned v2u32 __attribute__((ext_vector_type(2)));
 
+// (x & mask) | bits in one instruction, which the compiler makes two of where both are constants.
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
+    uint32_t r;
+    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "s"(mask), "v"(bits));
+    return r;
+}
+
 // What 8 columns are as operands of v_mfma_*_16x16x32, of a token (from memory) and of a feature (from a word of codes), and
 // how a group's products become a number: sums[i] * kUnit * scale.
 template <typename X>
@@ -108,12 +115,17 @@ struct Operand<half_t> {
     __device__ __forceinline__ void weights(uint32_t word) {
         uint32_t pair[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t biased = (word >> (4 * j) & 0x000f000fu) | 0x64006400u;  // 1024 + 8 + code
-            pair[j] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2f16, biased) - v2f16{(half_t) 1032.f, (half_t) 1032.f});
+        for (int j = 0; j < 4; j += 2) {
+            const uint32_t part = j == 0 ? word : word >> 8;
+            const uint32_t low = and_or(part, 0x000f000fu, 0x64006400u), high = and_or(part, 0x00f000f0u, 0x64006400u);
+            // 1024 + (8 + code), and 1024 + 16 (8 + code): both exact
+            pair[j] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2f16, low) - v2f16{(half_t) 1032.f, (half_t) 1032.f});
+            pair[j + 1] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(v2f16, high), v2f16{(half_t) 0.0625f, (half_t) 0.0625f},
+                                                                                 v2f16{(half_t) -72.f, (half_t) -72.f}));
         }
         w = __builtin_bit_cast(v8f16, v4u32{pair[0], pair[1], pair[2], pair[3]});
     }
+    __device__ __forceinline__ static Raw ready(const Raw &x) { return x; }
     __device__ __forceinline__ static Sums add(const Raw &x, const Operand &o, Sums sums) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8f16, x), o.w, sums, 0, 0, 0);
     }
@@ -130,18 +142,24 @@ struct Operand<int8_t> {
         word ^= 0x88888888u;
         w = __builtin_bit_cast(long, v2u32{word << 4 & 0xf0f0f0f0u, word & 0xf0f0f0f0u});
     }
-    __device__ __forceinline__ static Sums add(const Raw &x, const Operand &o, Sums sums) {
-        const v2u32 turned = {__builtin_amdgcn_perm(x[1], x[0], 0x05010400u), __builtin_amdgcn_perm(x[1], x[0], 0x07030602u)};
-        return __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, turned), o.w, sums, 0, 0, 0);
+    __device__ __forceinline__ static long ready(const Raw &x) {
+        return __builtin_bit_cast(long, v2u32{__builtin_amdgcn_perm(x[1], x[0], 0x05010400u), __builtin_amdgcn_perm(x[1], x[0], 0x07030602u)});
+    }
+    __device__ __forceinline__ static Sums add(long x, const Operand &o, Sums sums) {
+        return __builtin_amdgcn_mfma_i32_16x16x32_i8(x, o.w, sums, 0, 0, 0);
     }
 };
 
 // An fp32 value is the sum of three bf16 numbers, its leading, middle and last 8 bits, and codes are bf16 numbers: every
-// product is exact, anywhere in fp32's range.
+// product is exact, anywhere in fp32's range.  (fp32 matrix instructions, a sixteenth as fast: 16 tokens, 4096 x 16384, 29 us
+// against 19.)
 template <>
 struct Operand<float> {
     struct Raw {
         v4f32 part[2];
+    };
+    struct Ready {
+        v8bf16 term[3];
     };
     typedef v4f32 Sums;
     static constexpr float kUnit = 1.f;
@@ -154,151 +172,172 @@ struct Operand<float> {
             const int nibble = e / 2 + 4 * (e & 1);
             f[e] = (float) ((nibble & 1 ? high : low) >> (8 * (nibble / 2)) & 0xffu) - 8.f;
         }
-        w = top_halves(f);
+        w = leading(f);
     }
-    __device__ __forceinline__ static v8bf16 top_halves(const float (&f)[8]) {
+    __device__ __forceinline__ static v8bf16 leading(const float (&f)[8]) {
         v4u32 r;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             r[i] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, f[2 * i + 1]), __builtin_bit_cast(uint32_t, f[2 * i]), 0x07060302u);
         return __builtin_bit_cast(v8bf16, r);
     }
-    __device__ __forceinline__ static float top(float x) {
+    __device__ __forceinline__ static float lead(float x) {
         return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & 0xffff0000u);
     }
-    struct Terms {
-        v8bf16 t[3];
-    };
-    __device__ __forceinline__ static Terms terms(const Raw &x) {
-        float a[8], b[8];
+    __device__ __forceinline__ static Ready ready(const Raw &x) {
+        float a[8];
+        Ready r;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            a[e] = x.part[e / 4][e % 4];
-            const float lead = top(a[e]);
-            b[e] = a[e] == lead ? 0.f : a[e] - lead;  // (an infinity is its own first term; a NaN stays one in the second)
+        for (int e = 0; e < 8; ++e) a[e] = x.part[e / 4][e % 4];
+        r.term[0] = leading(a);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {  // (an infinity is its own first term; a NaN stays one in the second)
+            const float top = lead(a[e]);
+            a[e] = a[e] == top ? 0.f : a[e] - top;
         }
-        Terms r;
-        r.t[0] = top_halves(a);
-        r.t[1] = top_halves(b);
+        r.term[1] = leading(a);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) b[e] -= top(b[e]);
-        r.t[2] = top_halves(b);
+        for (int e = 0; e < 8; ++e) a[e] -= lead(a[e]);
+        r.term[2] = leading(a);
         return r;
     }
-    __device__ __forceinline__ static Sums add(const Terms &x, const Operand &o, Sums sums) {
-        sums = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.t[2], o.w, sums, 0, 0, 0);
-        sums = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.t[1], o.w, sums, 0, 0, 0);
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.t[0], o.w, sums, 0, 0, 0);
+    __device__ __forceinline__ static Sums add(const Ready &x, const Operand &o, Sums sums) {
+#pragma unroll
+        for (int n = 2; n >= 0; --n) sums = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.term[n], o.w, sums, 0, 0, 0);
+        return sums;
     }
 };
 
-__device__ __forceinline__ v4f32 prepared(const v4f32 &x) { return x; }
-__device__ __forceinline__ v2u32 prepared(const v2u32 &x) { return x; }
-__device__ __forceinline__ Operand<float>::Terms prepared(const Operand<float>::Raw &x) { return Operand<float>::terms(x); }
+// The scales of a lane's feature in a block: 128 / group = EACH halves.
+template <int EACH>
+struct Scales {
+    Vec<half_t, EACH> v;
 
-// The scales of a lane's feature in a block, 128 / group of them, as the low halves of one number.
-__device__ __forceinline__ unsigned long long load_scales(const half_t *scales, size_t row, int each) {
-    if (each == 4) return *reinterpret_cast<const unsigned long long *>(scales + row * 4);
-    if (each == 2) return *reinterpret_cast<const unsigned *>(scales + row * 2);
-    return *reinterpret_cast<const unsigned short *>(scales + row);
-}
+    __device__ __forceinline__ void load(const half_t *scales, size_t row) { v = load_vec<half_t, EACH>(scales + row * EACH); }
+};
 
-// A workgroup has 16 FT features and 16 TT tokens; its W wavefronts take every W-th block of 128 columns, so that all of a weight
-// row that fits is on its way at once, and their sums meet in LDS, in wavefront order.  The matrix product has tokens as rows
-// and features as columns: a lane keeps one feature per 16, whose scale it multiplies each group's sums with.
-template <typename X, typename T, int TT, int FT, int W>
-__global__ __launch_bounds__(W * kWave) void dense_w4_kernel(int tokens, int features, int width, const X *__restrict__ x, size_t ldx,
-                                                             const float *__restrict__ x_scales, const v4u32 *__restrict__ packed,
-                                                             int group, const T *__restrict__ bias, int activation,
-                                                             T *__restrict__ out, size_t ldo) {
+template <typename X, typename T>
+struct DenseArgs {
+    int tokens, features, steps;  // steps of 32 columns
+    int blocks, tiles, strips;    // of 128 columns, 16 features, 16 tokens
+    const X *x;
+    size_t ldx;
+    const float *x_scales;
+    const v4u32 *packed;
+    const half_t *scales;
+    const T *bias;
+    int activation;
+    T *out;
+    size_t ldo;
+};
+
+// The products of 16 tokens with 16 FT features over one block, whose operands are there.  The matrix product has tokens as rows and
+// features as columns: a lane keeps one feature per 16, whose scale it multiplies each group's sums with.
+template <typename X, int FT, int EACH>
+__device__ __forceinline__ void multiply_block(v4f32 (&acc)[FT], const typename Operand<X>::Raw (&piece)[4], const v4u32 (&codes)[FT],
+                                               const Scales<EACH> (&by)[FT]) {
     typedef Operand<X> Op;
-    __shared__ float traded[W][TT * 16][17];
-    const int wave = wave_in_block(), lane = threadIdx.x & (kWave - 1), col = lane & 15, quarter = lane >> 4;
-    const int tile0 = blockIdx.x * FT, token0 = blockIdx.y * (16 * TT);
-    const int blocks = (int) packed_blocks(width), tiles = (int) packed_tiles(features), each = kColumns / group;
-    const half_t *scales = reinterpret_cast<const half_t *>(packed + (size_t) blocks * tiles * kWave);
-    const X *rows[TT];
+    typename Op::Sums sums[FT];
 #pragma unroll
-    for (int t = 0; t < TT; ++t) {
-        const int token = token0 + 16 * t + col;
-        rows[t] = x + (size_t) (token < tokens ? token : tokens - 1) * ldx + 8 * quarter;  // (rows past the last are not stored)
-    }
-    size_t first[FT];  // block of a feature tile; tiles past the last repeat it and are not stored
-#pragma unroll
-    for (int f = 0; f < FT; ++f) first[f] = (size_t) (tile0 + f < tiles ? tile0 + f : tiles - 1) * blocks;
-
-    v4f32 acc[TT][FT] = {};
-    v4u32 codes[FT];
-    unsigned long long by[FT];
-    auto bring = [&](int block) {
+    for (int s = 0; s < 4; ++s) {
+        const auto x = Op::ready(piece[s]);
 #pragma unroll
         for (int f = 0; f < FT; ++f) {
-            codes[f] = packed[(first[f] + block) * kWave + lane];
-            by[f] = load_scales(scales, (first[f] + block) * kTile + col, each);
+            Op o;
+            o.weights(codes[f][s]);
+            sums[f] = Op::add(x, o, s % (4 / EACH) == 0 ? typename Op::Sums{} : sums[f]);
         }
-    };
-    if (wave < blocks) bring(wave);
-    for (int block = wave; block < blocks; block += W) {
-        v4u32 now[FT];
-        unsigned long long scale[FT];
+        if ((s + 1) % (4 / EACH) == 0) {  // the end of a group
 #pragma unroll
-        for (int f = 0; f < FT; ++f) now[f] = codes[f], scale[f] = by[f];
-        typename Op::Raw piece[TT][4];
-        const int steps = (width - block * kColumns) / 32;  // of this block, 4 but in the last one
+            for (int f = 0; f < FT; ++f) {
+                const float scale = (float) by[f].v.v[s * EACH / 4] * Op::kUnit;
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
-#pragma unroll
-            for (int t = 0; t < TT; ++t)  // (steps past the end read the last one again)
-                piece[t][s] = *reinterpret_cast<const typename Op::Raw *>(rows[t] + block * kColumns + 32 * (s < steps ? s : steps - 1));
-        if (block + W < blocks) bring(block + W);
-        typename Op::Sums sums[TT][FT] = {};
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            if (s < steps) {
-                Op o[FT];
-#pragma unroll
-                for (int f = 0; f < FT; ++f) o[f].weights(now[f][s]);
-#pragma unroll
-                for (int t = 0; t < TT; ++t) {
-                    const auto ready = prepared(piece[t][s]);
-#pragma unroll
-                    for (int f = 0; f < FT; ++f) sums[t][f] = Op::add(ready, o[f], sums[t][f]);
-                }
-                if ((s + 1) * 32 % group == 0) {
-#pragma unroll
-                    for (int f = 0; f < FT; ++f) {
-                        const float by_now = (float) __builtin_bit_cast(half_t, (unsigned short) (scale[f] >> (s * 32 / group * 16))) * Op::kUnit;
-#pragma unroll
-                        for (int t = 0; t < TT; ++t) {
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) acc[t][f][i] = fmaf((float) sums[t][f][i], by_now, acc[t][f][i]);
-                            sums[t][f] = typename Op::Sums{};
-                        }
-                    }
-                }
+                for (int i = 0; i < 4; ++i) acc[f][i] = fmaf((float) sums[f][i], scale, acc[f][i]);
             }
         }
     }
+}
+
+// A workgroup has 16 FT features and 16 tokens; its W wavefronts take every W-th block of 128 columns, the operands of the next one
+// on their way while they work on this one's, and their sums meet in LDS, in wavefront order.
+template <typename X, typename T, int EACH, int FT, int W>
+__global__ __launch_bounds__(W * kWave) void dense_w4_kernel(DenseArgs<X, T> a) {
+    typedef typename Operand<X>::Raw Raw;
+    __shared__ float traded[FT][W][kTile][17];
+    const int wave = wave_in_block(), lane = threadIdx.x & (kWave - 1);
+    // Workgroups are handed to the eight dies in turn: those of one feature tile, 16 tokens each, follow each other on one die,
+    // whose cache then has the weights.
+    const int on_die = blockIdx.x / 8, tile0 = (on_die / a.strips * 8 + blockIdx.x % 8) * FT, token0 = on_die % a.strips * kTile;
+    if (tile0 >= a.tiles) return;
+    const int token = token0 + (lane & 15);  // rows past the last repeat it and are not stored
+    const X *row = a.x + (size_t) (token < a.tokens ? token : a.tokens - 1) * a.ldx + 8 * (lane >> 4);
+    size_t first[FT];  // block of a feature tile; tiles past the last repeat it and are not stored
 #pragma unroll
-    for (int f = 0; f < FT; ++f) {
-        if (f > 0) __syncthreads();
+    for (int f = 0; f < FT; ++f) first[f] = (size_t) (tile0 + f < a.tiles ? tile0 + f : a.tiles - 1) * a.blocks;
+    v4f32 acc[FT] = {};
+    v4u32 codes[FT];
+    Scales<EACH> by[FT];
+    Raw piece[4];
+    auto bring = [&](int block) {
 #pragma unroll
-        for (int t = 0; t < TT; ++t)
+        for (int f = 0; f < FT; ++f) {
+            codes[f] = a.packed[(first[f] + block) * kWave + lane];
+            by[f].load(a.scales, (first[f] + block) * kTile + (lane & 15));
+        }
+        const X *at = row + (size_t) block * kColumns;
+        if (a.steps - 4 * block >= 4) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) traded[wave][16 * t + 4 * quarter + i][col] = acc[t][f][i];
-        __syncthreads();
-        for (int i = threadIdx.x; i < TT * 256; i += W * kWave) {
-            const int token = token0 + i / 16, feature = (tile0 + f) * kTile + i % 16;
-            if (token >= tokens || feature >= features) continue;
-            float sum = 0.f;
+            for (int s = 0; s < 4; ++s) piece[s] = *reinterpret_cast<const Raw *>(at + 32 * s);
+        } else {  // past the end of the rows there is nothing: zeros, as the codes there are
 #pragma unroll
-            for (int w = 0; w < W; ++w) sum += traded[w][i / 16][i % 16];
-            if (sizeof(X) == 1) sum *= x_scales[token];
-            if (bias != nullptr) sum += to_f32(bias[feature]);
-            if (activation != 0) sum = GeluOp<float>()(sum);
-            out[token * ldo + feature] = from_f32<T>(sum);
+            for (int s = 0; s < 4; ++s) piece[s] = 4 * block + s < a.steps ? *reinterpret_cast<const Raw *>(at + 32 * s) : Raw{};
+        }
+    };
+    if (wave < a.blocks) bring(wave);
+    for (int block = wave; block < a.blocks; block += W) {
+        multiply_block<X, FT, EACH>(acc, piece, codes, by);
+        if (block + W < a.blocks) bring(block + W);
+    }
+#pragma unroll
+    for (int f = 0; f < FT; ++f)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) traded[f][wave][4 * (lane >> 4) + i][lane & 15] = acc[f][i];
+    __syncthreads();
+    constexpr int kQuarter = W / 4;  // four threads to a result
+#pragma unroll
+    for (int i = threadIdx.x; i < FT * 1024; i += W * kWave) {
+        const int m = i / (FT * 64), n = i / 4 % (FT * 16), part = i % 4;
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kQuarter; ++w) sum += traded[n / 16][part * kQuarter + w][m][n % 16];
+        sum += dpp_move<kDppQuadXor1>(sum);
+        sum += dpp_move<kDppQuadXor2>(sum);
+        const int to = token0 + m, feature = tile0 * kTile + n;
+        if (part == 0 && to < a.tokens && feature < a.features) {
+            if (sizeof(X) == 1) sum *= a.x_scales[to];
+            if (a.bias != nullptr) sum += to_f32(a.bias[feature]);
+            if (a.activation != 0) sum = GeluOp<float>()(sum);
+            a.out[to * a.ldo + feature] = from_f32<T>(sum);
         }
     }
+}
+
+// How many features a workgroup has: more make less of reading and taking apart x again, fewer fill the card.  Microseconds with 16 /
+// 32 / 64 features: 16 fp16 tokens, 8192 x 32768 (2048 units of 16 features and 16 tokens) 65 / 40 / 34; 33 tokens, 4096 x 4096 (768)
+// 12 / 12 / 8.6; 1 token, 4096 x 16384 (1024) 10.8 / 9.5 / 10.1, 4096 x 1024 (64) 4.4 / 5.1 / 7.3.
+template <typename X, typename T, int EACH>
+int run_dense_w4(const DenseArgs<X, T> &a, hipStream_t s) {
+    const long long units = (long long) a.tiles * a.strips;
+    if (units >= 1 << 22) return CUBERT_UNSUPPORTED;  // a launch holds less than 2^32 threads
+    auto grid = [&](int ft) { return dim3((unsigned) (((a.tiles + ft - 1) / ft + 7) / 8 * 8 * a.strips)); };
+#ifdef VARIANT
+    VARIANT
+#endif
+    if (units > 1024 || (units > 512 && a.tokens > 8)) return launch(dense_w4_kernel<X, T, EACH, 4, 8>, grid(4), dim3(8 * kWave), s, a);
+    if (units > 256) return launch(dense_w4_kernel<X, T, EACH, 2, 8>, grid(2), dim3(8 * kWave), s, a);
+    // (sixteen wavefronts, 4096 x 1024: 1 token 3.9 us against 4.4 with eight, 64 tokens 7.0 against 6.7)
+    if (units <= 128 && a.blocks > 8) return launch(dense_w4_kernel<X, T, EACH, 1, 16>, grid(1), dim3(16 * kWave), s, a);
+    return launch(dense_w4_kernel<X, T, EACH, 1, 8>, grid(1), dim3(8 * kWave), s, a);
 }
 
 template <typename X, typename T>
@@ -310,31 +349,14 @@ int dense_w4(void *stream, int tokens, int features, int in, const X *x, int ldx
     if (x == nullptr || packed == nullptr || out == nullptr || (sizeof(X) == 1 && x_scales == nullptr)) return CUBERT_BAD_ARGUMENT;
     if (!good_group(group) || in % group != 0 || !is_aligned(x, 16) || (size_t) ldx * sizeof(X) % 16 != 0 || !is_aligned(packed, 16))
         return CUBERT_UNSUPPORTED;
-    const int tiles = (int) packed_tiles(features), blocks = (int) packed_blocks(in);
-    const int token_tiles = tokens <= 16 ? 1 : tokens <= 32 ? 2 : 4;
-    const int strips = (tokens + 16 * token_tiles - 1) / (16 * token_tiles);
-    if (strips > 65535) return CUBERT_UNSUPPORTED;
-    const bool wide = tiles >= 2048, deep = blocks >= 16;
+    DenseArgs<X, T> a;
+    a.tokens = tokens, a.features = features, a.steps = in / 32;
+    a.blocks = (int) packed_blocks(in), a.tiles = (int) packed_tiles(features), a.strips = (tokens + kTile - 1) / kTile;
+    a.x = x, a.ldx = ldx, a.x_scales = x_scales;
+    a.packed = (const v4u32 *) packed, a.scales = reinterpret_cast<const half_t *>(a.packed + (size_t) a.blocks * a.tiles * kWave);
+    a.bias = bias, a.activation = activation, a.out = out, a.ldo = ldo;
     const hipStream_t s = (hipStream_t) stream;
-#define RUN(TT, FT, W)                                                                                                        \
-    return launch(dense_w4_kernel<X, T, TT, FT, W>, dim3((tiles + FT - 1) / FT, strips), dim3(W * kWave), s, tokens, features, in, x, \
-                  ldx, x_scales, (const v4u32 *) packed, group, bias, activation, out, ldo);
-    // (with 64 tokens, fewer features or wavefronts keep the sums and the rows of x in registers)
-    constexpr int kWide4 = sizeof(X) == 4 ? 1 : sizeof(X) == 2 ? 2 : 4, kDeep4 = sizeof(X) == 4 ? 8 : 16;
-    if (wide) {
-        if (token_tiles == 1) RUN(1, 4, 8)
-        if (token_tiles == 2) RUN(2, 4, 8)
-        RUN(4, kWide4, 8)
-    }
-    if (deep) {
-        if (token_tiles == 1) RUN(1, 1, 16)
-        if (token_tiles == 2) RUN(2, 1, 16)
-        RUN(4, 1, kDeep4)
-    }
-    if (token_tiles == 1) RUN(1, 1, 8)
-    if (token_tiles == 2) RUN(2, 1, 8)
-    RUN(4, 1, 8)
-#undef RUN
+    return group == 128 ? run_dense_w4<X, T, 1>(a, s) : group == 64 ? run_dense_w4<X, T, 2>(a, s) : run_dense_w4<X, T, 4>(a, s);
 }
 
 template <typename T>
