@@ -135,9 +135,7 @@ __device__ __forceinline__ void attend(Rows<T, D> &r, const unsigned char *k, co
         r.top = high;
         r.sum *= shrink;
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) r.ctx[d][i] *= shrink;
+        for (int d = 0; d < D / 32; ++d) r.ctx[d] *= shrink;
     }
 #pragma unroll
     for (int n = 0; n < N; ++n) {
@@ -226,20 +224,46 @@ struct Tiles {
     __device__ __forceinline__ int base(int tile) const { return (tile < of_sinks ? tile : tile - of_sinks + first) * KEYS; }
 };
 
-// Whole 16-byte pieces of KEYS rows from row `base` on, brought to LDS by WAVES wavefronts; rows past the last are read from it.
+// 16 bytes per lane from `base` + `offset` to LDS at `to` + 16 * lane, without passing through registers.  As an instruction of its
+// own, not the builtin: behind that the compiler lets every transposing read of LDS wait for all that is on its way, also to other
+// buffers.  The waits are the callers' (landed, and the ones that count).
+__device__ __forceinline__ void copy_to_lds(const char *base, unsigned offset, unsigned to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory", "m0");
+}
+
+__device__ __forceinline__ unsigned lds_address(const unsigned char *p) {
+    return (unsigned) (uintptr_t) (const __attribute__((address_space(3))) unsigned char *) p;
+}
+
+// Whole 16-byte pieces of KEYS rows, brought to LDS by WAVES wavefronts: where a lane's pieces are in a tile, and the requests for a
+// tile from row `base` on; rows past the last are read from it.
 template <typename T, int D, int KEYS, int WAVES, bool IS_V>
-__device__ __forceinline__ void request(const T *from, int base, int rows, size_t pitch, unsigned char *to, int wave, int lane) {
-    constexpr int kRowBytes = D * (int) sizeof(T), kPieces = kRowBytes / 16, kRequests = KEYS * kPieces / (kWave * WAVES);
+struct Bring {
+    static constexpr int kRowBytes = D * (int) sizeof(T), kPieces = kRowBytes / 16, kRequests = KEYS * kPieces / (kWave * WAVES);
     static_assert(KEYS * kPieces % (kWave * WAVES) == 0, "whole requests");
-    const char *tile = reinterpret_cast<const char *>(from + (size_t) base * pitch);
-    const int last = rows - 1 - base;
-#pragma unroll
-    for (int i = 0; i < kRequests; ++i) {
+    unsigned offset[kRequests];
+
+    __device__ __forceinline__ static unsigned offset_of(int i, int wave, int lane, int last, unsigned pitch) {
         const int at = (i * WAVES + wave) * kWave + lane, key = at / kPieces, place = at % kPieces;
         const int piece = IS_V ? v_piece<T, kRowBytes>(key, place) : k_piece<kRowBytes>(key, place);  // (its own inverse)
-        load_to_lds(tile + (size_t) (key < last ? key : last) * (pitch * sizeof(T)) + piece * 16, to + (i * WAVES + wave) * 1024);
+        return (unsigned) (key < last ? key : last) * pitch + piece * 16;
     }
-}
+    __device__ __forceinline__ Bring(int wave, int lane, unsigned pitch) {
+#pragma unroll
+        for (int i = 0; i < kRequests; ++i) offset[i] = offset_of(i, wave, lane, KEYS, pitch);
+    }
+    __device__ __forceinline__ void operator()(const T *from, int base, int rows, unsigned pitch, unsigned to, int wave, int lane) const {
+        const char *tile = reinterpret_cast<const char *>(from) + (size_t) base * pitch;
+        if (base + KEYS <= rows) {
+#pragma unroll
+            for (int i = 0; i < kRequests; ++i) copy_to_lds(tile, offset[i], to + (i * WAVES + wave) * 1024);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kRequests; ++i)
+                copy_to_lds(tile, offset_of(i, wave, lane, rows - 1 - base, pitch), to + (i * WAVES + wave) * 1024);
+        }
+    }
+};
 
 // A key that nobody sees has probability 0, but 0 times what its row of V may hold need not be 0.
 template <typename T, int D, int KEYS, int THREADS>
@@ -300,10 +324,13 @@ __global__ __launch_bounds__(kBlock) void attention_window_shared_kernel(WindowA
 
     Rows<T, D> r;
     r.load((const T *) a.q + ((size_t) at.b * a.q_rows + query) * a.ldq + (size_t) head * D, lane >> 5, a.negate);
+    const unsigned pitch = (unsigned) a.ldkv * sizeof(T), lds = lds_address(smem);
+    const Bring<T, D, kKeys, 4, false> bring_k(wave, lane, pitch);
+    const Bring<T, D, kKeys, 4, true> bring_v(wave, lane, pitch);
     auto bring = [&](int tile, int buffer) {
-        unsigned char *to = smem + buffer * 2 * kTileBytes;
-        request<T, D, kKeys, 4, false>(k, tiles.base(tile), a.kv_rows, a.ldkv, to, wave, lane);
-        request<T, D, kKeys, 4, true>(v, tiles.base(tile), a.kv_rows, a.ldkv, to + kTileBytes, wave, lane);
+        const unsigned to = lds + buffer * 2 * kTileBytes;
+        bring_k(k, tiles.base(tile), a.kv_rows, pitch, to, wave, lane);
+        bring_v(v, tiles.base(tile), a.kv_rows, pitch, to + kTileBytes, wave, lane);
     };
     auto mask_byte = [&](int tile) -> int {
         const int j = tiles.base(tile) + lane;
@@ -314,7 +341,8 @@ __global__ __launch_bounds__(kBlock) void attention_window_shared_kernel(WindowA
         bring(0, 0);
         kept = mask_byte(0);
     }
-    for (int tile = 0; tile < tiles.count; ++tile) {
+    // One tile of the workgroup's: everybody waits for it, brings a share of the next one and, `busy`, works on it.
+    auto take = [&](int tile, bool busy) {
         landed();
         const unsigned long long kept_bits = __ballot(kept != 0);
         __syncthreads();  // everybody's; and nobody reads the other buffer any more
@@ -329,13 +357,24 @@ __global__ __launch_bounds__(kBlock) void attention_window_shared_kernel(WindowA
             clear_rows<T, D, kKeys, kBlock>(vt, seen, threadIdx.x);
             __syncthreads();
         }
-        if (mine.any && (mine.of(base, a.sinks) & kept_bits & whole) != 0) {
-            const bool all = mine.all(base, kKeys, a.sinks) && (kept_bits & whole) == whole;
-            const unsigned long long visible =
-                    all ? ~0ull : bits_below(end - base) & (~bits_below(begin - base) | bits_below(a.sinks - base)) & kept_bits;
-            attend<T, D, kKeys / 32>(r, kt, vt, a.scale, all, visible, lane);
-        }
+        if (!busy) return;
+        const bool all = mine.all(base, kKeys, a.sinks) && (kept_bits & whole) == whole;
+        const unsigned long long visible =
+                all ? ~0ull : bits_below(end - base) & (~bits_below(begin - base) | bits_below(a.sinks - base)) & kept_bits;
+        attend<T, D, kKeys / 32>(r, kt, vt, a.scale, all, visible, lane);
+    };
+    // This wavefront's tiles are those of the sinks (which reach into the window's where there is no gap between them) and a run
+    // among those of the window.  (Tiles passed over by loops of their own: a branch around the work has the compiler copy every
+    // accumulator.)
+    const int my_sinks = a.sinks < mine.last_end ? a.sinks : mine.last_end, sinks_end = mine.any ? (my_sinks + kKeys - 1) / kKeys : 0;
+    const int from = mine.any ? tiles.of_sinks + mine.first_begin / kKeys - tiles.first : tiles.count;
+    const int until = mine.any ? tiles.of_sinks + (mine.last_end + kKeys - 1) / kKeys - tiles.first : tiles.count;
+    int tile = 0;
+    for (int part = 0; part < 2; ++part) {
+        for (; tile < (part == 0 ? 0 : from); ++tile) take(tile, false);
+        for (; tile < (part == 0 ? sinks_end : until); ++tile) take(tile, true);
     }
+    for (; tile < tiles.count; ++tile) take(tile, false);
     if (row >= rows) return;
     const float sum = r.sum + __shfl_xor(r.sum, 32, kWave);
     const float by = there && sum > 0.f ? 1.f / sum : 0.f;
@@ -389,10 +428,13 @@ __global__ __launch_bounds__(kBlock) void attention_window_spread_kernel(WindowA
     const int each = tiles.count / pieces, more = tiles.count - each * pieces;
     const int until = piece * each + (piece < more ? piece : more) + each + (piece < more ? 1 : 0);
     int tile = piece * each + (piece < more ? piece : more) + wave;
+    const unsigned pitch = (unsigned) a.ldkv * sizeof(T), lds = lds_address(buffers);
+    const Bring<T, D, 32, 1, false> bring_k(0, lane, pitch);
+    const Bring<T, D, 32, 1, true> bring_v(0, lane, pitch);
     auto bring = [&](int t, int buffer) {
-        unsigned char *to = buffers + buffer * 2 * S::kTileBytes;
-        request<T, D, 32, 1, false>(k, tiles.base(t), a.kv_rows, a.ldkv, to, 0, lane);
-        request<T, D, 32, 1, true>(v, tiles.base(t), a.kv_rows, a.ldkv, to + S::kTileBytes, 0, lane);
+        const unsigned to = lds + buffer * 2 * S::kTileBytes;
+        bring_k(k, tiles.base(t), a.kv_rows, pitch, to, 0, lane);
+        bring_v(v, tiles.base(t), a.kv_rows, pitch, to + S::kTileBytes, 0, lane);
     };
     auto mask_byte = [&](int t) -> int {
         const int j = tiles.base(t) + lane;
@@ -625,6 +667,7 @@ int attention_window(const T *q, int ldq, const T *k, const T *v, int ldkv, cons
     if (!is_aligned(q, 16) || !is_aligned(k, 16) || !is_aligned(v, 16) || !is_aligned(ctx, 16) || ldq % piece != 0 ||
         ldkv % piece != 0 || ld_ctx % piece != 0)
         return CUBERT_UNSUPPORTED;
+    if (ldkv > 1 << 22) return CUBERT_UNSUPPORTED;  // (pieces of a tile are addressed with 32 bits)
     if (head_size != 32 && head_size != 64 && head_size != 128) return CUBERT_UNSUPPORTED;
     const unsigned long long rows = (unsigned long long) batch * q_rows * heads;
     if (rows >= 1u << 24) return CUBERT_UNSUPPORTED;  // a launch holds less than 2^32 threads
