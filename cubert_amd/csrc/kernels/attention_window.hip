@@ -41,7 +41,8 @@ typedef float v2f32 __attribute__((ext_vector_type(2)));
 typedef float v16f32 __attribute__((ext_vector_type(16)));
 
 constexpr float kNone = -3e38f;  // the maximum of no scores: finite, so that differences to it are numbers
-constexpr float kSlack = 8.f;    // how far a maximum may rise, in powers of two, before sums are scaled anew
+constexpr float kSlack = 8.f;    // how far a maximum may rise, in powers of two, before sums are scaled anew (fp32)
+constexpr float kMost = 1024.f;  // what the probabilities of a tile may add up to in half a row before that (fp16)
 
 // 32 rows (queries and heads of one key head) meet 32 keys in one matrix product with the keys as its rows: lane l has row
 // l % 32 and, in accumulator i, key 8 (i / 4) + 4 (l / 32) + i % 4.  The probabilities are then the second operand of the
@@ -122,40 +123,52 @@ __device__ __forceinline__ void attend(Rows<T, D> &r, const unsigned char *k, co
             for (int i = 0; i < 16; ++i) s[n][i] = word >> (8 * (i / 4) + i % 4) & 1u ? s[n][i] : -INFINITY;
         }
     }
-    float top = s[0][0];
-#pragma unroll
-    for (int n = 0; n < N; ++n)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[n][i]);
-    top *= scale;
-    // Sums are scaled anew only when some maximum has risen by a factor of 2^8, which a probability and the sums bear.
-    if (__any(top > r.top + kSlack)) {
+    // Sums are scaled anew only when some maximum has risen by a factor that a probability in 16 bits and the sums bear.
+    auto rescale = [&](float top) {
         const float high = fmaxf(r.top, fmaxf(top, __shfl_xor(top, 32, kWave)));
         const float shrink = __builtin_amdgcn_exp2f(r.top - high);
         r.top = high;
         r.sum *= shrink;
 #pragma unroll
         for (int d = 0; d < D / 32; ++d) r.ctx[d] *= shrink;
-    }
+    };
+    auto largest = [&]() {
+        float top = s[0][0];
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
+        for (int n = 0; n < N; ++n)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[n][i] = __builtin_amdgcn_exp2f(fmaf(s[n][i], scale, -r.top));
-    }
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[n][i]);
+        return top * scale;
+    };
     if constexpr (sizeof(T) == 2) {
+        // Probabilities against the maximum so far; their sum, which is wanted anyway, says whether it was too small by far, and
+        // only then the scores' maximum is looked for.
+        v8f16 p[N][2];
+        auto weigh = [&]() {
+            float sum = 0.f;
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const v2f16 pair = __builtin_convertvector((v2f32{__builtin_amdgcn_exp2f(fmaf(s[n][i], scale, -r.top)),
+                                                                      __builtin_amdgcn_exp2f(fmaf(s[n][i + 1], scale, -r.top))}), v2f16);
+                    p[n][i / 8][i % 8] = pair[0], p[n][i / 8][i % 8 + 1] = pair[1];
+                    // (a sum of the probabilities as the product takes them)
+                    sum = __builtin_amdgcn_fdot2(pair, v2f16{(half_t) 1.f, (half_t) 1.f}, sum, false);
+                }
+            return sum;
+        };
+        float sum = weigh();
+        if (__any(!(sum <= kMost))) {
+            rescale(largest());
+            sum = weigh();
+        }
+        r.sum += sum;
         const int patch = lane & 15, side = (lane >> 4) & 1;
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
+        for (int n = 0; n < N; ++n)
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                v8f16 p;
-#pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    const v2f16 pair = __builtin_convertvector((v2f32{s[n][8 * ks + e], s[n][8 * ks + e + 1]}), v2f16);
-                    p[e] = pair[0], p[e + 1] = pair[1];
-                    // the sum is one of the probabilities as the product takes them
-                    r.sum = __builtin_amdgcn_fdot2(pair, v2f16{(half_t) 1.f, (half_t) 1.f}, r.sum, false);
-                }
+            for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
                 for (int d = 0; d < D / 32; ++d) {
                     v4f16 part[2];
@@ -165,15 +178,16 @@ __device__ __forceinline__ void attend(Rows<T, D> &r, const unsigned char *k, co
                         part[h] = read_transposed(v + key * R::kRowBytes + v_piece<T, R::kRowBytes>(key, at) * 16 + (patch & 1) * 8);
                     }
                     const v8f16 a = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
-                    r.ctx[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, p, r.ctx[d], 0, 0, 0);
+                    r.ctx[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, p[n][ks], r.ctx[d], 0, 0, 0);
                 }
-            }
-        }
     } else {
+        const float top = largest();
+        if (__any(top > r.top + kSlack)) rescale(top);
 #pragma unroll
         for (int n = 0; n < N; ++n)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
+                s[n][i] = __builtin_amdgcn_exp2f(fmaf(s[n][i], scale, -r.top));
                 r.sum += s[n][i];
                 const int key = 32 * n + 8 * (i / 4) + 4 * half_wave + i % 4;
 #pragma unroll
@@ -279,8 +293,7 @@ __device__ __forceinline__ void clear_rows(unsigned char *v, unsigned long long 
 struct Problem {
     int b, kv_head, length, first;
 
-    __device__ __forceinline__ Problem(const WindowArgs &a, int problem) {
-        b = problem / a.kv_heads, kv_head = problem - b * a.kv_heads;
+    __device__ __forceinline__ Problem(const WindowArgs &a, int b_, int kv_head_) : b(b_), kv_head(kv_head_) {
         length = a.lengths != nullptr ? clamp_to(a.lengths[b], 0, a.kv_rows) : a.kv_rows;
         first = a.first != nullptr ? clamp_to(a.first[b], -kFar, kFar) : 0;
     }
@@ -297,15 +310,66 @@ __device__ __forceinline__ void landed() {  // what this wavefront requested is 
     asm volatile("" ::: "memory");
 }
 
+// Which 128 rows a workgroup takes.  Workgroups are handed to the eight dies in turn and to the units of a die as they come free, so
+// the ones with work come first: handed out with the others between them, which end at once, one unit got 8 of 1280 and another 2
+// (4 sequences of 1024 to 4096 tokens, 99 us for 56 us of work).  A die has consecutive ones, which read the same keys.
+struct Place {
+    int b, kv_head, tile;
+
+    // `count` things, those of a die consecutive: the number of the die's first one
+    __device__ __forceinline__ static int before(int count, int die) { return die * (count / 8) + (die < count % 8 ? die : count % 8); }
+
+    __device__ __forceinline__ Place(const WindowArgs &a, int share, int row_tiles, int lane) {
+        const int die = blockIdx.x % 8, on_die = blockIdx.x / 8, total = a.batch * a.kv_heads * row_tiles;
+        if ((a.lengths == nullptr && a.first == nullptr) || a.batch > kWave) {
+            const int i = before(total, die) + on_die, problem = i / row_tiles;
+            tile = i - problem * row_tiles, b = problem / a.kv_heads, kv_head = problem - b * a.kv_heads;
+            return;
+        }
+        // a lane per sequence: the tiles with a query inside of it
+        int from = 0, count = 0;
+        if (lane < a.batch) {
+            const int length = a.lengths != nullptr ? clamp_to(a.lengths[lane], 0, a.kv_rows) : a.kv_rows;
+            const int first = a.first != nullptr ? clamp_to(a.first[lane], -kFar, kFar) : 0;
+            const int low = first < 0 ? -first : 0, high = length - first < a.q_rows ? length - first : a.q_rows;
+            if (low < high) from = low * share / 128, count = (high * share + 127) / 128 - from;
+        }
+        int active = count;
+#pragma unroll
+        for (int n = 1; n < kWave; n *= 2) active += __shfl_xor(active, n, kWave);
+        active *= a.kv_heads;
+        const int mine = before(active, die + 1) - before(active, die);
+        const bool works = on_die < mine;
+        int i = works ? before(active, die) + on_die : before(total, die) - before(active, die) + on_die - mine;
+        const int each = works ? count : row_tiles - count;  // of a sequence and key head
+        int upto = (lane < a.batch ? each : 0) * a.kv_heads;
+#pragma unroll
+        for (int n = 1; n < kWave; n *= 2) {
+            const int other = __shfl_up(upto, n, kWave);
+            upto += lane >= n ? other : 0;
+        }
+        b = __builtin_amdgcn_readfirstlane(__builtin_ctzll(__ballot(upto > i)));
+        i -= b > 0 ? __builtin_amdgcn_readlane(upto, b - 1) : 0;
+        const int n = __builtin_amdgcn_readlane(each, b), begin = __builtin_amdgcn_readlane(from, b);
+        i = __builtin_amdgcn_readfirstlane(i);
+        kv_head = i / n;
+        tile = i - kv_head * n;
+        tile += works ? begin : tile < begin ? 0 : __builtin_amdgcn_readlane(count, b);
+        // (the same in every lane, which the compiler has to be told)
+        b = __builtin_amdgcn_readfirstlane(b), kv_head = __builtin_amdgcn_readfirstlane(kv_head), tile = __builtin_amdgcn_readfirstlane(tile);
+    }
+};
+
 // Four wavefronts of 32 rows each share every tile of K and V, the next one on its way while they work on this one.
 template <typename T, int D>
 __global__ __launch_bounds__(kBlock) void attention_window_shared_kernel(WindowArgs a, int row_tiles) {
     constexpr int kKeys = sizeof(T) == 2 ? 64 : 32, kTileBytes = kKeys * D * (int) sizeof(T);
     extern __shared__ __align__(16) unsigned char smem[];  // two buffers of K and V
     const int wave = wave_in_block(), lane = threadIdx.x & (kWave - 1);
-    const int problem = blockIdx.x / row_tiles, row0 = (blockIdx.x - problem * row_tiles) * 128;
-    const Problem at(a, problem);
     const int share = a.heads / a.kv_heads, rows = a.q_rows * share;
+    const Place place(a, share, row_tiles, lane);
+    const int row0 = place.tile * 128;
+    const Problem at(a, place.b, place.kv_head);
     const int row = row0 + 32 * wave + (lane & 31), my_row = row < rows ? row : rows - 1;
     const int query = my_row / share, head = at.kv_head * share + my_row - query * share;
     const int p = at.first + query;
@@ -407,7 +471,7 @@ __global__ __launch_bounds__(kBlock) void attention_window_spread_kernel(WindowA
     const int wave = wave_in_block(), lane = threadIdx.x & (kWave - 1);
     const int piece = blockIdx.x % pieces, tile_at = blockIdx.x / pieces;
     const int problem = tile_at / row_tiles, row0 = (tile_at - problem * row_tiles) * 32;
-    const Problem at(a, problem);
+    const Problem at(a, problem / a.kv_heads, problem % a.kv_heads);
     const int share = a.heads / a.kv_heads, rows = a.q_rows * share;
     const int row = row0 + (lane & 31), my_row = row < rows ? row : rows - 1;
     const int query = my_row / share, head = at.kv_head * share + my_row - query * share;

@@ -354,6 +354,8 @@ WIDE = {
     "wide and nothing left": (2, 140, 140, 48, 48, 5, 5, 0, None, None, "nothing"),
     "wide before the sequence": (3, 150, 164, 40, 40, 10, 0, 1, "end", (164, 7, 120), "no"),
     "wide window of one": (2, 129, 129, 49, 49, 0, 0, 0, None, None, "no"),
+    "wide, 64 sequences": (64, 140, 150, 4, 2, 30, 0, 2, "end", tuple(150 - 2 * i for i in range(64)), "no"),
+    "wide, 70 sequences": (70, 40, 60, 4, 4, 11, 3, 2, None, tuple(max(0, 60 - i) for i in range(70)), "no"),
     "wide sinks alone": (5, 40, 900, 80, 20, 3, 0, 40, "end", (900, 100, 800, 40, 41), "no"),
 }
 ATTENTION.update(WIDE)
