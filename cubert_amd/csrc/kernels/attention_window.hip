@@ -57,6 +57,7 @@ struct Rows {
     v4f32 q[kSteps];  // pieces 2 s + l / 32 of the row
     v16f32 ctx[D / 32];
     float top, sum;
+    bool fresh = true;  // no key yet (the same in every lane)
 
     __device__ __forceinline__ void load(const T *row, int half_wave, bool negate) {
 #pragma unroll
@@ -158,6 +159,8 @@ __device__ __forceinline__ void attend(Rows<T, D> &r, const unsigned char *k, co
                 }
             return sum;
         };
+        if (r.fresh) rescale(largest());
+        r.fresh = false;
         float sum = weigh();
         if (__any(!(sum <= kMost))) {
             rescale(largest());
@@ -334,24 +337,20 @@ struct Place {
             const int low = first < 0 ? -first : 0, high = length - first < a.q_rows ? length - first : a.q_rows;
             if (low < high) from = low * share / 128, count = (high * share + 127) / 128 - from;
         }
-        int active = count;
-#pragma unroll
-        for (int n = 1; n < kWave; n *= 2) active += __shfl_xor(active, n, kWave);
+        int active = 0;
+        for (int n = 0; n < a.batch; ++n) active += __builtin_amdgcn_readlane(count, n);
         active *= a.kv_heads;
         const int mine = before(active, die + 1) - before(active, die);
         const bool works = on_die < mine;
         int i = works ? before(active, die) + on_die : before(total, die) - before(active, die) + on_die - mine;
-        const int each = works ? count : row_tiles - count;  // of a sequence and key head
-        int upto = (lane < a.batch ? each : 0) * a.kv_heads;
-#pragma unroll
-        for (int n = 1; n < kWave; n *= 2) {
-            const int other = __shfl_up(upto, n, kWave);
-            upto += lane >= n ? other : 0;
+        int n = 0;  // tiles of a sequence and key head
+        for (b = 0; b < a.batch; ++b) {
+            n = __builtin_amdgcn_readlane(count, b);
+            n = works ? n : row_tiles - n;
+            if (i < n * a.kv_heads) break;
+            i -= n * a.kv_heads;
         }
-        b = __builtin_amdgcn_readfirstlane(__builtin_ctzll(__ballot(upto > i)));
-        i -= b > 0 ? __builtin_amdgcn_readlane(upto, b - 1) : 0;
-        const int n = __builtin_amdgcn_readlane(each, b), begin = __builtin_amdgcn_readlane(from, b);
-        i = __builtin_amdgcn_readfirstlane(i);
+        const int begin = __builtin_amdgcn_readlane(from, b);
         kv_head = i / n;
         tile = i - kv_head * n;
         tile += works ? begin : tile < begin ? 0 : __builtin_amdgcn_readlane(count, b);
@@ -371,7 +370,7 @@ __global__ __launch_bounds__(kBlock) void attention_window_shared_kernel(WindowA
     const int row0 = place.tile * 128;
     const Problem at(a, place.b, place.kv_head);
     const int row = row0 + 32 * wave + (lane & 31), my_row = row < rows ? row : rows - 1;
-    const int query = my_row / share, head = at.kv_head * share + my_row - query * share;
+    const int query = share == 1 ? my_row : my_row / share, head = at.kv_head * share + my_row - query * share;
     const int p = at.first + query;
     const bool there = row < rows && p >= 0 && p < at.length;
     const int begin = p > a.left ? p - a.left : 0, end = p < at.length - a.right ? p + a.right + 1 : at.length;
@@ -386,8 +385,6 @@ __global__ __launch_bounds__(kBlock) void attention_window_shared_kernel(WindowA
     Reach mine(a, at.first + wave_row / share, at.first + wave_last / share, at.length);
     mine.any = mine.any && wave_row < rows;
 
-    Rows<T, D> r;
-    r.load((const T *) a.q + ((size_t) at.b * a.q_rows + query) * a.ldq + (size_t) head * D, lane >> 5, a.negate);
     const unsigned pitch = (unsigned) a.ldkv * sizeof(T), lds = lds_address(smem);
     const Bring<T, D, kKeys, 4, false> bring_k(wave, lane, pitch);
     const Bring<T, D, kKeys, 4, true> bring_v(wave, lane, pitch);
@@ -405,10 +402,12 @@ __global__ __launch_bounds__(kBlock) void attention_window_shared_kernel(WindowA
         bring(0, 0);
         kept = mask_byte(0);
     }
+    Rows<T, D> r;
+    r.load((const T *) a.q + ((size_t) at.b * a.q_rows + query) * a.ldq + (size_t) head * D, lane >> 5, a.negate);
     // One tile of the workgroup's: everybody waits for it, brings a share of the next one and, `busy`, works on it.
     auto take = [&](int tile, bool busy) {
         landed();
-        const unsigned long long kept_bits = __ballot(kept != 0);
+        const unsigned long long kept_bits = mask != nullptr ? __ballot(kept != 0) : ~0ull;
         __syncthreads();  // everybody's; and nobody reads the other buffer any more
         if (tile + 1 < tiles.count) {
             bring(tile + 1, (tile + 1) & 1);
@@ -416,15 +415,15 @@ __global__ __launch_bounds__(kBlock) void attention_window_shared_kernel(WindowA
         }
         unsigned char *kt = smem + (tile & 1) * 2 * kTileBytes, *vt = kt + kTileBytes;
         const int base = tiles.base(tile);
-        const unsigned long long seen = reach.of(base, a.sinks) & kept_bits, whole = bits_below(kKeys);
-        if ((seen & whole) != whole) {
-            clear_rows<T, D, kKeys, kBlock>(vt, seen, threadIdx.x);
+        const bool kept_all = mask == nullptr || (kept_bits & bits_below(kKeys)) == bits_below(kKeys);
+        if (!kept_all || base + kKeys > reach.last_end || (base < reach.first_begin && base + kKeys > a.sinks)) {
+            clear_rows<T, D, kKeys, kBlock>(vt, reach.of(base, a.sinks) & kept_bits, threadIdx.x);
             __syncthreads();
         }
         if (!busy) return;
-        const bool all = mine.all(base, kKeys, a.sinks) && (kept_bits & whole) == whole;
-        const unsigned long long visible =
-                all ? ~0ull : bits_below(end - base) & (~bits_below(begin - base) | bits_below(a.sinks - base)) & kept_bits;
+        const bool all = kept_all && mine.all(base, kKeys, a.sinks);
+        unsigned long long visible = ~0ull;
+        if (!all) visible = bits_below(end - base) & (~bits_below(begin - base) | bits_below(a.sinks - base)) & kept_bits;
         attend<T, D, kKeys / 32>(r, kt, vt, a.scale, all, visible, lane);
     };
     // This wavefront's tiles are those of the sinks (which reach into the window's where there is no gap between them) and a run
@@ -455,7 +454,9 @@ __global__ __launch_bounds__(kBlock) void attention_window_shared_kernel(WindowA
 template <typename T, int D>
 struct Spread {
     static constexpr int kTileBytes = 32 * D * (int) sizeof(T);                // of K, and of V
-    static constexpr int kBuffers = kTileBytes * 2 * 2 * 4 <= 128 * 1024 ? 2 : 1;
+    // (two where two workgroups with them fit a compute unit: 32 tokens over 4096 keys of 128, fp16, 62 us with one workgroup of two
+    // buffers to a wavefront, 54 with two of one)
+    static constexpr int kBuffers = kTileBytes * 2 * 2 * 4 <= 64 * 1024 ? 2 : 1;
     static constexpr int kWaveBytes = kBuffers * 2 * kTileBytes;
     static constexpr int kPitch = D + 4;                                       // floats between rows of a wavefront's results
     static constexpr int kMergeBytes = 4 * 32 * kPitch * 4;
@@ -465,7 +466,7 @@ struct Spread {
 // 32 rows per workgroup, whose four wavefronts take every fourth tile of 32 keys of this workgroup's piece of the axis; their
 // sums meet in LDS, in wavefront order, and go out as results or, where the axis is cut, as sums for the kernel below.
 template <typename T, int D>
-__global__ __launch_bounds__(kBlock) void attention_window_spread_kernel(WindowArgs a, int row_tiles, int pieces) {
+__global__ __launch_bounds__(kBlock, sizeof(T) * D == 512 ? 1 : 2) void attention_window_spread_kernel(WindowArgs a, int row_tiles, int pieces) {
     typedef Spread<T, D> S;
     extern __shared__ __align__(16) unsigned char smem[];
     const int wave = wave_in_block(), lane = threadIdx.x & (kWave - 1);
@@ -686,8 +687,10 @@ WindowPlan plan_window(int batch, int heads, int kv_heads, int q_rows, int kv_ro
     long long reach = kv_rows;
     if (left >= 0 && right >= 0) reach = (long long) left + right + 33 + sinks < reach ? (long long) left + right + 33 + sinks : reach;
     const long long tiles = (reach + 31) / 32, blocks = problems * plan.row_tiles;
-    long long pieces = blocks > 0 ? (1024 + blocks - 1) / blocks : 1;
-    pieces = pieces < (tiles + 7) / 8 ? pieces : (tiles + 7) / 8;  // two tiles to a wavefront at least
+    // About 384 workgroups, three for two units, with two tiles to a wavefront at least.  Microseconds with 256 / 384 / 512 / 768:
+    // fp16, 48 tokens over up to 1000 keys 20 / 20 / 24 / 23, 2 x 100 over 6000 28 / 23 / 27 / 26, 32 over 4096 52 / 54 / 52 / 53.
+    long long pieces = blocks > 0 ? (384 + blocks - 1) / blocks : 1;
+    pieces = pieces < (tiles + 7) / 8 ? pieces : (tiles + 7) / 8;
     plan.pieces = (int) (pieces < 1 ? 1 : pieces > kMaxPieces ? kMaxPieces : pieces);
     if (plan.pieces > 1) plan.floats = (size_t) blocks * plan.pieces * 32 * (head_size + 4);
     return plan;
@@ -708,8 +711,8 @@ int run_window(const WindowArgs &a, WindowPlan plan, hipStream_t stream) {
                               Spread<T, D>::kLds, stream, a, plan.row_tiles, plan.pieces);
     if (rc != 0 || plan.pieces == 1) return rc;
     const int total = problems * a.q_rows * (a.heads / a.kv_heads), per_block = kBlock / (D / 4);
-    // (18612 rows of 2 pieces: 5 us so, 22 us with a workgroup per row; 16 rows of 128: 4.4 us with one)
-    if (plan.pieces <= 8)
+    // (18612 rows of 2 pieces: 5 us so, 22 us with a workgroup per row; 512 rows of 8 pieces 6.6 and 4.7 us, 16 rows of 128 137 and 4.4)
+    if (plan.pieces <= 8 && total > 2048)
         return launch(attention_window_join_few_kernel<T, D>, dim3((total + per_block - 1) / per_block), dim3(kBlock), stream, a,
                       plan.row_tiles, plan.pieces, total);
     return launch(attention_window_join_kernel<T, D>, dim3(total), dim3(kBlock), stream, a,
