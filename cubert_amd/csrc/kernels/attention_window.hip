@@ -94,8 +94,18 @@ __device__ __forceinline__ v4f16 read_transposed(const unsigned char *p) {
     return __builtin_bit_cast(v4f16, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16 *) p));
 }
 
+// The wait states that an ordinary instruction needs before it reads what matrix instructions above wrote.  The compiler puts them in,
+// but behind a branch that follows such an instruction it was seen to count from the other way into the block, and 9 were missing.
+__device__ __forceinline__ void products_done() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 15");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 // 32 N keys of K and V in LDS, keys of bits 0 in `visible` left out where not all of them are seen
-template <typename T, int D, int N>
+// EXACT: probabilities in 16 bits as sums of two numbers, for kernels that wait for memory; their error is otherwise as large as that of
+// rounding the results, 2^-12 of them on average.
+template <typename T, int D, int N, bool EXACT = false>
 __device__ __forceinline__ void attend(Rows<T, D> &r, const unsigned char *k, const unsigned char *v, float scale, bool all,
                                        unsigned long long visible, int lane) {
     typedef Rows<T, D> R;
@@ -116,6 +126,7 @@ __device__ __forceinline__ void attend(Rows<T, D> &r, const unsigned char *k, co
             }
         }
     }
+    products_done();
     if (!all) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
@@ -144,18 +155,24 @@ __device__ __forceinline__ void attend(Rows<T, D> &r, const unsigned char *k, co
     if constexpr (sizeof(T) == 2) {
         // Probabilities against the maximum so far; their sum, which is wanted anyway, says whether it was too small by far, and
         // only then the scores' maximum is looked for.
-        v8f16 p[N][2];
+        v8f16 p[N][2], low[N][2];
         auto weigh = [&]() {
             float sum = 0.f;
 #pragma unroll
             for (int n = 0; n < N; ++n)
 #pragma unroll
                 for (int i = 0; i < 16; i += 2) {
-                    const v2f16 pair = __builtin_convertvector((v2f32{__builtin_amdgcn_exp2f(fmaf(s[n][i], scale, -r.top)),
-                                                                      __builtin_amdgcn_exp2f(fmaf(s[n][i + 1], scale, -r.top))}), v2f16);
+                    const v2f32 e = {__builtin_amdgcn_exp2f(fmaf(s[n][i], scale, -r.top)),
+                                     __builtin_amdgcn_exp2f(fmaf(s[n][i + 1], scale, -r.top))};
+                    const v2f16 pair = __builtin_convertvector(e, v2f16);
                     p[n][i / 8][i % 8] = pair[0], p[n][i / 8][i % 8 + 1] = pair[1];
-                    // (a sum of the probabilities as the product takes them)
-                    sum = __builtin_amdgcn_fdot2(pair, v2f16{(half_t) 1.f, (half_t) 1.f}, sum, false);
+                    if constexpr (EXACT) {
+                        const v2f16 left = __builtin_convertvector((v2f32{e[0] - (float) pair[0], e[1] - (float) pair[1]}), v2f16);
+                        low[n][i / 8][i % 8] = left[0], low[n][i / 8][i % 8 + 1] = left[1];
+                        sum += e[0] + e[1];
+                    } else {  // (a sum of the probabilities as the product takes them)
+                        sum = __builtin_amdgcn_fdot2(pair, v2f16{(half_t) 1.f, (half_t) 1.f}, sum, false);
+                    }
                 }
             return sum;
         };
@@ -181,6 +198,7 @@ __device__ __forceinline__ void attend(Rows<T, D> &r, const unsigned char *k, co
                         part[h] = read_transposed(v + key * R::kRowBytes + v_piece<T, R::kRowBytes>(key, at) * 16 + (patch & 1) * 8);
                     }
                     const v8f16 a = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
+                    if constexpr (EXACT) r.ctx[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, low[n][ks], r.ctx[d], 0, 0, 0);
                     r.ctx[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, p[n][ks], r.ctx[d], 0, 0, 0);
                 }
     } else {
@@ -313,7 +331,7 @@ __device__ __forceinline__ void landed() {  // what this wavefront requested is 
     asm volatile("" ::: "memory");
 }
 
-// Which 128 rows a workgroup takes.  Workgroups are handed to the eight dies in turn and to the units of a die as they come free, so
+// Which rows a workgroup takes, `rows` of them.  Workgroups are handed to the eight dies in turn and to the units of a die as they come free, so
 // the ones with work come first: handed out with the others between them, which end at once, one unit got 8 of 1280 and another 2
 // (4 sequences of 1024 to 4096 tokens, 99 us for 56 us of work).  A die has consecutive ones, which read the same keys.
 struct Place {
@@ -322,7 +340,7 @@ struct Place {
     // `count` things, those of a die consecutive: the number of the die's first one
     __device__ __forceinline__ static int before(int count, int die) { return die * (count / 8) + (die < count % 8 ? die : count % 8); }
 
-    __device__ __forceinline__ Place(const WindowArgs &a, int share, int row_tiles, int lane) {
+    __device__ __forceinline__ Place(const WindowArgs &a, int share, int rows, int row_tiles, int lane) {
         const int die = blockIdx.x % 8, on_die = blockIdx.x / 8, total = a.batch * a.kv_heads * row_tiles;
         if ((a.lengths == nullptr && a.first == nullptr) || a.batch > kWave) {
             const int i = before(total, die) + on_die, problem = i / row_tiles;
@@ -335,7 +353,7 @@ struct Place {
             const int length = a.lengths != nullptr ? clamp_to(a.lengths[lane], 0, a.kv_rows) : a.kv_rows;
             const int first = a.first != nullptr ? clamp_to(a.first[lane], -kFar, kFar) : 0;
             const int low = first < 0 ? -first : 0, high = length - first < a.q_rows ? length - first : a.q_rows;
-            if (low < high) from = low * share / 128, count = (high * share + 127) / 128 - from;
+            if (low < high) from = low * share / rows, count = (high * share + rows - 1) / rows - from;
         }
         int active = 0;
         for (int n = 0; n < a.batch; ++n) active += __builtin_amdgcn_readlane(count, n);
@@ -359,96 +377,360 @@ struct Place {
     }
 };
 
-// Four wavefronts of 32 rows each share every tile of K and V, the next one on its way while they work on this one.
-template <typename T, int D>
+// What a workgroup of four wavefronts works on, KEYS keys at a time: its rows, and which tiles of keys they reach.  A wavefront has
+// 32 rows and, where only ROWS / 32 of them have rows of their own, one of the parts of a tile.
+template <typename T, int D, int KEYS, int ROWS>
+struct Strip {
+    static constexpr int kRowGroups = ROWS / 32, kParts = 4 / kRowGroups;
+    const WindowArgs &a;
+    int share, rows, row0, row, query, head, begin, end;  // this wavefront's first row; a lane's, its query and head, the bounds of its window
+    Place place;
+    Problem at;
+    bool there;
+    Reach reach, mine;  // of the workgroup's rows, and of this wavefront's
+    Tiles<KEYS> tiles;
+    const T *k, *v;
+    const int8_t *mask;
+
+    __device__ __forceinline__ static int last_of(int row, int count, int rows) { return (row + count < rows ? row + count : rows) - 1; }
+    __device__ __forceinline__ Strip(const WindowArgs &args, int row_tiles, int wave, int lane)
+        : a(args), share(a.heads / a.kv_heads), rows(a.q_rows * share), row0(0), place(a, share, ROWS, row_tiles, lane),
+          at(a, place.b, place.kv_head), reach(a, at.first + place.tile * ROWS / share, at.first + last_of(place.tile * ROWS, ROWS, rows) / share, at.length),
+          mine(a, at.first + (place.tile * ROWS + 32 * (wave % kRowGroups)) / share,
+               at.first + last_of(place.tile * ROWS + 32 * (wave % kRowGroups), 32, rows) / share, at.length),
+          tiles(reach, a.sinks) {
+        row0 = place.tile * ROWS + 32 * (wave % kRowGroups), row = row0 + (lane & 31);
+        mine.any = mine.any && row0 < rows;
+        const int my_row = row < rows ? row : rows - 1;
+        query = share == 1 ? my_row : my_row / share, head = at.kv_head * share + my_row - query * share;
+        const int p = at.first + query;
+        there = row < rows && p >= 0 && p < at.length;
+        begin = p > a.left ? p - a.left : 0, end = p < at.length - a.right ? p + a.right + 1 : at.length;
+        k = (const T *) a.k + (size_t) at.b * a.kv_rows * a.ldkv + at.kv_head * D;
+        v = (const T *) a.v + (size_t) at.b * a.kv_rows * a.ldkv + at.kv_head * D;
+        mask = a.mask != nullptr ? a.mask + (size_t) at.b * a.kv_rows : nullptr;
+    }
+    __device__ __forceinline__ const T *q() const { return (const T *) a.q + ((size_t) at.b * a.q_rows + query) * a.ldq + (size_t) head * D; }
+    __device__ __forceinline__ int mask_byte(int key) const { return mask != nullptr && key < a.kv_rows ? mask[key] : 1; }
+    // of the keys base .. base + 63 that the mask keeps, those that this lane's row sees
+    __device__ __forceinline__ unsigned long long visible(int base, unsigned long long kept) const {
+        return bits_below(end - base) & (~bits_below(begin - base) | bits_below(a.sinks - base)) & kept;
+    }
+    // take(tile, busy) for every tile of the workgroup's, in order.  This wavefront's are those of the sinks (which reach into the
+    // window's where there is no gap between them) and a run among those of the window.  (Tiles passed over by loops of their own:
+    // a branch around the work has the compiler copy every accumulator.)
+    template <typename Take>
+    __device__ __forceinline__ void walk(Take take) const {
+        const int my_sinks = a.sinks < mine.last_end ? a.sinks : mine.last_end, sinks_end = mine.any ? (my_sinks + KEYS - 1) / KEYS : 0;
+        const int from = mine.any ? tiles.of_sinks + mine.first_begin / KEYS - tiles.first : tiles.count;
+        const int until = mine.any ? tiles.of_sinks + (mine.last_end + KEYS - 1) / KEYS - tiles.first : tiles.count;
+        int tile = 0;
+        for (int part = 0; part < 2; ++part) {
+            for (; tile < (part == 0 ? 0 : from); ++tile) take(tile, false);
+            for (; tile < (part == 0 ? sinks_end : until); ++tile) take(tile, true);
+        }
+        for (; tile < tiles.count; ++tile) take(tile, false);
+    }
+    // The rows' results: sums relative to their maxima, of all parts of the tiles, which meet in LDS (`traded`, kTraded bytes) in order.
+    static constexpr int kPitch = D + 4, kTraded = (kParts - 1) * ROWS * kPitch * 4;
+    __device__ __forceinline__ void store(v16f32 (&sums)[D / 32], float top, float sum, unsigned char *traded, int wave, int lane) const {
+        const int half_wave = lane >> 5;
+        products_done();
+        sum += __shfl_xor(sum, 32, kWave);
+        if constexpr (kParts > 1) {
+            static_assert(kParts == 2, "one other part");
+            float *with = reinterpret_cast<float *>(traded) + (32 * (wave % kRowGroups) + (lane & 31)) * kPitch;
+            __syncthreads();  // nobody reads tiles any more
+            if (wave >= kRowGroups) {
+#pragma unroll
+                for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4)
+                        *reinterpret_cast<v4f32 *>(with + 32 * d + 2 * i + 4 * half_wave) = v4f32{sums[d][i], sums[d][i + 1], sums[d][i + 2], sums[d][i + 3]};
+                if (half_wave == 0) with[D] = top, with[D + 1] = sum;
+            }
+            __syncthreads();
+            if (wave >= kRowGroups) return;
+            const float other = with[D], high = fmaxf(top, other);
+            const float mine_by = __builtin_amdgcn_exp2f(top - high), other_by = __builtin_amdgcn_exp2f(other - high);
+            sum = sum * mine_by + with[D + 1] * other_by;
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const v4f32 x = *reinterpret_cast<const v4f32 *>(with + 32 * d + 2 * i + 4 * half_wave);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sums[d][i + e] = sums[d][i + e] * mine_by + x[e] * other_by;
+                }
+        }
+        if (row >= rows) return;
+        const float by = there && sum > 0.f ? 1.f / sum : 0.f;
+        T *ctx = (T *) a.ctx + ((size_t) at.b * a.q_rows + query) * a.ld_ctx + (size_t) head * D + 4 * half_wave;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                if (by != 0.f) store4(ctx + 32 * d + 2 * i, sums[d][i] * by, sums[d][i + 1] * by, sums[d][i + 2] * by, sums[d][i + 3] * by);
+                else store4(ctx + 32 * d + 2 * i, 0.f, 0.f, 0.f, 0.f);
+            }
+    }
+};
+
+// fp16, many rows: four wavefronts share every tile of K and V, the next one on its way while they work on this one.  A wavefront has 64
+// keys of a tile with its 32 rows: ROWS = 128, the same ones for all, 64, either half of 128.
+template <int D, int ROWS>
 __global__ __launch_bounds__(kBlock) void attention_window_shared_kernel(WindowArgs a, int row_tiles) {
-    constexpr int kKeys = sizeof(T) == 2 ? 64 : 32, kTileBytes = kKeys * D * (int) sizeof(T);
+    typedef half_t T;
+    constexpr int kKeys = 64 * 128 / ROWS, kTileBytes = kKeys * D * (int) sizeof(T), kPartBytes = 64 * D * (int) sizeof(T);
+    typedef Strip<T, D, kKeys, ROWS> Work;
     extern __shared__ __align__(16) unsigned char smem[];  // two buffers of K and V
-    const int wave = wave_in_block(), lane = threadIdx.x & (kWave - 1);
-    const int share = a.heads / a.kv_heads, rows = a.q_rows * share;
-    const Place place(a, share, row_tiles, lane);
-    const int row0 = place.tile * 128;
-    const Problem at(a, place.b, place.kv_head);
-    const int row = row0 + 32 * wave + (lane & 31), my_row = row < rows ? row : rows - 1;
-    const int query = share == 1 ? my_row : my_row / share, head = at.kv_head * share + my_row - query * share;
-    const int p = at.first + query;
-    const bool there = row < rows && p >= 0 && p < at.length;
-    const int begin = p > a.left ? p - a.left : 0, end = p < at.length - a.right ? p + a.right + 1 : at.length;
-
-    const T *k = (const T *) a.k + (size_t) at.b * a.kv_rows * a.ldkv + at.kv_head * D;
-    const T *v = (const T *) a.v + (size_t) at.b * a.kv_rows * a.ldkv + at.kv_head * D;
-    const int8_t *mask = a.mask != nullptr ? a.mask + (size_t) at.b * a.kv_rows : nullptr;
-    const int last_row = (row0 + 128 < rows ? row0 + 128 : rows) - 1;
-    const Reach reach(a, at.first + row0 / share, at.first + last_row / share, at.length);
-    const Tiles<kKeys> tiles(reach, a.sinks);
-    const int wave_row = row0 + 32 * wave, wave_last = wave_row + 31 < rows ? wave_row + 31 : rows - 1;
-    Reach mine(a, at.first + wave_row / share, at.first + wave_last / share, at.length);
-    mine.any = mine.any && wave_row < rows;
-
+    static_assert(4 * kTileBytes >= Work::kTraded, "room for what is traded");
+    const int wave = wave_in_block(), lane = threadIdx.x & (kWave - 1), part = wave / Work::kRowGroups;
+    const Work strip(a, row_tiles, wave, lane);
     const unsigned pitch = (unsigned) a.ldkv * sizeof(T), lds = lds_address(smem);
     const Bring<T, D, kKeys, 4, false> bring_k(wave, lane, pitch);
     const Bring<T, D, kKeys, 4, true> bring_v(wave, lane, pitch);
     auto bring = [&](int tile, int buffer) {
         const unsigned to = lds + buffer * 2 * kTileBytes;
-        bring_k(k, tiles.base(tile), a.kv_rows, pitch, to, wave, lane);
-        bring_v(v, tiles.base(tile), a.kv_rows, pitch, to + kTileBytes, wave, lane);
-    };
-    auto mask_byte = [&](int tile) -> int {
-        const int j = tiles.base(tile) + lane;
-        return mask != nullptr && lane < kKeys && j < a.kv_rows ? mask[j] : 1;
+        bring_k(strip.k, strip.tiles.base(tile), a.kv_rows, pitch, to, wave, lane);
+        bring_v(strip.v, strip.tiles.base(tile), a.kv_rows, pitch, to + kTileBytes, wave, lane);
     };
     int kept = 1;
-    if (tiles.count > 0) {
+    if (strip.tiles.count > 0) {
         bring(0, 0);
-        kept = mask_byte(0);
+        kept = strip.mask_byte(strip.tiles.base(0) + 64 * part + lane);
     }
     Rows<T, D> r;
-    r.load((const T *) a.q + ((size_t) at.b * a.q_rows + query) * a.ldq + (size_t) head * D, lane >> 5, a.negate);
+    r.load(strip.q(), lane >> 5, a.negate);
     // One tile of the workgroup's: everybody waits for it, brings a share of the next one and, `busy`, works on it.
-    auto take = [&](int tile, bool busy) {
+    strip.walk([&](int tile, bool busy) {
         landed();
-        const unsigned long long kept_bits = mask != nullptr ? __ballot(kept != 0) : ~0ull;
+        const unsigned long long kept_bits = strip.mask != nullptr ? __ballot(kept != 0) : ~0ull;
         __syncthreads();  // everybody's; and nobody reads the other buffer any more
-        if (tile + 1 < tiles.count) {
+        if (tile + 1 < strip.tiles.count) {
             bring(tile + 1, (tile + 1) & 1);
-            kept = mask_byte(tile + 1);
-        }
-        unsigned char *kt = smem + (tile & 1) * 2 * kTileBytes, *vt = kt + kTileBytes;
-        const int base = tiles.base(tile);
-        const bool kept_all = mask == nullptr || (kept_bits & bits_below(kKeys)) == bits_below(kKeys);
-        if (!kept_all || base + kKeys > reach.last_end || (base < reach.first_begin && base + kKeys > a.sinks)) {
-            clear_rows<T, D, kKeys, kBlock>(vt, reach.of(base, a.sinks) & kept_bits, threadIdx.x);
-            __syncthreads();
+            kept = strip.mask_byte(strip.tiles.base(tile + 1) + 64 * part + lane);
         }
         if (!busy) return;
-        const bool all = kept_all && mine.all(base, kKeys, a.sinks);
+        unsigned char *kt = smem + (tile & 1) * 2 * kTileBytes + part * kPartBytes, *vt = kt + kTileBytes;
+        const int base = strip.tiles.base(tile) + 64 * part;
+        const bool all = kept_bits == ~0ull && strip.mine.all(base, 64, a.sinks);
         unsigned long long visible = ~0ull;
-        if (!all) visible = bits_below(end - base) & (~bits_below(begin - base) | bits_below(a.sinks - base)) & kept_bits;
-        attend<T, D, kKeys / 32>(r, kt, vt, a.scale, all, visible, lane);
-    };
-    // This wavefront's tiles are those of the sinks (which reach into the window's where there is no gap between them) and a run
-    // among those of the window.  (Tiles passed over by loops of their own: a branch around the work has the compiler copy every
-    // accumulator.)
-    const int my_sinks = a.sinks < mine.last_end ? a.sinks : mine.last_end, sinks_end = mine.any ? (my_sinks + kKeys - 1) / kKeys : 0;
-    const int from = mine.any ? tiles.of_sinks + mine.first_begin / kKeys - tiles.first : tiles.count;
-    const int until = mine.any ? tiles.of_sinks + (mine.last_end + kKeys - 1) / kKeys - tiles.first : tiles.count;
-    int tile = 0;
-    for (int part = 0; part < 2; ++part) {
-        for (; tile < (part == 0 ? 0 : from); ++tile) take(tile, false);
-        for (; tile < (part == 0 ? sinks_end : until); ++tile) take(tile, true);
-    }
-    for (; tile < tiles.count; ++tile) take(tile, false);
-    if (row >= rows) return;
-    const float sum = r.sum + __shfl_xor(r.sum, 32, kWave);
-    const float by = there && sum > 0.f ? 1.f / sum : 0.f;
-    T *ctx = (T *) a.ctx + ((size_t) at.b * a.q_rows + query) * a.ld_ctx + (size_t) head * D + 4 * (lane >> 5);
-#pragma unroll
-    for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            if (by != 0.f) store4(ctx + 32 * d + 2 * i, r.ctx[d][i] * by, r.ctx[d][i + 1] * by, r.ctx[d][i + 2] * by, r.ctx[d][i + 3] * by);
-            else store4(ctx + 32 * d + 2 * i, 0.f, 0.f, 0.f, 0.f);
+        if (!all) {
+            visible = strip.visible(base, kept_bits);
+            // (each wavefront that reads these rows clears them, with the same zeros)
+            const unsigned long long seen = strip.reach.of(base, a.sinks) & kept_bits;
+            if (seen != ~0ull) {
+                clear_rows<T, D, 64, kWave>(vt, seen, lane);
+                asm volatile("" ::: "memory");
+                __builtin_amdgcn_wave_barrier();
+            }
         }
+        attend<T, D, 2>(r, kt, vt, a.scale, all, visible, lane);
+    });
+    strip.store(r.ctx, r.top, r.sum, smem, wave, lane);
+}
+
+// ---- fp32, many rows ------------------------------------------------------
+// An fp32 number is the sum of three bf16 numbers: its leading, middle and last 8 bits.  Of the nine products of two such sums
+// the three smallest are below 2^-24 of the whole and left out; the six others run on the bf16 matrix cores, whose rate is sixteen
+// times that of fp32's, with fp32 sums.  K and V are taken apart on their way into LDS, once for the four wavefronts that read
+// them; the probabilities in their lanes.
+
+typedef __bf16 v8bf16 __attribute__((ext_vector_type(8)));
+typedef unsigned v2u32 __attribute__((ext_vector_type(2)));
+typedef unsigned v4u32 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ float lead(float x) { return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, x) & 0xffff0000u); }
+__device__ __forceinline__ unsigned lead_pair(float a, float b) {
+    return __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, b), __builtin_bit_cast(unsigned, a), 0x07060302u);
+}
+// What is left of x behind its leading bits.  (Of an infinity a NaN: what it reaches is not finite either way, and two
+// instructions more for every number of K, V and the probabilities would be a fifth of the kernel's time.)
+__device__ __forceinline__ float rest(float x) { return x - lead(x); }
+
+struct Terms {  // of 8 numbers
+    v8bf16 t[3];
+
+    __device__ __forceinline__ Terms() {}
+    __device__ __forceinline__ explicit Terms(const float (&x)[8]) {
+        v4u32 r[3];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float a = x[2 * i], b = x[2 * i + 1];
+#pragma unroll
+            for (int n = 0; n < 3; ++n) {
+                r[n][i] = lead_pair(a, b);
+                a = rest(a), b = rest(b);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < 3; ++n) t[n] = __builtin_bit_cast(v8bf16, r[n]);
+    }
+};
+
+// sums + one of the six products of a and b, of which the smallest come first
+__device__ __forceinline__ v16f32 multiply_term(int m, const v8bf16 (&a)[3], const v8bf16 (&b)[3], v16f32 sums) {
+    constexpr int kA[6] = {2, 1, 0, 1, 0, 0}, kB[6] = {0, 1, 2, 0, 1, 0};
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[kA[m]], b[kB[m]], sums, 0, 0, 0);
+}
+
+// As above; a wavefront has 32 keys of a tile with its 32 rows: ROWS = 128, the same ones for all, 64, either half of 64.
+template <int D, int ROWS>
+__global__ __launch_bounds__(kBlock, D == 128 ? 1 : 2) void attention_window_terms_kernel(WindowArgs a, int row_tiles) {
+    constexpr int kKeys = 32 * 128 / ROWS, kRowBytes = 2 * D, kPlane = kKeys * kRowBytes, kQuads = D / 4, kMine = kKeys * kQuads / kBlock;
+    typedef Strip<float, D, kKeys, ROWS> Work;
+    extern __shared__ __align__(16) unsigned char smem[];
+    static_assert(6 * kPlane >= Work::kTraded, "room for what is traded");
+    unsigned char *planes = smem;  // of K, then of V
+    const int wave = wave_in_block(), lane = threadIdx.x & (kWave - 1), col = lane & 31, half_wave = lane >> 5;
+    const int part = wave / Work::kRowGroups;
+    const Work strip(a, row_tiles, wave, lane);
+    // a thread's pieces of a tile: 16 bytes of `kMine` rows of K and of V
+    v4f32 next[2][kMine];
+    const unsigned pitch = (unsigned) a.ldkv * 4u;
+    auto offset_of = [&](int i, int last) {
+        const int at = i * kBlock + threadIdx.x, key = at / kQuads;
+        return (unsigned) (key < last ? key : last) * pitch + at % kQuads * 16;
+    };
+    unsigned offset[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) offset[i] = offset_of(i, kKeys);
+    auto bring = [&](int tile) {
+        const int base = strip.tiles.base(tile);
+        const char *k = (const char *) strip.k + (size_t) base * pitch, *v = (const char *) strip.v + (size_t) base * pitch;
+        const bool whole = base + kKeys <= a.kv_rows;  // (rows past the last are read from it)
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            const unsigned from = whole ? offset[i] : offset_of(i, a.kv_rows - 1 - base);
+            next[0][i] = *reinterpret_cast<const v4f32 *>(k + from);
+            next[1][i] = *reinterpret_cast<const v4f32 *>(v + from);
+        }
+    };
+    int kept = 1;
+    if (strip.tiles.count > 0) {
+        bring(0);
+        kept = strip.mask_byte(strip.tiles.base(0) + lane);
+    }
+    Terms q[D / 16];
+    {
+        const float *from = strip.q() + 8 * half_wave;
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = a.negate ? -from[16 * t + e] : from[16 * t + e];
+            q[t] = Terms(x);
+        }
+    }
+    v16f32 ctx[D / 32] = {};
+    float top = kNone, sum = 0.f;
+    const int patch = lane & 15, side = (lane >> 4) & 1;
+
+    strip.walk([&](int tile, bool busy) {
+        const unsigned long long kept_bits = strip.mask != nullptr ? __ballot(kept != 0) : ~0ull;
+        const int base = strip.tiles.base(tile) + 32 * part;
+        const unsigned long long seen = strip.reach.of(strip.tiles.base(tile), a.sinks) & kept_bits;
+        __syncthreads();  // nobody reads the tile before any more
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+                const int at = i * kBlock + threadIdx.x, key = at / kQuads, quad = at % kQuads;
+                // (a key that nobody sees has probability 0, but 0 times what its row of V may hold need not be 0)
+                const bool use = w == 0 || (seen >> key & 1ull);
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = use ? next[w][i][e] : 0.f;
+                const int piece = w == 0 ? k_piece<kRowBytes>(key, quad / 2) : v_piece<half_t, kRowBytes>(key, quad / 2);
+                unsigned char *to = planes + w * 3 * kPlane + key * kRowBytes + piece * 16 + (quad & 1) * 8;
+#pragma unroll
+                for (int n = 0; n < 3; ++n) {
+                    *reinterpret_cast<v2u32 *>(to + n * kPlane) = v2u32{lead_pair(x[0], x[1]), lead_pair(x[2], x[3])};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = rest(x[e]);
+                }
+            }
+        if (tile + 1 < strip.tiles.count) {
+            bring(tile + 1);
+            kept = strip.mask_byte(strip.tiles.base(tile + 1) + lane);
+        }
+        __syncthreads();
+        if (!busy) return;
+        const unsigned kept_part = (unsigned) (kept_bits >> (32 * part));
+        const bool all = kept_part == ~0u && strip.mine.all(base, 32, a.sinks);
+        // (two sums in turn: a product waits for the one before it in its sum)
+        v16f32 s = {}, odd = {};
+#pragma unroll
+        for (int t = 0; t < D / 16; t += 2) {
+            v8bf16 k[2][3];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int n = 0; n < 3; ++n)
+                    k[u][n] = *reinterpret_cast<const v8bf16 *>(planes + n * kPlane + (32 * part + col) * kRowBytes +
+                                                                k_piece<kRowBytes>(col, 2 * (t + u) + half_wave) * 16);
+#pragma unroll
+            for (int m = 0; m < 6; ++m) {
+                s = multiply_term(m, k[0], q[t].t, s);
+                odd = multiply_term(m, k[1], q[t + 1].t, odd);
+            }
+        }
+        products_done();
+        s += odd;
+        if (!all) {
+            const unsigned word = (unsigned) strip.visible(base, kept_part) >> (4 * half_wave);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = word >> (8 * (i / 4) + i % 4) & 1u ? s[i] : -INFINITY;
+        }
+        float high = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) high = fmaxf(high, s[i]);
+        high *= a.scale;
+        if (__any(high > top + kSlack)) {
+            high = fmaxf(top, fmaxf(high, __shfl_xor(high, 32, kWave)));
+            const float shrink = __builtin_amdgcn_exp2f(top - high);
+            top = high;
+            sum *= shrink;
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) ctx[d] *= shrink;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale, -top));
+            sum += s[i];
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = s[8 * ks + e];
+            const Terms p(x);
+            constexpr int kTogether = D == 32 ? 1 : 2;  // columns of 32 whose sums take turns
+#pragma unroll
+            for (int d = 0; d < D / 32; d += kTogether) {
+                v8bf16 v[kTogether][3];
+#pragma unroll
+                for (int u = 0; u < kTogether; ++u)
+#pragma unroll
+                    for (int n = 0; n < 3; ++n) {
+                        v4f16 from[2];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int key = 16 * ks + 8 * h + 4 * half_wave + patch / 4, at = 4 * (d + u) + 2 * side + (patch & 3) / 2;
+                            from[h] = read_transposed(planes + (3 + n) * kPlane + (32 * part + key) * kRowBytes +
+                                                      v_piece<half_t, kRowBytes>(key, at) * 16 + (patch & 1) * 8);
+                        }
+                        v[u][n] = __builtin_bit_cast(v8bf16, __builtin_shufflevector(from[0], from[1], 0, 1, 2, 3, 4, 5, 6, 7));
+                    }
+#pragma unroll
+                for (int m = 0; m < 6; ++m)
+#pragma unroll
+                    for (int u = 0; u < kTogether; ++u) ctx[d + u] = multiply_term(m, v[u], p.t, ctx[d + u]);
+            }
+        }
+    });
+    strip.store(ctx, top, sum, smem, wave, lane);
 }
 
 template <typename T, int D>
@@ -537,7 +819,7 @@ __global__ __launch_bounds__(kBlock, sizeof(T) * D == 512 ? 1 : 2) void attentio
             const bool all = reach.all(base, 32, a.sinks) && (kept_bits & whole) == whole;
             const unsigned long long visible =
                     all ? ~0ull : bits_below(end - base) & (~bits_below(begin - base) | bits_below(a.sinks - base)) & kept_bits;
-            attend<T, D, 1>(r, kt, vt, a.scale, all, visible, lane);
+            attend<T, D, 1, true>(r, kt, vt, a.scale, all, visible, lane);
         }
         if (S::kBuffers == 2) {
             buffer ^= 1;
@@ -553,6 +835,7 @@ __global__ __launch_bounds__(kBlock, sizeof(T) * D == 512 ? 1 : 2) void attentio
         }
     }
     // the four wavefronts' sums, 32 rows of D + 4 floats each: results, maximum, sum
+    products_done();
     __syncthreads();
     float *merge = reinterpret_cast<float *>(smem);
     const float sum = r.sum + __shfl_xor(r.sum, 32, kWave);
@@ -665,24 +948,28 @@ __global__ __launch_bounds__(kBlock) void attention_window_join_kernel(WindowArg
     else store4(ctx, 0.f, 0.f, 0.f, 0.f);
 }
 
-// How a call is run: rows of a workgroup, and into how many pieces the axis is cut.
+// How a call is run: rows of a workgroup (32: the spread kernel), and into how many pieces the axis is cut.
 struct WindowPlan {
-    bool shared;
-    int row_tiles, pieces;
+    int rows, row_tiles, pieces;
     size_t floats;
 };
 
-WindowPlan plan_window(int batch, int heads, int kv_heads, int q_rows, int kv_rows, int head_size, int left, int right, int sinks) {
+// The rule, measured on heads of 64 with 128 / 64 / 32 rows, microseconds.  fp16: 4 x 4096 tokens of 16 heads, window 512 (2048 workgroups of
+// 128) 78 / 106 / 164; 32 x 128 of 12 (384) 13 / 17 / 19; 2 x 4096 of 4 (256) 59 / 41 / 71; 3 x 517 of 12 (180) 24 / 23 / 26; 1 x 600
+// (60) 15 / 11 / 15; 1 x 64 over 1000 (12) 19 / 13 / 12.  fp32: 2 x 2000 of 16 (512) 195 / 231 / 301; 3 x 517 (180) 55 / 47 / 54; 1 x 600
+// (60) 46 / 31 / 26.  Heads of 128, 2 x 400 over 6000 in fp16 (104): 131 / 91 / 74.
+WindowPlan plan_window(bool half_precision, int batch, int heads, int kv_heads, int q_rows, int kv_rows, int head_size, int left, int right, int sinks) {
     WindowPlan plan;
     const long long rows = (long long) q_rows * (heads / kv_heads), problems = (long long) batch * kv_heads;
-    const long long shared_tiles = (rows + 127) / 128 * problems;
-    plan.shared = rows > 32 && shared_tiles >= 192;
+    const long long of_128 = (rows + 127) / 128 * problems, of_64 = (rows + 63) / 64 * problems;
+    const int enough = !half_precision ? 192 : head_size == 128 ? 256 : 96;
+    plan.rows = rows <= 32 ? 32 : of_128 >= 320 ? 128 : of_64 >= enough ? 64 : 32;
+#ifdef PLAN
+    plan.rows = rows <= 32 ? 32 : PLAN;
+#endif
+    plan.row_tiles = (int) ((rows + plan.rows - 1) / plan.rows);
     plan.pieces = 1, plan.floats = 0;
-    if (plan.shared) {
-        plan.row_tiles = (int) ((rows + 127) / 128);
-        return plan;
-    }
-    plan.row_tiles = (int) ((rows + 31) / 32);
+    if (plan.rows > 32) return plan;
     // the most keys that 32 rows reach
     long long reach = kv_rows;
     if (left >= 0 && right >= 0) reach = (long long) left + right + 33 + sinks < reach ? (long long) left + right + 33 + sinks : reach;
@@ -696,15 +983,26 @@ WindowPlan plan_window(int batch, int heads, int kv_heads, int q_rows, int kv_ro
     return plan;
 }
 
+template <typename T, int D, int ROWS>
+int run_window_rows(const WindowArgs &a, int row_tiles, hipStream_t stream) {
+    static std::atomic<unsigned long long> done{0};
+    const dim3 grid(a.batch * a.kv_heads * row_tiles);
+    if constexpr (sizeof(T) == 4) {
+        constexpr int kLds = 6 * (32 * 128 / ROWS) * 2 * D;
+        if (kLds > 48 * 1024 && !allow_large_lds(attention_window_terms_kernel<D, ROWS>, done)) return CUBERT_UNSUPPORTED;
+        return launch_lds(attention_window_terms_kernel<D, ROWS>, grid, dim3(kBlock), kLds, stream, a, row_tiles);
+    } else {
+        constexpr int kLds = 4 * (64 * 128 / ROWS) * 2 * D;
+        if (kLds > 48 * 1024 && !allow_large_lds(attention_window_shared_kernel<D, ROWS>, done)) return CUBERT_UNSUPPORTED;
+        return launch_lds(attention_window_shared_kernel<D, ROWS>, grid, dim3(kBlock), kLds, stream, a, row_tiles);
+    }
+}
+
 template <typename T, int D>
 int run_window(const WindowArgs &a, WindowPlan plan, hipStream_t stream) {
     const int problems = a.batch * a.kv_heads;
-    if (plan.shared) {
-        constexpr int kLds = 4 * (sizeof(T) == 2 ? 64 : 32) * D * (int) sizeof(T);
-        static std::atomic<unsigned long long> done{0};
-        if (kLds > 48 * 1024 && !allow_large_lds(attention_window_shared_kernel<T, D>, done)) return CUBERT_UNSUPPORTED;
-        return launch_lds(attention_window_shared_kernel<T, D>, dim3(problems * plan.row_tiles), dim3(kBlock), kLds, stream, a, plan.row_tiles);
-    }
+    if (plan.rows == 128) return run_window_rows<T, D, 128>(a, plan.row_tiles, stream);
+    if (plan.rows == 64) return run_window_rows<T, D, 64>(a, plan.row_tiles, stream);
     static std::atomic<unsigned long long> done{0};
     if (Spread<T, D>::kLds > 48 * 1024 && !allow_large_lds(attention_window_spread_kernel<T, D>, done)) return CUBERT_UNSUPPORTED;
     const int rc = launch_lds(attention_window_spread_kernel<T, D>, dim3(problems * plan.row_tiles * plan.pieces), dim3(kBlock),
@@ -748,7 +1046,7 @@ int attention_window(const T *q, int ldq, const T *k, const T *v, int ldkv, cons
     a.batch = batch, a.heads = heads, a.kv_heads = kv_heads, a.q_rows = q_rows, a.kv_rows = kv_rows;
     a.left = left < 0 || left > kFar ? kFar : left, a.right = right < 0 || right > kFar ? kFar : right;
     a.sinks = sinks;
-    WindowPlan plan = plan_window(batch, heads, kv_heads, q_rows, kv_rows, head_size, left, right, sinks);
+    WindowPlan plan = plan_window(sizeof(T) == 2, batch, heads, kv_heads, q_rows, kv_rows, head_size, left, right, sinks);
     if ((unsigned long long) batch * kv_heads * plan.row_tiles * plan.pieces >= 1u << 24) return CUBERT_UNSUPPORTED;
     if (plan.pieces > 1 && (partials == nullptr || partial_floats < plan.floats || !is_aligned(partials, 16))) plan.pieces = 1;
     if (head_size == 32) return run_window<T, 32>(a, plan, (hipStream_t) stream);
@@ -765,9 +1063,8 @@ extern "C" {
 
 size_t cubert_attention_window_partials(int half_precision, int batch, int heads, int kv_heads, int q_rows, int kv_rows,
                                         int head_size, int left, int right, int sinks) {
-    (void) half_precision;
     if (batch < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || q_rows < 1 || kv_rows < 1 || head_size < 1) return 0;
-    return cubert::plan_window(batch, heads, kv_heads, q_rows, kv_rows, head_size, left, right, sinks).floats;
+    return cubert::plan_window(half_precision != 0, batch, heads, kv_heads, q_rows, kv_rows, head_size, left, right, sinks).floats;
 }
 
 int cubert_attention_window_f32(const float *q, int ldq, const float *k, const float *v, int ldkv, const int *first,
