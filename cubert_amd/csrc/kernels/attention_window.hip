@@ -239,6 +239,9 @@ struct Reach {
     __device__ __forceinline__ unsigned long long of(int base, int sinks) const {
         return bits_below(last_end - base) & (~bits_below(first_begin - base) | bits_below(sinks - base));
     }
+    __device__ __forceinline__ void cut(int end) {  // nothing is seen from `end` on
+        first_end = first_end < end ? first_end : end, last_end = last_end < end ? last_end : end;
+    }
     __device__ __forceinline__ bool all(int base, int keys, int sinks) const {
         return base + keys <= first_end && (base >= last_begin || base + keys <= sinks);
     }
@@ -254,7 +257,7 @@ struct Tiles {
         const int end = (reach.last_end + KEYS - 1) / KEYS, far = sinks > reach.last_end ? reach.last_end : sinks;
         of_sinks = (far + KEYS - 1) / KEYS;
         of_sinks = of_sinks < first ? of_sinks : first;
-        count = reach.any ? of_sinks + end - first : 0;
+        count = reach.any ? of_sinks + (end > first ? end - first : 0) : 0;
     }
     __device__ __forceinline__ int base(int tile) const { return (tile < of_sinks ? tile : tile - of_sinks + first) * KEYS; }
 };
@@ -300,15 +303,44 @@ struct Bring {
     }
 };
 
-// A key that nobody sees has probability 0, but 0 times what its row of V may hold need not be 0.
-template <typename T, int D, int KEYS, int THREADS>
-__device__ __forceinline__ void clear_rows(unsigned char *v, unsigned long long seen, int thread) {
+// A key that nobody sees has probability 0, but 0 times what its row of V may hold need not be 0.  A wavefront clears these rows, one at a
+// time where they are few (holes in a mask).
+template <typename T, int D, int KEYS>
+__device__ __forceinline__ void clear_rows(unsigned char *v, unsigned long long seen, int lane) {
     constexpr int kPieces = D * (int) sizeof(T) / 16;
+    unsigned long long unseen = ~seen & (KEYS == 64 ? ~0ull : (1ull << (KEYS % 64)) - 1);
+    if (__builtin_popcountll(unseen) <= 12) {
+        for (; unseen != 0; unseen &= unseen - 1)
+            if (lane < kPieces) *reinterpret_cast<v4f32 *>(v + (__builtin_ctzll(unseen) * kPieces + lane) * 16) = v4f32{};
+    } else {
 #pragma unroll
-    for (int i = 0; i < KEYS * kPieces / THREADS; ++i) {
-        const int at = i * THREADS + thread;
-        if (!(seen >> (at / kPieces) & 1ull)) *reinterpret_cast<v4f32 *>(v + at * 16) = v4f32{};
+        for (int i = 0; i < KEYS * kPieces / kWave; ++i) {
+            const int at = i * kWave + lane;
+            if (!(seen >> (at / kPieces) & 1ull)) *reinterpret_cast<v4f32 *>(v + at * 16) = v4f32{};
+        }
     }
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// The number of keys up to the last one below `end` that the mask keeps (padding is given as a mask, and is not to be computed).
+__device__ __forceinline__ int kept_end(const int8_t *mask, int end, int lane) {
+    while (end > 0) {
+        int byte[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int j = end - 1 - (64 * i + lane);
+            byte[i] = mask[j > 0 ? j : 0];
+            byte[i] = j >= 0 ? byte[i] : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const unsigned long long kept = __ballot(byte[i] != 0);
+            if (kept != 0) return end - 64 * i - __builtin_ctzll(kept);
+        }
+        end -= 512;
+    }
+    return 0;
 }
 
 struct Problem {
@@ -388,9 +420,9 @@ struct Strip {
     Problem at;
     bool there;
     Reach reach, mine;  // of the workgroup's rows, and of this wavefront's
+    const int8_t *mask;
     Tiles<KEYS> tiles;
     const T *k, *v;
-    const int8_t *mask;
 
     __device__ __forceinline__ static int last_of(int row, int count, int rows) { return (row + count < rows ? row + count : rows) - 1; }
     __device__ __forceinline__ Strip(const WindowArgs &args, int row_tiles, int wave, int lane)
@@ -398,7 +430,7 @@ struct Strip {
           at(a, place.b, place.kv_head), reach(a, at.first + place.tile * ROWS / share, at.first + last_of(place.tile * ROWS, ROWS, rows) / share, at.length),
           mine(a, at.first + (place.tile * ROWS + 32 * (wave % kRowGroups)) / share,
                at.first + last_of(place.tile * ROWS + 32 * (wave % kRowGroups), 32, rows) / share, at.length),
-          tiles(reach, a.sinks) {
+          mask(a.mask != nullptr ? a.mask + (size_t) at.b * a.kv_rows : nullptr), tiles(cut_to_mask(lane), a.sinks) {
         row0 = place.tile * ROWS + 32 * (wave % kRowGroups), row = row0 + (lane & 31);
         mine.any = mine.any && row0 < rows;
         const int my_row = row < rows ? row : rows - 1;
@@ -408,7 +440,13 @@ struct Strip {
         begin = p > a.left ? p - a.left : 0, end = p < at.length - a.right ? p + a.right + 1 : at.length;
         k = (const T *) a.k + (size_t) at.b * a.kv_rows * a.ldkv + at.kv_head * D;
         v = (const T *) a.v + (size_t) at.b * a.kv_rows * a.ldkv + at.kv_head * D;
-        mask = a.mask != nullptr ? a.mask + (size_t) at.b * a.kv_rows : nullptr;
+    }
+    __device__ __forceinline__ const Reach &cut_to_mask(int lane) {
+        if (mask != nullptr && reach.any) {
+            const int kept = kept_end(mask, reach.last_end, lane);
+            reach.cut(kept), mine.cut(kept);
+        }
+        return reach;
     }
     __device__ __forceinline__ const T *q() const { return (const T *) a.q + ((size_t) at.b * a.q_rows + query) * a.ldq + (size_t) head * D; }
     __device__ __forceinline__ int mask_byte(int key) const { return mask != nullptr && key < a.kv_rows ? mask[key] : 1; }
@@ -421,9 +459,10 @@ struct Strip {
     // a branch around the work has the compiler copy every accumulator.)
     template <typename Take>
     __device__ __forceinline__ void walk(Take take) const {
-        const int my_sinks = a.sinks < mine.last_end ? a.sinks : mine.last_end, sinks_end = mine.any ? (my_sinks + KEYS - 1) / KEYS : 0;
-        const int from = mine.any ? tiles.of_sinks + mine.first_begin / KEYS - tiles.first : tiles.count;
-        const int until = mine.any ? tiles.of_sinks + (mine.last_end + KEYS - 1) / KEYS - tiles.first : tiles.count;
+        const int my_sinks = a.sinks < mine.last_end ? a.sinks : mine.last_end, sinks_end = mine.any && my_sinks > 0 ? (my_sinks + KEYS - 1) / KEYS : 0;
+        int from = mine.any ? tiles.of_sinks + mine.first_begin / KEYS - tiles.first : tiles.count;
+        int until = mine.any ? tiles.of_sinks + (mine.last_end + KEYS - 1) / KEYS - tiles.first : tiles.count;
+        from = from < tiles.count ? from : tiles.count, until = until < tiles.count ? until : tiles.count;
         int tile = 0;
         for (int part = 0; part < 2; ++part) {
             for (; tile < (part == 0 ? 0 : from); ++tile) take(tile, false);
@@ -520,11 +559,7 @@ __global__ __launch_bounds__(kBlock) void attention_window_shared_kernel(WindowA
             visible = strip.visible(base, kept_bits);
             // (each wavefront that reads these rows clears them, with the same zeros)
             const unsigned long long seen = strip.reach.of(base, a.sinks) & kept_bits;
-            if (seen != ~0ull) {
-                clear_rows<T, D, 64, kWave>(vt, seen, lane);
-                asm volatile("" ::: "memory");
-                __builtin_amdgcn_wave_barrier();
-            }
+            if (seen != ~0ull) clear_rows<T, D, 64>(vt, seen, lane);
         }
         attend<T, D, 2>(r, kt, vt, a.scale, all, visible, lane);
     });
@@ -765,7 +800,8 @@ __global__ __launch_bounds__(kBlock, sizeof(T) * D == 512 ? 1 : 2) void attentio
     const T *v = (const T *) a.v + (size_t) at.b * a.kv_rows * a.ldkv + at.kv_head * D;
     const int8_t *mask = a.mask != nullptr ? a.mask + (size_t) at.b * a.kv_rows : nullptr;
     const int last_row = (row0 + 32 < rows ? row0 + 32 : rows) - 1;
-    const Reach reach(a, at.first + row0 / share, at.first + last_row / share, at.length);
+    Reach reach(a, at.first + row0 / share, at.first + last_row / share, at.length);
+    if (mask != nullptr && reach.any) reach.cut(kept_end(mask, reach.last_end, lane));
     const Tiles<32> tiles(reach, a.sinks);
 
     Rows<T, D> r;
@@ -810,11 +846,7 @@ __global__ __launch_bounds__(kBlock, sizeof(T) * D == 512 ? 1 : 2) void attentio
         unsigned char *kt = buffers + buffer * 2 * S::kTileBytes, *vt = kt + S::kTileBytes;
         const int base = tiles.base(tile);
         const unsigned long long seen = reach.of(base, a.sinks) & kept_bits, whole = bits_below(32);
-        if ((seen & whole) != whole) {
-            clear_rows<T, D, 32, kWave>(vt, seen, lane);
-            asm volatile("" ::: "memory");
-            __builtin_amdgcn_wave_barrier();
-        }
+        if ((seen & whole) != whole) clear_rows<T, D, 32>(vt, seen, lane);
         if ((seen & whole) != 0) {
             const bool all = reach.all(base, 32, a.sinks) && (kept_bits & whole) == whole;
             const unsigned long long visible =
@@ -974,10 +1006,11 @@ WindowPlan plan_window(bool half_precision, int batch, int heads, int kv_heads, 
     long long reach = kv_rows;
     if (left >= 0 && right >= 0) reach = (long long) left + right + 33 + sinks < reach ? (long long) left + right + 33 + sinks : reach;
     const long long tiles = (reach + 31) / 32, blocks = problems * plan.row_tiles;
-    // About 384 workgroups, three for two units, with two tiles to a wavefront at least.  Microseconds with 256 / 384 / 512 / 768:
+    // About 384 workgroups, three for two units, with a tile to every wavefront at least.  Microseconds with 256 / 384 / 512 / 768:
     // fp16, 48 tokens over up to 1000 keys 20 / 20 / 24 / 23, 2 x 100 over 6000 28 / 23 / 27 / 26, 32 over 4096 52 / 54 / 52 / 53.
     long long pieces = blocks > 0 ? (384 + blocks - 1) / blocks : 1;
-    pieces = pieces < (tiles + 7) / 8 ? pieces : (tiles + 7) / 8;
+    const long long most = (tiles + 3) / 4;
+    pieces = pieces < most ? pieces : most;
     plan.pieces = (int) (pieces < 1 ? 1 : pieces > kMaxPieces ? kMaxPieces : pieces);
     if (plan.pieces > 1) plan.floats = (size_t) blocks * plan.pieces * 32 * (head_size + 4);
     return plan;

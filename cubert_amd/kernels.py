@@ -546,16 +546,16 @@ def dense_w4_i8(x, x_scales, w, bias=None, gelu=False, dtype=torch.float16, out=
     return _dense_w4(x, x_scales, w, bias, gelu, dtype, out)
 
 
-def _heads_ptr(t, what):
-    """Of a [batch, rows, heads, size] tensor whose rows are a fixed pitch apart, in rows of contiguous heads; and that pitch."""
+def _heads_pitch(t, what):
+    """The pitch of the rows of a [batch, rows, heads, size] tensor, one for all of them, whose heads stand side by side."""
     batch, rows, heads, size = t.shape
     b, r, h, d = t.stride()
     pitch = r if rows > 1 else b if batch > 1 else heads * size
     if t.numel() == 0:
-        return t.data_ptr(), heads * size
+        return heads * size
     if not heads * size <= pitch < 1 << 31 or (size > 1 and d != 1) or (heads > 1 and h != size) or (batch > 1 and b != rows * pitch):
         raise ValueError("%s: heads side by side in rows of one pitch expected, got strides %s of %s" % (what, t.stride(), tuple(t.shape)))
-    return t.data_ptr(), pitch
+    return pitch
 
 
 def attention_window(q, k, v, left=-1, right=-1, sinks=0, first=None, lengths=None, mask=None, alpha=None):
@@ -579,13 +579,13 @@ def attention_window(q, k, v, left=-1, right=-1, sinks=0, first=None, lengths=No
         raise ValueError("mask: int8 (%d, %d) expected, got %s %s" % (batch, kv_rows, mask.dtype, tuple(mask.shape)))
     left, right, sinks = max(min(left, 1 << 30), -1), max(min(right, 1 << 30), -1), min(sinks, 1 << 30)
     suffix = _SUFFIXES.get(q.dtype) or _suffix(q)
-    (qp, ldq), (kp, ldkv), (vp, ldv) = _heads_ptr(q, "q"), _heads_ptr(k, "k"), _heads_ptr(v, "v")
-    if ldkv != ldv:
-        raise ValueError("k and v at one row pitch expected, got %d and %d" % (ldkv, ldv))
-    ctx = torch.empty((batch, q_rows, heads, size), dtype=q.dtype, device=q.device)
+    ldq, ldkv = _heads_pitch(q, "q"), _heads_pitch(k, "k")
+    if v.stride() != k.stride() and _heads_pitch(v, "v") != ldkv:
+        raise ValueError("k and v at one row pitch expected, got strides %s and %s" % (k.stride(), v.stride()))
+    ctx = torch.empty_like(q, memory_format=torch.contiguous_format)
     floats = lib().cubert_attention_window_partials(suffix == "f16", batch, heads, kv_heads, q_rows, kv_rows, size, left, right, sinks)
     partials = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
-    args = (qp, ldq, kp, vp, ldkv, None if first is None else _whole_ptr(first), None if lengths is None else _whole_ptr(lengths),
+    args = (q.data_ptr(), ldq, k.data_ptr(), v.data_ptr(), ldkv, None if first is None else _whole_ptr(first), None if lengths is None else _whole_ptr(lengths),
             None if mask is None else _whole_ptr(mask), ctx.data_ptr(), heads * size, size ** -0.5 if alpha is None else float(alpha),
             batch, heads, kv_heads, q_rows, kv_rows, size, left, right, sinks, partials.data_ptr() if floats else None, floats,
             _raw_stream(device))

@@ -99,12 +99,12 @@ def test_wrappers_refuse_host_tensors():
 
 
 def test_strided_heads_are_recognised():
-    from cubert_amd.kernels import _heads_ptr
+    from cubert_amd.kernels import _heads_pitch
     packed = torch.zeros(3, 5, 8, 64)
-    assert _heads_ptr(packed[:, :, 2:4], "k")[1] == 8 * 64
-    assert _heads_ptr(packed[:1, :, :4], "q")[1] == 8 * 64
-    assert _heads_ptr(packed[:, :1].contiguous()[:, :, 4:], "q")[1] == 8 * 64
+    assert _heads_pitch(packed[:, :, 2:4], "k") == 8 * 64
+    assert _heads_pitch(packed[:1, :, :4], "q") == 8 * 64
+    assert _heads_pitch(packed[:, :1].contiguous()[:, :, 4:], "q") == 8 * 64
     for wrong in (packed[:, :, ::2], packed[..., ::2], packed.transpose(1, 2), packed[:, 1:4], packed[::2],
                   packed[:, :1].expand(3, 5, 8, 64)):
         with pytest.raises(ValueError):
-            _heads_ptr(wrong, "k")
+            _heads_pitch(wrong, "k")

@@ -356,6 +356,8 @@ WIDE = {
     "wide window of one": (2, 129, 129, 49, 49, 0, 0, 0, None, None, "no"),
     "wide, 64 sequences": (64, 140, 150, 4, 2, 30, 0, 2, "end", tuple(150 - 2 * i for i in range(64)), "no"),
     "wide, 70 sequences": (70, 40, 60, 4, 4, 11, 3, 2, None, tuple(max(0, 60 - i) for i in range(70)), "no"),
+    "wide and masked from the middle on": (2, 300, 1500, 96, 96, 200, 0, 3, "end", (1500, 1200), "middle"),
+    "masked from the middle on": (2, 3, 3000, 4, 2, 700, 0, 3, "end", (3000, 1800), "middle"),
     "wide sinks alone": (5, 40, 900, 80, 20, 3, 0, 40, "end", (900, 100, 800, 40, 41), "no"),
 }
 ATTENTION.update(WIDE)
@@ -377,6 +379,8 @@ def attention_inputs(name, t, size, seed=0):
     elif masked == "holes":
         mask = (torch.rand(batch, kv_rows, generator=g, device="cuda") > 0.2).to(torch.int8) * 3
         mask[0, :kv_rows // 3] = 0
+    elif masked == "middle":                               # nothing kept in the last windows but the sinks
+        mask = (torch.arange(kv_rows, device="cuda") < torch.tensor([[kv_rows // 2], [kv_rows // 3]], device="cuda")).to(torch.int8)
     elif masked == "nothing":
         mask = torch.zeros(batch, kv_rows, dtype=torch.int8, device="cuda")
         mask[1, 20] = -1
@@ -445,6 +449,7 @@ def test_attention_window(K, name, t, size):
 
 
 @pytest.mark.parametrize("name", ["one query", "masked encoder", "piece", "few tokens", "long", "encoder", "nothing left", "wide encoder",
+                                  "wide and masked from the middle on", "masked from the middle on",
                                   "wide masked encoder", "wide piece", "wide and nothing left"])
 @pytest.mark.parametrize("t", ["f32", "f16"])
 @pytest.mark.parametrize("filler", [math.nan, math.inf])
