@@ -221,6 +221,86 @@ __device__ __forceinline__ void attend(Rows<T, D> &r, const unsigned char *k, co
     }
 }
 
+// At most 16 rows in fp32, whose matrix instructions take as long as four times the rows need: tiles of 16 x 16.  Lane l has row l % 16
+// and, of every 16 keys or columns, the four from 4 (l / 16) on.  (8 x 1 over 4096 keys of 128, 4 rows: 56 us with tiles of 32, 40 with
+// these; 32 x 1 over up to 4096 of 64, 1 row: 98 and 90, where the bytes take 78.)
+template <int D>
+struct FewRows {
+    v4f32 q[D / 16], ctx[D / 16];
+    float top, sum;
+
+    __device__ __forceinline__ void load(const float *row, int quarter, bool negate) {
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) {
+            q[s] = *reinterpret_cast<const v4f32 *>(row + 16 * s + 4 * quarter);
+            if (negate) q[s] = -q[s];
+            ctx[s] = v4f32{};
+        }
+        top = kNone, sum = 0.f;
+    }
+};
+
+__device__ __forceinline__ float quarters_max(float x) {
+    x = fmaxf(x, __shfl_xor(x, 16, kWave));
+    return fmaxf(x, __shfl_xor(x, 32, kWave));
+}
+
+// 32 keys, those with bits 0 in `visible` left out unless all of them are seen
+template <int D>
+__device__ __forceinline__ void attend_few(FewRows<D> &r, const unsigned char *k, const unsigned char *v, float scale, bool all,
+                                           unsigned visible, int lane) {
+    constexpr int kRowBytes = D * 4;
+    const int col = lane & 15, quarter = lane >> 4;
+    v4f32 s[2] = {};
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) {
+        v4f32 piece[2];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const int key = 16 * n + col;
+            piece[n] = *reinterpret_cast<const v4f32 *>(k + key * kRowBytes + k_piece<kRowBytes>(key, 4 * t + quarter) * 16);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) s[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(piece[n][e], r.q[t][e], s[n], 0, 0, 0);
+    }
+    products_done();
+    if (!all) {
+        const unsigned word = visible >> (4 * quarter);
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[n][i] = word >> (16 * n + i) & 1u ? s[n][i] : -INFINITY;
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, s[n][i]);
+    top *= scale;
+    if (__any(top > r.top + kSlack)) {
+        const float high = fmaxf(r.top, quarters_max(top)), shrink = __builtin_amdgcn_exp2f(r.top - high);
+        r.top = high;
+        r.sum *= shrink;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) r.ctx[d] *= shrink;
+    }
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            s[n][i] = __builtin_amdgcn_exp2f(fmaf(s[n][i], scale, -r.top));
+            r.sum += s[n][i];
+            const int key = 16 * n + 4 * quarter + i;
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+                const float a = *reinterpret_cast<const float *>(v + key * kRowBytes + v_piece<float, kRowBytes>(key, 4 * d + col / 4) * 16 + (col & 3) * 4);
+                r.ctx[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, s[n][i], r.ctx[d], 0, 0, 0);
+            }
+        }
+}
+
 __device__ __forceinline__ unsigned long long bits_below(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; }
 
 // The keys that queries at the positions low..high of a sequence see between them, and those that each of them sees.
@@ -780,18 +860,29 @@ struct Spread {
     static constexpr int kLds = 4 * kWaveBytes > kMergeBytes ? 4 * kWaveBytes : kMergeBytes;
 };
 
-// 32 rows per workgroup, whose four wavefronts take every fourth tile of 32 keys of this workgroup's piece of the axis; their
+// Few rows, 32 of them per workgroup, whose four wavefronts take every fourth tile of 32 keys of this workgroup's piece of the axis; their
 // sums meet in LDS, in wavefront order, and go out as results or, where the axis is cut, as sums for the kernel below.
+template <typename T, int D, bool FEW>
+struct SpreadRows {
+    typedef Rows<T, D> type;
+};
 template <typename T, int D>
-__global__ __launch_bounds__(kBlock, sizeof(T) * D == 512 ? 1 : 2) void attention_window_spread_kernel(WindowArgs a, int row_tiles, int pieces) {
+struct SpreadRows<T, D, true> {
+    typedef FewRows<D> type;
+};
+
+// FEW: at most 16 rows in fp32.
+template <typename T, int D, bool FEW>
+__global__ __launch_bounds__(kBlock, sizeof(T) * D == 512 && !FEW ? 1 : 2) void attention_window_spread_kernel(WindowArgs a, int row_tiles, int pieces) {
     typedef Spread<T, D> S;
+    constexpr int kRows = FEW ? 16 : 32;
     extern __shared__ __align__(16) unsigned char smem[];
     const int wave = wave_in_block(), lane = threadIdx.x & (kWave - 1);
     const int piece = blockIdx.x % pieces, tile_at = blockIdx.x / pieces;
     const int problem = tile_at / row_tiles, row0 = (tile_at - problem * row_tiles) * 32;
     const Problem at(a, problem / a.kv_heads, problem % a.kv_heads);
     const int share = a.heads / a.kv_heads, rows = a.q_rows * share;
-    const int row = row0 + (lane & 31), my_row = row < rows ? row : rows - 1;
+    const int row = row0 + (lane & (kRows - 1)), my_row = row < rows ? row : rows - 1;
     const int query = my_row / share, head = at.kv_head * share + my_row - query * share;
     const int p = at.first + query;
     const int begin = p > a.left ? p - a.left : 0, end = p < at.length - a.right ? p + a.right + 1 : at.length;
@@ -804,8 +895,8 @@ __global__ __launch_bounds__(kBlock, sizeof(T) * D == 512 ? 1 : 2) void attentio
     if (mask != nullptr && reach.any) reach.cut(kept_end(mask, reach.last_end, lane));
     const Tiles<32> tiles(reach, a.sinks);
 
-    Rows<T, D> r;
-    r.load((const T *) a.q + ((size_t) at.b * a.q_rows + query) * a.ldq + (size_t) head * D, lane >> 5, a.negate);
+    typename SpreadRows<T, D, FEW>::type r;
+    r.load((const T *) a.q + ((size_t) at.b * a.q_rows + query) * a.ldq + (size_t) head * D, lane / kRows, a.negate);
     unsigned char *buffers = smem + wave * S::kWaveBytes;
     // pieces of the axis: whole tiles, the first ones one more where they do not divide
     const int each = tiles.count / pieces, more = tiles.count - each * pieces;
@@ -851,7 +942,8 @@ __global__ __launch_bounds__(kBlock, sizeof(T) * D == 512 ? 1 : 2) void attentio
             const bool all = reach.all(base, 32, a.sinks) && (kept_bits & whole) == whole;
             const unsigned long long visible =
                     all ? ~0ull : bits_below(end - base) & (~bits_below(begin - base) | bits_below(a.sinks - base)) & kept_bits;
-            attend<T, D, 1, true>(r, kt, vt, a.scale, all, visible, lane);
+            if constexpr (FEW) attend_few<D>(r, kt, vt, a.scale, all, (unsigned) visible, lane);
+            else attend<T, D, 1, true>(r, kt, vt, a.scale, all, visible, lane);
         }
         if (S::kBuffers == 2) {
             buffer ^= 1;
@@ -870,14 +962,20 @@ __global__ __launch_bounds__(kBlock, sizeof(T) * D == 512 ? 1 : 2) void attentio
     products_done();
     __syncthreads();
     float *merge = reinterpret_cast<float *>(smem);
-    const float sum = r.sum + __shfl_xor(r.sum, 32, kWave);
-    float *to = merge + (wave * 32 + (lane & 31)) * S::kPitch;
+    float sum = r.sum + __shfl_xor(r.sum, 32, kWave);
+    float *to = merge + (wave * 32 + (lane & (kRows - 1))) * S::kPitch;
+    if constexpr (FEW) {
+        sum += __shfl_xor(sum, 16, kWave);
 #pragma unroll
-    for (int d = 0; d < D / 32; ++d)
+        for (int d = 0; d < D / 16; ++d) *reinterpret_cast<v4f32 *>(to + 16 * d + 4 * (lane >> 4)) = r.ctx[d];
+    } else {
 #pragma unroll
-        for (int i = 0; i < 16; i += 4)
-            *reinterpret_cast<v4f32 *>(to + 32 * d + 2 * i + 4 * (lane >> 5)) = v4f32{r.ctx[d][i], r.ctx[d][i + 1], r.ctx[d][i + 2], r.ctx[d][i + 3]};
-    if (lane < 32) to[D] = r.top, to[D + 1] = sum;
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<v4f32 *>(to + 32 * d + 2 * i + 4 * (lane >> 5)) = v4f32{r.ctx[d][i], r.ctx[d][i + 1], r.ctx[d][i + 2], r.ctx[d][i + 3]};
+    }
+    if (lane < kRows) to[D] = r.top, to[D + 1] = sum;
     __syncthreads();
     constexpr int kQuads = D / 4;  // a thread has four columns of a row
     for (int i = threadIdx.x; i < (last_row - row0 + 1) * kQuads; i += kBlock) {
@@ -996,9 +1094,6 @@ WindowPlan plan_window(bool half_precision, int batch, int heads, int kv_heads, 
     const long long of_128 = (rows + 127) / 128 * problems, of_64 = (rows + 63) / 64 * problems;
     const int enough = !half_precision ? 192 : head_size == 128 ? 256 : 96;
     plan.rows = rows <= 32 ? 32 : of_128 >= 320 ? 128 : of_64 >= enough ? 64 : 32;
-#ifdef PLAN
-    plan.rows = rows <= 32 ? 32 : PLAN;
-#endif
     plan.row_tiles = (int) ((rows + plan.rows - 1) / plan.rows);
     plan.pieces = 1, plan.floats = 0;
     if (plan.rows > 32) return plan;
@@ -1007,7 +1102,8 @@ WindowPlan plan_window(bool half_precision, int batch, int heads, int kv_heads, 
     if (left >= 0 && right >= 0) reach = (long long) left + right + 33 + sinks < reach ? (long long) left + right + 33 + sinks : reach;
     const long long tiles = (reach + 31) / 32, blocks = problems * plan.row_tiles;
     // About 384 workgroups, three for two units, with a tile to every wavefront at least.  Microseconds with 256 / 384 / 512 / 768:
-    // fp16, 48 tokens over up to 1000 keys 20 / 20 / 24 / 23, 2 x 100 over 6000 28 / 23 / 27 / 26, 32 over 4096 52 / 54 / 52 / 53.
+    // fp16, 48 tokens over up to 1000 keys 20 / 20 / 24 / 23, 2 x 100 over 6000 28 / 23 / 27 / 26, 32 over 4096 52 / 54 / 52 / 53.  (Pieces of 8
+    // tiles at least and of 4: fp32, 7 x 1 over 413 keys of 128 20 and 14 us, 12 x 1 over 396 15 and 12; fp16, 1 x 1 over 4096 both 12.)
     long long pieces = blocks > 0 ? (384 + blocks - 1) / blocks : 1;
     const long long most = (tiles + 3) / 4;
     pieces = pieces < most ? pieces : most;
@@ -1031,15 +1127,21 @@ int run_window_rows(const WindowArgs &a, int row_tiles, hipStream_t stream) {
     }
 }
 
+template <typename T, int D, bool FEW>
+int run_spread(const WindowArgs &a, WindowPlan plan, hipStream_t stream) {
+    static std::atomic<unsigned long long> done{0};
+    if (Spread<T, D>::kLds > 48 * 1024 && !allow_large_lds(attention_window_spread_kernel<T, D, FEW>, done)) return CUBERT_UNSUPPORTED;
+    return launch_lds(attention_window_spread_kernel<T, D, FEW>, dim3(a.batch * a.kv_heads * plan.row_tiles * plan.pieces), dim3(kBlock),
+                      Spread<T, D>::kLds, stream, a, plan.row_tiles, plan.pieces);
+}
+
 template <typename T, int D>
 int run_window(const WindowArgs &a, WindowPlan plan, hipStream_t stream) {
     const int problems = a.batch * a.kv_heads;
     if (plan.rows == 128) return run_window_rows<T, D, 128>(a, plan.row_tiles, stream);
     if (plan.rows == 64) return run_window_rows<T, D, 64>(a, plan.row_tiles, stream);
-    static std::atomic<unsigned long long> done{0};
-    if (Spread<T, D>::kLds > 48 * 1024 && !allow_large_lds(attention_window_spread_kernel<T, D>, done)) return CUBERT_UNSUPPORTED;
-    const int rc = launch_lds(attention_window_spread_kernel<T, D>, dim3(problems * plan.row_tiles * plan.pieces), dim3(kBlock),
-                              Spread<T, D>::kLds, stream, a, plan.row_tiles, plan.pieces);
+    const int rows = a.q_rows * (a.heads / a.kv_heads);
+    const int rc = sizeof(T) == 4 && rows <= 16 ? run_spread<T, D, sizeof(T) == 4>(a, plan, stream) : run_spread<T, D, false>(a, plan, stream);
     if (rc != 0 || plan.pieces == 1) return rc;
     const int total = problems * a.q_rows * (a.heads / a.kv_heads), per_block = kBlock / (D / 4);
     // (18612 rows of 2 pieces: 5 us so, 22 us with a workgroup per row; 512 rows of 8 pieces 6.6 and 4.7 us, 16 rows of 128 137 and 4.4)

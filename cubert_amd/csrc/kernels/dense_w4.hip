@@ -330,9 +330,6 @@ int run_dense_w4(const DenseArgs<X, T> &a, hipStream_t s) {
     const long long units = (long long) a.tiles * a.strips;
     if (units >= 1 << 22) return CUBERT_UNSUPPORTED;  // a launch holds less than 2^32 threads
     auto grid = [&](int ft) { return dim3((unsigned) (((a.tiles + ft - 1) / ft + 7) / 8 * 8 * a.strips)); };
-#ifdef VARIANT
-    VARIANT
-#endif
     if (units > 1024 || (units > 512 && a.tokens > 8)) return launch(dense_w4_kernel<X, T, EACH, 4, 8>, grid(4), dim3(8 * kWave), s, a);
     if (units > 256) return launch(dense_w4_kernel<X, T, EACH, 2, 8>, grid(2), dim3(8 * kWave), s, a);
     // (sixteen wavefronts, 4096 x 1024: 1 token 3.9 us against 4.4 with eight, 64 tokens 7.0 against 6.7)
