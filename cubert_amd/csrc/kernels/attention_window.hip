@@ -16,7 +16,7 @@ namespace cubert {
 namespace {
 
 constexpr int kMaxPieces = 128;  // of an axis that is cut
-constexpr int kFar = 1 << 30;  // a bound, position or length that no sequence reaches
+constexpr int kFar = (1 << 30) - 1;  // a bound, position or length that no sequence reaches
 
 struct WindowArgs {
     const void *q, *k, *v;
@@ -38,6 +38,7 @@ typedef _Float16 v4f16 __attribute__((ext_vector_type(4)));
 typedef _Float16 v2f16 __attribute__((ext_vector_type(2)));
 typedef float v4f32 __attribute__((ext_vector_type(4)));
 typedef float v2f32 __attribute__((ext_vector_type(2)));
+typedef int v4i32 __attribute__((ext_vector_type(4)));
 typedef float v16f32 __attribute__((ext_vector_type(16)));
 
 constexpr float kNone = -3e38f;  // the maximum of no scores: finite, so that differences to it are numbers
@@ -403,24 +404,39 @@ __device__ __forceinline__ void clear_rows(unsigned char *v, unsigned long long 
     __builtin_amdgcn_wave_barrier();
 }
 
-// The number of keys up to the last one below `end` that the mask keeps (padding is given as a mask, and is not to be computed).
+// A bound of the keys below `end` that the mask keeps (padding is given as a mask, and is not to be computed): behind the last one, or,
+// where that is far, up to 16 behind it.
 __device__ __forceinline__ int kept_end(const int8_t *mask, int end, int lane) {
-    while (end > 0) {
-        int byte[8];
+    int byte[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int j = end - 1 - (64 * i + lane);
-            byte[i] = mask[j > 0 ? j : 0];
-            byte[i] = j >= 0 ? byte[i] : 0;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const unsigned long long kept = __ballot(byte[i] != 0);
-            if (kept != 0) return end - 64 * i - __builtin_ctzll(kept);
-        }
-        end -= 512;
+    for (int i = 0; i < 8; ++i) {
+        const int j = end - 1 - (64 * i + lane);
+        byte[i] = mask[j > 0 ? j : 0];
+        byte[i] = j >= 0 ? byte[i] : 0;
     }
-    return 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const unsigned long long kept = __ballot(byte[i] != 0);
+        if (kept != 0) return end - 64 * i - __builtin_ctzll(kept);
+    }
+    if (end <= 512) return 0;
+    end -= 512;
+    end += -(int) (uintptr_t) (mask + end) & 15;  // to whole 16-byte pieces, with some bytes seen already
+    for (; end >= 16; end -= 4096) {
+        v4i32 piece[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int j = end - 16 * (64 * i + lane + 1);
+            piece[i] = j >= 0 ? *reinterpret_cast<const v4i32 *>(mask + j) : v4i32{};
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned long long kept = __ballot((piece[i][0] | piece[i][1] | piece[i][2] | piece[i][3]) != 0);
+            if (kept != 0) return end - 16 * (64 * i + __builtin_ctzll(kept));
+        }
+        if (end <= 4096) return end & 15;  // (bytes before the first whole piece)
+    }
+    return end;
 }
 
 struct Problem {
@@ -583,7 +599,7 @@ struct Strip {
                 }
         }
         if (row >= rows) return;
-        const float by = there && sum > 0.f ? 1.f / sum : 0.f;
+        const float by = there && sum != 0.f ? 1.f / sum : 0.f;  // (a sum that is no number stays none)
         T *ctx = (T *) a.ctx + ((size_t) at.b * a.q_rows + query) * a.ld_ctx + (size_t) head * D + 4 * half_wave;
 #pragma unroll
         for (int d = 0; d < D / 32; ++d)
@@ -998,9 +1014,9 @@ __global__ __launch_bounds__(kBlock, sizeof(T) * D == 512 && !FEW ? 1 : 2) void 
         if (pieces > 1) {
             float *out = a.partials + ((size_t) blockIdx.x * 32 + m) * S::kPitch;
             *reinterpret_cast<v4f32 *>(out + d) = out_there ? x : v4f32{};
-            if (d == 0) out[D] = top, out[D + 1] = out_there ? total : 0.f;
+            if (d == 0) out[D] = out_there ? top : kNone, out[D + 1] = out_there ? total : 0.f;
         } else {
-            const float by = out_there && total > 0.f ? 1.f / total : 0.f;
+            const float by = out_there && total != 0.f ? 1.f / total : 0.f;
             T *ctx = (T *) a.ctx + ((size_t) at.b * a.q_rows + out_query) * a.ld_ctx + (size_t) out_head * D + d;
             if (by != 0.f) store4(ctx, x[0] * by, x[1] * by, x[2] * by, x[3] * by);
             else store4(ctx, 0.f, 0.f, 0.f, 0.f);
@@ -1030,7 +1046,7 @@ __global__ __launch_bounds__(kBlock) void attention_window_join_few_kernel(Windo
     }
     const int query = row / share, head = kv_head * share + row - query * share;
     T *ctx = (T *) a.ctx + ((size_t) b * a.q_rows + query) * a.ld_ctx + (size_t) head * D + d;
-    const float by = sum > 0.f ? 1.f / sum : 0.f;
+    const float by = sum != 0.f ? 1.f / sum : 0.f;
     if (by != 0.f) store4(ctx, x[0] * by, x[1] * by, x[2] * by, x[3] * by);
     else store4(ctx, 0.f, 0.f, 0.f, 0.f);
 }
@@ -1073,7 +1089,7 @@ __global__ __launch_bounds__(kBlock) void attention_window_join_kernel(WindowArg
     for (int n = 1; n < kAtOnce; ++n) x += parts[n][thread];
     const int query = row / share, head = kv_head * share + row - query * share;
     T *ctx = (T *) a.ctx + ((size_t) b * a.q_rows + query) * a.ld_ctx + (size_t) head * D + d;
-    const float by = sum > 0.f ? 1.f / sum : 0.f;
+    const float by = sum != 0.f ? 1.f / sum : 0.f;
     if (by != 0.f) store4(ctx, x[0] * by, x[1] * by, x[2] * by, x[3] * by);
     else store4(ctx, 0.f, 0.f, 0.f, 0.f);
 }
@@ -1156,8 +1172,8 @@ template <typename T>
 int attention_window(const T *q, int ldq, const T *k, const T *v, int ldkv, const int *first, const int *lengths, const int8_t *mask,
                      T *ctx, int ld_ctx, float alpha, int batch, int heads, int kv_heads, int q_rows, int kv_rows, int head_size,
                      int left, int right, int sinks, float *partials, size_t partial_floats, void *stream) {
-    if (batch < 0 || heads < 1 || kv_heads < 1 ||
-        heads % kv_heads != 0 || !(alpha > -INFINITY && alpha < INFINITY) || q_rows < 0 || kv_rows < 0 || head_size < 1 || sinks < 0 || kv_rows > kFar || q_rows > kFar)
+    if (batch < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || !(alpha > -INFINITY && alpha < INFINITY) || q_rows < 0 ||
+        kv_rows < 0 || head_size < 1 || sinks < 0 || kv_rows > kFar || q_rows > kFar)
         return CUBERT_BAD_ARGUMENT;
     const long long width = (long long) heads * head_size, kv_width = (long long) kv_heads * head_size;
     if (ldq < width || ldkv < kv_width || ld_ctx < width) return CUBERT_BAD_ARGUMENT;
@@ -1169,8 +1185,9 @@ int attention_window(const T *q, int ldq, const T *k, const T *v, int ldkv, cons
         return CUBERT_UNSUPPORTED;
     if (ldkv > 1 << 22) return CUBERT_UNSUPPORTED;  // (pieces of a tile are addressed with 32 bits)
     if (head_size != 32 && head_size != 64 && head_size != 128) return CUBERT_UNSUPPORTED;
-    const unsigned long long rows = (unsigned long long) batch * q_rows * heads;
-    if (rows >= 1u << 24) return CUBERT_UNSUPPORTED;  // a launch holds less than 2^32 threads
+    // a launch holds less than 2^32 threads, and rows of a key head are counted in 32 bits
+    const unsigned long long problems = (unsigned long long) batch * kv_heads, rows = (unsigned long long) q_rows * (heads / kv_heads);
+    if (problems >= 1u << 24 || rows >= 1u << 30) return CUBERT_UNSUPPORTED;
     WindowArgs a;
     a.q = q, a.k = k, a.v = v, a.ctx = ctx, a.first = first, a.lengths = lengths, a.mask = mask;
     a.partials = partials;
@@ -1182,7 +1199,7 @@ int attention_window(const T *q, int ldq, const T *k, const T *v, int ldkv, cons
     a.left = left < 0 || left > kFar ? kFar : left, a.right = right < 0 || right > kFar ? kFar : right;
     a.sinks = sinks;
     WindowPlan plan = plan_window(sizeof(T) == 2, batch, heads, kv_heads, q_rows, kv_rows, head_size, left, right, sinks);
-    if ((unsigned long long) batch * kv_heads * plan.row_tiles * plan.pieces >= 1u << 24) return CUBERT_UNSUPPORTED;
+    if (problems * plan.row_tiles * plan.pieces >= 1u << 24) return CUBERT_UNSUPPORTED;
     if (plan.pieces > 1 && (partials == nullptr || partial_floats < plan.floats || !is_aligned(partials, 16))) plan.pieces = 1;
     if (head_size == 32) return run_window<T, 32>(a, plan, (hipStream_t) stream);
     if (head_size == 64) return run_window<T, 64>(a, plan, (hipStream_t) stream);
@@ -1199,6 +1216,7 @@ extern "C" {
 size_t cubert_attention_window_partials(int half_precision, int batch, int heads, int kv_heads, int q_rows, int kv_rows,
                                         int head_size, int left, int right, int sinks) {
     if (batch < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || q_rows < 1 || kv_rows < 1 || head_size < 1) return 0;
+    if ((long long) batch * kv_heads >= 1 << 24) return 0;  // refused
     return cubert::plan_window(half_precision != 0, batch, heads, kv_heads, q_rows, kv_rows, head_size, left, right, sinks).floats;
 }
 

@@ -24,8 +24,8 @@ constexpr int kBlockBytes = kTile * kColumns / 2;
 
 bool good_group(int group) { return group == 32 || group == 64 || group == 128; }
 
-__host__ __device__ inline size_t packed_blocks(int width) { return (width + kColumns - 1) / kColumns; }
-__host__ __device__ inline size_t packed_tiles(int features) { return (features + kTile - 1) / kTile; }
+__host__ __device__ inline size_t packed_blocks(int width) { return ((size_t) width + kColumns - 1) / kColumns; }
+__host__ __device__ inline size_t packed_tiles(int features) { return ((size_t) features + kTile - 1) / kTile; }
 
 // ---- preparing weights (once per model) -----------------------------------
 
@@ -328,8 +328,9 @@ __global__ __launch_bounds__(W * kWave) void dense_w4_kernel(DenseArgs<X, T> a) 
 template <typename X, typename T, int EACH>
 int run_dense_w4(const DenseArgs<X, T> &a, hipStream_t s) {
     const long long units = (long long) a.tiles * a.strips;
-    if (units >= 1 << 22) return CUBERT_UNSUPPORTED;  // a launch holds less than 2^32 threads
-    auto grid = [&](int ft) { return dim3((unsigned) (((a.tiles + ft - 1) / ft + 7) / 8 * 8 * a.strips)); };
+    auto groups = [&](int ft) { return ((long long) a.tiles + 8 * ft - 1) / (8 * ft) * 8 * a.strips; };
+    auto grid = [&](int ft) { return dim3((unsigned) groups(ft)); };
+    if (units > 1024 && groups(4) * 8 * kWave >= 1ll << 32) return CUBERT_UNSUPPORTED;  // (what a launch holds)
     if (units > 1024 || (units > 512 && a.tokens > 8)) return launch(dense_w4_kernel<X, T, EACH, 4, 8>, grid(4), dim3(8 * kWave), s, a);
     if (units > 256) return launch(dense_w4_kernel<X, T, EACH, 2, 8>, grid(2), dim3(8 * kWave), s, a);
     // (sixteen wavefronts, 4096 x 1024: 1 token 3.9 us against 4.4 with eight, 64 tokens 7.0 against 6.7)
@@ -348,7 +349,7 @@ int dense_w4(void *stream, int tokens, int features, int in, const X *x, int ldx
         return CUBERT_UNSUPPORTED;
     DenseArgs<X, T> a;
     a.tokens = tokens, a.features = features, a.steps = in / 32;
-    a.blocks = (int) packed_blocks(in), a.tiles = (int) packed_tiles(features), a.strips = (tokens + kTile - 1) / kTile;
+    a.blocks = (int) packed_blocks(in), a.tiles = (int) packed_tiles(features), a.strips = (int) (((long long) tokens + kTile - 1) / kTile);
     a.x = x, a.ldx = ldx, a.x_scales = x_scales;
     a.packed = (const v4u32 *) packed, a.scales = reinterpret_cast<const half_t *>(a.packed + (size_t) a.blocks * a.tiles * kWave);
     a.bias = bias, a.activation = activation, a.out = out, a.ldo = ldo;
@@ -386,6 +387,7 @@ int cubert_w4_quantize_f16(const cubert_half *w, int features, int in, int group
 size_t cubert_w4_packed_bytes(int features, int in, int group) {
     if (features < 1 || in < 1 || !cubert::good_group(group) || in % group != 0) return 0;
     const size_t blocks = cubert::packed_blocks(in) * cubert::packed_tiles(features);
+    if (blocks * (cubert::kBlockBytes / 4) >= (size_t) 1 << 31) return 0;
     return blocks * cubert::kBlockBytes + blocks * (cubert::kColumns / group) * cubert::kTile * sizeof(half_t);
 }
 

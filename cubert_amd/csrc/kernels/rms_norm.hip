@@ -18,7 +18,6 @@ namespace cubert {
 namespace {
 
 constexpr int kMaxHidden = 32768;
-constexpr int kMaxRows = 1 << 21;  // a launch holds less than 2^32 threads
 
 // WAVES wavefronts per row, ROWS rows to a workgroup; a lane has CHUNKS runs of VEC elements, WAVES * 64 runs apart.
 template <typename T, int VEC, int CHUNKS, int WAVES, int ROWS, bool CODES>
@@ -78,7 +77,7 @@ __global__ __launch_bounds__(WAVES * ROWS * kWave) void rms_norm_kernel(const T 
             if (CODES) top = fmaxf(top, traded[1][w]);
         }
     }
-    const float rstd = 1.f / sqrtf(squares / (float) hidden + eps);
+    const float power = squares / (float) hidden + eps, rstd = power == 0.f ? 0.f : 1.f / sqrtf(power);
     // A NaN is lost in a maximum and an infinity leaves no finite factor: such a row's scale is NaN and its codes are 0.
     const bool finite = squares < INFINITY;
     // 127 / m leaves fp32's range for m below 2^-121: rows that small are raised by a power of two first, which is exact.
@@ -109,7 +108,7 @@ template <typename T, bool CODES>
 int rms_norm(const T *x, const T *residual, const T *gamma, float eps, T *sum_out, T *out, int8_t *codes, float *scales, int rows,
              int hidden, void *stream) {
     if (rows < 0 || hidden < 1 || !(eps >= 0.f) || !(eps < INFINITY)) return CUBERT_BAD_ARGUMENT;
-    if (hidden > kMaxHidden || rows > kMaxRows) return CUBERT_UNSUPPORTED;
+    if (hidden > kMaxHidden) return CUBERT_UNSUPPORTED;
     if (rows == 0) return 0;
     if (x == nullptr || gamma == nullptr || (CODES ? codes == nullptr || scales == nullptr : out == nullptr)) return CUBERT_BAD_ARGUMENT;
     const hipStream_t s = (hipStream_t) stream;
@@ -117,15 +116,17 @@ int rms_norm(const T *x, const T *residual, const T *gamma, float eps, T *sum_ou
     const bool whole = hidden % kVec == 0 && is_aligned(x, 16) && is_aligned(gamma, 16) && (residual == nullptr || is_aligned(residual, 16)) &&
                        (sum_out == nullptr || is_aligned(sum_out, 16)) && (CODES ? is_aligned(codes, kVec) : is_aligned(out, 16));
 #define RUN(VEC, CHUNKS, WAVES, ROWS)                                                                                         \
-    if (hidden <= VEC * CHUNKS * WAVES * kWave)                                                                               \
-        return launch(rms_norm_kernel<T, VEC, CHUNKS, WAVES, ROWS, CODES>, dim3((rows + ROWS - 1) / ROWS), dim3(WAVES * ROWS * kWave), s, \
-                      x, residual, gamma, eps, sum_out, out, codes, scales, rows, hidden);
+    if (hidden <= VEC * CHUNKS * WAVES * kWave) {                                                                             \
+        if ((rows + (ROWS - 1ll)) / ROWS * (WAVES * ROWS * kWave) >= 1ll << 32) return CUBERT_UNSUPPORTED;                    \
+        return launch(rms_norm_kernel<T, VEC, CHUNKS, WAVES, ROWS, CODES>, dim3((rows + (ROWS - 1ll)) / ROWS),         \
+                      dim3(WAVES * ROWS * kWave), s, x, residual, gamma, eps, sum_out, out, codes, scales, rows, hidden);     \
+    }
     if (whole && rows >= 1024) {
         RUN(kVec, 1, 1, 4) RUN(kVec, 2, 1, 4) RUN(kVec, 4, 1, 4)
     }
     if (whole) {
         RUN(kVec, 1, 4, 1) RUN(kVec, 2, 4, 1) RUN(kVec, 1, 16, 1) RUN(kVec, 4, 16, 1)
-        if (sizeof(T) == 4) RUN(kVec, 8, 16, 1)
+        if constexpr (sizeof(T) == 4) RUN(kVec, 8, 16, 1)
     }
     RUN(1, 4, 4, 1) RUN(1, 4, 16, 1) RUN(1, 32, 16, 1)
 #undef RUN

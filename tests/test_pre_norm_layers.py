@@ -28,6 +28,9 @@ def test_rms_norm_refuses(L, t, codes):
     if codes:
         assert norm(L, t, codes, scales=None) == BAD_ARGUMENT
     assert norm(L, t, codes, hidden=32769) == UNSUPPORTED
+    assert norm(L, t, codes, rows=1 << 26) == UNSUPPORTED                  # more rows than a launch holds
+    assert norm(L, t, codes, rows=1 << 24, hidden=1) == UNSUPPORTED
+    assert norm(L, t, codes, rows=1 << 22, hidden=32768) == UNSUPPORTED
     assert norm(L, t, codes, rows=0, x=None, out=None) == 0
 
 
@@ -45,6 +48,8 @@ def test_dense_w4_refuses(L, name):
     for other in (dict(group=16), dict(group=96), dict(width=96, group=64), dict(x=P + 8), dict(ldx=258), dict(packed=P + 4)):
         assert dense(L, name, **other) == UNSUPPORTED, other
     assert dense(L, name, tokens=0, x=None, out=None) == 0
+    assert dense(L, name, tokens=(1 << 31) - 1) == UNSUPPORTED             # more than a launch holds
+    assert dense(L, name, tokens=1 << 24, features=(1 << 31) - 1) == UNSUPPORTED
 
 
 def test_w4_sizes_and_refusals(L):
@@ -53,7 +58,7 @@ def test_w4_sizes_and_refusals(L):
     assert L.cubert_w4_packed_bytes(17, 160, 32) == 4 * (1024 + 4 * 32)
     assert L.cubert_w4_packed_bytes(1, 64, 64) == 1024 + 2 * 32
     assert L.cubert_w4_packed_bytes(32768, 65536, 128) == 2048 * 512 * (1024 + 32)
-    for sizes in ((0, 128, 128), (16, 0, 128), (16, 128, 16), (16, 96, 64)):
+    for sizes in ((0, 128, 128), (16, 0, 128), (16, 128, 16), (16, 96, 64), ((1 << 31) - 1, 1 << 20, 128)):
         assert L.cubert_w4_packed_bytes(*sizes) == 0
     for t in ("f32", "f16"):
         quantize = getattr(L, "cubert_w4_quantize_" + t)
@@ -64,26 +69,45 @@ def test_w4_sizes_and_refusals(L):
     assert L.cubert_w4_pack(P, None, 16, 128, 64, P, None) == BAD_ARGUMENT
     assert L.cubert_w4_pack(P, P, 16, 128, 48, P, None) == UNSUPPORTED
     assert L.cubert_w4_pack(P, P, 16, 128, 64, P + 8, None) == UNSUPPORTED
+    assert L.cubert_w4_pack(P, P, (1 << 31) - 1, 1 << 20, 64, P, None) == UNSUPPORTED
 
 
 def attention(L, t, q=P, ldq=None, k=P, v=P, ldkv=None, ctx=P, ld_ctx=None, batch=2, heads=4, kv_heads=2, q_rows=3, kv_rows=50, size=64,
-              left=-1, right=0, sinks=0):
+              left=-1, right=0, sinks=0, alpha=1.0):
     return getattr(L, "cubert_attention_window_" + t)(
         q, heads * size if ldq is None else ldq, k, v, kv_heads * size if ldkv is None else ldkv, None, None, None, ctx,
-        heads * size if ld_ctx is None else ld_ctx, 1.0, batch, heads, kv_heads, q_rows, kv_rows, size, left, right, sinks, None, 0, None)
+        heads * size if ld_ctx is None else ld_ctx, alpha, batch, heads, kv_heads, q_rows, kv_rows, size, left, right, sinks, None, 0, None)
 
 
 @pytest.mark.parametrize("t", ["f32", "f16"])
 def test_attention_window_refuses(L, t):
     for wrong in (dict(q=None), dict(k=None), dict(v=None), dict(ctx=None), dict(batch=-1), dict(heads=0), dict(kv_heads=0), dict(kv_heads=3),
                   dict(q_rows=-1), dict(kv_rows=-1), dict(size=0), dict(sinks=-1), dict(ldq=255), dict(ldkv=127), dict(ld_ctx=255),
-                  dict(kv_rows=(1 << 30) + 1)):
+                  dict(kv_rows=1 << 30), dict(q_rows=1 << 30), dict(alpha=float("nan")), dict(alpha=float("inf")), dict(alpha=float("-inf"))):
         assert attention(L, t, **wrong) == BAD_ARGUMENT, wrong
     for other in (dict(size=48), dict(size=256), dict(q=P + 8), dict(k=P + 8), dict(v=P + 8), dict(ctx=P + 8), dict(ldq=258), dict(ldkv=130),
-                  dict(ld_ctx=258)):
+                  dict(ld_ctx=258), dict(ldkv=(1 << 22) + 64), dict(batch=1 << 23), dict(batch=(1 << 31) - 1, kv_heads=4),
+                  dict(q_rows=(1 << 30) - 1, heads=4, kv_heads=1), dict(batch=1 << 20, q_rows=1 << 20)):
         assert attention(L, t, **other) == UNSUPPORTED, other
     assert attention(L, t, batch=0, q=None) == 0
     assert attention(L, t, q_rows=0, q=None) == 0
+
+
+def test_attention_window_partials(L):
+    """Floats for 32 rows of head size + 4 per piece of the axis, and none where nothing is cut."""
+    for half in (0, 1):
+        def floats(batch, heads, kv_heads, q_rows, kv_rows, size, left=-1, right=0, sinks=0):
+            return L.cubert_attention_window_partials(half, batch, heads, kv_heads, q_rows, kv_rows, size, left, right, sinks)
+        assert floats(1, 16, 2, 1, 131072, 128) == 2 * 128 * 32 * 132
+        assert floats(4, 8, 4, 1, 2048, 64) == 16 * 16 * 32 * 68       # 64 tiles of 32 keys, four of them to a piece
+        assert floats(4, 8, 4, 1, 8192, 64, left=95) == 0              # 128 keys are one piece
+        assert floats(4, 8, 4, 1, 8192, 64, left=96) == 16 * 2 * 32 * 68
+        assert floats(1, 4, 4, 1, 128, 64) == 0
+        assert floats(512, 12, 12, 1, 4096, 64) == 0
+        assert floats(8, 12, 12, 512, 512, 64) == 0
+        for nothing in ((0, 4, 2, 1, 50, 64), (1, 4, 3, 1, 50, 64), (1, 4, 0, 1, 50, 64), (1, 4, 2, 0, 50, 64), (1, 4, 2, 1, 0, 64),
+                        (1, 4, 2, 1, 50, 0), (1 << 30, 1 << 20, 1 << 20, 1, 5000, 64)):
+            assert floats(*nothing) == 0
 
 
 def test_wrappers_refuse_host_tensors():

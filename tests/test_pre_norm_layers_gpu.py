@@ -123,6 +123,11 @@ def test_rms_norm_of_rows_without_a_norm(K, t, hidden):
     assert (codes[4:] == 127).all()
     assert abs(float(scales[5]) * 127 - 1) < 1e-5
     assert (out[5].float() - 1).abs().max() < 1e-3
+    # a row of zeros has no direction: its norm is zero, whatever is added below the root
+    codes, scales, _ = K.res_rms_norm_i8(x, None, gamma, 0.0)
+    out, _ = K.res_rms_norm(x, None, gamma, 0.0)
+    assert bool((codes[0] == 0).all()) and float(scales[0]) == 0 and bool((out[0] == 0).all())
+    assert bool(torch.isnan(out[1]).all()) and math.isnan(scales[1])
 
 
 def test_rms_norm_in_place(K):
@@ -485,6 +490,89 @@ def test_attention_window_of_large_scores(K, t):
     assert bool(torch.isfinite(got).all())
     want, bound = attention_reference(q, k, v, **at)
     within(got, want, bound, "large")
+
+
+@pytest.mark.parametrize("name", ["one query", "few tokens", "long", "long window", "piece", "masked encoder", "wide piece", "wide masked encoder",
+                                  "wide causal", "causal", "encoder"])
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("where", ["q", "k"])
+def test_attention_window_of_no_number(K, name, t, where):
+    """What is no number in a query or a key makes none of the results that take it, and of no others."""
+    q, k, v, at = attention_inputs(name, TYPES[t], 64)
+    want, bound = attention_reference(q, k, v, **at)
+    seen, share = visible(q, k, **at)[:, 0], q.shape[2] // k.shape[2]      # [batch, q_rows, kv_rows]
+    b, i = (int(x) for x in seen.any(2).nonzero()[seen.any(2).sum() // 2])
+    bad = torch.zeros(q.shape[:3], dtype=torch.bool, device="cuda")
+    if where == "q":
+        q = q.clone()
+        q[b, i, 1, 5] = math.nan
+        bad[b, i, 1] = True
+    else:
+        j = int(seen[b, i].nonzero()[0])
+        k = k.clone()
+        k[b, j, 0, 63] = math.nan
+        bad[b, :, :share] = seen[b, :, j, None]
+    got = K.attention_window(q, k, v, **at)
+    assert bool(torch.isnan(got[bad]).all())
+    within(torch.where(bad[..., None], 0, got), torch.where(bad[..., None], 0.0, want), bound, name)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("q_rows,heads", [(1, 2), (3, 8), (50, 60)])
+@pytest.mark.parametrize("kv_rows", [9001, 8992, 4624])
+def test_attention_window_of_long_padding(K, t, q_rows, heads, kv_rows):
+    """Masks that keep nothing from some key on, near and far from the end, at any address: the same as shorter sequences."""
+    ends = (0, 1, 15, 500, 513, 528, 4090, 4113, 4624)
+    g, t = gen(12), TYPES[t]
+    q = normal(g, len(ends), q_rows, heads, 32).to(t)
+    k, v = (normal(g, len(ends), kv_rows, 2, 32).to(t) for _ in "kv")
+    mask = (torch.arange(kv_rows, device="cuda") < torch.tensor(ends, device="cuda")[:, None]).to(torch.int8)
+    at = dict(left=-1, right=-1, sinks=0, first=None, lengths=None, mask=mask)
+    got = K.attention_window(q, k, v, **at)
+    cut = slice(0, max(ends))
+    at["mask"] = mask[:, cut].contiguous()
+    for i in range(0, heads, heads // 2):                  # (a head of each key head at a time: the reference is large)
+        h = slice(i, i + 1)
+        kv = slice(2 * i // heads, 2 * i // heads + 1)
+        want, bound = attention_reference(q[:, :, h], k[:, cut, kv], v[:, cut, kv], **at)
+        within(got[:, :, h], want, bound, "head %d" % i)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+def test_attention_window_without_scores(K, t):
+    """A scale of 0: the mean of what is seen."""
+    for name in ("few tokens", "one query", "masked encoder", "wide masked encoder", "long"):
+        q, k, v, at = attention_inputs(name, TYPES[t], 64)
+        want, bound = attention_reference(q, k, v, alpha=0.0, **at)
+        within(K.attention_window(q, k, v, alpha=0.0, **at), want, bound, name)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+def test_attention_window_in_two_graphs(K, t):
+    """Calls over a cut axis, two captured and one eager, each with its own partial sums, in turns."""
+    calls = [attention_inputs("long", TYPES[t], size, seed) for size, seed in ((64, 1), (64, 2), (128, 3))]
+    for q, k, v, at in calls:
+        K.attention_window(q, k, v, **at)
+    torch.cuda.synchronize()
+    graphs = []
+    for q, k, v, at in calls[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = K.attention_window(q, k, v, **at)
+        graphs.append((graph, out))
+    for turn in range(4):
+        for q, k, v, at in calls:
+            q.copy_(normal(gen(70 + turn), *q.shape))
+        for graph, _ in graphs:
+            graph.replay()
+        eager = K.attention_window(*calls[2][:3], **calls[2][3])
+        graphs[0][0].replay()
+        got = [out.clone() for _, out in graphs] + [eager]
+        torch.cuda.synchronize()
+        for out, (q, k, v, at) in zip(got, calls):
+            assert torch.equal(out, K.attention_window(q, k, v, **at))
+            want, bound = attention_reference(q, k, v, **at)
+            within(out, want, bound, "turn %d" % turn)
 
 
 def test_attention_window_cut_and_uncut(K):
