@@ -228,8 +228,9 @@ int cubert_transpose_f16(const cubert_half *in, int rows, int cols, cubert_half 
 /* residual + root-mean-square norm (beside cubert_bias_res_ln_*):
  *   s = in[r] + residual[r];   out[r] = gamma * s / sqrt(mean(s^2) + eps)
  * `residual` may be NULL (s = in[r]).  s goes to sum_out, rounded to the storage type, as the residual of the next layer
- * (NULL = not wanted); sum_out may be `in` or `residual` itself, `out` may be neither of the three.  The norm is taken of the unrounded fp32 s, whose
- * squares have to stay within fp32's range.  hidden up to 32768 (more: CUBERT_UNSUPPORTED), eps >= 0. */
+ * (NULL = not wanted); sum_out may be `in` or `residual` itself, `out` may be none of the three.  The norm is taken of the
+ * unrounded fp32 s, whose squares have to stay within fp32's range; a row of zeros gives zeros for any eps >= 0.  hidden up to
+ * 32768 and as many rows as a launch holds, 2^21 at least (more: CUBERT_UNSUPPORTED). */
 int cubert_res_rms_norm_f32(const float *in, const float *residual, const float *gamma, float eps, float *sum_out, float *out,
                             int rows, int hidden, void *stream);
 int cubert_res_rms_norm_f16(const cubert_half *in, const cubert_half *residual, const cubert_half *gamma, float eps,
@@ -263,8 +264,9 @@ int cubert_w4_pack(const uint8_t *codes, const cubert_half *scales, int features
 /* A Dense layer on such weights (beside cubert_gemm_skinny_* and cubert_dense_*):
  *   out[t, f] = act(sum_k x[t, k] w[f, k] + bias[f]),  act = identity (0) or the erf-form GELU (1)
  * with fp32 sums and no rounding of a weight.  x [tokens, in] at ldx elements per row, 16-byte aligned with rows of whole
- * 16-byte pieces (otherwise CUBERT_UNSUPPORTED); `bias` may be NULL; out rows are ldo apart.  The _i8_ forms take rows of 8
- * bits and a scale per row, x[t, k] * x_scales[t].  Any number of tokens is right, few (up to 64) are what it is made for.
+ * 16-byte pieces (otherwise CUBERT_UNSUPPORTED); `bias` may be NULL; out rows are ldo apart and overlap nothing that is read.
+ * The _i8_ forms take rows of 8 bits and a scale per row, x[t, k] * x_scales[t].  Any number of tokens that a launch holds is
+ * right (2^17 of them with 32768 features are), few (up to 64) are what it is made for: 16 at a time read the weights.
  * Asynchronous on `stream`; needs no handle and no workspace, and the same call gives the same bits. */
 int cubert_dense_w4_f32(void *stream, int tokens, int features, int in, const float *x, int ldx, const void *packed, int group,
                         const float *bias, int activation, float *out, int ldo);
@@ -285,8 +287,12 @@ int cubert_dense_w4_i8_f16(void *stream, int tokens, int features, int in, const
  * q is [batch * q_rows, heads * head_size] at ldq elements per row, k and v [batch * kv_rows, kv_heads * head_size] at ldkv
  * (kv_rows: the rows a sequence has in the cache, whatever its length), ctx like q at ld_ctx.  `first` (NULL: 0) and
  * `lengths` (NULL: kv_rows; larger ones count as kv_rows) are device arrays of `batch` ints, `mask` (NULL: all kept) is
- * int8 [batch, kv_rows].  K and V behind a sequence's length, and where the mask is 0, may hold anything.  A negative left or right is no bound; a right of 0 is causal.
- * head_size 32, 64 or 128, pointers and rows of whole 16-byte pieces; otherwise CUBERT_UNSUPPORTED.
+ * int8 [batch, kv_rows].  A negative left or right is no bound; a right of 0 is causal.  alpha is finite.
+ * K and V that no query of a sequence sees may hold anything: behind its length, where the mask is 0, outside all windows.  A V that is
+ * not finite and that some queries see may make other queries of the same call, which do not see it, NaN as well; a Q or K that is
+ * not a number reaches the results of that query or of those that see the key, and no others.
+ * head_size 32, 64 or 128, pointers and rows of whole 16-byte pieces, ldkv up to 2^22, and fewer than 2^24 workgroups of at least 32 rows
+ * (q_rows * heads / kv_heads of every sequence and key head); otherwise CUBERT_UNSUPPORTED.  ctx overlaps nothing that is read.
  * Few rows over a long axis are cut along it, into `partials`: cubert_attention_window_partials floats of device memory,
  * 16-byte aligned, that no other call uses before this one is done.  With less (or NULL) the same call runs uncut. */
 size_t cubert_attention_window_partials(int half_precision, int batch, int heads, int kv_heads, int q_rows, int kv_rows,
