@@ -468,8 +468,8 @@ struct Place {
     // `count` things, those of a die consecutive: the number of the die's first one
     __device__ __forceinline__ static int before(int count, int die) { return die * (count / 8) + (die < count % 8 ? die : count % 8); }
 
-    __device__ __forceinline__ Place(const WindowArgs &a, int share, int rows, int row_tiles, int lane) {
-        const int die = blockIdx.x % 8, on_die = blockIdx.x / 8, total = a.batch * a.kv_heads * row_tiles;
+    __device__ __forceinline__ Place(const WindowArgs &a, int share, int rows, int row_tiles, int block, int lane) {
+        const int die = block % 8, on_die = block / 8, total = a.batch * a.kv_heads * row_tiles;
         if ((a.lengths == nullptr && a.first == nullptr) || a.batch > kWave) {
             const int i = before(total, die) + on_die, problem = i / row_tiles;
             tile = i - problem * row_tiles, b = problem / a.kv_heads, kv_head = problem - b * a.kv_heads;
@@ -512,17 +512,20 @@ struct Strip {
     static constexpr int kRowGroups = ROWS / 32, kParts = 4 / kRowGroups;
     const WindowArgs &a;
     int share, rows, row0, row, query, head, begin, end;  // this wavefront's first row; a lane's, its query and head, the bounds of its window
+    int pieces, piece;  // of the axis, and which one this is
     Place place;
     Problem at;
     bool there;
     Reach reach, mine;  // of the workgroup's rows, and of this wavefront's
     const int8_t *mask;
     Tiles<KEYS> tiles;
+    int low, high;  // the piece's tiles
     const T *k, *v;
 
     __device__ __forceinline__ static int last_of(int row, int count, int rows) { return (row + count < rows ? row + count : rows) - 1; }
-    __device__ __forceinline__ Strip(const WindowArgs &args, int row_tiles, int wave, int lane)
-        : a(args), share(a.heads / a.kv_heads), rows(a.q_rows * share), row0(0), place(a, share, ROWS, row_tiles, lane),
+    __device__ __forceinline__ Strip(const WindowArgs &args, int row_tiles, int pieces_, int wave, int lane)
+        : a(args), share(a.heads / a.kv_heads), rows(a.q_rows * share), row0(0), pieces(pieces_), piece(pieces == 1 ? 0 : blockIdx.x * pieces / gridDim.x),
+          place(a, share, ROWS, row_tiles, blockIdx.x - piece * (gridDim.x / pieces), lane),
           at(a, place.b, place.kv_head), reach(a, at.first + place.tile * ROWS / share, at.first + last_of(place.tile * ROWS, ROWS, rows) / share, at.length),
           mine(a, at.first + (place.tile * ROWS + 32 * (wave % kRowGroups)) / share,
                at.first + last_of(place.tile * ROWS + 32 * (wave % kRowGroups), 32, rows) / share, at.length),
@@ -536,6 +539,11 @@ struct Strip {
         begin = p > a.left ? p - a.left : 0, end = p < at.length - a.right ? p + a.right + 1 : at.length;
         k = (const T *) a.k + (size_t) at.b * a.kv_rows * a.ldkv + at.kv_head * D;
         v = (const T *) a.v + (size_t) at.b * a.kv_rows * a.ldkv + at.kv_head * D;
+        low = 0, high = tiles.count;
+        if (pieces > 1) {
+            const int each = tiles.count / pieces, more = tiles.count - each * pieces;
+            low = piece * each + (piece < more ? piece : more), high = low + each + (piece < more ? 1 : 0);
+        }
     }
     __device__ __forceinline__ const Reach &cut_to_mask(int lane) {
         if (mask != nullptr && reach.any) {
@@ -550,7 +558,7 @@ struct Strip {
     __device__ __forceinline__ unsigned long long visible(int base, unsigned long long kept) const {
         return bits_below(end - base) & (~bits_below(begin - base) | bits_below(a.sinks - base)) & kept;
     }
-    // take(tile, busy) for every tile of the workgroup's, in order.  This wavefront's are those of the sinks (which reach into the
+    // take(tile, busy) for every tile of the workgroup's piece, in order.  This wavefront's are those of the sinks (which reach into the
     // window's where there is no gap between them) and a run among those of the window.  (Tiles passed over by loops of their own:
     // a branch around the work has the compiler copy every accumulator.)
     template <typename Take>
@@ -558,13 +566,14 @@ struct Strip {
         const int my_sinks = a.sinks < mine.last_end ? a.sinks : mine.last_end, sinks_end = mine.any && my_sinks > 0 ? (my_sinks + KEYS - 1) / KEYS : 0;
         int from = mine.any ? tiles.of_sinks + mine.first_begin / KEYS - tiles.first : tiles.count;
         int until = mine.any ? tiles.of_sinks + (mine.last_end + KEYS - 1) / KEYS - tiles.first : tiles.count;
-        from = from < tiles.count ? from : tiles.count, until = until < tiles.count ? until : tiles.count;
-        int tile = 0;
+        from = from < high ? from : high, until = until < high ? until : high;
+        const int sinks_until = sinks_end < high ? sinks_end : high;
+        int tile = low;
         for (int part = 0; part < 2; ++part) {
-            for (; tile < (part == 0 ? 0 : from); ++tile) take(tile, false);
-            for (; tile < (part == 0 ? sinks_end : until); ++tile) take(tile, true);
+            for (; tile < (part == 0 ? low : from); ++tile) take(tile, false);
+            for (; tile < (part == 0 ? sinks_until : until); ++tile) take(tile, true);
         }
-        for (; tile < tiles.count; ++tile) take(tile, false);
+        for (; tile < high; ++tile) take(tile, false);
     }
     // The rows' results: sums relative to their maxima, of all parts of the tiles, which meet in LDS (`traded`, kTraded bytes) in order.
     static constexpr int kPitch = D + 4, kTraded = (kParts - 1) * ROWS * kPitch * 4;
@@ -588,7 +597,7 @@ struct Strip {
             if (wave >= kRowGroups) return;
             const float other = with[D], high = fmaxf(top, other);
             const float mine_by = __builtin_amdgcn_exp2f(top - high), other_by = __builtin_amdgcn_exp2f(other - high);
-            sum = sum * mine_by + with[D + 1] * other_by;
+            sum = sum * mine_by + with[D + 1] * other_by, top = high;
 #pragma unroll
             for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -599,6 +608,18 @@ struct Strip {
                 }
         }
         if (row >= rows) return;
+        if (pieces > 1) {
+            const size_t tile32 = (size_t) (at.b * a.kv_heads + at.kv_head) * ((rows + ROWS - 1) / ROWS * kRowGroups) + row0 / 32;
+            float *out = a.partials + ((tile32 * pieces + piece) * 32 + (lane & 31)) * kPitch;
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4)
+                    *reinterpret_cast<v4f32 *>(out + 32 * d + 2 * i + 4 * half_wave) =
+                            there ? v4f32{sums[d][i], sums[d][i + 1], sums[d][i + 2], sums[d][i + 3]} : v4f32{};
+            if (half_wave == 0) out[D] = there ? top : kNone, out[D + 1] = there ? sum : 0.f;
+            return;
+        }
         const float by = there && sum != 0.f ? 1.f / sum : 0.f;  // (a sum that is no number stays none)
         T *ctx = (T *) a.ctx + ((size_t) at.b * a.q_rows + query) * a.ld_ctx + (size_t) head * D + 4 * half_wave;
 #pragma unroll
@@ -621,7 +642,7 @@ __global__ __launch_bounds__(kBlock) void attention_window_shared_kernel(WindowA
     extern __shared__ __align__(16) unsigned char smem[];  // two buffers of K and V
     static_assert(4 * kTileBytes >= Work::kTraded, "room for what is traded");
     const int wave = wave_in_block(), lane = threadIdx.x & (kWave - 1), part = wave / Work::kRowGroups;
-    const Work strip(a, row_tiles, wave, lane);
+    const Work strip(a, row_tiles, 1, wave, lane);  // (an axis in one piece)
     const unsigned pitch = (unsigned) a.ldkv * sizeof(T), lds = lds_address(smem);
     const Bring<T, D, kKeys, 4, false> bring_k(wave, lane, pitch);
     const Bring<T, D, kKeys, 4, true> bring_v(wave, lane, pitch);
@@ -631,9 +652,9 @@ __global__ __launch_bounds__(kBlock) void attention_window_shared_kernel(WindowA
         bring_v(strip.v, strip.tiles.base(tile), a.kv_rows, pitch, to + kTileBytes, wave, lane);
     };
     int kept = 1;
-    if (strip.tiles.count > 0) {
-        bring(0, 0);
-        kept = strip.mask_byte(strip.tiles.base(0) + 64 * part + lane);
+    if (strip.low < strip.high) {
+        bring(strip.low, strip.low & 1);
+        kept = strip.mask_byte(strip.tiles.base(strip.low) + 64 * part + lane);
     }
     Rows<T, D> r;
     r.load(strip.q(), lane >> 5, a.negate);
@@ -642,7 +663,7 @@ __global__ __launch_bounds__(kBlock) void attention_window_shared_kernel(WindowA
         landed();
         const unsigned long long kept_bits = strip.mask != nullptr ? __ballot(kept != 0) : ~0ull;
         __syncthreads();  // everybody's; and nobody reads the other buffer any more
-        if (tile + 1 < strip.tiles.count) {
+        if (tile + 1 < strip.high) {
             bring(tile + 1, (tile + 1) & 1);
             kept = strip.mask_byte(strip.tiles.base(tile + 1) + 64 * part + lane);
         }
@@ -708,7 +729,7 @@ __device__ __forceinline__ v16f32 multiply_term(int m, const v8bf16 (&a)[3], con
 
 // As above; a wavefront has 32 keys of a tile with its 32 rows: ROWS = 128, the same ones for all, 64, either half of 64.
 template <int D, int ROWS>
-__global__ __launch_bounds__(kBlock, D == 128 ? 1 : 2) void attention_window_terms_kernel(WindowArgs a, int row_tiles) {
+__global__ __launch_bounds__(kBlock, D == 128 ? 1 : 2) void attention_window_terms_kernel(WindowArgs a, int row_tiles, int pieces) {
     constexpr int kKeys = 32 * 128 / ROWS, kRowBytes = 2 * D, kPlane = kKeys * kRowBytes, kQuads = D / 4, kMine = kKeys * kQuads / kBlock;
     typedef Strip<float, D, kKeys, ROWS> Work;
     extern __shared__ __align__(16) unsigned char smem[];
@@ -716,7 +737,7 @@ __global__ __launch_bounds__(kBlock, D == 128 ? 1 : 2) void attention_window_ter
     unsigned char *planes = smem;  // of K, then of V
     const int wave = wave_in_block(), lane = threadIdx.x & (kWave - 1), col = lane & 31, half_wave = lane >> 5;
     const int part = wave / Work::kRowGroups;
-    const Work strip(a, row_tiles, wave, lane);
+    const Work strip(a, row_tiles, pieces, wave, lane);
     // a thread's pieces of a tile: 16 bytes of `kMine` rows of K and of V
     v4f32 next[2][kMine];
     const unsigned pitch = (unsigned) a.ldkv * 4u;
@@ -739,9 +760,9 @@ __global__ __launch_bounds__(kBlock, D == 128 ? 1 : 2) void attention_window_ter
         }
     };
     int kept = 1;
-    if (strip.tiles.count > 0) {
-        bring(0);
-        kept = strip.mask_byte(strip.tiles.base(0) + lane);
+    if (strip.low < strip.high) {
+        bring(strip.low);
+        kept = strip.mask_byte(strip.tiles.base(strip.low) + lane);
     }
     Terms q[D / 16];
     {
@@ -782,7 +803,7 @@ __global__ __launch_bounds__(kBlock, D == 128 ? 1 : 2) void attention_window_ter
                     for (int e = 0; e < 4; ++e) x[e] = rest(x[e]);
                 }
             }
-        if (tile + 1 < strip.tiles.count) {
+        if (tile + 1 < strip.high) {
             bring(tile + 1);
             kept = strip.mask_byte(strip.tiles.base(tile + 1) + lane);
         }
@@ -1102,40 +1123,47 @@ struct WindowPlan {
 
 // The rule, measured on heads of 64 with 128 / 64 / 32 rows, microseconds.  fp16: 4 x 4096 tokens of 16 heads, window 512 (2048 workgroups of
 // 128) 78 / 106 / 164; 32 x 128 of 12 (384) 13 / 17 / 19; 2 x 4096 of 4 (256) 59 / 41 / 71; 3 x 517 of 12 (180) 24 / 23 / 26; 1 x 600
-// (60) 15 / 11 / 15; 1 x 64 over 1000 (12) 19 / 13 / 12.  fp32: 2 x 2000 of 16 (512) 195 / 231 / 301; 3 x 517 (180) 55 / 47 / 54; 1 x 600
-// (60) 46 / 31 / 26.  Heads of 128, 2 x 400 over 6000 in fp16 (104): 131 / 91 / 74.
+// (60) 15 / 11 / 15; 1 x 64 over 1000 (12) 19 / 13 / 12.  Heads of 128, 2 x 400 over 6000 (104): 131 / 91 / 74.  fp32: 2 x 2000 of 16 (512)
+// 184 / 216 / 300; 3 x 517 (180) 46 / 40 / 54; 2 x 400 (168 of 64) - / 22 / 31; 1 x 64 over 1000 (12) - / 19 / 13.
 WindowPlan plan_window(bool half_precision, int batch, int heads, int kv_heads, int q_rows, int kv_rows, int head_size, int left, int right, int sinks) {
     WindowPlan plan;
     const long long rows = (long long) q_rows * (heads / kv_heads), problems = (long long) batch * kv_heads;
     const long long of_128 = (rows + 127) / 128 * problems, of_64 = (rows + 63) / 64 * problems;
-    const int enough = !half_precision ? 192 : head_size == 128 ? 256 : 96;
+    const int enough = !half_precision ? 16 : head_size == 128 ? 256 : 96;
     plan.rows = rows <= 32 ? 32 : of_128 >= 320 ? 128 : of_64 >= enough ? 64 : 32;
     plan.row_tiles = (int) ((rows + plan.rows - 1) / plan.rows);
     plan.pieces = 1, plan.floats = 0;
-    if (plan.rows > 32) return plan;
-    // the most keys that 32 rows reach
+    // the most tiles of 32 keys that a workgroup's rows reach
     long long reach = kv_rows;
-    if (left >= 0 && right >= 0) reach = (long long) left + right + 33 + sinks < reach ? (long long) left + right + 33 + sinks : reach;
+    if (left >= 0 && right >= 0) reach = (long long) left + right + plan.rows + 1 + sinks < reach ? (long long) left + right + plan.rows + 1 + sinks : reach;
     const long long tiles = (reach + 31) / 32, blocks = problems * plan.row_tiles;
-    // About 384 workgroups, three for two units, with a tile to every wavefront at least.  Microseconds with 256 / 384 / 512 / 768:
-    // fp16, 48 tokens over up to 1000 keys 20 / 20 / 24 / 23, 2 x 100 over 6000 28 / 23 / 27 / 26, 32 over 4096 52 / 54 / 52 / 53.  (Pieces of 8
-    // tiles at least and of 4: fp32, 7 x 1 over 413 keys of 128 20 and 14 us, 12 x 1 over 396 15 and 12; fp16, 1 x 1 over 4096 both 12.)
-    long long pieces = blocks > 0 ? (384 + blocks - 1) / blocks : 1;
-    const long long most = (tiles + 3) / 4;
+    long long pieces = 1, most = 1;
+    if (plan.rows == 32) {
+        // About 384 workgroups, three for two units, with a tile to every wavefront at least.  Microseconds with 256 / 384 / 512 / 768:
+        // fp16, 48 tokens over up to 1000 keys 20 / 20 / 24 / 23, 2 x 100 over 6000 28 / 23 / 27 / 26, 32 over 4096 52 / 54 / 52 / 53.  (Pieces
+        // of 8 tiles at least and of 4: fp32, 7 x 1 over 413 keys of 128 20 and 14 us, 12 x 1 over 396 15 and 12; fp16, 1 x 1 over 4096 both 12.)
+        pieces = blocks > 0 ? (384 + blocks - 1) / blocks : 1, most = (tiles + 3) / 4;
+    } else if (plan.rows == 64 && !half_precision) {
+        // 512 workgroups, which two units share, with 512 keys at least.  Microseconds uncut (or with 32 rows, where 64 are too few) / so: 4 x 64
+        // of 32 heads to 8 of 128 over 8192 312 / 272; 2048 causal tokens of 12 heads of 64 91 / 75; 2 x 100 of 14 to 2 over 6000 53 / 46;
+        // 430 over 7327 of 8 to 2 of 32 79 / 71.  With 256 keys at least 3 x 517 45 / 48, 2 x 1000 of 7 to 1, window 300, 35 / 44.  Not in
+        // fp16, which has less to do for the sums that it would write and read again: 2048 causal tokens 26 / 34, 600 of 12 11 / 15.
+        pieces = (512 + blocks - 1) / blocks, most = tiles / 16;
+    }
     pieces = pieces < most ? pieces : most;
     plan.pieces = (int) (pieces < 1 ? 1 : pieces > kMaxPieces ? kMaxPieces : pieces);
-    if (plan.pieces > 1) plan.floats = (size_t) blocks * plan.pieces * 32 * (head_size + 4);
+    if (plan.pieces > 1) plan.floats = (size_t) blocks * plan.pieces * plan.rows * (head_size + 4);
     return plan;
 }
 
 template <typename T, int D, int ROWS>
-int run_window_rows(const WindowArgs &a, int row_tiles, hipStream_t stream) {
+int run_window_rows(const WindowArgs &a, int row_tiles, int pieces, hipStream_t stream) {
     static std::atomic<unsigned long long> done{0};
-    const dim3 grid(a.batch * a.kv_heads * row_tiles);
+    const dim3 grid(a.batch * a.kv_heads * row_tiles * pieces);
     if constexpr (sizeof(T) == 4) {
         constexpr int kLds = 6 * (32 * 128 / ROWS) * 2 * D;
         if (kLds > 48 * 1024 && !allow_large_lds(attention_window_terms_kernel<D, ROWS>, done)) return CUBERT_UNSUPPORTED;
-        return launch_lds(attention_window_terms_kernel<D, ROWS>, grid, dim3(kBlock), kLds, stream, a, row_tiles);
+        return launch_lds(attention_window_terms_kernel<D, ROWS>, grid, dim3(kBlock), kLds, stream, a, row_tiles, pieces);
     } else {
         constexpr int kLds = 4 * (64 * 128 / ROWS) * 2 * D;
         if (kLds > 48 * 1024 && !allow_large_lds(attention_window_shared_kernel<D, ROWS>, done)) return CUBERT_UNSUPPORTED;
@@ -1153,19 +1181,19 @@ int run_spread(const WindowArgs &a, WindowPlan plan, hipStream_t stream) {
 
 template <typename T, int D>
 int run_window(const WindowArgs &a, WindowPlan plan, hipStream_t stream) {
-    const int problems = a.batch * a.kv_heads;
-    if (plan.rows == 128) return run_window_rows<T, D, 128>(a, plan.row_tiles, stream);
-    if (plan.rows == 64) return run_window_rows<T, D, 64>(a, plan.row_tiles, stream);
-    const int rows = a.q_rows * (a.heads / a.kv_heads);
-    const int rc = sizeof(T) == 4 && rows <= 16 ? run_spread<T, D, sizeof(T) == 4>(a, plan, stream) : run_spread<T, D, false>(a, plan, stream);
+    const int problems = a.batch * a.kv_heads, rows = a.q_rows * (a.heads / a.kv_heads), row_tiles = plan.row_tiles * (plan.rows / 32);
+    int rc;
+    if (plan.rows == 128) rc = run_window_rows<T, D, 128>(a, plan.row_tiles, plan.pieces, stream);
+    else if (plan.rows == 64) rc = run_window_rows<T, D, 64>(a, plan.row_tiles, plan.pieces, stream);
+    else if (sizeof(T) == 4 && rows <= 16) rc = run_spread<T, D, sizeof(T) == 4>(a, plan, stream);
+    else rc = run_spread<T, D, false>(a, plan, stream);
     if (rc != 0 || plan.pieces == 1) return rc;
-    const int total = problems * a.q_rows * (a.heads / a.kv_heads), per_block = kBlock / (D / 4);
+    const int total = problems * rows, per_block = kBlock / (D / 4);
     // (18612 rows of 2 pieces: 5 us so, 22 us with a workgroup per row; 512 rows of 8 pieces 6.6 and 4.7 us, 16 rows of 128 137 and 4.4)
     if (plan.pieces <= 8 && total > 2048)
-        return launch(attention_window_join_few_kernel<T, D>, dim3((total + per_block - 1) / per_block), dim3(kBlock), stream, a,
-                      plan.row_tiles, plan.pieces, total);
-    return launch(attention_window_join_kernel<T, D>, dim3(total), dim3(kBlock), stream, a,
-                  plan.row_tiles, plan.pieces);
+        return launch(attention_window_join_few_kernel<T, D>, dim3((total + per_block - 1) / per_block), dim3(kBlock), stream, a, row_tiles,
+                      plan.pieces, total);
+    return launch(attention_window_join_kernel<T, D>, dim3(total), dim3(kBlock), stream, a, row_tiles, plan.pieces);
 }
 
 template <typename T>

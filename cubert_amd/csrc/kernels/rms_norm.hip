@@ -19,6 +19,10 @@ namespace {
 
 constexpr int kMaxHidden = 32768;
 
+// Bound by memory where there are many rows: fp16, 32768 x 1024 with a residual, 268 MB in 48.8 us, 5.5 TB/s (a large copy reaches 5.1);
+// fp32 in 8 bits, 4099 x 1000, 53 MB in 10.2 us, 5.2 TB/s.  A few rows are one read, two exchanges and one write behind each other:
+// 1 x 768 2.0 us, 8 x 4096 in 8 bits 4.2 us, of which launching anything takes 1.5.
+//
 // WAVES wavefronts per row, ROWS rows to a workgroup; a lane has CHUNKS runs of VEC elements, WAVES * 64 runs apart.
 template <typename T, int VEC, int CHUNKS, int WAVES, int ROWS, bool CODES>
 __global__ __launch_bounds__(WAVES * ROWS * kWave) void rms_norm_kernel(const T *x, const T *residual, const T *__restrict__ gamma, float eps,
@@ -121,7 +125,10 @@ int rms_norm(const T *x, const T *residual, const T *gamma, float eps, T *sum_ou
         return launch(rms_norm_kernel<T, VEC, CHUNKS, WAVES, ROWS, CODES>, dim3((rows + (ROWS - 1ll)) / ROWS),         \
                       dim3(WAVES * ROWS * kWave), s, x, residual, gamma, eps, sum_out, out, codes, scales, rows, hidden);     \
     }
-    if (whole && rows >= 1024) {
+    // A wavefront per row where a row is one run of its lanes or the rows fill the card, otherwise four (or sixteen) per row.  Microseconds
+    // with one / four: fp16, 16384 x 256 9.3 / 17.4, 128 x 256 2.6 / 2.7, 4096 x 1024 8.3 / 8.5, 1024 x 1024 4.5 / 3.5, 64 x 1024
+    // 3.2 / 2.7, 4096 x 2000 15.3 / 16.0, 300 x 2000 4.7 / 3.2; fp32 in 8 bits, 512 x 256 2.7 / 2.9, 1024 x 1024 5.2 / 5.0.
+    if (whole && (rows >= 2048 || hidden <= kVec * kWave)) {
         RUN(kVec, 1, 1, 4) RUN(kVec, 2, 1, 4) RUN(kVec, 4, 1, 4)
     }
     if (whole) {

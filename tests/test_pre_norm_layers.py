@@ -94,7 +94,7 @@ def test_attention_window_refuses(L, t):
 
 
 def test_attention_window_partials(L):
-    """Floats for 32 rows of head size + 4 per piece of the axis, and none where nothing is cut."""
+    """Floats for the rows of a workgroup, head size + 4 each, per piece of the axis, and none where nothing is cut."""
     for half in (0, 1):
         def floats(batch, heads, kv_heads, q_rows, kv_rows, size, left=-1, right=0, sinks=0):
             return L.cubert_attention_window_partials(half, batch, heads, kv_heads, q_rows, kv_rows, size, left, right, sinks)
@@ -105,6 +105,9 @@ def test_attention_window_partials(L):
         assert floats(1, 4, 4, 1, 128, 64) == 0
         assert floats(512, 12, 12, 1, 4096, 64) == 0
         assert floats(8, 12, 12, 512, 512, 64) == 0
+        assert floats(2, 8, 4, 100, 3000, 64) == (32 * 5 * 64 * 68 if not half else 56 * 7 * 32 * 68)
+        assert floats(1, 12, 12, 2048, 2048, 64) == (384 * 2 * 64 * 68 if not half else 0)
+        assert half or floats(1, 12, 12, 600, 600, 64, right=-1) == 0
         for nothing in ((0, 4, 2, 1, 50, 64), (1, 4, 3, 1, 50, 64), (1, 4, 0, 1, 50, 64), (1, 4, 2, 0, 50, 64), (1, 4, 2, 1, 0, 64),
                         (1, 4, 2, 1, 50, 0), (1 << 30, 1 << 20, 1 << 20, 1, 5000, 64)):
             assert floats(*nothing) == 0

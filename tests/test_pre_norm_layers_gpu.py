@@ -367,6 +367,17 @@ WIDE = {
 }
 ATTENTION.update(WIDE)
 
+# so many rows, and a long axis: 64 of them share their tiles, and in fp32 the axis is cut as well
+ATTENTION.update({
+    "cut piece": (2, 100, 3000, 8, 4, -1, 0, 3, "end", (3000, 1700), "holes"),
+    "cut piece with a window": (1, 300, 2500, 14, 2, 1500, 20, 40, "end", (2477,), "no"),
+    "cut causal": (1, 1100, 1100, 4, 4, -1, 0, 0, None, None, "no"),
+    "cut encoder": (3, 520, 1030, 6, 6, -1, -1, 0, None, (1030, 33, 0), "no"),
+    "cut before the sequence": (2, 200, 2000, 8, 2, 700, 500, 2, "end", (2000, 150), "no"),
+    "cut and masked from the middle on": (2, 130, 2100, 9, 3, 1100, 0, 3, "end", (2100, 1500), "middle"),
+    "cut and nothing left": (2, 140, 1600, 4, 4, 1100, 5, 0, None, None, "nothing"),
+})
+
 
 def attention_inputs(name, t, size, seed=0):
     batch, q_rows, kv_rows, heads, kv_heads, left, right, sinks, first, lengths, masked = ATTENTION[name]
@@ -455,7 +466,8 @@ def test_attention_window(K, name, t, size):
 
 @pytest.mark.parametrize("name", ["one query", "masked encoder", "piece", "few tokens", "long", "encoder", "nothing left", "wide encoder",
                                   "wide and masked from the middle on", "masked from the middle on",
-                                  "wide masked encoder", "wide piece", "wide and nothing left"])
+                                  "wide masked encoder", "wide piece", "wide and nothing left", "cut piece", "cut and nothing left",
+                                  "cut encoder", "cut piece with a window", "cut and masked from the middle on"])
 @pytest.mark.parametrize("t", ["f32", "f16"])
 @pytest.mark.parametrize("filler", [math.nan, math.inf])
 def test_attention_window_past_what_it_sees(K, name, t, filler):
@@ -493,7 +505,7 @@ def test_attention_window_of_large_scores(K, t):
 
 
 @pytest.mark.parametrize("name", ["one query", "few tokens", "long", "long window", "piece", "masked encoder", "wide piece", "wide masked encoder",
-                                  "wide causal", "causal", "encoder"])
+                                  "wide causal", "causal", "encoder", "cut piece", "cut causal", "cut before the sequence"])
 @pytest.mark.parametrize("t", ["f32", "f16"])
 @pytest.mark.parametrize("where", ["q", "k"])
 def test_attention_window_of_no_number(K, name, t, where):
@@ -579,7 +591,7 @@ def test_attention_window_cut_and_uncut(K):
     """A call without room for its pieces runs uncut, with the same result within its bound; and twice gives the same bits."""
     from cubert_amd._lib import lib
     for t in (torch.float32, torch.float16):
-        for name in ("long", "long window", "one query", "few tokens"):
+        for name in ("long", "long window", "one query", "few tokens", "cut piece", "cut before the sequence"):
             q, k, v, at = attention_inputs(name, t, 64)
             want, bound = attention_reference(q, k, v, **at)
             got = K.attention_window(q, k, v, **at)
