@@ -549,10 +549,10 @@ def dense_w4_i8(x, x_scales, w, bias=None, gelu=False, dtype=torch.float16, out=
 def _heads_pitch(t, what):
     """The pitch of the rows of a [batch, rows, heads, size] tensor, one for all of them, whose heads stand side by side."""
     batch, rows, heads, size = t.shape
+    if t.is_contiguous():
+        return heads * size
     b, r, h, d = t.stride()
     pitch = r if rows > 1 else b if batch > 1 else heads * size
-    if t.numel() == 0:
-        return heads * size
     if not heads * size <= pitch < 1 << 31 or (size > 1 and d != 1) or (heads > 1 and h != size) or (batch > 1 and b != rows * pitch):
         raise ValueError("%s: heads side by side in rows of one pitch expected, got strides %s of %s" % (what, t.stride(), tuple(t.shape)))
     return pitch
@@ -565,22 +565,23 @@ def attention_window(q, k, v, left=-1, right=-1, sinks=0, first=None, lengths=No
     projection or of a cache), first and lengths int32 [batch], mask int8 [batch, kv_rows].  Queries that see nothing, or
     stand outside their sequence, give zeros.  None when the head size or the alignment does not fit."""
     device = _device(q, k, v, first, lengths, mask)
+    t, cache = q.dtype, k.shape
     batch, q_rows, heads, size = q.shape
-    kv_rows, kv_heads = k.shape[1], k.shape[2]
-    if k.dtype != q.dtype or v.dtype != q.dtype or k.shape != v.shape or k.shape[0] != batch or k.shape[3] != size:
-        raise ValueError("k and v like q expected, got %s, %s and %s" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    if len(cache) != 4 or k.dtype != t or v.dtype != t or v.shape != cache or cache[0] != batch or cache[3] != size:
+        raise ValueError("k and v like q expected, got %s, %s and %s" % (tuple(q.shape), tuple(cache), tuple(v.shape)))
+    kv_rows, kv_heads = cache[1], cache[2]
     if kv_heads < 1 or heads % kv_heads:
         raise ValueError("%d heads cannot share %d" % (heads, kv_heads))
-    if first is not None and (first.dtype != torch.int32 or first.shape != (batch,)):
-        raise ValueError("first: int32 (%d,) expected, got %s %s" % (batch, first.dtype, tuple(first.shape)))
-    if lengths is not None and (lengths.dtype != torch.int32 or lengths.shape != (batch,)):
-        raise ValueError("lengths: int32 (%d,) expected, got %s %s" % (batch, lengths.dtype, tuple(lengths.shape)))
+    for n, what in ((first, "first"), (lengths, "lengths")):
+        if n is not None and (n.dtype != torch.int32 or n.shape != (batch,)):
+            raise ValueError("%s: int32 (%d,) expected, got %s %s" % (what, batch, n.dtype, tuple(n.shape)))
     if mask is not None and (mask.dtype != torch.int8 or mask.shape != (batch, kv_rows)):
         raise ValueError("mask: int8 (%d, %d) expected, got %s %s" % (batch, kv_rows, mask.dtype, tuple(mask.shape)))
-    left, right, sinks = max(min(left, 1 << 30), -1), max(min(right, 1 << 30), -1), min(sinks, 1 << 30)
-    suffix = _SUFFIXES.get(q.dtype) or _suffix(q)
+    if not (-1 <= left <= 1 << 30 and -1 <= right <= 1 << 30 and sinks <= 1 << 30):  # (the C interface has 32 bits)
+        left, right, sinks = max(min(left, 1 << 30), -1), max(min(right, 1 << 30), -1), min(sinks, 1 << 30)
+    suffix = _SUFFIXES.get(t) or _suffix(q)
     ldq, ldkv = _heads_pitch(q, "q"), _heads_pitch(k, "k")
-    if v.stride() != k.stride() and _heads_pitch(v, "v") != ldkv:
+    if _heads_pitch(v, "v") != ldkv:
         raise ValueError("k and v at one row pitch expected, got strides %s and %s" % (k.stride(), v.stride()))
     ctx = torch.empty_like(q, memory_format=torch.contiguous_format)
     floats = lib().cubert_attention_window_partials(suffix == "f16", batch, heads, kv_heads, q_rows, kv_rows, size, left, right, sinks)
