@@ -339,8 +339,9 @@ int run_dense_w4(const DenseArgs<X, T> &a, hipStream_t s) {
     if (units > 1024 && groups(4) * 8 * kWave >= 1ll << 32) return CUBERT_UNSUPPORTED;  // (what a launch holds)
     if (units > 1024 || (units > 512 && a.tokens > 8)) return launch(dense_w4_kernel<X, T, EACH, 4, 8>, grid(4), dim3(8 * kWave), s, a);
     if (units > 256) return launch(dense_w4_kernel<X, T, EACH, 2, 8>, grid(2), dim3(8 * kWave), s, a);
-    // (sixteen wavefronts, 4096 x 1024: 1 token 3.9 us against 4.4 with eight, 64 tokens 7.0 against 6.7)
-    if (units <= 128 && a.blocks > 8) return launch(dense_w4_kernel<X, T, EACH, 1, 16>, grid(1), dim3(16 * kWave), s, a);
+    // (sixteen wavefronts / eight: 1 token, 4096 x 1024 4.0 / 4.4 us, 8192 x 4096 7.0 / 8.5; 8 tokens, 8192 x 4096 8.8 / 9.2; 16 tokens, 4096 x
+    // 4096 7.2 / 6.8)
+    if ((units <= 128 || (units <= 256 && a.tokens <= 8)) && a.blocks > 8) return launch(dense_w4_kernel<X, T, EACH, 1, 16>, grid(1), dim3(16 * kWave), s, a);
     return launch(dense_w4_kernel<X, T, EACH, 1, 8>, grid(1), dim3(8 * kWave), s, a);
 }
 
