@@ -16,6 +16,7 @@ namespace cubert {
 namespace {
 
 constexpr int kMaxPieces = 128;  // of an axis that is cut
+constexpr int kFewPieces = 8;    // that one thread takes
 constexpr int kFar = (1 << 30) - 1;  // a bound, position or length that no sequence reaches
 
 struct WindowArgs {
@@ -1052,7 +1053,7 @@ __global__ __launch_bounds__(kBlock, sizeof(T) * D == 512 && !FEW ? 1 : 2) void 
     }
 }
 
-// The pieces' sums of a row joined, where they are few: D / 4 lanes to a row.
+// The pieces' sums of a row joined, where they are at most kFewPieces: D / 4 lanes to a row.
 template <typename T, int D>
 __global__ __launch_bounds__(kBlock) void attention_window_join_few_kernel(WindowArgs a, int row_tiles, int pieces, int total_rows) {
     constexpr int kPitch = Spread<T, D>::kPitch, kQuads = D / 4;
@@ -1062,15 +1063,27 @@ __global__ __launch_bounds__(kBlock) void attention_window_join_few_kernel(Windo
     const int problem = i / rows, row = i - problem * rows, b = problem / a.kv_heads, kv_head = problem - b * a.kv_heads;
     const float *from = a.partials + ((size_t) (problem * row_tiles + row / 32) * pieces * 32 + row % 32) * kPitch;
     const size_t step = (size_t) 32 * kPitch;
-    float top = kNone;
-    for (int n = 0; n < pieces; ++n) top = fmaxf(top, from[n * step + D]);
+    // all that there is to read at once (past the last piece the first one again)
+    v4f32 part[kFewPieces];
+    float tops[kFewPieces], sums[kFewPieces];
+#pragma unroll
+    for (int n = 0; n < kFewPieces; ++n) {
+        const float *at = from + (n < pieces ? n : 0) * step;
+        part[n] = *reinterpret_cast<const v4f32 *>(at + d);
+        tops[n] = at[D], sums[n] = at[D + 1];
+    }
+    float top = tops[0];
+#pragma unroll
+    for (int n = 1; n < kFewPieces; ++n) top = fmaxf(top, tops[n]);
     v4f32 x = v4f32{};
     float sum = 0.f;
-#pragma unroll 4
-    for (int n = 0; n < pieces; ++n) {
-        const float f = __builtin_amdgcn_exp2f(from[n * step + D] - top);
-        sum += from[n * step + D + 1] * f;
-        x += *reinterpret_cast<const v4f32 *>(from + n * step + d) * f;
+#pragma unroll
+    for (int n = 0; n < kFewPieces; ++n) {
+        if (n < pieces) {
+            const float f = __builtin_amdgcn_exp2f(tops[n] - top);
+            sum += sums[n] * f;
+            x += part[n] * f;
+        }
     }
     const int query = row / share, head = kv_head * share + row - query * share;
     T *ctx = (T *) a.ctx + ((size_t) b * a.q_rows + query) * a.ld_ctx + (size_t) head * D + d;
@@ -1196,8 +1209,9 @@ int run_window(const WindowArgs &a, WindowPlan plan, hipStream_t stream) {
     else rc = run_spread<T, D, false>(a, plan, stream);
     if (rc != 0 || plan.pieces == 1) return rc;
     const int total = problems * rows, per_block = kBlock / (D / 4);
-    // (18612 rows of 2 pieces: 5 us so, 22 us with a workgroup per row; 512 rows of 8 pieces 6.6 and 4.7 us, 16 rows of 128 137 and 4.4)
-    if (plan.pieces <= 8 && total > 2048)
+    // (the whole call with D / 4 threads to a row / a workgroup: 8 x 1 of 16 heads over up to 2048 keys, 6 pieces, 14.0 / 14.6 us, 12 x 1 of 12
+    // over up to 1000, 3 pieces, 14.5 / 15.1; the join alone, 18612 rows of 2 pieces, 5 / 22)
+    if (plan.pieces <= kFewPieces)
         return launch(attention_window_join_few_kernel<T, D>, dim3((total + per_block - 1) / per_block), dim3(kBlock), stream, a, row_tiles,
                       plan.pieces, total);
     return launch(attention_window_join_kernel<T, D>, dim3(total), dim3(kBlock), stream, a, row_tiles, plan.pieces);
