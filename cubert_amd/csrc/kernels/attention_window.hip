@@ -903,8 +903,8 @@ struct Spread {
     static constexpr int kLds = 4 * kWaveBytes > kMergeBytes ? 4 * kWaveBytes : kMergeBytes;
 };
 
-// Few rows, bound by reading K and V: 32 tokens over up to 4096 keys of 4 heads of 128 in fp16, 219 MB in 49 us (4.5 TB/s); 1 token over
-// 131072 keys of 2 heads, 134 MB in 25 us (5.3 TB/s), and 4 us for the join.  32 rows per workgroup, whose four wavefronts take every
+// Few rows, bound by reading K and V: 32 tokens over up to 4096 keys of 4 heads of 128 in fp16, 219 MB in 50 us (4.4 TB/s); 1 token over
+// 131072 keys of 2 heads, 134 MB in 25 us (5.3 TB/s), and 4.7 us for the join.  32 rows per workgroup, whose four wavefronts take every
 // fourth tile of 32 keys of this workgroup's piece of the axis; their sums meet in LDS, in wavefront order, and go out as results or, where
 // the axis is cut, as sums for the kernel below.
 template <typename T, int D, bool FEW>

@@ -262,7 +262,7 @@ __device__ __forceinline__ void multiply_block(v4f32 (&acc)[FT], const typename 
 // wavefront order.  The operands come straight into registers, where the matrix instructions take them: weights are used once per 16
 // tokens, and so many wavefronts fit a unit that the others cover one's wait.  (Operands of the next block in registers of their own:
 // 16 x 8192 x 32768 33 and 31 us, 64 x 4096 x 4096 10 and 11.)
-// Few tokens on large layers are bound by reading the weights: 16 rows of 8 bits, 8192 x 32768, 140 MB in 29.8 us, 4.7 TB/s; 1 token in
+// Few tokens on large layers are bound by reading the weights: 16 rows of 8 bits, 8192 x 32768, 140 MB in 29 us, 4.8 TB/s; 1 token in
 // fp16 29.6 us.  Small layers by latency: 1 x 1024 x 4096 3.2 us.  More tokens by the loads of x, which every 64 features repeat in 16
 // rows of 64 bytes: 64 x 4096 x 16384 in fp16 27 us, where the weights take 6.7; codes unpacked once for 32 or 64 tokens left that
 // as it was (26 and 27 us).

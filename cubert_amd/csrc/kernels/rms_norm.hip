@@ -19,9 +19,9 @@ namespace {
 
 constexpr int kMaxHidden = 32768;
 
-// Bound by memory where there are many rows: fp16, 32768 x 1024 with a residual, 268 MB in 48.8 us, 5.5 TB/s (a large copy reaches 5.1);
-// fp32 in 8 bits, 4099 x 1000, 53 MB in 10.2 us, 5.2 TB/s.  A few rows are one read, two exchanges and one write behind each other:
-// 1 x 768 2.0 us, 8 x 4096 in 8 bits 4.2 us.
+// Bound by memory where there are many rows: fp16, 32768 x 1024 with a residual, 268 MB in 48 us, 5.6 TB/s (a large copy reaches 5.1);
+// fp32 in 8 bits, 4099 x 1000, 53 MB in 10.4 us, 5.1 TB/s.  A few rows are one read, two exchanges and one write behind each other:
+// 1 x 768 1.8 us, 8 x 4096 in 8 bits 4.2 us.
 //
 // WAVES wavefronts per row, ROWS rows to a workgroup; a lane has CHUNKS runs of VEC elements, WAVES * 64 runs apart.
 template <typename T, int VEC, int CHUNKS, int WAVES, int ROWS, bool CODES>
