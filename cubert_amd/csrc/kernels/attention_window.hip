@@ -43,8 +43,8 @@ typedef int v4i32 __attribute__((ext_vector_type(4)));
 typedef float v16f32 __attribute__((ext_vector_type(16)));
 
 constexpr float kNone = -3e38f;  // the maximum of no scores: finite, so that differences to it are numbers
-constexpr float kSlack = 8.f;    // how far a maximum may rise, in powers of two, before sums are scaled anew (fp32)
-constexpr float kMost = 1024.f;  // what the probabilities of a tile may add up to in half a row before that (fp16)
+constexpr float kSlack = 8.f;    // how far a maximum may rise, in powers of two, before sums are scaled anew
+constexpr float kMost = 1024.f;  // what the probabilities of a tile may add up to in half a row before that (fp16, many rows)
 
 // 32 rows (queries and heads of one key head) meet 32 keys in one matrix product with the keys as its rows: lane l has row
 // l % 32 and, in accumulator i, key 8 (i / 4) + 4 (l / 32) + i % 4.  The probabilities are then the second operand of the
@@ -104,39 +104,49 @@ __device__ __forceinline__ void products_done() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
-// 32 N keys of K and V in LDS, keys of bits 0 in `visible` left out where not all of them are seen
-// EXACT: probabilities in 16 bits as sums of two numbers, for kernels that wait for memory; their error is otherwise as large as that of
-// rounding the results, 2^-12 of them on average.
-template <typename T, int D, int N, bool EXACT = false>
+// e as a sum of two fp16 numbers, exact to 22 bits: pairs of `high` and `low`
+__device__ __forceinline__ void two_terms(float e0, float e1, v2f16 &high, v2f16 &low) {
+    high = __builtin_convertvector((v2f32{e0, e1}), v2f16);
+    float minus = -1.f;
+    asm("" : "+v"(minus));  // (as a constant it makes a conversion and a subtraction of one instruction)
+    low = __builtin_convertvector((v2f32{fmaf((float) high[0], minus, e0), fmaf((float) high[1], minus, e1)}), v2f16);
+}
+
+// 32 N keys of K and V in LDS, keys of bits 0 in `visible` left out where not all of them are seen.  The product with V takes
+// probabilities in 16 bits as sums of two numbers, so that a result is rounded once, at the end.  (As single numbers their error is as
+// large as that rounding, 2^-12 of them on average, and one query would differ with the number of rows it comes with.)
+template <typename T, int D, int N>
 __device__ __forceinline__ void attend(Rows<T, D> &r, const unsigned char *k, const unsigned char *v, float scale, bool all,
                                        unsigned long long visible, int lane) {
     typedef Rows<T, D> R;
     const int col = lane & 31, half_wave = lane >> 5;
     v16f32 s[N];
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-        s[n] = v16f32{};
-        const int key = 32 * n + col;
-#pragma unroll
-        for (int t = 0; t < R::kSteps; ++t) {
-            const v4f32 piece = *reinterpret_cast<const v4f32 *>(k + key * R::kRowBytes + k_piece<R::kRowBytes>(key, 2 * t + half_wave) * 16);
-            if constexpr (sizeof(T) == 2) {
-                s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8f16, piece), __builtin_bit_cast(v8f16, r.q[t]), s[n], 0, 0, 0);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(piece[e], r.q[t][e], s[n], 0, 0, 0);
-            }
-        }
-    }
-    products_done();
-    if (!all) {
+    auto products = [&]() {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const unsigned word = (unsigned) (visible >> (32 * n)) >> (4 * half_wave);
+            s[n] = v16f32{};
+            const int key = 32 * n + col;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[n][i] = word >> (8 * (i / 4) + i % 4) & 1u ? s[n][i] : -INFINITY;
+            for (int t = 0; t < R::kSteps; ++t) {
+                const v4f32 piece = *reinterpret_cast<const v4f32 *>(k + key * R::kRowBytes + k_piece<R::kRowBytes>(key, 2 * t + half_wave) * 16);
+                if constexpr (sizeof(T) == 2) {
+                    s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8f16, piece), __builtin_bit_cast(v8f16, r.q[t]), s[n], 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(piece[e], r.q[t][e], s[n], 0, 0, 0);
+                }
+            }
         }
-    }
+        products_done();
+        if (!all) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const unsigned word = (unsigned) (visible >> (32 * n)) >> (4 * half_wave);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[n][i] = word >> (8 * (i / 4) + i % 4) & 1u ? s[n][i] : -INFINITY;
+            }
+        }
+    };
     // Sums are scaled anew only when some maximum has risen by a factor that a probability in 16 bits and the sums bear.
     auto rescale = [&](float top) {
         const float high = fmaxf(r.top, fmaxf(top, __shfl_xor(top, 32, kWave)));
@@ -154,43 +164,48 @@ __device__ __forceinline__ void attend(Rows<T, D> &r, const unsigned char *k, co
             for (int i = 0; i < 16; ++i) top = fmaxf(top, s[n][i]);
         return top * scale;
     };
+    products();
     if constexpr (sizeof(T) == 2) {
-        // Probabilities against the maximum so far; their sum, which is wanted anyway, says whether it was too small by far, and
-        // only then the scores' maximum is looked for.
-        v8f16 p[N][2], low[N][2];
         auto weigh = [&]() {
             float sum = 0.f;
 #pragma unroll
             for (int n = 0; n < N; ++n)
 #pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    const v2f32 e = {__builtin_amdgcn_exp2f(fmaf(s[n][i], scale, -r.top)),
-                                     __builtin_amdgcn_exp2f(fmaf(s[n][i + 1], scale, -r.top))};
-                    const v2f16 pair = __builtin_convertvector(e, v2f16);
-                    p[n][i / 8][i % 8] = pair[0], p[n][i / 8][i % 8 + 1] = pair[1];
-                    if constexpr (EXACT) {
-                        const v2f16 left = __builtin_convertvector((v2f32{e[0] - (float) pair[0], e[1] - (float) pair[1]}), v2f16);
-                        low[n][i / 8][i % 8] = left[0], low[n][i / 8][i % 8 + 1] = left[1];
-                        sum += e[0] + e[1];
-                    } else {  // (a sum of the probabilities as the product takes them)
-                        sum = __builtin_amdgcn_fdot2(pair, v2f16{(half_t) 1.f, (half_t) 1.f}, sum, false);
-                    }
+                for (int i = 0; i < 16; ++i) {
+                    s[n][i] = __builtin_amdgcn_exp2f(fmaf(s[n][i], scale, -r.top));
+                    sum += s[n][i];
                 }
             return sum;
         };
-        if (r.fresh) rescale(largest());
-        r.fresh = false;
-        float sum = weigh();
-        if (__any(!(sum <= kMost))) {
-            rescale(largest());
-            sum = weigh();
+        if constexpr (N == 1) {  // (for kernels that wait for memory)
+            const float top = largest();
+            if (__any(top > r.top + kSlack)) rescale(top);
+            r.sum += weigh();
+        } else {
+            // Probabilities against the maximum so far, in the scores' place; their sum, which is wanted anyway, says whether it was
+            // too small by far, and only then the scores are made again and their maximum is looked for.
+            if (r.fresh) rescale(largest());
+            r.fresh = false;
+            float sum = weigh();
+            if (__any(!(sum <= kMost))) {
+                products();
+                rescale(largest());
+                sum = weigh();
+            }
+            r.sum += sum;
         }
-        r.sum += sum;
         const int patch = lane & 15, side = (lane >> 4) & 1;
 #pragma unroll
         for (int n = 0; n < N; ++n)
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks)
+            for (int ks = 0; ks < 2; ++ks) {
+                v8f16 p, low;
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    v2f16 a, b;
+                    two_terms(s[n][8 * ks + i], s[n][8 * ks + i + 1], a, b);
+                    p[i] = a[0], p[i + 1] = a[1], low[i] = b[0], low[i + 1] = b[1];
+                }
 #pragma unroll
                 for (int d = 0; d < D / 32; ++d) {
                     v4f16 part[2];
@@ -200,9 +215,10 @@ __device__ __forceinline__ void attend(Rows<T, D> &r, const unsigned char *k, co
                         part[h] = read_transposed(v + key * R::kRowBytes + v_piece<T, R::kRowBytes>(key, at) * 16 + (patch & 1) * 8);
                     }
                     const v8f16 a = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
-                    if constexpr (EXACT) r.ctx[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, low[n][ks], r.ctx[d], 0, 0, 0);
-                    r.ctx[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, p[n][ks], r.ctx[d], 0, 0, 0);
+                    r.ctx[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, low, r.ctx[d], 0, 0, 0);
+                    r.ctx[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, p, r.ctx[d], 0, 0, 0);
                 }
+            }
     } else {
         const float top = largest();
         if (__any(top > r.top + kSlack)) rescale(top);
@@ -633,13 +649,14 @@ struct Strip {
     }
 };
 
-// fp16, many rows, bound by exponentials, matrix instructions and reads of LDS, about a quarter of the time each, that three wavefronts to a
-// SIMD overlap in part: 4 x up to 4096 tokens of 16 heads of 64, window 512, 39 Gflop in 77 us (500 Tflop/s); 2 x 4096 causal tokens of 16
-// heads of 128, 137 Gflop in 206 us (670).  Four wavefronts share every tile of K and V, the next one on its way while they work on this
-// one.  (Two on their way: 80 and 77 us, but 214 and 280 for heads of 128.)  A wavefront has 64
+// fp16, many rows, bound by exponentials and what else the probabilities take, matrix instructions and reads of LDS, that three wavefronts to
+// a SIMD overlap in part: 4 x up to 4096 tokens of 16 heads of 64, window 512, 39 Gflop in 96 us (400 Tflop/s); 2 x 4096 causal tokens of
+// 16 heads of 128, 137 Gflop in 259 us (530).  (The probabilities in one fp16 term each: 88 and 214 us, with a second rounding as
+// large as that of the results.)  Four wavefronts share every tile of K and V, the next one on its way while they work on this
+// one.  (Two on their way: 80 and 77 us, but 214 and 280 for heads of 128, with one term.)  A wavefront has 64
 // keys of a tile with its 32 rows: ROWS = 128, the same ones for all, 64, either half of 128.
 template <int D, int ROWS>
-__global__ __launch_bounds__(kBlock) void attention_window_shared_kernel(WindowArgs a, int row_tiles) {
+__global__ __launch_bounds__(kBlock, D == 128 && ROWS == 128 ? 2 : 1) void attention_window_shared_kernel(WindowArgs a, int row_tiles) {
     typedef half_t T;
     constexpr int kKeys = 64 * 128 / ROWS, kTileBytes = kKeys * D * (int) sizeof(T), kPartBytes = 64 * D * (int) sizeof(T);
     typedef Strip<T, D, kKeys, ROWS> Work;
@@ -988,7 +1005,7 @@ __global__ __launch_bounds__(kBlock, sizeof(T) * D == 512 && !FEW ? 1 : 2) void 
             const unsigned long long visible =
                     all ? ~0ull : bits_below(end - base) & (~bits_below(begin - base) | bits_below(a.sinks - base)) & kept_bits;
             if constexpr (FEW) attend_few<D>(r, kt, vt, a.scale, all, (unsigned) visible, lane);
-            else attend<T, D, 1, true>(r, kt, vt, a.scale, all, visible, lane);
+            else attend<T, D, 1>(r, kt, vt, a.scale, all, visible, lane);
         }
         if (S::kBuffers == 2) {
             buffer ^= 1;

@@ -639,6 +639,48 @@ def test_attention_window_far_into_a_cache(K):
     within(got, want, bound, "far")
 
 
+def exact_scores(g, t, batch, q_rows, kv_rows, heads, kv_heads, size):
+    """Queries and keys of -1, 0 and 1: every order of summation gives the same scores, whole numbers of at most `size`."""
+    q = torch.randint(-1, 2, (batch, q_rows, heads, size), generator=g, device="cuda").to(t)
+    return q, torch.randint(-1, 2, (batch, kv_rows, kv_heads, size), generator=g, device="cuda").to(t)
+
+
+# batch, q_rows, kv_rows, heads, kv_heads, left, right, sinks: single tokens, few rows, 64 rows to a workgroup, 128 rows
+ROUNDED_ONCE = [(3, 1, 2000, 8, 2, -1, 0, 0), (2, 4, 90, 8, 4, 3, 0, 1), (2, 300, 300, 12, 12, 2, 0, 1), (4, 300, 300, 32, 32, 2, 0, 0),
+                (4, 300, 300, 32, 32, 1, 1, 2), (4, 330, 330, 32, 16, -1, 0, 0)]
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("size", [32, 64, 128])
+@pytest.mark.parametrize("at", ROUNDED_ONCE)
+def test_attention_window_rounds_results_once(K, t, size, at):
+    """A result is off by its own rounding and by what fp32 loses on the way, however many rows come with it."""
+    batch, q_rows, kv_rows, heads, kv_heads, left, right, sinks = at
+    t, g = TYPES[t], gen(size + q_rows)
+    q, k = exact_scores(g, t, batch, q_rows, kv_rows, heads, kv_heads, size)
+    v = normal(g, batch, kv_rows, kv_heads, size).to(t)
+    first = torch.full((batch,), kv_rows - q_rows, dtype=torch.int32, device="cuda")
+    at = dict(left=left, right=right, sinks=sinks, first=first, lengths=None, mask=None)
+    got = K.attention_window(q, k, v, alpha=0.125, **at)
+    want, _ = attention_reference(q, k, v, alpha=0.125, **at)
+    share, seen = heads // kv_heads, visible(q, k, **at)
+    Q, KT = q.double().permute(0, 2, 1, 3), k.double().repeat_interleave(share, 2).permute(0, 2, 3, 1).contiguous()
+    V = v.double().abs().repeat_interleave(share, 2).permute(0, 2, 1, 3).contiguous()
+    z = torch.where(seen, (Q @ KT) * 0.125, -math.inf)
+    e = torch.exp(z - z.amax(3, keepdim=True))
+    total, back = e.sum(3, keepdim=True), lambda x: x.permute(0, 2, 1, 3)
+    # An exponent is a whole number times alpha log2(e), at most size / 8 * 1.443, less a maximum that is as large: the factor is off by
+    # 2 u of it, the maximum by 3 u, the difference by u of twice that, and e's exponential of that by log 2 times it.
+    exponent = math.log(2) * size / 8 * 1.443 * 8 * U
+    # An exponential: 2^-22; a probability in two terms of 11 bits: 2^-22; sums of it and of the products: 3 n u.  The same for the sum.
+    count = float(seen.sum(3).max())
+    off = (e @ V) / total * (2 * exponent + 2.0 ** -21 + 2.0 ** -22 + 4 * count * U)
+    if t == torch.float16:  # terms among fp16's subnormals: 2^-25 of the largest probability, for every key
+        off = off + 2.0 ** -25 * (seen.double().expand(e.shape) @ V) / total
+    off = back(off)
+    within(got, want, (want.abs() + off) * HALF[t] + off + SMALL[t], "rounded once")
+
+
 # ---------------------------------------------------------------------------- streams, graphs, a run of them
 
 
