@@ -23,6 +23,11 @@ constexpr int kMaxHidden = 32768;
 // fp32 in 8 bits, 4099 x 1000, 53 MB in 10.4 us, 5.1 TB/s.  A few rows are one read, two exchanges and one write behind each other:
 // 1 x 768 1.8 us, 8 x 4096 in 8 bits 4.2 us.
 //
+// The largest, or a NaN where there is one (fmaxf takes the number).
+struct LargestOp {
+    __device__ __forceinline__ float operator()(float a, float b) const { return __builtin_elementwise_maximum(a, b); }
+};
+
 // WAVES wavefronts per row, ROWS rows to a workgroup; a lane has CHUNKS runs of VEC elements, WAVES * 64 runs apart.
 template <typename T, int VEC, int CHUNKS, int WAVES, int ROWS, bool CODES>
 __global__ __launch_bounds__(WAVES * ROWS * kWave) void rms_norm_kernel(const T *x, const T *residual, const T *__restrict__ gamma, float eps,
@@ -62,12 +67,12 @@ __global__ __launch_bounds__(WAVES * ROWS * kWave) void rms_norm_kernel(const T 
                 s[c][i] = to_f32(a[c].v[i]);
                 if (residual != nullptr) s[c][i] += to_f32(r[c].v[i]);
                 squares = fmaf(s[c][i], s[c][i], squares);
-                if (CODES) top = fmaxf(top, fabsf(to_f32(g[c].v[i]) * s[c][i]));
+                if (CODES) top = LargestOp()(top, fabsf(to_f32(g[c].v[i]) * s[c][i]));
             }
         }
     }
     squares = wave_sum(squares);
-    if (CODES) top = wave_max(top);
+    if (CODES) top = group_reduce<kWave>(top, LargestOp());
     if constexpr (WAVES > 1) {
         if ((threadIdx.x & (kWave - 1)) == 0) {
             traded[0][wave] = squares;
@@ -78,12 +83,12 @@ __global__ __launch_bounds__(WAVES * ROWS * kWave) void rms_norm_kernel(const T 
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) {
             squares += traded[0][w];
-            if (CODES) top = fmaxf(top, traded[1][w]);
+            if (CODES) top = LargestOp()(top, traded[1][w]);
         }
     }
     const float power = squares / (float) hidden + eps, rstd = power == 0.f ? 0.f : 1.f / sqrtf(power);
-    // A NaN is lost in a maximum and an infinity leaves no finite factor: such a row's scale is NaN and its codes are 0.
-    const bool finite = squares < INFINITY;
+    // Neither a NaN nor an infinity leaves a finite factor: such a row's scale is NaN and its codes are 0.  gamma may bring them as well.
+    const bool finite = squares < INFINITY && top < INFINITY;
     // 127 / m leaves fp32's range for m below 2^-121: rows that small are raised by a power of two first, which is exact.
     const float raise = top < 0x1p-60f ? 0x1p80f : 1.f;
     const float inverse = top > 0.f && finite ? 127.f / (top * raise) : 0.f;

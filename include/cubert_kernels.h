@@ -237,8 +237,8 @@ int cubert_res_rms_norm_f16(const cubert_half *in, const cubert_half *residual, 
                             cubert_half *sum_out, cubert_half *out, int rows, int hidden, void *stream);
 /* The same in 8 bits, as cubert_dense_w4_i8_* takes its rows: the result is out[r, c] * scales[r] with
  *   t = gamma * s,  m = max |t|,  out = rint(t * (127 / m)),  scales[r] = m / (127 sqrt(mean(s^2) + eps)),
- * in fp32.  A row of zeros has scale 0 and codes 0; a row with a value (or a sum of squares) that is not finite has
- * scale NaN and codes 0, so that whatever is made of it is NaN. */
+ * in fp32.  A row of zeros has scale 0 and codes 0; a row with a value s, a t (by a gamma that is not finite, or beyond fp32's range) or
+ * a sum of squares that is not finite has scale NaN and codes 0, so that whatever is made of it is NaN. */
 int cubert_res_rms_norm_i8_f32(const float *in, const float *residual, const float *gamma, float eps, float *sum_out, int8_t *out,
                                float *scales, int rows, int hidden, void *stream);
 int cubert_res_rms_norm_i8_f16(const cubert_half *in, const cubert_half *residual, const cubert_half *gamma, float eps,

@@ -130,6 +130,26 @@ def test_rms_norm_of_rows_without_a_norm(K, t, hidden):
     assert bool(torch.isnan(out[1]).all()) and math.isnan(scales[1])
 
 
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("rows,hidden", [(3, 64), (3, 100), (3, 1024), (3, 5000), (2050, 1024), (2, 8192)])
+def test_rms_norm_by_a_gamma_that_is_not_finite(K, t, rows, hidden):
+    """Rows that such a gamma leaves no norm have scale NaN and codes 0, wherever in the row it stands; rows that are 0 there too."""
+    t, g = TYPES[t], gen(hidden)
+    x = normal(g, rows, hidden).to(t)
+    for at in (0, hidden // 3, hidden - 1):
+        for bad in (math.nan, math.inf, -math.inf) + ((2.0 ** 127,) if t == torch.float32 else ()):
+            gamma = torch.ones(hidden, device="cuda", dtype=t)
+            gamma[at] = bad
+            y = x.clone()
+            y[:, at] = 8                                   # (8 * 2^127 is beyond fp32, and its square is not)
+            y[1, at] = 0
+            codes, scales, _ = K.res_rms_norm_i8(y, None, gamma)
+            none = torch.ones(rows, dtype=torch.bool, device="cuda")
+            none[1] = bad != 2.0 ** 127                    # (0 times it is 0)
+            assert bool((codes[none] == 0).all()) and bool(torch.isnan(scales[none]).all()), (at, bad)
+            assert bool(torch.isfinite(scales[~none]).all())
+
+
 def test_rms_norm_in_place(K):
     """The sum may be written over either input, as the C interface says."""
     from cubert_amd._lib import lib
