@@ -718,8 +718,8 @@ __device__ __forceinline__ float lead(float x) { return __builtin_bit_cast(float
 __device__ __forceinline__ unsigned lead_pair(float a, float b) {
     return __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, b), __builtin_bit_cast(unsigned, a), 0x07060302u);
 }
-// What is left of x behind its leading bits.  (Of an infinity a NaN: what it reaches is not finite either way, and two
-// instructions more for every number of K, V and the probabilities would be a fifth of the kernel's time.)
+// What is left of x behind its leading bits.  (Of an infinity a NaN, and an infinite term times a term of 0 is one as well: scores that are
+// none are made again from the numbers themselves, below.  Of an infinite V both are as good: what sees it is not finite.)
 __device__ __forceinline__ float rest(float x) { return x - lead(x); }
 
 struct Terms {  // of 8 numbers
@@ -747,6 +747,9 @@ __device__ __forceinline__ v16f32 multiply_term(int m, const v8bf16 (&a)[3], con
     constexpr int kA[6] = {2, 1, 0, 1, 0, 0}, kB[6] = {0, 1, 2, 0, 1, 0};
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[kA[m]], b[kB[m]], sums, 0, 0, 0);
 }
+
+// The largest, or a NaN where there is one (fmaxf takes the number).
+__device__ __forceinline__ float largest_or_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 // Bound by the matrix instructions and, next to them, by taking K and V apart and reading the terms: 16 x 512 tokens of 16 heads of 64, 17
 // Gflop in 112 us, 154 Tflop/s, what a large fp32 matrix product reaches on fp32's own matrix instructions.
@@ -853,16 +856,41 @@ __global__ __launch_bounds__(kBlock, D == 128 ? 1 : 2) void attention_window_ter
         }
         products_done();
         s += odd;
+        unsigned word = ~0u;
         if (!all) {
-            const unsigned word = (unsigned) strip.visible(base, kept_part) >> (4 * half_wave);
+            word = (unsigned) strip.visible(base, kept_part) >> (4 * half_wave);
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = word >> (8 * (i / 4) + i % 4) & 1u ? s[i] : -INFINITY;
         }
         float high = s[0];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) high = fmaxf(high, s[i]);
+        for (int i = 1; i < 16; ++i) high = largest_or_nan(high, s[i]);
         high *= a.scale;
-        if (__any(high > top + kSlack)) {
+        if (__any(!(high <= top + kSlack))) {
+            if (__any(high != high)) {
+                // Something infinite, or no number: these scores from Q and K themselves.  An infinite K against a q of the other sign is a
+                // score of -infinity and no more.
+                const float *qr = strip.q();
+#pragma unroll 1
+                for (int i = 0; i < 16; ++i) {
+                    float score = s[0];
+#pragma unroll
+                    for (int j = 1; j < 16; ++j) score = i == j ? s[j] : score;
+                    const int at = 8 * (i / 4) + i % 4;
+                    if (score != score && (word >> at & 1u)) {
+                        const float *kr = strip.k + (size_t) (base + 4 * half_wave + at) * a.ldkv;
+                        score = 0.f;
+#pragma unroll 1
+                        for (int d = 0; d < D; ++d) score = fmaf(a.negate ? -qr[d] : qr[d], kr[d], score);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) s[j] = i == j ? score : s[j];
+                }
+                high = s[0];
+#pragma unroll
+                for (int i = 1; i < 16; ++i) high = fmaxf(high, s[i]);
+                high *= a.scale;
+            }
             high = fmaxf(top, fmaxf(high, __shfl_xor(high, 32, kWave)));
             const float shrink = __builtin_amdgcn_exp2f(top - high);
             top = high;

@@ -290,8 +290,9 @@ int cubert_dense_w4_i8_f16(void *stream, int tokens, int features, int in, const
  * `lengths` (NULL: kv_rows; larger ones count as kv_rows) are device arrays of `batch` ints, `mask` (NULL: all kept) is
  * int8 [batch, kv_rows].  A negative left or right is no bound; a right of 0 is causal.  alpha is finite.
  * K and V that no query of a sequence sees may hold anything: behind its length, where the mask is 0, outside all windows.  A V that is
- * not finite and that some queries see may make other queries of the same call, which do not see it, NaN as well; a Q or K that is
- * not a number reaches the results of that query or of those that see the key, and no others.
+ * not finite and that some queries see leaves their results infinite or no numbers, and may make other queries of the same call, which do
+ * not see it, NaN as well; a Q or K that is not a number reaches the results of that query or of those that see the key, and no others.
+ * An infinite Q or K makes the scores that fp32 arithmetic makes of it: a key whose score is -infinity is as good as not there.
  * head_size 32, 64 or 128, pointers and rows of whole 16-byte pieces, ldkv up to 2^22, and fewer than 2^24 workgroups of at least 32 rows
  * (q_rows * heads / kv_heads of every sequence and key head); otherwise CUBERT_UNSUPPORTED.  ctx overlaps nothing that is read.
  * Few rows over a long axis are cut along it, into `partials`: cubert_attention_window_partials floats of device memory,

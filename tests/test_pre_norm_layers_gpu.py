@@ -549,6 +549,33 @@ def test_attention_window_of_no_number(K, name, t, where):
     within(torch.where(bad[..., None], 0, got), torch.where(bad[..., None], 0.0, want), bound, name)
 
 
+@pytest.mark.parametrize("name", ["one query", "few tokens", "long", "piece", "masked encoder", "wide piece", "wide masked encoder", "wide causal", "causal",
+                                  "encoder", "cut piece", "cut causal", "cut before the sequence"])
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("size", [32, 64, 128])
+@pytest.mark.parametrize("alpha", [0.125, -0.125])
+def test_attention_window_of_infinite_keys(K, name, t, size, alpha):
+    """An infinite key is a score of -infinity for a query of the other sign, as if it were not there, and no number for the others."""
+    q, k, v, at = attention_inputs(name, TYPES[t], size)
+    q, k = q.clone(), k.clone()
+    q[..., 5] = torch.where(q[..., 5] < 0, -0.5, 0.5).to(q.dtype)
+    seen, share = visible(q, k, **at)[:, 0], q.shape[2] // k.shape[2]      # [batch, q_rows, kv_rows]
+    b, i = (int(x) for x in seen.any(2).nonzero()[seen.any(2).sum() // 2])
+    j = int(seen[b, i].nonzero()[0])
+    without = dict(at, mask=torch.ones(k.shape[:2], dtype=torch.int8, device="cuda") if at["mask"] is None else at["mask"].clone())
+    without["mask"][b, j] = 0
+    want, bound = attention_reference(q, k, v, alpha=alpha, **at)
+    want_without, bound_without = attention_reference(q, k, v, alpha=alpha, **without)
+    meets = torch.zeros(q.shape[:3], dtype=torch.bool, device="cuda")
+    meets[b, :, :share] = seen[b, :, j, None]
+    none = meets & (q[..., 5] * alpha > 0)
+    want, bound = torch.where(meets[..., None], want_without, want), torch.where(meets[..., None], bound_without, bound)
+    k[b, j, 0, 5] = math.inf
+    got = K.attention_window(q, k, v, alpha=alpha, **at)
+    assert bool(torch.isnan(got[none]).all())
+    within(torch.where(none[..., None], 0, got), torch.where(none[..., None], 0.0, want), bound, name)
+
+
 @pytest.mark.parametrize("t", ["f32", "f16"])
 @pytest.mark.parametrize("q_rows,heads", [(1, 2), (3, 8), (50, 60)])
 @pytest.mark.parametrize("kv_rows", [9001, 8992, 4624])
