@@ -43,8 +43,20 @@ typedef int v4i32 __attribute__((ext_vector_type(4)));
 typedef float v16f32 __attribute__((ext_vector_type(16)));
 
 constexpr float kNone = -3e38f;  // the maximum of no scores: finite, so that differences to it are numbers
-constexpr float kSlack = 8.f;    // how far a maximum may rise, in powers of two, before sums are scaled anew
-constexpr float kMost = 1024.f;  // what the probabilities of a tile may add up to in half a row before that (fp16, many rows)
+constexpr float kSlack = 8.f;    // how far a maximum may rise, in powers of two, before sums are scaled anew (fp32)
+// Probabilities in 16 bits are taken relative to a number 2^kRaise below the maximum, so that fp16's subnormals begin far below it: a
+// probability loses 2^-25 of that number at most, 2^-35 or 2^-37 of the largest, and a long axis of small ones is not lost next to one
+// large.  At the top end what a maximum may rise before sums are scaled anew keeps them within fp16.
+template <int N>
+struct Range;
+template <>
+struct Range<1> {  // few rows: the maximum is looked at
+    static constexpr float kRaise = 12.f, kSlack = 3.f;
+};
+template <>
+struct Range<2> {  // many: what the probabilities of a tile add up to in half a row, 32 of them
+    static constexpr float kRaise = 10.f, kMost = 60000.f;
+};
 
 // 32 rows (queries and heads of one key head) meet 32 keys in one matrix product with the keys as its rows: lane l has row
 // l % 32 and, in accumulator i, key 8 (i / 4) + 4 (l / 32) + i % 4.  The probabilities are then the second operand of the
@@ -149,7 +161,8 @@ __device__ __forceinline__ void attend(Rows<T, D> &r, const unsigned char *k, co
     };
     // Sums are scaled anew only when some maximum has risen by a factor that a probability in 16 bits and the sums bear.
     auto rescale = [&](float top) {
-        const float high = fmaxf(r.top, fmaxf(top, __shfl_xor(top, 32, kWave)));
+        constexpr float kRaise = sizeof(T) == 2 ? Range<N>::kRaise : 0.f;
+        const float high = fmaxf(r.top, fmaxf(top, __shfl_xor(top, 32, kWave)) - kRaise);
         const float shrink = __builtin_amdgcn_exp2f(r.top - high);
         r.top = high;
         r.sum *= shrink;
@@ -179,7 +192,7 @@ __device__ __forceinline__ void attend(Rows<T, D> &r, const unsigned char *k, co
         };
         if constexpr (N == 1) {  // (for kernels that wait for memory)
             const float top = largest();
-            if (__any(top > r.top + kSlack)) rescale(top);
+            if (__any(top > r.top + (Range<N>::kRaise + Range<N>::kSlack))) rescale(top);
             r.sum += weigh();
         } else {
             // Probabilities against the maximum so far, in the scores' place; their sum, which is wanted anyway, says whether it was
@@ -187,7 +200,7 @@ __device__ __forceinline__ void attend(Rows<T, D> &r, const unsigned char *k, co
             if (r.fresh) rescale(largest());
             r.fresh = false;
             float sum = weigh();
-            if (__any(!(sum <= kMost))) {
+            if (__any(!(sum <= Range<N>::kMost))) {
                 products();
                 rescale(largest());
                 sum = weigh();

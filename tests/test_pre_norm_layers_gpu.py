@@ -728,6 +728,27 @@ def test_attention_window_rounds_results_once(K, t, size, at):
     within(got, want, (want.abs() + off) * HALF[t] + off + SMALL[t], "rounded once")
 
 
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("q_rows", [1, 3, 768, 5120])
+@pytest.mark.parametrize("at", [0, 70000, 131071])
+def test_attention_window_of_a_long_axis_next_to_one_key(K, t, q_rows, at):
+    """One key stands so far out that each of 131071 others is less than half of fp16's smallest number next to it; together they
+    are 3 thousandths of the result."""
+    t, keys, size, score = TYPES[t], 131072, 64, 17.5
+    q = torch.ones(1, q_rows, 8, size, device="cuda", dtype=t)
+    k, v = torch.zeros(1, keys, 1, size, device="cuda", dtype=t), torch.ones(1, keys, 1, size, device="cuda", dtype=t)
+    k[:, at], v[:, at] = 1, 0
+    got = K.attention_window(q, k, v, alpha=score / size)
+    others = (keys - 1) * math.exp(-score)
+    want = torch.full(got.shape, others / (1 + others), dtype=torch.float64, device="cuda")
+    # The exponents are score log2(e), in fp32: 6 u of 26; exponentials 2^-22; a lane adds up to half of the keys one by one, each
+    # addition off by u of what is there, in the sum and in the products.
+    off = want * (math.log(2) * 26 * 6 * U + 2.0 ** -21 + 2 * (keys / 2 + 64) * U)
+    if t == torch.float16:
+        off = off + keys * 2.0 ** -35
+    within(got, want, want * HALF[t] + off + SMALL[t], "others")
+
+
 # ---------------------------------------------------------------------------- streams, graphs, a run of them
 
 
