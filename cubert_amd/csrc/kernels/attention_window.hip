@@ -718,22 +718,31 @@ __global__ __launch_bounds__(kBlock, D == 128 && ROWS == 128 ? 2 : 1) void atten
 }
 
 // ---- fp32, many rows ------------------------------------------------------
-// An fp32 number is the sum of three bf16 numbers: its leading, middle and last 8 bits.  Of the nine products of two such sums
-// the three smallest are below 2^-24 of the whole and left out; the six others run on the bf16 matrix cores, whose rate is sixteen
-// times that of fp32's, with fp32 sums.  K and V are taken apart on their way into LDS, once for the four wavefronts that read
-// them; the probabilities in their lanes.
+// An fp32 number is the sum of three bf16 numbers, each the nearest to what those before it leave: the second is at most 2^-8 of the
+// leading power of two, the third at most 2^-17, and nothing is left.  Of the nine products of two such sums the three smallest are
+// left out, 2 * 2^-25 of the product together and of either sign; the six others run on the bf16 matrix cores, whose rate is sixteen times that
+// of fp32's, with fp32 sums.  (Terms cut off instead of rounded take as many instructions, but leave out up to 2^-21, always of the product's
+// sign.)  V's first term is cut off, because the nearest to the largest fp32 numbers is infinite; its second is then at most 2^-7 and its third
+// 2^-16, and what is left out of its products with probabilities 2 * 2^-24.  K and V are taken apart on their way into LDS, once for the
+// four wavefronts that read them; the probabilities in their lanes.
 
 typedef __bf16 v8bf16 __attribute__((ext_vector_type(8)));
 typedef unsigned v2u32 __attribute__((ext_vector_type(2)));
 typedef unsigned v4u32 __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ float lead(float x) { return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, x) & 0xffff0000u); }
-__device__ __forceinline__ unsigned lead_pair(float a, float b) {
-    return __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, b), __builtin_bit_cast(unsigned, a), 0x07060302u);
+typedef __bf16 v2bf16 __attribute__((ext_vector_type(2)));
+
+// The next terms of two numbers, and in their place what those leave; CUT: the leading bits as they are.  (Of an infinity a NaN is left, and
+// an infinite term times a term of 0 is one as well: scores that are none are made again from the numbers themselves, below.  Of an infinite V
+// both are as good: what sees it is not finite.)
+template <bool CUT>
+__device__ __forceinline__ unsigned next_terms(float &a, float &b) {
+    unsigned pair;
+    if constexpr (CUT) pair = __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, b), __builtin_bit_cast(unsigned, a), 0x07060302u);
+    else pair = __builtin_bit_cast(unsigned, __builtin_convertvector((v2f32{a, b}), v2bf16));
+    a -= __builtin_bit_cast(float, pair << 16), b -= __builtin_bit_cast(float, pair & 0xffff0000u);
+    return pair;
 }
-// What is left of x behind its leading bits.  (Of an infinity a NaN, and an infinite term times a term of 0 is one as well: scores that are
-// none are made again from the numbers themselves, below.  Of an infinite V both are as good: what sees it is not finite.)
-__device__ __forceinline__ float rest(float x) { return x - lead(x); }
 
 struct Terms {  // of 8 numbers
     v8bf16 t[3];
@@ -745,10 +754,7 @@ struct Terms {  // of 8 numbers
         for (int i = 0; i < 4; ++i) {
             float a = x[2 * i], b = x[2 * i + 1];
 #pragma unroll
-            for (int n = 0; n < 3; ++n) {
-                r[n][i] = lead_pair(a, b);
-                a = rest(a), b = rest(b);
-            }
+            for (int n = 0; n < 3; ++n) r[n][i] = next_terms<false>(a, b);
         }
 #pragma unroll
         for (int n = 0; n < 3; ++n) t[n] = __builtin_bit_cast(v8bf16, r[n]);
@@ -835,12 +841,11 @@ __global__ __launch_bounds__(kBlock, D == 128 ? 1 : 2) void attention_window_ter
                 for (int e = 0; e < 4; ++e) x[e] = use ? next[w][i][e] : 0.f;
                 const int piece = w == 0 ? k_piece<kRowBytes>(key, quad / 2) : v_piece<half_t, kRowBytes>(key, quad / 2);
                 unsigned char *to = planes + w * 3 * kPlane + key * kRowBytes + piece * 16 + (quad & 1) * 8;
+                *reinterpret_cast<v2u32 *>(to) = w == 0 ? v2u32{next_terms<false>(x[0], x[1]), next_terms<false>(x[2], x[3])}
+                                                        : v2u32{next_terms<true>(x[0], x[1]), next_terms<true>(x[2], x[3])};
 #pragma unroll
-                for (int n = 0; n < 3; ++n) {
-                    *reinterpret_cast<v2u32 *>(to + n * kPlane) = v2u32{lead_pair(x[0], x[1]), lead_pair(x[2], x[3])};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = rest(x[e]);
-                }
+                for (int n = 1; n < 3; ++n)
+                    *reinterpret_cast<v2u32 *>(to + n * kPlane) = v2u32{next_terms<false>(x[0], x[1]), next_terms<false>(x[2], x[3])};
             }
         if (tile + 1 < strip.high) {
             bring(tile + 1);

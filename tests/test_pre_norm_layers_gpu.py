@@ -749,6 +749,32 @@ def test_attention_window_of_a_long_axis_next_to_one_key(K, t, q_rows, at):
     within(got, want, want * HALF[t] + off + SMALL[t], "others")
 
 
+@pytest.mark.parametrize("size", [32, 64, 128])
+@pytest.mark.parametrize("batch,heads", [(1, 1), (3, 2), (4, 8)])
+def test_attention_window_of_scores_that_cancel(K, size, batch, heads):
+    """fp32 scores that are a millionth of the two products that make them: what a product leaves out stays below its own rounding."""
+    g, rows = gen(size), 1300
+    # numbers just below a step of 8 bits, whose parts below are as large as they get, and any numbers
+    step = 1 + torch.randint(1, 9, (2, batch, rows, heads), generator=g, device="cuda") * 2.0 ** -7 - 2.0 ** -23
+    some = 1 + torch.rand(2, batch, rows, heads, generator=g, device="cuda") / 16
+    x, y = torch.where(torch.arange(rows, device="cuda")[:, None] % 2 == 0, step, some)
+    y = y * 2.0 ** 20
+    q, k = (torch.zeros(batch, rows, heads, size, device="cuda") for _ in "qk")
+    q[..., 0], q[..., 1] = x, 1
+    k[..., 0], k[..., 1] = y, -(x * y)
+    v = torch.ones_like(k)
+    k[:, 0], v[:, 0] = 0, 0                                # the first key has score 0 and value 0; a query sees it and its own
+    got = K.attention_window(q, k, v, left=0, right=0, sinks=1, alpha=1.0)
+    product = x.double() * y.double()
+    want = torch.sigmoid(product - (x * y).double())
+    want[:, 0] = 0
+    # The product leaves out u of it.  It and the other, as large, meet in the last matrix instruction, whose two sums are off by a step
+    # (2 u) each; the instructions before have 2^-7 of that.  A sigmoid's slope is a quarter; exponentials and the quotient: 2^-20.
+    bound = 0.25 * 5.25 * U * product + 2.0 ** -20
+    within(got[..., 0], want, bound, "cancelled")
+    assert bool((got == got[..., :1]).all())
+
+
 # ---------------------------------------------------------------------------- streams, graphs, a run of them
 
 
