@@ -42,10 +42,13 @@ typedef float v2f32 __attribute__((ext_vector_type(2)));
 typedef int v4i32 __attribute__((ext_vector_type(4)));
 typedef float v16f32 __attribute__((ext_vector_type(16)));
 
+// Probabilities are 2^(scale (s - top)) of scores s and a maximum `top` of them, both as the products leave them: the difference is
+// taken first.  (One fused 2^(scale s - top), with a scaled maximum, is an instruction less, but that maximum's rounding grows with the
+// scores: beyond 2^26 the largest probability itself was 0 or infinite.)
 constexpr float kNone = -3e38f;  // the maximum of no scores: finite, so that differences to it are numbers
 constexpr float kSlack = 8.f;    // how far a maximum may rise, in powers of two, before sums are scaled anew (fp32)
-// Probabilities in 16 bits are taken relative to a number 2^kRaise below the maximum, so that fp16's subnormals begin far below it: a
-// probability loses 2^-25 of that number at most, 2^-35 or 2^-37 of the largest, and a long axis of small ones is not lost next to one
+// Probabilities in 16 bits are 2^kRaise times as large, so that fp16's subnormals begin far below the maximum: a
+// probability loses 2^-25 of that at most, 2^-35 or 2^-37 of the largest, and a long axis of small ones is not lost next to one
 // large.  At the top end what a maximum may rise before sums are scaled anew keeps them within fp16.
 template <int N>
 struct Range;
@@ -161,9 +164,8 @@ __device__ __forceinline__ void attend(Rows<T, D> &r, const unsigned char *k, co
     };
     // Sums are scaled anew only when some maximum has risen by a factor that a probability in 16 bits and the sums bear.
     auto rescale = [&](float top) {
-        constexpr float kRaise = sizeof(T) == 2 ? Range<N>::kRaise : 0.f;
-        const float high = fmaxf(r.top, fmaxf(top, __shfl_xor(top, 32, kWave)) - kRaise);
-        const float shrink = __builtin_amdgcn_exp2f(r.top - high);
+        const float high = fmaxf(r.top, fmaxf(top, __shfl_xor(top, 32, kWave)));
+        const float shrink = __builtin_amdgcn_exp2f((r.top - high) * scale);
         r.top = high;
         r.sum *= shrink;
 #pragma unroll
@@ -175,7 +177,7 @@ __device__ __forceinline__ void attend(Rows<T, D> &r, const unsigned char *k, co
         for (int n = 0; n < N; ++n)
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(top, s[n][i]);
-        return top * scale;
+        return top;
     };
     products();
     if constexpr (sizeof(T) == 2) {
@@ -185,14 +187,14 @@ __device__ __forceinline__ void attend(Rows<T, D> &r, const unsigned char *k, co
             for (int n = 0; n < N; ++n)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    s[n][i] = __builtin_amdgcn_exp2f(fmaf(s[n][i], scale, -r.top));
+                    s[n][i] = __builtin_amdgcn_exp2f(fmaf(s[n][i] - r.top, scale, Range<N>::kRaise));
                     sum += s[n][i];
                 }
             return sum;
         };
         if constexpr (N == 1) {  // (for kernels that wait for memory)
             const float top = largest();
-            if (__any(top > r.top + (Range<N>::kRaise + Range<N>::kSlack))) rescale(top);
+            if (__any((top - r.top) * scale > Range<N>::kSlack)) rescale(top);
             r.sum += weigh();
         } else {
             // Probabilities against the maximum so far, in the scores' place; their sum, which is wanted anyway, says whether it was
@@ -234,12 +236,12 @@ __device__ __forceinline__ void attend(Rows<T, D> &r, const unsigned char *k, co
             }
     } else {
         const float top = largest();
-        if (__any(top > r.top + kSlack)) rescale(top);
+        if (__any((top - r.top) * scale > kSlack)) rescale(top);
 #pragma unroll
         for (int n = 0; n < N; ++n)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[n][i] = __builtin_amdgcn_exp2f(fmaf(s[n][i], scale, -r.top));
+                s[n][i] = __builtin_amdgcn_exp2f((s[n][i] - r.top) * scale);
                 r.sum += s[n][i];
                 const int key = 32 * n + 8 * (i / 4) + 4 * half_wave + i % 4;
 #pragma unroll
@@ -309,9 +311,8 @@ __device__ __forceinline__ void attend_few(FewRows<D> &r, const unsigned char *k
     for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) top = fmaxf(top, s[n][i]);
-    top *= scale;
-    if (__any(top > r.top + kSlack)) {
-        const float high = fmaxf(r.top, quarters_max(top)), shrink = __builtin_amdgcn_exp2f(r.top - high);
+    if (__any((top - r.top) * scale > kSlack)) {
+        const float high = fmaxf(r.top, quarters_max(top)), shrink = __builtin_amdgcn_exp2f((r.top - high) * scale);
         r.top = high;
         r.sum *= shrink;
 #pragma unroll
@@ -321,7 +322,7 @@ __device__ __forceinline__ void attend_few(FewRows<D> &r, const unsigned char *k
     for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            s[n][i] = __builtin_amdgcn_exp2f(fmaf(s[n][i], scale, -r.top));
+            s[n][i] = __builtin_amdgcn_exp2f((s[n][i] - r.top) * scale);
             r.sum += s[n][i];
             const int key = 16 * n + 4 * quarter + i;
 #pragma unroll
@@ -626,7 +627,7 @@ struct Strip {
             __syncthreads();
             if (wave >= kRowGroups) return;
             const float other = with[D], high = fmaxf(top, other);
-            const float mine_by = __builtin_amdgcn_exp2f(top - high), other_by = __builtin_amdgcn_exp2f(other - high);
+            const float mine_by = __builtin_amdgcn_exp2f((top - high) * a.scale), other_by = __builtin_amdgcn_exp2f((other - high) * a.scale);
             sum = sum * mine_by + with[D + 1] * other_by, top = high;
 #pragma unroll
             for (int d = 0; d < D / 32; ++d)
@@ -883,8 +884,7 @@ __global__ __launch_bounds__(kBlock, D == 128 ? 1 : 2) void attention_window_ter
         float high = s[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) high = largest_or_nan(high, s[i]);
-        high *= a.scale;
-        if (__any(!(high <= top + kSlack))) {
+        if (__any(!((high - top) * a.scale <= kSlack))) {
             if (__any(high != high)) {
                 // Something infinite, or no number: these scores from Q and K themselves.  An infinite K against a q of the other sign is a
                 // score of -infinity and no more.
@@ -907,10 +907,9 @@ __global__ __launch_bounds__(kBlock, D == 128 ? 1 : 2) void attention_window_ter
                 high = s[0];
 #pragma unroll
                 for (int i = 1; i < 16; ++i) high = fmaxf(high, s[i]);
-                high *= a.scale;
             }
             high = fmaxf(top, fmaxf(high, __shfl_xor(high, 32, kWave)));
-            const float shrink = __builtin_amdgcn_exp2f(top - high);
+            const float shrink = __builtin_amdgcn_exp2f((top - high) * a.scale);
             top = high;
             sum *= shrink;
 #pragma unroll
@@ -918,7 +917,7 @@ __global__ __launch_bounds__(kBlock, D == 128 ? 1 : 2) void attention_window_ter
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale, -top));
+            s[i] = __builtin_amdgcn_exp2f((s[i] - top) * a.scale);
             sum += s[i];
         }
 #pragma unroll
@@ -1096,7 +1095,7 @@ __global__ __launch_bounds__(kBlock, sizeof(T) * D == 512 && !FEW ? 1 : 2) void 
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             const float *from = merge + (w * 32 + m) * S::kPitch;
-            const float f = __builtin_amdgcn_exp2f(from[D] - top);
+            const float f = __builtin_amdgcn_exp2f((from[D] - top) * a.scale);
             total += from[D + 1] * f;
             x += *reinterpret_cast<const v4f32 *>(from + d) * f;
         }
@@ -1143,7 +1142,7 @@ __global__ __launch_bounds__(kBlock) void attention_window_join_few_kernel(Windo
 #pragma unroll
     for (int n = 0; n < kFewPieces; ++n) {
         if (n < pieces) {
-            const float f = __builtin_amdgcn_exp2f(tops[n] - top);
+            const float f = __builtin_amdgcn_exp2f((tops[n] - top) * a.scale);
             sum += sums[n] * f;
             x += part[n] * f;
         }
@@ -1175,7 +1174,7 @@ __global__ __launch_bounds__(kBlock) void attention_window_join_kernel(WindowArg
     float top = tops[0];
 #pragma unroll
     for (int w = 1; w < kBlock / kWave; ++w) top = fmaxf(top, tops[w]);
-    const float weight = __builtin_amdgcn_exp2f(my_top - top);
+    const float weight = __builtin_amdgcn_exp2f((my_top - top) * a.scale);
     if (mine) weights[thread] = weight;
     const float wave_total = wave_sum(weight * my_sum);
     if ((thread & (kWave - 1)) == 0) sums[thread / kWave] = wave_total;
@@ -1304,8 +1303,8 @@ int attention_window(const T *q, int ldq, const T *k, const T *v, int ldkv, cons
     a.q = q, a.k = k, a.v = v, a.ctx = ctx, a.first = first, a.lengths = lengths, a.mask = mask;
     a.partials = partials;
     a.negate = alpha < 0.f;
-    // (a factor of 0 would make numbers of the infinities that stand for keys left out)
-    a.scale = fmaxf(fabsf(alpha) * 1.44269504089f, 1e-30f);
+    // (a factor of 0 would make numbers of the infinities that stand for keys left out, an infinite one no number of a difference of 0)
+    a.scale = fminf(fmaxf(fabsf(alpha) * 1.44269504089f, 1e-30f), 3e38f);
     a.ldq = ldq, a.ldkv = ldkv, a.ld_ctx = ld_ctx;
     a.batch = batch, a.heads = heads, a.kv_heads = kv_heads, a.q_rows = q_rows, a.kv_rows = kv_rows;
     a.left = left < 0 || left > kFar ? kFar : left, a.right = right < 0 || right > kFar ? kFar : right;

@@ -775,6 +775,46 @@ def test_attention_window_of_scores_that_cancel(K, size, batch, heads):
     assert bool((got == got[..., :1]).all())
 
 
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("rows,heads", [(1, 1), (40, 2), (300, 8), (400, 40)])
+@pytest.mark.parametrize("alpha", [0.5, -0.5])
+def test_attention_window_of_the_largest_numbers(K, t, rows, heads, alpha):
+    """The largest numbers as keys and as values (the nearest in 16 bits to fp32's is infinite), and scores as large as they make."""
+    t = TYPES[t]
+    most = torch.finfo(t).max
+    q, k, v = (torch.zeros(2, rows, heads, 64, device="cuda", dtype=t) for _ in "qkv")
+    if t == torch.float32:
+        q[..., 0] = 0.25
+    else:
+        q[:] = most                                        # 64 products of 4.3e9
+    up = math.copysign(most, alpha)                        # (a key whose score is above 0)
+    k[0], k[1], v[..., :32] = -up, up, 1
+    k[:, 0] = 0                                            # a query sees the first key, whose score is 0, its own and the one before
+    v[:, 0, :, 32:] = most
+    got = K.attention_window(q, k, v, left=1, right=0, sinks=1, alpha=alpha)
+    want = torch.zeros(got.shape, dtype=torch.float64, device="cuda")
+    want[0, :, :, :32], want[0, :, :, 32:] = 1, most       # scores so low that the first key is all there is, or so high that it is not
+    want[1, :, :, :32] = 1
+    want[:, 0, :, :32], want[:, 0, :, 32:] = 1, most
+    within(got, want, want.abs() * 16 * U, "largest")
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("name", ["one query", "few tokens", "piece", "wide piece", "cut piece", "long"])
+@pytest.mark.parametrize("alpha", [2.0 ** 40, -3e38])
+def test_attention_window_of_a_large_scale(K, t, name, alpha):
+    """Scores that are whole numbers, times so much that only the largest of them count: the mean of their values."""
+    q, k, v, at = attention_inputs(name, TYPES[t], 64)
+    g = gen(14)
+    q, k = exact_scores(g, q.dtype, q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], 64)
+    got = K.attention_window(q, k, v, alpha=alpha, **at)
+    want, _ = attention_reference(q, k, v, alpha=math.copysign(1e4, alpha), **at)
+    # sums of the values that count, in fp32, over as many; one rounding
+    count = float(visible(q, k, **at).sum(3).max())
+    bound = 4.0 * count * U * float(v.double().abs().max())
+    within(got, want, want.abs() * HALF[q.dtype] + bound + SMALL[q.dtype], name)
+
+
 # ---------------------------------------------------------------------------- streams, graphs, a run of them
 
 
