@@ -111,14 +111,6 @@ __device__ __forceinline__ v4f16 read_transposed(const unsigned char *p) {
     return __builtin_bit_cast(v4f16, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16 *) p));
 }
 
-// The wait states that an ordinary instruction needs before it reads what matrix instructions above wrote.  The compiler puts them in,
-// but behind a branch that follows such an instruction it was seen to count from the other way into the block, and 9 were missing.
-__device__ __forceinline__ void products_done() {
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_nop 15");
-    __builtin_amdgcn_sched_barrier(0);
-}
-
 // e as a sum of two fp16 numbers, exact to 22 bits: pairs of `high` and `low`
 __device__ __forceinline__ void two_terms(float e0, float e1, v2f16 &high, v2f16 &low) {
     high = __builtin_convertvector((v2f32{e0, e1}), v2f16);

@@ -137,6 +137,15 @@ __device__ __forceinline__ float group_reduce(float v, Op op) {
 __device__ __forceinline__ float wave_sum(float v) { return group_reduce<kWave>(v, SumOp()); }
 __device__ __forceinline__ float wave_max(float v) { return group_reduce<kWave>(v, MaxOp()); }
 
+// The states that an ordinary instruction needs between itself and the matrix instructions above whose results it takes: 18 behind
+// v_mfma_f32_32x32x2_f32, the longest used here, 12 behind 32x32x16, 10 behind 16x16x4_f32, 8 behind 16x16x32; these are 20.  The compiler
+// puts them in, but behind a branch that follows such an instruction it was seen to count from the other way into the block, and 9 were missing.
+__device__ __forceinline__ void products_done() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 15\n\ts_nop 3");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 // Wavefront index inside the workgroup as a scalar (SGPR) value, so that
 // addresses derived from it use scalar arithmetic and scalar loads.
 __device__ __forceinline__ int wave_in_block() {
