@@ -535,6 +535,7 @@ __global__ __launch_bounds__(KT * kWave) void attention_fused_kernel(const T *__
             }
         }
     }
+    if constexpr (RAGGED) products_done();  // (a branch around the first row is what follows)
     // lane holds output column jt*32 + r and 16 query rows
     const size_t first_row = (size_t) b * seq + qt * 32;
     bool over = false;
@@ -1119,6 +1120,7 @@ __global__ __launch_bounds__(WAVES * kWave, 3) void attention_spread_kernel(
     sum += __shfl_xor(sum, 32, kWave);
     if (hh == 0) s_sum[w][r] = sum;
     float *s_part = s_tiles + kTileFloats;  // (over the wavefront's own keys)
+    products_done();  // (after the last tile of a short sequence a branch leads here)
 #pragma unroll
     for (int jt = 0; jt < kColTiles; ++jt)
 #pragma unroll

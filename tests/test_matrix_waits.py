@@ -174,3 +174,11 @@ def test_the_guard_alone_is_long_enough(functions):
                 if x.text == "s_nop 15":
                     runs.append(16 + (int(y.operands[0], 0) + 1 if y.op == "s_nop" else 0))
             assert max(runs, default=0) > max(STATES.values()), kind
+
+
+def test_results_of_matrix_instructions_are_waited_for(functions):
+    assert sum(any(x.op.startswith("v_mfma") for x in body) for _, body in functions) > 50
+    unknown = {x.op for _, body in functions for x in body if x.op.startswith("v_mfma")} - set(STATES)
+    assert not unknown, "states of %s" % sorted(unknown)
+    wrong = [(name,) + f for name, body in functions for f in too_early(body)]
+    assert not wrong, "%d ways, such as %s" % (len(wrong), "; ".join("%s: %s -> %s, %d states and %d" % w for w in wrong[:4]))
