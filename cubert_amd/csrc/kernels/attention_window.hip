@@ -368,9 +368,14 @@ struct Tiles {
 
 // 16 bytes per lane from `base` + `offset` to LDS at `to` + 16 * lane, without passing through registers.  As an instruction of its
 // own, not the builtin: behind that the compiler lets every transposing read of LDS wait for all that is on its way, also to other
-// buffers.  The waits are the callers' (landed, and the ones that count).
+// buffers.  The waits are the callers' (landed, and the ones that count).  The compiler does not look into the statement, so it has the
+// five states that a load needs behind a vector instruction that wrote its scalar base (one, behind m0), and leaves m0 as it was.
 __device__ __forceinline__ void copy_to_lds(const char *base, unsigned offset, unsigned to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory", "m0");
+    unsigned m0;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 2\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0)
+                 : "s"(to), "v"(offset), "s"(base)
+                 : "memory");
 }
 
 __device__ __forceinline__ unsigned lds_address(const unsigned char *p) {

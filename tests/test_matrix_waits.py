@@ -176,6 +176,25 @@ def test_the_guard_alone_is_long_enough(functions):
             assert max(runs, default=0) > max(STATES.values()), kind
 
 
+def test_copies_to_lds_count_on_nothing_else(functions):
+    """Their statement has the five states that a scalar base written by a vector instruction needs, and gives m0 back."""
+    copies = 0
+    for name, body in functions:
+        if "attention_window" not in name:
+            continue
+        for i, x in enumerate(body):
+            if x.op == "global_load_lds_dwordx4" and x.operands[1].startswith("s["):
+                copies += 1
+                states, j = 0, i - 1
+                while body[j].op in ("s_nop", "s_mov_b32") and body[j].operands[-1] != "m0":
+                    states += int(body[j].operands[0], 0) + 1 if body[j].op == "s_nop" else 1
+                    j -= 1
+                kept = body[j].operands
+                assert body[j].op == "s_mov_b32" and kept[1] == "m0" and states + 1 >= 5, (name, x.text)
+                assert body[i + 1].op == "s_mov_b32" and body[i + 1].operands == ["m0", kept[0]], (name, x.text)
+    assert copies > 100
+
+
 def test_results_of_matrix_instructions_are_waited_for(functions):
     assert sum(any(x.op.startswith("v_mfma") for x in body) for _, body in functions) > 50
     unknown = {x.op for _, body in functions for x in body if x.op.startswith("v_mfma")} - set(STATES)
