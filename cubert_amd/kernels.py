@@ -480,6 +480,8 @@ class W4Weights(object):
 def w4_quantize(w, group=128, overflow=None):
     """(codes uint8 [features, width / 2], scales fp16 [features, width / group]) of weights [features, width]; overflow: an int32
     that becomes 1 where a group has a weight that is not finite or a scale beyond fp16."""
+    if overflow is not None and (overflow.dtype != torch.int32 or overflow.numel() < 1):
+        raise ValueError("overflow: an int32 expected, got %s %s" % (overflow.dtype, tuple(overflow.shape)))
     device = _device(w, overflow)
     features, width = w.shape
     if group not in (32, 64, 128) or width % group:

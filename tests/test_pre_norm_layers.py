@@ -135,3 +135,12 @@ def test_strided_heads_are_recognised():
                   packed[:, :1].expand(3, 5, 8, 64)):
         with pytest.raises(ValueError):
             _heads_pitch(wrong, "k")
+
+
+def test_quantize_wants_an_int_to_write_to():
+    """4 bytes are written there."""
+    from cubert_amd import kernels
+    for overflow in (torch.zeros(1, dtype=torch.int8), torch.zeros(1, dtype=torch.bool), torch.zeros(1, dtype=torch.int64),
+                     torch.zeros(1), torch.zeros(0, dtype=torch.int32)):
+        with pytest.raises(ValueError, match="int32"):
+            kernels.w4_quantize(torch.zeros(2, 64), 64, overflow)
