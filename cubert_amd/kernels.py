@@ -579,8 +579,8 @@ def attention_window(q, k, v, left=-1, right=-1, sinks=0, first=None, lengths=No
             raise ValueError("%s: int32 (%d,) expected, got %s %s" % (what, batch, n.dtype, tuple(n.shape)))
     if mask is not None and (mask.dtype != torch.int8 or mask.shape != (batch, kv_rows)):
         raise ValueError("mask: int8 (%d, %d) expected, got %s %s" % (batch, kv_rows, mask.dtype, tuple(mask.shape)))
-    if not (-1 <= left <= 1 << 30 and -1 <= right <= 1 << 30 and sinks <= 1 << 30):  # (the C interface has 32 bits)
-        left, right, sinks = max(min(left, 1 << 30), -1), max(min(right, 1 << 30), -1), min(sinks, 1 << 30)
+    if not (-1 <= left <= 1 << 30 and -1 <= right <= 1 << 30 and 0 <= sinks <= 1 << 30):  # (the C interface has 32 bits)
+        left, right, sinks = (max(min(n, 1 << 30), -1) for n in (left, right, sinks))
     suffix = _SUFFIXES.get(t) or _suffix(q)
     ldq, ldkv = _heads_pitch(q, "q"), _heads_pitch(k, "k")
     if _heads_pitch(v, "v") != ldkv:

@@ -144,3 +144,15 @@ def test_quantize_wants_an_int_to_write_to():
                      torch.zeros(1), torch.zeros(0, dtype=torch.int32)):
         with pytest.raises(ValueError, match="int32"):
             kernels.w4_quantize(torch.zeros(2, 64), 64, overflow)
+
+
+def test_a_negative_number_of_sinks_stays_one(monkeypatch):
+    from cubert_amd import kernels
+    calls = []
+    monkeypatch.setattr(kernels, "_device", lambda *tensors: 0)
+    monkeypatch.setattr(kernels, "_raw_stream", lambda device: 0)
+    monkeypatch.setattr(kernels, "_run_on", lambda device, name, args: calls.append(args) or True)
+    q = torch.zeros(1, 3, 2, 64)
+    for sinks, sent in ((4, 4), (0, 0), (-1, -1), (5 - (1 << 32), -1), (1 << 40, 1 << 30)):
+        kernels.attention_window(q, q, q, left=7, right=0, sinks=sinks)
+        assert calls[-1][-6:-3] == (7, 0, sent), sinks      # left, right, sinks, partials, their number, stream
