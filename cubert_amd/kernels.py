@@ -423,6 +423,12 @@ def _run_on(device, name, args, declines=True):
     _check(rc, name)
 
 
+def _fits(largest):
+    """The C interface has 32 bits for sizes and pitches, and what does not fit them would arrive as another number."""
+    if largest >= 1 << 31:
+        raise ValueError("sizes and pitches below 2**31 expected, got %d" % largest)
+
+
 def _like(t, ref, shape, what):
     if t.dtype != ref.dtype or t.shape != shape:
         raise ValueError("%s: %s %s expected, got %s %s" % (what, ref.dtype, tuple(shape), t.dtype, tuple(t.shape)))
@@ -435,12 +441,13 @@ def _whole_ptr(t):
 
 
 def _rms_norm(x, residual, gamma, eps, codes):
-    device = _device(x, residual, gamma)
-    suffix = _SUFFIXES.get(x.dtype) or _suffix(x)
     hidden = x.shape[-1]
     rows = x.numel() // hidden if hidden else 0
     if hidden == 0 or rows >= 1 << 31:
         raise ValueError("rows expected, got %s" % (tuple(x.shape),))
+    _fits(hidden)
+    device = _device(x, residual, gamma)
+    suffix = _SUFFIXES.get(x.dtype) or _suffix(x)
     _like(gamma, x, (hidden,), "gamma")
     args = (_whole_ptr(x),)
     total = None
@@ -482,8 +489,9 @@ def w4_quantize(w, group=128, overflow=None):
     that becomes 1 where a group has a weight that is not finite or a scale beyond fp16."""
     if overflow is not None and (overflow.dtype != torch.int32 or overflow.numel() < 1):
         raise ValueError("overflow: an int32 expected, got %s %s" % (overflow.dtype, tuple(overflow.shape)))
-    device = _device(w, overflow)
     features, width = w.shape
+    _fits(max(features, width))
+    device = _device(w, overflow)
     if group not in (32, 64, 128) or width % group:
         raise ValueError("groups of 32, 64 or 128 columns that divide %d expected, got %d" % (width, group))
     codes = torch.empty((features, width // 2), dtype=torch.uint8, device=w.device)
@@ -495,8 +503,9 @@ def w4_quantize(w, group=128, overflow=None):
 
 def w4_pack(codes, scales, group=128):
     """W4Weights of codes and scales as w4_quantize gives them (two's complement, two to a byte, the even column low)."""
-    device = _device(codes, scales)
     features, width = codes.shape[0], 2 * codes.shape[1]
+    _fits(max(features, width))
+    device = _device(codes, scales)
     size = lib().cubert_w4_packed_bytes(features, width, group)
     if size == 0:
         raise ValueError("groups of 32, 64 or 128 columns that divide %d expected, got %d" % (width, group))
@@ -510,12 +519,13 @@ def w4_pack(codes, scales, group=128):
 
 
 def _dense_w4(x, x_scales, w, bias, gelu, dtype, out):
+    tokens, width = x.shape
+    features = w.features
+    _fits(max(tokens, width, x.stride(0), 0 if out is None else out.stride(0)))
     device = _device(x, x_scales, w.packed, bias, out)
     suffix = _SUFFIXES.get(dtype)
     if suffix is None:
         raise TypeError("float32 or float16 expected, got %s" % dtype)
-    tokens, width = x.shape
-    features = w.features
     if width != w.width:
         raise ValueError("rows of %d expected, got %d" % (w.width, width))
     if out is None:
@@ -566,8 +576,9 @@ def attention_window(q, k, v, left=-1, right=-1, sinks=0, first=None, lengths=No
     left or right is no bound.  q [batch, q_rows, heads, size], k and v [batch, kv_rows, kv_heads, size] (views of a packed
     projection or of a cache), first and lengths int32 [batch], mask int8 [batch, kv_rows].  Queries that see nothing, or
     stand outside their sequence, give zeros.  None when the head size or the alignment does not fit."""
-    device = _device(q, k, v, first, lengths, mask)
     t, cache = q.dtype, k.shape
+    _fits(max(*q.shape, *cache))
+    device = _device(q, k, v, first, lengths, mask)
     batch, q_rows, heads, size = q.shape
     if len(cache) != 4 or k.dtype != t or v.dtype != t or v.shape != cache or cache[0] != batch or cache[3] != size:
         raise ValueError("k and v like q expected, got %s, %s and %s" % (tuple(q.shape), tuple(cache), tuple(v.shape)))

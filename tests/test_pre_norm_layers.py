@@ -156,3 +156,25 @@ def test_a_negative_number_of_sinks_stays_one(monkeypatch):
     for sinks, sent in ((4, 4), (0, 0), (-1, -1), (5 - (1 << 32), -1), (1 << 40, 1 << 30)):
         kernels.attention_window(q, q, q, left=7, right=0, sinks=sinks)
         assert calls[-1][-6:-3] == (7, 0, sent), sinks      # left, right, sinks, partials, their number, stream
+
+
+def test_wrappers_refuse_what_32_bits_do_not_hold():
+    """The C interface has 32 bits for sizes and pitches: 2**32 + 64 would arrive as 64."""
+    from cubert_amd import kernels
+
+    def empty(*shape, dtype=torch.float16):
+        return torch.empty(shape, dtype=dtype, device="meta")
+
+    large = (1 << 32) + 64
+    w = kernels.W4Weights(empty(8, dtype=torch.uint8), 16, 64, 64)
+    apart = torch.empty_strided((2, 64), (large, 1), dtype=torch.float16, device="meta")
+    for call in (lambda: kernels.res_rms_norm(empty(1, large), None, empty(large)),
+                 lambda: kernels.res_rms_norm_i8(empty(1, large), None, empty(large)),
+                 lambda: kernels.w4_quantize(empty(1, large), 64), lambda: kernels.w4_quantize(empty(large, 64), 64),
+                 lambda: kernels.w4_pack(empty(1, large // 2, dtype=torch.uint8), empty(1, large // 64), 64),
+                 lambda: kernels.dense_w4(empty(large, 64), w), lambda: kernels.dense_w4(apart, w),
+                 lambda: kernels.dense_w4(empty(2, 64), w, out=torch.empty_strided((2, 16), (large, 1), dtype=torch.float16, device="meta")),
+                 lambda: kernels.attention_window(empty(1, large, 1, 64), empty(1, 9, 1, 64), empty(1, 9, 1, 64)),
+                 lambda: kernels.attention_window(empty(1, 9, 1, 64), empty(1, large, 1, 64), empty(1, large, 1, 64))):
+        with pytest.raises(ValueError, match="2\\*\\*31"):
+            call()
