@@ -102,6 +102,18 @@ def test_rms_norm_8_bits(K, t, rows, hidden, with_residual):
     within(codes.double() * want[:, None], y, want[:, None] * (0.5 + 127 * 8 * U) + y.abs() * 8 * U, "values")
 
 
+# so many rows that a wavefront has one to itself, of one, two and four runs of its lanes, and of more, or of no whole pieces
+MANY_ROWS = [(2300, 256), (2048, 512), (2051, 1000), (2049, 1024), (2100, 1792), (2050, 2048), (2049, 4104), (2050, 1001)]
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("rows,hidden", MANY_ROWS)
+@pytest.mark.parametrize("with_residual", [False, True])
+def test_rms_norm_of_many_rows(K, t, rows, hidden, with_residual):
+    test_rms_norm(K, t, rows, hidden, with_residual)
+    test_rms_norm_8_bits(K, t, rows, hidden, with_residual)
+
+
 @pytest.mark.parametrize("t", ["f32", "f16"])
 @pytest.mark.parametrize("hidden", [64, 100, 1024, 5000])
 def test_rms_norm_of_rows_without_a_norm(K, t, hidden):
@@ -247,6 +259,36 @@ def test_dense_w4(K, tokens, width, features, group, x_type, t, plain):
     want, bound = dense_bound(x, w, y, width, group, not plain, t)
     assert out.dtype == t
     within(out, want, bound, "out")
+
+
+# Tokens, width, features, group, so that a workgroup has 32 or 64 features, or 16 and sixteen wavefronts: on both sides of where that
+# changes (tiles of 16 features times strips of 16 tokens: 128, 256, 512 and 1024; 8 tokens), with tiles left over and ends inside them
+WIDE_DENSE = [(3, 2048, 4000, 128), (8, 1280, 4096, 64), (9, 1280, 2048, 32), (7, 160, 4100, 32), (17, 256, 2064, 64), (8, 128, 8208, 128),
+              (5, 416, 12000, 32), (9, 128, 8208, 64), (33, 768, 4100, 128), (1, 128, 16385, 64), (16, 256, 16500, 128), (40, 96, 8200, 32),
+              (200, 512, 1300, 64), (64, 1152, 5003, 128)]
+
+
+@pytest.mark.parametrize("tokens,width,features,group", WIDE_DENSE)
+@pytest.mark.parametrize("x_type,t", [("f32", "f32"), ("f16", "f16"), ("i8", "f32"), ("i8", "f16")])
+@pytest.mark.parametrize("plain", [True, False])
+def test_dense_w4_of_many_features(K, tokens, width, features, group, x_type, t, plain):
+    test_dense_w4(K, tokens, width, features, group, x_type, t, plain)
+
+
+def test_dense_w4_of_many_features_stays_in_its_rows(K):
+    """What lies between rows of out stays where a workgroup has 32 or 64 features, and the same call gives the same bits."""
+    g = gen(6)
+    for tokens, features in ((7, 4100), (20, 8195)):
+        codes, scales, w = weights(g, features, 160, 32)
+        packed = K.w4_pack(codes, scales, 32)
+        x = normal(g, tokens, 160).half()
+        held = torch.full((tokens, features + 13), 7.0, device="cuda", dtype=torch.float16)
+        K.dense_w4(x, packed, out=held[:, :features])
+        want, bound = dense_bound(x.double(), w, x.double() @ w.t(), 160, 32, False, torch.float16)
+        within(held[:, :features], want, bound, "out")
+        assert bool((held[:, features:] == 7).all())
+        for _ in range(3):
+            assert torch.equal(K.dense_w4(x, packed), held[:, :features])
 
 
 def test_dense_w4_rows_apart(K):
