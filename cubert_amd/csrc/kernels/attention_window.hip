@@ -667,7 +667,7 @@ struct Strip {
 // one.  (Two on their way: 80 and 77 us, but 214 and 280 for heads of 128, with one term.)  A wavefront has 64
 // keys of a tile with its 32 rows: ROWS = 128, the same ones for all, 64, either half of 128.
 template <int D, int ROWS>
-__global__ __launch_bounds__(kBlock, D == 128 && ROWS == 128 ? 2 : 1) void attention_window_shared_kernel(WindowArgs a, int row_tiles) {
+__global__ __launch_bounds__(kBlock, D == 128 ? 2 : 1) void attention_window_shared_kernel(WindowArgs a, int row_tiles) {
     typedef half_t T;
     constexpr int kKeys = 64 * 128 / ROWS, kTileBytes = kKeys * D * (int) sizeof(T), kPartBytes = 64 * D * (int) sizeof(T);
     typedef Strip<T, D, kKeys, ROWS> Work;
@@ -1201,15 +1201,17 @@ struct WindowPlan {
 };
 
 // The rule, measured on heads of 64 with 128 / 64 / 32 rows, microseconds.  fp16: 4 x 4096 tokens of 16 heads, window 512 (2048 workgroups of
-// 128) 78 / 106 / 164; 32 x 128 of 12 (384) 13 / 17 / 19; 2 x 4096 of 4 (256) 59 / 41 / 71; 3 x 517 of 12 (180) 24 / 23 / 26; 1 x 600
-// (60) 15 / 11 / 15; 1 x 64 over 1000 (12) 19 / 13 / 12.  Heads of 128, 2 x 400 over 6000 (104): 131 / 91 / 74.  fp32: 2 x 2000 of 16 (512)
-// 184 / 216 / 300; 3 x 517 (180) 46 / 40 / 54; 2 x 400 (168 of 64) - / 22 / 31; 1 x 64 over 1000 (12) - / 19 / 13.
+// 128) 109 / 135 / 179; 32 x 128 of 12 (384) 13 / 19 / 19; 2 x 4096 of 4 (256) 84 / 57 / 80; 2 x 512 of 12 over 8192 (192 of 64) 161 / 93 / 104;
+// 3 x 517 of 12 (180) 32 / 28 / 28; 1 x 600 (60) 18 / 13 / 16; 1 x 64 over 1000 (12) 25 / 17 / 10.  Heads of 128, whose tiles for 64 rows
+// leave room for one workgroup to a unit: 2048 causal tokens of 16 (256 of 128) 68 / 75 / 73; 1024 of 32 to 8 over 16384 (256) 467 / 597 / 512;
+// 2 x 800 of 16 to 4 over 6000 (200) 176 / 209 / 138; 512 of 32 to 8 over 16384 (128) 464 / 321 / 280; 1000 of 16 (128) 38 / 27 / 28.
+// fp32: 2 x 2000 of 16 (512) 189 / 211 / 303; 3 x 517 (180) 47 / 43 / 59; 2 x 400 of 12 (168 of 64) 29 / 22 / 31; 1 x 64 over 1000 (12) 57 / 27 / 13.
 WindowPlan plan_window(bool half_precision, int batch, int heads, int kv_heads, int q_rows, int kv_rows, int head_size, int left, int right, int sinks) {
     WindowPlan plan;
     const long long rows = (long long) q_rows * (heads / kv_heads), problems = (long long) batch * kv_heads;
     const long long of_128 = (rows + 127) / 128 * problems, of_64 = (rows + 63) / 64 * problems;
-    const int enough = !half_precision ? 16 : head_size == 128 ? 256 : 96;
-    plan.rows = rows <= 32 ? 32 : of_128 >= 320 ? 128 : of_64 >= enough ? 64 : 32;
+    if (half_precision && head_size == 128) plan.rows = rows <= 32 || of_128 < 256 ? 32 : 128;
+    else plan.rows = rows <= 32 ? 32 : of_128 >= 320 ? 128 : of_64 >= (half_precision ? 96 : 16) ? 64 : 32;
     plan.row_tiles = (int) ((rows + plan.rows - 1) / plan.rows);
     plan.pieces = 1, plan.floats = 0;
     // the most tiles of 32 keys that a workgroup's rows reach
@@ -1262,8 +1264,9 @@ template <typename T, int D>
 int run_window(const WindowArgs &a, WindowPlan plan, hipStream_t stream) {
     const int problems = a.batch * a.kv_heads, rows = a.q_rows * (a.heads / a.kv_heads), row_tiles = plan.row_tiles * (plan.rows / 32);
     int rc;
+    constexpr int kHalfRows = sizeof(T) == 2 && D == 128 ? 128 : 64;  // (heads of 128 in fp16 have no rows in between)
     if (plan.rows == 128) rc = run_window_rows<T, D, 128>(a, plan.row_tiles, plan.pieces, stream);
-    else if (plan.rows == 64) rc = run_window_rows<T, D, 64>(a, plan.row_tiles, plan.pieces, stream);
+    else if (plan.rows == 64) rc = run_window_rows<T, D, kHalfRows>(a, plan.row_tiles, plan.pieces, stream);
     else if (sizeof(T) == 4 && rows <= 16) rc = run_spread<T, D, sizeof(T) == 4>(a, plan, stream);
     else rc = run_spread<T, D, false>(a, plan, stream);
     if (rc != 0 || plan.pieces == 1) return rc;
