@@ -661,8 +661,8 @@ struct Strip {
 };
 
 // fp16, many rows, bound by exponentials and what else the probabilities take, matrix instructions and reads of LDS, that three wavefronts to
-// a SIMD overlap in part: 4 x up to 4096 tokens of 16 heads of 64, window 512, 39 Gflop in 96 us (400 Tflop/s); 2 x 4096 causal tokens of
-// 16 heads of 128, 137 Gflop in 259 us (530).  (The probabilities in one fp16 term each: 88 and 214 us, with a second rounding as
+// a SIMD overlap in part: 4 x up to 4096 tokens of 16 heads of 64, window 512, 39 Gflop in 97 us (400 Tflop/s); 2 x 4096 causal tokens of
+// 16 heads of 128, 137 Gflop in 265 us (520).  (The probabilities in one fp16 term each: 88 and 214 us, with a second rounding as
 // large as that of the results.)  Four wavefronts share every tile of K and V, the next one on its way while they work on this
 // one.  (Two on their way: 80 and 77 us, but 214 and 280 for heads of 128, with one term.)  A wavefront has 64
 // keys of a tile with its 32 rows: ROWS = 128, the same ones for all, 64, either half of 128.
@@ -769,7 +769,7 @@ __device__ __forceinline__ v16f32 multiply_term(int m, const v8bf16 (&a)[3], con
 __device__ __forceinline__ float largest_or_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 // Bound by the matrix instructions and, next to them, by taking K and V apart and reading the terms: 16 x 512 tokens of 16 heads of 64, 17
-// Gflop in 112 us, 154 Tflop/s, what a large fp32 matrix product reaches on fp32's own matrix instructions.
+// Gflop in 110 to 119 us, 150 Tflop/s, what a large fp32 matrix product reaches on fp32's own matrix instructions.
 // As above; a wavefront has 32 keys of a tile with its 32 rows: ROWS = 128, the same ones for all, 64, either half of 64.
 template <int D, int ROWS>
 __global__ __launch_bounds__(kBlock, D == 128 ? 1 : 2) void attention_window_terms_kernel(WindowArgs a, int row_tiles, int pieces) {
@@ -963,7 +963,7 @@ struct Spread {
 };
 
 // Few rows, bound by reading K and V: 32 tokens over up to 4096 keys of 4 heads of 128 in fp16, 219 MB in 50 us (4.4 TB/s); 1 token over
-// 131072 keys of 2 heads, 134 MB in 25 us (5.3 TB/s), and 4.7 us for the join.  32 rows per workgroup, whose four wavefronts take every
+// 131072 keys of 2 heads, 134 MB in 26 us (5.2 TB/s), and 4.3 us for the join.  32 rows per workgroup, whose four wavefronts take every
 // fourth tile of 32 keys of this workgroup's piece of the axis; their sums meet in LDS, in wavefront order, and go out as results or, where
 // the axis is cut, as sums for the kernel below.
 template <typename T, int D, bool FEW>

@@ -330,7 +330,9 @@ __global__ __launch_bounds__(W * kWave) void dense_w4_kernel(DenseArgs<X, T> a) 
 
 // How many features a workgroup has: more make less of reading and taking apart x again, fewer fill the card.  Microseconds with 16 /
 // 32 / 64 features: 16 fp16 tokens, 8192 x 32768 (2048 units of 16 features and 16 tokens) 65 / 40 / 34; 33 tokens, 4096 x 4096 (768)
-// 12 / 12 / 8.6; 1 token, 4096 x 16384 (1024) 10.8 / 9.5 / 10.1, 4096 x 1024 (64) 4.4 / 5.1 / 7.3.
+// 12 / 12 / 8.6; 1 token, 4096 x 16384 (1024) 10.8 / 9.5 / 10.1, 4096 x 1024 (64) 4.4 / 5.1 / 7.3.  Up to 8 tokens, 16 features and sixteen
+// wavefronts / 32 and eight: 7 tokens, 4096 x 4100 (257) 7.6 / 6.3, 4096 x 5120 (320) 8.2 / 6.3, in 8 bits 7.6 / 6.0, in fp32 15 / 12, 4096 x
+// 8192 (512) 9.0 / 7.8; 1 token, 4096 x 4100 5.3 / 5.5, 1024 x 8192 3.7 / 3.8.
 template <typename X, typename T, int EACH>
 int run_dense_w4(const DenseArgs<X, T> &a, hipStream_t s) {
     const long long units = (long long) a.tiles * a.strips;

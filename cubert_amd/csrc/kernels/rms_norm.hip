@@ -8,8 +8,9 @@
 //     t = gamma * s,  m = max |t|,  code = rint(t * (127 / m)),  scale = m / (127 sqrt(mean(s^2) + eps)).
 //
 // The norm's factor is the same for a whole row, so it divides out of the codes: they follow from fp32 operations on
-// single elements and a maximum, and no order of a sum can move one across a border.  A row lives in registers between
-// the statistics and the results, so that the sum may be written over either input.
+// single elements and a maximum, and no order of a sum can move one across a border.  A thread keeps its part of a row between
+// the statistics and the results, so that the sum may be written over either input: in registers, but for rows of more than 4096 elements
+// that are no whole 16-byte pieces, which have 34 of them in scratch memory.
 
 #include "cubert_kernels.h"
 #include "device_common.h"
@@ -19,8 +20,8 @@ namespace {
 
 constexpr int kMaxHidden = 32768;
 
-// Bound by memory where there are many rows: fp16, 32768 x 1024 with a residual, 268 MB in 48 us, 5.6 TB/s (a large copy reaches 5.1);
-// fp32 in 8 bits, 4099 x 1000, 53 MB in 10.4 us, 5.1 TB/s.  A few rows are one read, two exchanges and one write behind each other:
+// Bound by memory where there are many rows: fp16, 32768 x 1024 with a residual, 268 MB in 49 us, 5.5 TB/s (a large copy reaches 5.1);
+// fp32 in 8 bits, 4099 x 1000, 53 MB in 10.2 us, 5.2 TB/s.  A few rows are one read, two exchanges and one write behind each other:
 // 1 x 768 1.8 us, 8 x 4096 in 8 bits 4.2 us.
 //
 // The largest, or a NaN where there is one (fmaxf takes the number).
@@ -140,6 +141,9 @@ int rms_norm(const T *x, const T *residual, const T *gamma, float eps, T *sum_ou
         RUN(kVec, 1, 4, 1) RUN(kVec, 2, 4, 1) RUN(kVec, 1, 16, 1) RUN(kVec, 4, 16, 1)
         if constexpr (sizeof(T) == 4) RUN(kVec, 8, 16, 1)
     }
+    // Rows of no whole 16-byte pieces, an element at a time; microseconds against rows of pieces as long: fp16, 4096 x 1001 13 and 8, 32768
+    // x 1025 200 and 53, 4096 x 4100 132 and 28; fp32, 4096 x 1001 16 and 14, 32768 x 1025 161 and 94, 1024 x 32767 195
+    // and 106.
     RUN(1, 4, 4, 1) RUN(1, 4, 16, 1) RUN(1, 32, 16, 1)
 #undef RUN
     return CUBERT_UNSUPPORTED;
