@@ -284,7 +284,8 @@ int cubert_dense_w4_i8_f16(void *stream, int tokens, int features, int in, const
  *   ctx[b, i, a, :] = sum_j softmax_j(alpha Q[b, i, a, :] . K[b, j, a', :]) V[b, j, a', :],  a' = a / (heads / kv_heads)
  * over the keys it sees.  A query that sees none, or that stands outside its sequence (p < 0 or p >= lengths[b]), gets
  * zeros; unlike in cubert_attention_fused_* a masked key is no key at all.  Scores, probabilities and sums are held in fp32, or in
- * two terms of 16 bits where a matrix product takes them: a result is rounded to the storage type once, however many rows are asked for.
+ * two or three terms of 16 bits where a matrix product takes them: a result is rounded to the storage type once, however many rows
+ * are asked for.
  * q is [batch * q_rows, heads * head_size] at ldq elements per row, k and v [batch * kv_rows, kv_heads * head_size] at ldkv
  * (kv_rows: the rows a sequence has in the cache, whatever its length), ctx like q at ld_ctx.  `first` (NULL: 0) and
  * `lengths` (NULL: kv_rows; larger ones count as kv_rows) are device arrays of `batch` ints, `mask` (NULL: all kept) is
