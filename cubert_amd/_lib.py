@@ -124,6 +124,9 @@ SIGNATURES = {
     "cubert_w4_packed_bytes": (ctypes.c_size_t, [ci, ci, ci]),
     "cubert_w4_pack": (ci, [vp, vp, ci, ci, ci, vp, vp]),
     "cubert_attention_window_partials": (ctypes.c_size_t, [ci, ci, ci, ci, ci, ci, ci, ci, ci, ci]),
+    "cubert_paged_extend": (ci, [vp, ci, ci, vp, vp, vp, vp, ci, ci, ci, ci, vp, vp, vp, vp]),
+    "cubert_paged_cut": (ci, [vp, ci, ci, vp, vp, vp, vp, ci, ci, ci, vp, vp, vp, vp]),
+    "cubert_attention_paged_partials": (ctypes.c_size_t, [ci, ci, ci, ci, ci, ci, ci, ci, ci, ci]),
     "cubert_blas_create": (vp, []),
     "cubert_blas_destroy": (ci, [vp]),
     "cubert_blas_set_stream": (ci, [vp, vp]),
@@ -162,6 +165,9 @@ for _t in ("f32", "f16"):
         "cubert_dense_w4_i8_" + _t: (ci, [vp, ci, ci, ci, vp, ci, vp, vp, ci, vp, ci, vp, ci]),
         "cubert_attention_window_" + _t: (ci, [vp, ci, vp, vp, ci, vp, vp, vp, vp, ci, cf, ci, ci, ci, ci, ci, ci, ci, ci, ci, vp,
                                                ctypes.c_size_t, vp]),
+        "cubert_paged_write_" + _t: (ci, [vp, vp, ci, vp, ci, vp, vp, cll, cll, cll, ci, ci, ci, ci, vp]),
+        "cubert_attention_paged_" + _t: (ci, [vp, ci, vp, vp, cll, cll, cll, vp, ci, ci, vp, vp, vp, ci, cf, ci, ci, ci, ci, ci, ci, ci, ci,
+                                              ci, vp, ctypes.c_size_t, vp]),
         "cubert_gemm_strided_batch_" + _t: (ci, [vp, ci, ci, ci, ci, ci, cf, vp, ci, cll, vp, ci, cll, cf, vp, ci, cll, ci]),
         "cubert_gemm_batch_" + _t: (ci, [vp, ci, ci, ci, ci, ci, cf, vp, ci, vp, ci, cf, vp, ci, ci]),
     })

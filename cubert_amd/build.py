@@ -28,6 +28,7 @@ HOST_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-command-line-a
 
 DEVICE_SOURCES = ["kernels/layernorm.hip", "kernels/softmax.hip", "kernels/elementwise.hip", "kernels/attention.hip", "kernels/gemm_skinny.hip", "kernels/dense_mid.hip", "kernels/dense_large.hip", "kernels/gemm_batch.hip", "kernels/split.hip",
                   "kernels/rms_norm.hip", "kernels/dense_w4.hip", "kernels/attention_window.hip",
+                  "kernels/paged_cache.hip", "kernels/attention_paged.hip",
                   "runtime.hip"]
 HOST_SOURCES = ["host/Transformer.cpp", "host/Bert.cpp", "host/BertM.cpp", "host/Graph.cpp", "host/tokenization.cpp",
                 "host/api.cpp"]

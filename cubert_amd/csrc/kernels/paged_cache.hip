@@ -1,0 +1,321 @@
+// A key/value cache in pages: which page of a sequence is which, where new tokens go, and keys and values on their way there.
+//
+//     page i of sequence b is table[b, i]; its token at position p has slot table[b, p / page] * page + p % page
+//
+// Pages of nobody stand on a stack, free[0 .. *free_count), and are taken from its top.
+
+#include "cubert_kernels.h"
+#include "device_common.h"
+#include "paged.h"
+
+namespace cubert {
+namespace {
+
+__device__ __forceinline__ int clamp_to(int x, int low, int high) { return x < low ? low : x > high ? high : x; }
+__device__ __forceinline__ int pages_of(int tokens, int shift) { return tokens == 0 ? 0 : ((tokens - 1) >> shift) + 1; }
+
+constexpr int kSpan = 1024;  // slots of a workgroup
+
+struct ExtendArgs {
+    int *table;
+    const int *lengths, *counts, *free, *free_count;
+    int *slots, *lengths_out, *free_out;
+    int width, ld_table, pages, shift, batch, rows;
+};
+
+// What a sequence has and asks for: `need` pages more for `count` tokens; none, and no tokens, where its table has no room for them.
+struct Growth {
+    int length, count, need;
+    bool fits;
+
+    __device__ __forceinline__ Growth(const ExtendArgs &a, int b) {
+        const int room = a.width << a.shift;
+        length = clamp_to(a.lengths[b], 0, room);
+        count = a.counts != nullptr ? clamp_to(a.counts[b], 0, a.rows) : a.rows;
+        fits = count <= room - length;
+        need = fits ? pages_of(length + count, a.shift) - pages_of(length, a.shift) : 0;
+    }
+};
+
+// The sum over a workgroup's threads.
+__device__ __forceinline__ int block_sum(int x, int *shared) {
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) x += __shfl_xor(x, d, kWave);
+    if ((threadIdx.x & (kWave - 1)) == 0) shared[threadIdx.x / kWave] = x;
+    __syncthreads();
+    int sum = 0;
+#pragma unroll
+    for (int w = 0; w < kBlock / kWave; ++w) sum += shared[w];
+    __syncthreads();
+    return sum;
+}
+
+// A sequence is served if it needs no page, or if all that is asked for up to it is there.  A workgroup has kSpan slots; it adds up what the
+// sequences before them ask for (a few bytes per sequence, which the cache has), so that none waits for another.
+__global__ __launch_bounds__(kBlock) void paged_extend_kernel(ExtendArgs a) {
+    __shared__ int shared[kBlock / kWave], starts[kSpan], lengths[kSpan], counts[kSpan];
+    const int rows = a.rows > 0 ? a.rows : 1, total = a.batch * rows, thread = threadIdx.x, lane = thread & (kWave - 1);
+    const int from = blockIdx.x * kSpan, until = total - from < kSpan ? total : from + kSpan;
+    const int first = from / rows, last = (until - 1) / rows;  // the sequences that these slots belong to
+    const int there = clamp_to(*a.free_count, 0, a.pages);
+    if (total == 0) {
+        if (thread == 0) *a.free_out = there;
+        return;
+    }
+    int before = 0;
+    for (int b = thread; b < first; b += kBlock) before += Growth(a, b).need;
+    before = block_sum(before, shared);
+    // sequences in runs of kSpan / kBlock to a thread
+    constexpr int kRun = kSpan / kBlock;
+    int need[kRun], sum = 0;
+#pragma unroll
+    for (int n = 0; n < kRun; ++n) {
+        const int at = thread * kRun + n;
+        need[n] = 0;
+        if (first + at <= last) {
+            const Growth g(a, first + at);
+            need[n] = g.need, lengths[at] = g.length, counts[at] = g.fits ? g.count : 0;
+        }
+        sum += need[n];
+    }
+    int through = sum;
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+        const int other = __shfl_up(through, d, kWave);
+        through += lane >= d ? other : 0;
+    }
+    if (lane == kWave - 1) shared[thread / kWave] = through;
+    __syncthreads();
+    int start = before + through - sum;
+#pragma unroll
+    for (int w = 0; w < kBlock / kWave; ++w)
+        if (w < thread / kWave) start += shared[w];
+#pragma unroll
+    for (int n = 0; n < kRun; ++n) {
+        const int at = thread * kRun + n, b = first + at;
+        if (b <= last) {
+            starts[at] = start;
+            const bool granted = need[n] == 0 || start + need[n] <= there;
+            if (!granted) counts[at] = 0;
+            // what stays on the stack is what the first one left that did not get its pages, or else the last one (several workgroups may
+            // have its slots, and all write this)
+            if (start <= there && (start + need[n] > there || b == a.batch - 1)) *a.free_out = there - start - (granted ? need[n] : 0);
+        }
+        start += need[n];
+    }
+    __syncthreads();
+    for (int i = from + thread; i < until; i += kBlock) {
+        const int b = i / rows, t = i - b * rows, at = b - first, length = lengths[at], count = counts[at];
+        if (t == 0) a.lengths_out[b] = length + count;
+        if (a.rows == 0) continue;
+        int slot = -1;
+        if (t < count) {
+            const int p = length + t, index = p >> a.shift, held = pages_of(length, a.shift);
+            int *entry = a.table + (size_t) b * a.ld_table + index;
+            int page;
+            if (index < held) {
+                page = *entry;
+            } else {
+                page = a.free[there - 1 - (starts[at] + index - held)];
+                if ((p & ((1 << a.shift) - 1)) == 0) *entry = page;
+            }
+            if (page >= 0 && page < a.pages) slot = (page << a.shift) + (p & ((1 << a.shift) - 1));
+        }
+        a.slots[i] = slot;
+    }
+}
+
+// ---- and back ---------------------------------------------------------------
+
+struct CutArgs {
+    const int *table, *lengths, *keep;
+    int *free;
+    const int *free_count;
+    int *lengths_out, *free_out, *returned;
+    int width, ld_table, pages, shift, batch;
+};
+
+struct Shrink {
+    int keep, begin, end;  // the entries of the table's row that go
+
+    __device__ __forceinline__ Shrink(const CutArgs &a, int b) {
+        const int length = clamp_to(a.lengths[b], 0, a.width << a.shift);
+        keep = a.keep != nullptr ? clamp_to(a.keep[b], 0, length) : 0;
+        begin = pages_of(keep, a.shift), end = pages_of(length, a.shift);
+    }
+};
+
+constexpr int kAhead = 8;  // entries of a lane that are on their way together
+
+// How many pages a sequence gives back: entries that are no pages (a window has passed them, and they were taken out) do not count.
+__global__ __launch_bounds__(kBlock) void paged_cut_count_kernel(CutArgs a) {
+    const int b = blockIdx.x * (kBlock / kWave) + wave_in_block(), lane = threadIdx.x & (kWave - 1);
+    if (b >= a.batch) return;
+    const Shrink s(a, b);
+    const int *row = a.table + (size_t) b * a.ld_table;
+    int count = 0;
+    for (int i = s.begin + lane; i < s.end; i += kWave * kAhead) {
+        int page[kAhead];
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n) page[n] = i + n * kWave < s.end ? row[i + n * kWave] : -1;
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n) count += page[n] >= 0 && page[n] < a.pages ? 1 : 0;
+    }
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) count += __shfl_xor(count, d, kWave);
+    if (lane == 0) a.returned[b] = count, a.lengths_out[b] = s.keep;
+}
+
+// A wavefront per sequence puts them onto the stack, behind those of the sequences before it.
+__global__ __launch_bounds__(kBlock) void paged_cut_kernel(CutArgs a) {
+    const int b = blockIdx.x * (kBlock / kWave) + wave_in_block(), lane = threadIdx.x & (kWave - 1);
+    const int there = clamp_to(*a.free_count, 0, a.pages);
+    if (a.batch == 0 && blockIdx.x == 0 && threadIdx.x == 0) *a.free_out = there;
+    if (b >= a.batch) return;
+    const Shrink s(a, b);
+    long long before = 0;
+    for (int i = lane; i < b; i += kWave) before += a.returned[i];
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) before += __shfl_xor(before, d, kWave);
+    const long long height = there + before;
+    if (b == a.batch - 1 && lane == 0) {
+        const long long all = height + a.returned[b];
+        *a.free_out = (int) (all < a.pages ? all : a.pages);
+    }
+    const int *row = a.table + (size_t) b * a.ld_table;
+    const int free_places = height < a.pages ? a.pages - (int) height : 0;
+    int *to = a.free + height;
+    int at = 0;
+    for (int base = s.begin; base < s.end && at < free_places; base += kWave * kAhead) {
+        int page[kAhead];
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n) {
+            const int i = base + n * kWave + lane;
+            page[n] = i < s.end ? row[i] : -1;
+        }
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n) {
+            const bool is = page[n] >= 0 && page[n] < a.pages;
+            const unsigned long long all = __ballot(is);
+            const int place = at + __builtin_popcountll(all & ((1ull << lane) - 1));
+            if (is && place < free_places) to[place] = page[n];
+            at += __builtin_popcountll(all);
+        }
+    }
+}
+
+// ---- rows into pages ----------------------------------------------------------
+
+struct WriteArgs {
+    const char *k, *v;
+    char *k_pages, *v_pages;
+    const int *slots;
+    long long page_bytes, head_bytes, row_bytes, from_bytes;
+    unsigned tokens, slots_there;
+    int shift, pieces_of_head, pieces;  // of 16 bytes, of a head and of all of a token's
+};
+
+__global__ __launch_bounds__(kBlock) void paged_write_kernel(WriteArgs a) {
+    const unsigned long long i = (unsigned long long) blockIdx.x * kBlock + threadIdx.x;
+    const unsigned token = (unsigned) (i / (unsigned) a.pieces);
+    if (token >= a.tokens) return;
+    const int piece = (int) (i - (unsigned long long) token * a.pieces), head = piece / a.pieces_of_head;
+    const unsigned slot = (unsigned) a.slots[token];
+    if (slot >= a.slots_there) return;  // (a negative one is a large one)
+    const long long from = token * a.from_bytes + (long long) piece * 16;
+    const long long to = (long long) (slot >> a.shift) * a.page_bytes + (long long) (slot & ((1u << a.shift) - 1)) * a.row_bytes +
+                         head * a.head_bytes + (piece - head * a.pieces_of_head) * 16;
+    const Vec<float, 4> x = load_vec<float, 4>((const float *) (a.k + from)), y = load_vec<float, 4>((const float *) (a.v + from));
+    store_vec<float, 4>((float *) (a.k_pages + to), x);
+    store_vec<float, 4>((float *) (a.v_pages + to), y);
+}
+
+// What extend and cut have in common: sizes of tables and pages that 32 bits count.
+int check_tables(const void *table, int width, int ld_table, const void *lengths, const void *free, const void *free_count, int pages, int page, int batch,
+                 const void *lengths_out, const void *free_out) {
+    if (width < 1 || ld_table < width || pages < 1 || page < 1 || batch < 0) return CUBERT_BAD_ARGUMENT;
+    if (free == nullptr || free_count == nullptr || free_out == nullptr || free_out == free_count) return CUBERT_BAD_ARGUMENT;
+    if (batch > 0 && (table == nullptr || lengths == nullptr || lengths_out == nullptr || lengths_out == lengths)) return CUBERT_BAD_ARGUMENT;
+    if ((page & (page - 1)) != 0) return CUBERT_UNSUPPORTED;
+    const long long most = (1ll << 31) - 1;
+    if ((long long) width * page > most || (long long) pages * page > most) return CUBERT_UNSUPPORTED;
+    return 0;
+}
+
+int paged_write(const void *k, const void *v, int ld, const int *slots, int tokens, void *k_pages, void *v_pages, long long page_stride,
+                long long head_stride, long long row_stride, int pages, int page, int kv_heads, int head_size, int element, void *stream) {
+    if (tokens < 0 || pages < 1 || page < 1 || kv_heads < 1 || head_size < 1 || ld < (long long) kv_heads * head_size) return CUBERT_BAD_ARGUMENT;
+    if (!cubert::pages_apart(page_stride, head_stride, row_stride, pages, kv_heads, page, head_size)) return CUBERT_BAD_ARGUMENT;
+    if (tokens == 0) return 0;
+    if (k == nullptr || v == nullptr || slots == nullptr || k_pages == nullptr || v_pages == nullptr) return CUBERT_BAD_ARGUMENT;
+    if ((page & (page - 1)) != 0 || (long long) pages * page >= 1ll << 31) return CUBERT_UNSUPPORTED;
+    const int piece = 16 / element;
+    if (!is_aligned(k, 16) || !is_aligned(v, 16) || !is_aligned(k_pages, 16) || !is_aligned(v_pages, 16) || ld % piece != 0 || head_size % piece != 0 ||
+        page_stride % piece != 0 || head_stride % piece != 0 || row_stride % piece != 0)
+        return CUBERT_UNSUPPORTED;
+    WriteArgs a;
+    a.k = (const char *) k, a.v = (const char *) v, a.k_pages = (char *) k_pages, a.v_pages = (char *) v_pages, a.slots = slots;
+    a.page_bytes = page_stride * element, a.head_bytes = head_stride * element, a.row_bytes = row_stride * element;
+    a.from_bytes = (long long) ld * element;
+    a.tokens = (unsigned) tokens, a.slots_there = (unsigned) pages * (unsigned) page;
+    a.shift = __builtin_ctz((unsigned) page);
+    a.pieces_of_head = head_size / piece, a.pieces = kv_heads * a.pieces_of_head;
+    const unsigned long long blocks = ((unsigned long long) tokens * a.pieces + kBlock - 1) / kBlock;
+    if (blocks >= 1u << 24) return CUBERT_UNSUPPORTED;  // (a launch holds less than 2^32 threads)
+    return launch(paged_write_kernel, dim3((unsigned) blocks), dim3(kBlock), (hipStream_t) stream, a);
+}
+
+}  // namespace
+}  // namespace cubert
+
+extern "C" {
+
+int cubert_paged_extend(int *table, int width, int ld_table, const int *lengths, const int *counts, const int *free, const int *free_count, int pages,
+                        int page, int batch, int rows, int *slots, int *lengths_out, int *free_out, void *stream) {
+    using namespace cubert;
+    if (rows < 0) return CUBERT_BAD_ARGUMENT;
+    const int rc = check_tables(table, width, ld_table, lengths, free, free_count, pages, page, batch, lengths_out, free_out);
+    if (rc != 0) return rc;
+    if (batch > 0 && rows > 0 && slots == nullptr) return CUBERT_BAD_ARGUMENT;
+    const long long total = (long long) batch * (rows > 0 ? rows : 1);
+    if (total > (1ll << 31) - 1 - kSpan) return CUBERT_UNSUPPORTED;
+    ExtendArgs a;
+    a.table = table, a.lengths = lengths, a.counts = counts, a.free = free, a.free_count = free_count;
+    a.slots = slots, a.lengths_out = lengths_out, a.free_out = free_out;
+    a.width = width, a.ld_table = ld_table, a.pages = pages, a.shift = __builtin_ctz((unsigned) page), a.batch = batch, a.rows = rows;
+    const unsigned blocks = total > 0 ? (unsigned) ((total + kSpan - 1) / kSpan) : 1;
+    return launch(paged_extend_kernel, dim3(blocks), dim3(kBlock), (hipStream_t) stream, a);
+}
+
+int cubert_paged_cut(const int *table, int width, int ld_table, const int *lengths, const int *keep, int *free, const int *free_count, int pages,
+                     int page, int batch, int *lengths_out, int *free_out, int *work, void *stream) {
+    using namespace cubert;
+    const int rc = check_tables(table, width, ld_table, lengths, free, free_count, pages, page, batch, lengths_out, free_out);
+    if (rc != 0) return rc;
+    if (batch > 0 && work == nullptr) return CUBERT_BAD_ARGUMENT;
+    if (batch > 1 << 25) return CUBERT_UNSUPPORTED;
+    CutArgs a;
+    a.table = table, a.lengths = lengths, a.keep = keep, a.free = free, a.free_count = free_count;
+    a.lengths_out = lengths_out, a.free_out = free_out, a.returned = work;
+    a.width = width, a.ld_table = ld_table, a.pages = pages, a.shift = __builtin_ctz((unsigned) page), a.batch = batch;
+    constexpr int kEach = kBlock / kWave;
+    const unsigned blocks = batch > 0 ? (unsigned) ((batch + kEach - 1) / kEach) : 1;
+    if (batch > 0) {
+        const int failed = launch(paged_cut_count_kernel, dim3(blocks), dim3(kBlock), (hipStream_t) stream, a);
+        if (failed != 0) return failed;
+    }
+    return launch(paged_cut_kernel, dim3(blocks), dim3(kBlock), (hipStream_t) stream, a);
+}
+
+int cubert_paged_write_f32(const float *k, const float *v, int ld, const int *slots, int tokens, float *k_pages, float *v_pages, long long page_stride,
+                           long long head_stride, long long row_stride, int pages, int page, int kv_heads, int head_size, void *stream) {
+    return cubert::paged_write(k, v, ld, slots, tokens, k_pages, v_pages, page_stride, head_stride, row_stride, pages, page, kv_heads, head_size, 4, stream);
+}
+
+int cubert_paged_write_f16(const cubert_half *k, const cubert_half *v, int ld, const int *slots, int tokens, cubert_half *k_pages, cubert_half *v_pages,
+                           long long page_stride, long long head_stride, long long row_stride, int pages, int page, int kv_heads, int head_size,
+                           void *stream) {
+    return cubert::paged_write(k, v, ld, slots, tokens, k_pages, v_pages, page_stride, head_stride, row_stride, pages, page, kv_heads, head_size, 2, stream);
+}
+
+}  // extern "C"

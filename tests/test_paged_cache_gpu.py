@@ -1,0 +1,816 @@
+"""A key/value cache in pages against its definition: tables and slots, which are whole numbers, against a plain walk through the sequences;
+rows in pages bit for bit; attention over pages against its formula in 64 bits; and a run of them as a server makes it.
+
+Tolerances count roundings.  u = 2^-24 is half a step of fp32 relative to the value, 2^-11 of fp16; a sum of n terms that
+are added in fp32 in any order is off by at most (n - 1) u times the sum of their magnitudes."""
+import math
+import random
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+U = 2.0 ** -24
+HALF = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11}
+SMALL = {torch.float32: 2.0 ** -149, torch.float16: 2.0 ** -25}   # half a step among the subnormals
+TYPES = {"f32": torch.float32, "f16": torch.float16}
+
+
+@pytest.fixture(scope="module")
+def K():
+    if not torch.cuda.is_available():
+        pytest.fail("no GPU visible: the -m gpu tests must run on the MI355X box")
+    from cubert_amd import kernels
+    return kernels
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def normal(g, *shape):
+    return torch.randn(*shape, generator=g, device="cuda")
+
+
+def ints(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def up(n, page):
+    return -(-n // page)
+
+
+# ---------------------------------------------------------------------------- tables
+
+
+def extend_reference(table, lengths, counts, free, free_count, page, rows):
+    """What paged_extend gives, by a walk through the sequences: (slots, lengths, free_count, table)."""
+    width, pages = len(table[0]) if table else 1, len(free)
+    table, after = [list(r) for r in table], []
+    top, refused = min(max(free_count, 0), pages), False
+    slots = [[-1] * rows for _ in lengths]
+    for b, n in enumerate(lengths):
+        n = min(max(n, 0), width * page)
+        count = min(max(counts[b], 0), rows) if counts is not None else rows
+        after.append(n)
+        if n + count > width * page:
+            continue
+        need = up(n + count, page) - up(n, page)
+        refused = refused or need > top
+        if refused and need:
+            continue
+        for i in range(up(n, page), up(n + count, page)):
+            top -= 1
+            table[b][i] = free[top]
+        after[b] += count
+        for t in range(count):
+            own = table[b][(n + t) // page]
+            slots[b][t] = own * page + (n + t) % page if 0 <= own < pages else -1
+    return slots, after, top, table
+
+
+def cut_reference(table, lengths, keep, free, free_count, page):
+    """(lengths, free_count, free) of paged_cut."""
+    width, pages = len(table[0]) if table else 1, len(free)
+    free, top, after = list(free), min(max(free_count, 0), pages), []
+    for b, n in enumerate(lengths):
+        n = min(max(n, 0), width * page)
+        left = min(max(keep[b], 0), n) if keep is not None else 0
+        after.append(left)
+        for i in range(up(left, page), up(n, page)):
+            if 0 <= table[b][i] < pages and top < pages:
+                free[top] = table[b][i]
+                top += 1
+    return after, top, free
+
+
+def tables(seed, batch, width, page, pages, longest, held=True):
+    """Lengths up to `longest`, a table with pages that belong to nobody else, and a stack of the others."""
+    r = random.Random(seed)
+    order = list(range(pages))
+    r.shuffle(order)
+    lengths = [r.randint(0, longest) for _ in range(batch)]
+    table = [[-1] * width for _ in range(batch)]
+    for b in range(batch):
+        for i in range(up(lengths[b], page)):
+            table[b][i] = order.pop()
+    return table, lengths, order + [-7] * (pages - len(order)), len(order)
+
+
+# batch, rows, width, page, longest, pages to spare (of the stack), counts
+EXTEND = {
+    "one token": (1, 1, 4, 16, 40, 5, "rows"),
+    "one token that needs a page": (1, 1, 4, 1, 3, 5, "rows"),
+    "steps": (300, 1, 9, 16, 143, 300, "any"),
+    "steps of nobody": (40, 1, 9, 16, 100, 10, "none"),
+    "steps of four": (77, 4, 12, 16, 150, 100, "any"),
+    "short stack": (100, 5, 12, 4, 40, 30, "any"),
+    "empty stack": (100, 3, 12, 16, 150, 0, "any"),
+    "full tables": (64, 9, 5, 8, 40, 500, "any"),
+    "full tables and a short stack": (1500, 2, 5, 2, 10, 400, "any"),
+    "prompts": (7, 1000, 70, 16, 90, 700, "any"),
+    "prompts and a short stack": (9, 1000, 200, 16, 2000, 250, "any"),
+    "long prompts": (3, 5000, 400, 32, 7000, 500, "rows"),
+    "pages of one": (33, 20, 50, 1, 30, 660, "any"),
+    "large pages": (20, 300, 3, 1024, 2500, 20, "any"),
+    "many sequences": (5000, 1, 3, 16, 47, 5000, "any"),
+    "counts beyond the rows": (50, 6, 9, 16, 100, 100, "wild"),
+    "no rows": (20, 0, 4, 16, 60, 10, "any"),
+    "exactly one workgroup": (1024, 1, 4, 16, 60, 1024, "rows"),
+    "exactly two workgroups": (2, 1024, 70, 16, 60, 200, "rows"),
+}
+
+
+def counts_of(kind, batch, rows, seed):
+    r = random.Random(seed + 1)
+    if kind == "rows":
+        return None
+    if kind == "none":
+        return [0] * batch
+    if kind == "wild":
+        return [r.choice((-5, rows + 3, 1 << 30, -(1 << 31), (1 << 31) - 1, r.randint(0, rows))) for _ in range(batch)]
+    return [r.choice((0, rows, r.randint(0, rows))) for _ in range(batch)]
+
+
+@pytest.mark.parametrize("name", list(EXTEND))
+def test_extend(K, name):
+    batch, rows, width, page, longest, spare, kind = EXTEND[name]
+    table, lengths, _, _ = tables(len(name), batch, width, page, batch * width, longest)
+    pages = sum(up(n, page) for n in lengths) + spare + 3
+    table, lengths, free, there = tables(len(name), batch, width, page, pages, longest)
+    there = min(there, spare)
+    counts = counts_of(kind, batch, rows, len(name))
+    on = [ints(table), ints(lengths), None if counts is None else ints(counts), ints(free), ints([there])]
+    before = [None if x is None else x.clone() for x in on]
+    slots, after, left = K.paged_extend(*on, page, rows)
+    want = extend_reference(table, lengths, counts, free, there, page, rows)
+    assert slots.tolist() == want[0] and after.tolist() == want[1] and left.tolist() == [want[2]] and on[0].tolist() == want[3]
+    for x, y in zip(on[1:], before[1:]):                   # what it reads stays as it is
+        assert x is None or torch.equal(x, y)
+    assert [x.tolist() for x in K.paged_extend(*on, page, rows)] == [x.tolist() for x in (slots, after, left)]  # (and so a call may be repeated)
+
+
+def test_extend_of_what_no_program_hands_over(K):
+    """Lengths, heights and pages outside their ranges: cut to what there is, and never followed."""
+    page, low, high = 16, -(1 << 31), (1 << 31) - 1
+    table = [[5, -1, 3, 2], [high, low, 1, 0], [10, 9, 8, 7], [4, 4, 4, 4], [0, 1, 2, 3]]
+    lengths, counts = [low, 20, high, 17, 30], [3, 40, 1, 4, 34]
+    free = [6, -1, 11, high, low, 20, 0, 1, 2, 3, 4, 5]
+    for there in (12, 6, 4, 0, -5, high):
+        got_table = ints(table)
+        slots, after, left = K.paged_extend(got_table, ints(lengths), ints(counts), ints(free), ints([there]), page, 40)
+        want = extend_reference(table, lengths, counts, free, there, page, 40)
+        assert (slots.tolist(), after.tolist(), left.tolist()[0], got_table.tolist()) == want
+
+
+def test_tables_with_rows_apart(K):
+    """Tables that are a part of a larger one."""
+    table, lengths, free, there = tables(5, 30, 6, 16, 400, 70)
+    whole = torch.full((30, 11), -9, dtype=torch.int32, device="cuda")
+    part = whole[:, 2:8]
+    part.copy_(ints(table))
+    want = extend_reference(table, lengths, None, free, there, 16, 20)
+    slots, after, left = K.paged_extend(part, ints(lengths), None, ints(free), ints([there]), 16, 20)
+    assert (slots.tolist(), after.tolist(), left.tolist()[0], part.tolist()) == want
+    assert bool((whole[:, :2] == -9).all()) and bool((whole[:, 8:] == -9).all())
+    stack = ints(free)
+    after, left = K.paged_cut(part, ints(lengths), None, stack, ints([there]), 16)
+    assert (after.tolist(), left.tolist()[0], stack.tolist()) == cut_reference(want[3], lengths, None, free, there, 16)
+    assert part.tolist() == want[3] and bool((whole[:, 8:] == -9).all())
+
+
+def test_tables_of_nobody(K):
+    for call in (lambda t, n, f, c: K.paged_extend(t, n, n, f, c, 16, 3)[1:], lambda t, n, f, c: K.paged_cut(t, n, n, f, c, 16)):
+        for there in (3, 9, -4, 100):
+            after, left = call(torch.zeros(0, 4, dtype=torch.int32, device="cuda"), ints([]), ints([0] * 9), ints([there]))
+            assert after.shape == (0,) and left.tolist() == [min(max(there, 0), 9)]
+
+
+CUT = {
+    "one page": (1, 4, 16, 16, "none"),
+    "a few end": (8, 40, 16, 600, "few"),
+    "all end": (300, 20, 8, 160, "none"),
+    "proposals": (100, 12, 16, 190, "near"),
+    "anything": (70, 50, 4, 200, "any"),
+    "one long": (1, 9000, 16, 140000, "any"),
+    "few long": (5, 3000, 16, 48000, "none"),
+    "many": (3000, 3, 16, 48, "any"),
+    "pages of one": (20, 300, 1, 300, "any"),
+    "wild": (200, 7, 16, 100, "wild"),
+}
+
+
+@pytest.mark.parametrize("name", list(CUT))
+@pytest.mark.parametrize("holes", [False, True])
+def test_cut(K, name, holes):
+    batch, width, page, longest, kind = CUT[name]
+    r = random.Random(len(name))
+    table, lengths, free, there = tables(len(name), batch, width, page, batch * width + 9, longest)
+    if holes:                                              # pages that a window has passed, and entries that are nothing
+        for b in range(batch):
+            for i in range(width):
+                if r.random() < 0.3:
+                    table[b][i] = r.choice((-1, -(1 << 31), len(free), (1 << 31) - 1))
+    keep = {"none": [0] * batch, "few": [n if r.random() < 0.8 else 0 for n in lengths], "near": [n - r.randint(0, 5) for n in lengths],
+            "any": [r.randint(0, n) for n in lengths], "wild": [r.choice((-1, 1 << 30, n + 1, -(1 << 31))) for n in lengths]}[kind]
+    if kind == "none" and holes:
+        keep = None
+    stack, on = ints(free), (ints(table), ints(lengths))
+    after, left = K.paged_cut(*on, None if keep is None else ints(keep), stack, ints([there]), page)
+    want = cut_reference(table, lengths, keep, free, there, page)
+    assert after.tolist() == want[0] and left.tolist() == [want[1]] and stack.tolist() == want[2]
+    assert on[0].tolist() == table and on[1].tolist() == lengths
+
+
+def test_cut_of_more_than_the_stack_holds(K):
+    """Tables that have a page twice, and heights that are none: what there is no room for is left out, and nothing is written elsewhere."""
+    table = [[i % 10 for i in range(30)] for _ in range(7)]
+    lengths = [300, 480, 17, 480, (1 << 31) - 1, -3, 480]
+    for there in (0, 8, 10, 40, -1):
+        room = torch.full((30,), -8, dtype=torch.int32, device="cuda")
+        stack = room[10:20]
+        after, left = K.paged_cut(ints(table), ints(lengths), None, stack, ints([there]), 16)
+        want = cut_reference(table, lengths, None, [-8] * 10, there, 16)
+        assert after.tolist() == want[0] and left.tolist() == [want[1]] and stack.tolist() == want[2]
+        assert bool((room[:10] == -8).all()) and bool((room[20:] == -8).all())
+
+
+@pytest.mark.parametrize("page", [1, 16, 64])
+def test_pages_come_and_go(K, page):
+    """Steps of a server, growing and cutting back: no page belongs to two, none is lost."""
+    r = random.Random(page)
+    batch, width, pages = 40, 12, 200
+    table, stack, count = torch.full((batch, width), -1, dtype=torch.int32, device="cuda"), ints(list(range(pages))), ints([pages])
+    lengths = ints([0] * batch)
+    for step in range(25):
+        rows = r.choice((1, 1, 4, 3 * page))
+        counts = [r.randint(0, rows) for _ in range(batch)]
+        want = extend_reference(table.tolist(), lengths.tolist(), counts, stack.tolist(), int(count), page, rows)
+        slots, lengths, count = K.paged_extend(table, lengths, ints(counts), stack, count, page, rows)
+        assert (slots.tolist(), lengths.tolist(), int(count), table.tolist()) == want
+        keep = [r.choice((n, n, n - 1, 0, r.randint(0, max(n, 1)))) for n in want[1]]
+        want = cut_reference(want[3], want[1], keep, stack.tolist(), want[2], page)
+        lengths, count = K.paged_cut(table, lengths, ints(keep), stack, count, page)
+        assert (lengths.tolist(), int(count), stack.tolist()) == want
+        held = [p for row, n in zip(table.tolist(), lengths.tolist()) for p in row[:up(n, page)]]
+        assert sorted(held + stack.tolist()[:int(count)]) == list(range(pages))
+
+
+# ---------------------------------------------------------------------------- rows into pages
+
+
+def pool_of(layout, pages, kv_heads, page, size, t, seed):
+    """Two pools [pages, kv_heads, page, size] in memory as `layout` has it, and all of the memory around them."""
+    g = gen(seed)
+    if layout == "heads":
+        whole = normal(g, 2, pages, kv_heads, page, size).to(t)
+        return whole[0], whole[1], whole
+    if layout == "tokens":
+        whole = normal(g, 2, pages, page, kv_heads, size).to(t)
+        return whole[0].transpose(1, 2), whole[1].transpose(1, 2), whole
+    if layout == "by turns":                               # keys and values of a page behind each other
+        whole = normal(g, pages, 2, kv_heads, page, size).to(t)
+        return whole[:, 0], whole[:, 1], whole
+    if layout == "heads first":
+        whole = normal(g, 2, kv_heads, pages, page, size).to(t)
+        return whole[0].transpose(0, 1), whole[1].transpose(0, 1), whole
+    assert layout == "apart"                               # rows with something between them
+    whole = normal(g, 2, pages + 1, kv_heads + 1, page + 3, size + 8).to(t)
+    return whole[0, 1:, :kv_heads, 2:page + 2, :size], whole[1, 1:, :kv_heads, 2:page + 2, :size], whole
+
+
+LAYOUTS = ["heads", "tokens", "by turns", "heads first", "apart"]
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("batch,rows,heads,kv_heads,size,page", [(1, 1, 1, 1, 64, 16), (3, 1, 4, 2, 128, 16), (2, 37, 4, 4, 32, 1), (5, 200, 2, 12, 64, 32),
+                                                                 (1, 3, 1, 3, 8, 4), (2, 50, 3, 1, 80, 64)])
+def test_write(K, layout, t, batch, rows, heads, kv_heads, size, page):
+    t, g = TYPES[t], gen(rows)
+    pages = up(2 * batch * rows, page) + 2
+    k_pages, v_pages, whole = pool_of(layout, pages, kv_heads, page, size, t, 3)
+    packed = normal(g, batch, rows, heads + 2 * kv_heads, size).to(t)
+    k, v = packed[:, :, heads:heads + kv_heads], packed[:, :, heads + kv_heads:]
+    slots = torch.randperm(pages * page, generator=g, device="cuda")[:batch * rows].int().view(batch, rows)
+    slots.view(-1)[1::5] = -1
+    if batch * rows > 20:                                  # slots that no pool has
+        slots.view(-1)[[2, 7, 12]] = ints([pages * page, (1 << 31) - 1, -(1 << 31)])
+    want_k, want_v, want = pool_of(layout, pages, kv_heads, page, size, t, 3)
+    for b in range(batch):
+        for i in range(rows):
+            s = int(slots[b, i])
+            if 0 <= s < pages * page:
+                want_k[s // page, :, s % page], want_v[s // page, :, s % page] = k[b, i], v[b, i]
+    assert K.paged_write(k, v, slots, k_pages, v_pages) is not None
+    assert torch.equal(whole, want)                        # and nothing else has changed
+
+
+def test_write_refuses(K):
+    pool, q = torch.zeros(4, 2, 16, 64, device="cuda"), torch.zeros(2, 3, 4, 64, device="cuda")
+    slots = torch.zeros(2, 3, dtype=torch.int32, device="cuda")
+    assert K.paged_write(q[:, :, :2, :], q[:, :, 2:], slots - 1, pool, pool + 0) is not None
+    assert K.paged_write(q[:0, :, :2], q[:0, :, 2:], slots[:0], pool, pool + 0) is not None
+    odd = torch.zeros(2, 3, 2, 66, device="cuda")
+    assert K.paged_write(odd, odd, slots, torch.zeros(4, 2, 16, 66, device="cuda"), torch.zeros(4, 2, 16, 66, device="cuda")) is None
+    whole = torch.zeros(4 * 2 * 16 * 64 + 1, device="cuda")[1:].view(4, 2, 16, 64)
+    assert K.paged_write(q[:, :, :2], q[:, :, 2:], slots, whole, whole) is None
+    with pytest.raises(RuntimeError):                      # all heads of a page in one place
+        K.paged_write(q[:, :, :2], q[:, :, 2:], slots, pool[:, :1].expand(4, 2, 16, 64), pool[:, :1].expand(4, 2, 16, 64))
+
+
+# ---------------------------------------------------------------------------- attention over pages
+
+# batch, q_rows, heads, kv_heads, page, left, sinks, lengths, first (None: the last ones)
+ATTENTION = {
+    "one key": (1, 1, 1, 1, 16, -1, 0, (1,), None),
+    "one query": (2, 1, 4, 2, 16, -1, 0, (300, 77), None),
+    "no keys": (3, 1, 4, 1, 16, -1, 0, (0, 5, 0), None),
+    "nobody": (2, 1, 12, 12, 16, -1, 0, (0, 0), None),
+    "around a page": (9, 1, 3, 3, 16, -1, 0, (15, 16, 17, 31, 32, 33, 1, 2, 64), None),
+    "around large pages": (6, 1, 8, 2, 64, -1, 0, (63, 64, 65, 127, 129, 300), None),
+    "a few tokens": (4, 5, 8, 2, 16, -1, 0, (1000, 999, 64, 5), None),
+    "seven heads to one": (3, 3, 7, 1, 32, 50, 4, (333, 100, 2), None),
+    "many heads to one": (2, 1, 40, 1, 16, -1, 0, (500, 40), None),
+    "many rows": (2, 9, 16, 2, 16, 100, 1, (700, 7), None),
+    "a window": (3, 1, 4, 2, 16, 40, 0, (500, 41, 12), None),
+    "a window and sinks": (3, 2, 4, 2, 16, 100, 5, (500, 300, 12), None),
+    "a window of one": (2, 4, 2, 2, 16, 0, 0, (100, 17), None),
+    "sinks alone": (2, 3, 2, 1, 16, 0, 40, (300, 35), None),
+    "sinks up to the window": (2, 1, 2, 1, 16, 20, 70, (90, 95), None),
+    "sinks of everything": (2, 2, 4, 4, 32, 3, 1000, (90, 200), None),
+    "before the sequence": (3, 20, 2, 2, 16, 10, 1, (64, 7, 0), None),
+    "padded tokens": (4, 6, 4, 2, 16, -1, 0, (50, 51, 52, 53), (44, 50, 52, 60)),
+    "tokens in the middle": (2, 3, 4, 2, 16, 30, 2, (200, 100), (90, 20)),
+    "long": (1, 1, 4, 1, 16, -1, 0, (4999,), None),
+    "long of two heads": (2, 1, 16, 2, 128, -1, 0, (9000, 100), None),
+    "long window": (2, 2, 8, 1, 256, 4095, 4, (9000, 4500), None),
+    "unlike lengths": (33, 1, 4, 4, 16, -1, 0, tuple((37 * i * i) % 1500 for i in range(33)), None),
+    "many short": (300, 1, 2, 2, 16, -1, 0, tuple(i % 40 for i in range(300)), None),
+    "many and one long": (70, 1, 2, 1, 16, -1, 0, (3000,) + (3,) * 69, None),
+    "many and a long one at the end": (260, 1, 4, 2, 16, -1, 0, (3,) * 259 + (5000,), None),
+    "a prompt": (2, 130, 4, 2, 16, -1, 0, (130, 100), None),
+}
+
+
+def paged(name, t, size, layout="heads", seed=0, wide=3):
+    """Inputs of a case, and its keys and values as they would stand without pages."""
+    batch, q_rows, heads, kv_heads, page, left, sinks, lengths, first = ATTENTION[name]
+    g = gen(seed + size + len(name))
+    longest = max(max(lengths), 1)
+    width = up(longest, page) + wide
+    pages = sum(up(n, page) for n in lengths) + 3
+    q = normal(g, batch, q_rows, heads, size).to(t)
+    k, v = (normal(g, batch, longest, kv_heads, size).to(t) for _ in "kv")
+    order = torch.randperm(pages, generator=g, device="cuda").int().tolist()
+    rows = []
+    for n in lengths:
+        rows.append([order.pop() for _ in range(up(n, page))])
+        rows[-1] += [-1] * (width - len(rows[-1]))
+    table = ints(rows)
+    k_pages, v_pages, _ = pool_of(layout, pages, kv_heads, page, size, t, seed + 1)
+    for b, n in enumerate(lengths):
+        at = torch.arange(n, device="cuda")
+        own = table[b].long()[at // page]
+        k_pages[own, :, at % page], v_pages[own, :, at % page] = k[b, :n], v[b, :n]
+    at = dict(left=left, sinks=sinks, lengths=ints(lengths), first=None if first is None else ints(first))
+    return q, k_pages, v_pages, table, k, v, page, at
+
+
+def visible(q, k, page, left, sinks, lengths, first, table=None, pages=None):
+    """[batch, q_rows, keys]"""
+    q_rows, keys = q.shape[1], k.shape[1]
+    n = lengths.long()[:, None, None]
+    p = ((n[:, 0] - q_rows if first is None else first.long()[:, None]) + torch.arange(q_rows, device="cuda"))[:, :, None]
+    j = torch.arange(keys, device="cuda")
+    seen = (j <= p) & (j < n) & (p >= 0) & (p < n)
+    if left >= 0:
+        seen = seen & ((j >= p - left) | (j < sinks))
+    if table is not None:
+        there = (table >= 0) & (table < pages)
+        seen = seen & there.repeat_interleave(page, 1)[:, None, :keys]
+    return seen
+
+
+def reference(q, k, v, seen, alpha=None):
+    """The formula in 64 bits, and how far a kernel may be off it."""
+    t, size = q.dtype, q.shape[3]
+    alpha = size ** -0.5 if alpha is None else alpha
+    share = q.shape[2] // k.shape[2]
+    hold = seen.any(1)[:, :, None, None]                   # keys that nobody sees may hold anything
+    k, v = torch.where(hold, k, 0), torch.where(hold, v, 0)
+    seen = seen[:, None]
+    Q, KT = q.double().permute(0, 2, 1, 3), k.double().repeat_interleave(share, 2).permute(0, 2, 3, 1)
+    V = v.double().repeat_interleave(share, 2).permute(0, 2, 1, 3)
+    z = torch.where(seen, (Q @ KT) * alpha, -math.inf)
+    top = z.amax(3, keepdim=True)
+    e = torch.where(seen, torch.exp(z - torch.where(top == -math.inf, 0.0, top)), 0.0)
+    total = e.sum(3, keepdim=True)
+    some = torch.where(total > 0, total, 1.0)
+    out = (e @ V) / some
+    # A score is a sum of `size` products of which each is rounded once and each sum once, 2 size u of the products' magnitudes; the factor
+    # alpha log2(e) has 2 roundings, the difference to a maximum one and its product with the factor one, of at most twice the largest.
+    products = (Q.abs() @ KT.abs()) * abs(alpha)
+    slip = torch.where(seen, products, 0.0).amax(3, keepdim=True) * (2 * size + 8) * U
+    # An exponential is off by 2^-22 of itself, and sums are scaled anew by some (once for 16 keys, twice when they are joined); sums have as
+    # many terms as keys are seen, and a product each.
+    count = seen.double().sum(3, keepdim=True)
+    each = torch.expm1(2 * slip) + 3 * 2.0 ** -22 + (2 * count + 16) * U + (count / 16 + 2) * 2.0 ** -22
+    off = each * ((e @ V.abs()) / some)
+    bound = off + (out.abs() + off) * (HALF[t] + 4 * U) + SMALL[t]
+    back = lambda x: x.permute(0, 2, 1, 3)                 # noqa: E731
+    return back(out), back(bound)
+
+
+def within(got, want, bound, what):
+    """|got - want| <= bound element by element (want and bound in 64 bits)."""
+    torch.cuda.synchronize()
+    assert got.shape == want.shape
+    off = (got.double() - want).abs()
+    assert bool((off <= bound).all()), "%s: off by %.3g where %.3g is allowed, %d of %d elements" % (
+        what, float(off.nan_to_num(math.inf).max()), float(bound.flatten()[off.nan_to_num(math.inf).argmax()]),
+        int((~(off <= bound)).sum()), off.numel())
+
+
+@pytest.mark.parametrize("name", list(ATTENTION))
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("size", [32, 64, 128])
+def test_attention_paged(K, name, t, size):
+    q, k_pages, v_pages, table, k, v, page, at = paged(name, TYPES[t], size)
+    seen = visible(q, k, page, **at)
+    want, bound = reference(q, k, v, seen)
+    got = K.attention_paged(q, k_pages, v_pages, table, **at)
+    within(got, want, bound, name)
+    assert bool((got[~seen.any(2)] == 0).all())
+    assert torch.equal(got, K.attention_paged(q, k_pages, v_pages, table, **at))     # the same call gives the same bits
+
+
+@pytest.mark.parametrize("name", ["one query", "a few tokens", "a window and sinks", "long", "unlike lengths"])
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("layout", LAYOUTS[1:])
+@pytest.mark.parametrize("size", [32, 64, 128])
+def test_attention_paged_in_any_layout(K, name, t, layout, size):
+    """Pools of other strides, queries out of a packed projection, another scale."""
+    q, k_pages, v_pages, table, k, v, page, at = paged(name, TYPES[t], size, layout)
+    packed = torch.zeros(q.shape[0], q.shape[1], q.shape[2] + 3, size, dtype=q.dtype, device="cuda")
+    packed[:, :, 1:-2] = q
+    want, bound = reference(q, k, v, visible(q, k, page, **at), alpha=-0.03)
+    within(K.attention_paged(packed[:, :, 1:-2], k_pages, v_pages, table, alpha=-0.03, **at), want, bound, name)
+
+
+FEW = ["one query", "no keys", "around a page", "around large pages", "a few tokens", "seven heads to one", "a window and sinks", "sinks alone",
+       "before the sequence", "tokens in the middle", "long", "long window", "unlike lengths", "many short", "many rows"]
+
+
+@pytest.mark.parametrize("name", FEW)
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("filler", [math.nan, math.inf, -math.inf])
+def test_attention_paged_past_what_it_sees(K, name, t, filler):
+    """What no query sees may hold anything: the rest of a last page, what a window has passed, pages of nobody; and tables anything behind
+    the pages that are read."""
+    q, k_pages, v_pages, table, k, v, page, at = paged(name, TYPES[t], 64)
+    seen = visible(q, k, page, **at)
+    want, bound = reference(q, k, v, seen)
+    keep = torch.zeros(k_pages.shape[0] * page, dtype=torch.bool, device="cuda")
+    b, j = seen.any(1).nonzero(as_tuple=True)
+    keep[table[b, j // page].long() * page + j % page] = True
+    keep = keep.view(-1, 1, page, 1)
+    k_pages, v_pages = torch.where(keep, k_pages, filler), torch.where(keep, v_pages, filler)
+    need = torch.zeros(table.shape, dtype=torch.bool, device="cuda")
+    need[b, j // page] = True
+    wild = ints([-1, k_pages.shape[0], (1 << 31) - 1, -(1 << 31)]).repeat(table.numel() // 4 + 1)[:table.numel()].view(table.shape)
+    within(K.attention_paged(q, k_pages, v_pages, torch.where(need, table, wild), **at), want, bound, name)
+
+
+@pytest.mark.parametrize("name", FEW)
+@pytest.mark.parametrize("t", ["f32", "f16"])
+def test_attention_paged_without_some_pages(K, name, t):
+    """An entry that is no page takes its keys out of sight."""
+    q, k_pages, v_pages, table, k, v, page, at = paged(name, TYPES[t], 64)
+    gone = torch.rand(table.shape, generator=gen(4), device="cuda") < 0.3
+    gone[0] = True                                         # nothing left of the first sequence
+    table = torch.where(gone, ints([-1, k_pages.shape[0], (1 << 31) - 1, -(1 << 31)]).repeat(table.numel() // 4 + 1)[:table.numel()].view(table.shape), table)
+    seen = visible(q, k, page, table=table, pages=k_pages.shape[0], **at)
+    want, bound = reference(q, k, v, seen)
+    got = K.attention_paged(q, k_pages, v_pages, table, **at)
+    within(got, want, bound, name)
+    assert bool((got[~seen.any(2)] == 0).all())
+
+
+@pytest.mark.parametrize("name", ["one query", "a few tokens", "long", "a window and sinks", "seven heads to one", "unlike lengths"])
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("where", ["q", "k"])
+def test_attention_paged_of_no_number(K, name, t, where):
+    """What is no number in a query or a key makes none of the results that take it, and of no others."""
+    q, k_pages, v_pages, table, k, v, page, at = paged(name, TYPES[t], 64)
+    seen, share = visible(q, k, page, **at), q.shape[2] // k.shape[2]
+    want, bound = reference(q, k, v, seen)
+    b, i = (int(x) for x in seen.any(2).nonzero()[seen.any(2).sum() // 2])
+    bad = torch.zeros(q.shape[:3], dtype=torch.bool, device="cuda")
+    if where == "q":
+        q[b, i, 1, 5] = math.nan
+        bad[b, i, 1] = True
+    else:
+        j = int(seen[b, i].nonzero()[0])
+        k_pages[int(table[b, j // page]), 0, j % page, 63] = math.nan
+        bad[b, :, :share] = seen[b, :, j, None]
+    got = K.attention_paged(q, k_pages, v_pages, table, **at)
+    assert bool(torch.isnan(got[bad]).all())
+    within(torch.where(bad[..., None], 0, got), torch.where(bad[..., None], 0.0, want), bound, name)
+
+
+@pytest.mark.parametrize("name", ["one query", "a few tokens", "long", "a window and sinks", "seven heads to one", "unlike lengths"])
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("size", [32, 64, 128])
+@pytest.mark.parametrize("alpha", [0.125, -0.125])
+def test_attention_paged_of_infinite_keys(K, name, t, size, alpha):
+    """An infinite key is a score of -infinity for a query of the other sign, as if it were not there, and no number for the others."""
+    q, k_pages, v_pages, table, k, v, page, at = paged(name, TYPES[t], size)
+    q[..., 5] = torch.where(q[..., 5] < 0, -0.5, 0.5).to(q.dtype)
+    seen, share = visible(q, k, page, **at), q.shape[2] // k.shape[2]
+    b, i = (int(x) for x in seen.any(2).nonzero()[seen.any(2).sum() // 2])
+    j = int(seen[b, i].nonzero()[0])
+    without = seen.clone()
+    without[b, :, j] = False
+    want, bound = reference(q, k, v, seen, alpha=alpha)
+    want_without, bound_without = reference(q, k, v, without, alpha=alpha)
+    meets = torch.zeros(q.shape[:3], dtype=torch.bool, device="cuda")
+    meets[b, :, :share] = seen[b, :, j, None]
+    none = meets & (q[..., 5] * alpha > 0)
+    want, bound = torch.where(meets[..., None], want_without, want), torch.where(meets[..., None], bound_without, bound)
+    k_pages[int(table[b, j // page]), 0, j % page, 5] = math.inf
+    got = K.attention_paged(q, k_pages, v_pages, table, alpha=alpha, **at)
+    assert bool(torch.isnan(got[none]).all())
+    within(torch.where(none[..., None], 0, got), torch.where(none[..., None], 0.0, want), bound, name)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("at_key", [0, 17, 2999])
+def test_attention_paged_of_infinite_values(K, t, at_key):
+    """Infinite values reach the results of the heads that share them, in their column, and nothing else."""
+    t, g = TYPES[t], gen(15)
+    k_pages, v_pages, _ = pool_of("heads", 200, 2, 16, 64, t, 5)
+    table = torch.randperm(200, generator=g, device="cuda").int()[:190].view(1, -1).contiguous()
+    q, lengths = normal(g, 1, 1, 4, 64).to(t), ints([3000])
+    clean = K.attention_paged(q, k_pages, v_pages, table, lengths)
+    v_pages[int(table[0, at_key // 16]), 1, at_key % 16, 7] = -math.inf
+    got = K.attention_paged(q, k_pages, v_pages, table, lengths)
+    assert bool((got[0, 0, 2:, 7] == -math.inf).all())
+    got[0, 0, 2:, 7] = clean[0, 0, 2:, 7]
+    assert torch.equal(got, clean)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("size", [32, 64, 128])
+def test_attention_paged_of_large_scores(K, t, size):
+    """Scores far apart and far from zero, up to the largest that there are: the softmax picks single keys, and nothing leaves the range."""
+    t, g = TYPES[t], gen(10)
+    largest = 60000.0 if t == torch.float16 else 1e18
+    for q_by, k_by, alpha in ((30, 30, None), (30, 30, -0.7), (1000, 50, 0.3), (0, 0, None)):
+        k_pages, v_pages, _ = pool_of("heads", 60, 2, 16, size, t, 5)
+        k_pages *= k_by
+        if k_by == 0:                                      # one number each, of the largest there are, the others zero
+            k_pages[..., 3] = largest
+            k_pages[7, :, 5, 3] = largest / 2
+        table = torch.randperm(60, generator=g, device="cuda").int()[:50].view(2, 25).contiguous()
+        q = (q_by * normal(g, 2, 3, 4, size)).to(t)
+        if q_by == 0:
+            q[..., 3] = largest / 4
+        at = dict(left=-1, sinks=0, lengths=ints([400, 333]), first=None)
+        own = table.long()
+        k, v = (p.transpose(1, 2)[own].reshape(2, 400, 2, size) for p in (k_pages, v_pages))
+        got = K.attention_paged(q, k_pages, v_pages, table, alpha=alpha, **at)
+        assert bool(torch.isfinite(got).all())
+        want, bound = reference(q, k, v, visible(q, k, 16, **at), alpha=alpha)
+        within(got, want, bound, "%g %g" % (q_by, k_by))
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+def test_attention_paged_without_scores(K, t):
+    """A scale of 0: the mean of what is seen."""
+    for name in FEW:
+        q, k_pages, v_pages, table, k, v, page, at = paged(name, TYPES[t], 64)
+        want, bound = reference(q, k, v, visible(q, k, page, **at), alpha=0.0)
+        within(K.attention_paged(q, k_pages, v_pages, table, alpha=0.0, **at), want, bound, name)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+def test_attention_paged_keeps_a_long_axis_next_to_one_key(K, t):
+    """One key of a large score and very many of a small one, whose probabilities add up to as much."""
+    t, n, size = TYPES[t], 60000, 64
+    k_pages, v_pages, _ = pool_of("heads", n // 16, 1, 16, size, t, 5)
+    k_pages.zero_()
+    v_pages.fill_(1)
+    q = torch.zeros(1, 1, 2, size, dtype=t, device="cuda")
+    q[..., 0] = 1
+    table = torch.randperm(n // 16, generator=gen(3), device="cuda").int().view(1, -1).contiguous()
+    for where in (0, 30000, n - 1):
+        k_pages.zero_(), v_pages.fill_(1)
+        own = int(table[0, where // 16])
+        k_pages[own, 0, where % 16, 0] = 11.0
+        v_pages[own, 0, where % 16] = -1
+        got = K.attention_paged(q, k_pages, v_pages, table, ints([n]), alpha=1.0)
+        e = math.exp(11.0)
+        want = torch.full(got.shape, (n - 1 - e) / (n - 1 + e), dtype=torch.float64, device="cuda")
+        # (its terms cancel in part: 1 - 2 e / (n - 1 + e); sums of n terms, and the roundings of 11 in multiples of log 2)
+        within(got, want, torch.full_like(want, 2 * (2 * n + 64) * U + 2 * 2.0 ** -22 * n / 16) + want.abs() * HALF[t], "at %d" % where)
+
+
+def test_attention_paged_lengths_that_no_table_holds(K):
+    """Lengths and positions come from the device: ones beyond the table are cut to what it holds."""
+    low, high = -(1 << 31), (1 << 31) - 1
+    q, k_pages, v_pages, table, k, v, page, at = paged("a few tokens", torch.float16, 64, wide=0)
+    n = table.shape[1] * page
+    table = torch.where(table < 0, 0, table)
+    k, v = (p.transpose(1, 2)[table.long()].reshape(4, n, 2, 64) for p in (k_pages, v_pages))
+    at["lengths"], at["first"] = ints([high, 2000000000, -5, 5]), ints([995, 990, 0, low])
+    got = K.attention_paged(q, k_pages, v_pages, table, **at)
+    at["lengths"], at["first"] = ints([n, n, 0, 5]), ints([995, 990, 0, -100])
+    want, bound = reference(q, k, v, visible(q, k, page, **at))
+    within(got, want, bound, "cut")
+    for first in ([high] * 4, [low] * 4, [n] * 4):
+        assert bool((K.attention_paged(q, k_pages, v_pages, table, at["lengths"], first=ints(first)) == 0).all())
+
+
+def test_attention_paged_far_into_a_pool(K):
+    """Pages more than 2^31 elements in, keys and values by turns."""
+    pages, kv, page, size = 70000, 8, 32, 128              # 4.6e9 elements, 9.2 GB
+    pool = torch.zeros(pages, 2, kv, page, size, dtype=torch.float16, device="cuda")
+    k_pages, v_pages = pool[:, 0], pool[:, 1]
+    g = gen(11)
+    table = ints([[69999, 1, 35000, 69998, 32768, 65537, 0]])
+    for own in table[0].tolist():
+        pool[own] = normal(g, 2, kv, page, size).half()
+    q, lengths = normal(g, 1, 2, 16, size).half(), ints([7 * page - 3])
+    k, v = (p.transpose(1, 2)[table.long()].reshape(1, 7 * page, kv, size) for p in (k_pages, v_pages))
+    at = dict(left=150, sinks=3, lengths=lengths, first=None)
+    want, bound = reference(q, k, v, visible(q, k, page, **at))
+    within(K.attention_paged(q, k_pages, v_pages, table, **at), want, bound, "far")
+    row = normal(g, 1, 1, 2 * kv, size).half()
+    K.paged_write(row[:, :, :kv], row[:, :, kv:], ints([[69997 * page + 5]]), k_pages, v_pages)
+    assert torch.equal(pool[69997, :, :, 5].reshape(-1, size), row[0, 0])
+    pool[69997] = 0
+    assert bool((pool[69990:69998] == 0).all())
+
+
+def test_attention_paged_cut_and_uncut(K):
+    """A call without room for its pieces runs uncut, with the same result within its bound."""
+    from cubert_amd._lib import lib
+    for t in (torch.float32, torch.float16):
+        for name in ("long", "long of two heads", "long window", "one query", "a few tokens", "unlike lengths", "many and one long", "many rows", "nobody"):
+            q, k_pages, v_pages, table, k, v, page, at = paged(name, t, 64)
+            want, bound = reference(q, k, v, visible(q, k, page, **at))
+            out = torch.full_like(q, math.nan)
+            batch, q_rows, heads, size = q.shape
+            rc = getattr(lib(), "cubert_attention_paged_" + ("f32" if t == torch.float32 else "f16"))(
+                q.data_ptr(), heads * size, k_pages.data_ptr(), v_pages.data_ptr(), *k_pages.stride()[:3], table.data_ptr(), table.shape[1], table.shape[1],
+                at["lengths"].data_ptr(), None, out.data_ptr(), heads * size, size ** -0.5, batch, heads, k_pages.shape[1], q_rows, k_pages.shape[0], page,
+                size, at["left"], at["sinks"], None, 0, torch.cuda.current_stream().cuda_stream)
+            assert rc == 0
+            within(out, want, bound, name)
+
+
+def test_attention_paged_declines(K):
+    pool, q = torch.zeros(4, 2, 16, 64, device="cuda"), torch.zeros(2, 3, 4, 64, device="cuda")
+    table, n = torch.zeros(2, 3, dtype=torch.int32, device="cuda"), ints([0, 0])
+    assert K.attention_paged(q[..., :48].contiguous(), pool[..., :48], pool[..., :48], table, n) is None
+    assert K.attention_paged(q, pool[:, :, :8].contiguous(), pool[:, :, :8].contiguous(), table, n) is None
+    assert K.attention_paged(q[:0], pool, pool, table[:0], n[:0]).shape == (0, 3, 4, 64)
+    assert K.attention_paged(q[:, :0], pool, pool, table, n).shape == (2, 0, 4, 64)
+    assert bool((K.attention_paged(q + 1, pool, pool, table, n) == 0).all())
+    with pytest.raises(RuntimeError):
+        K.attention_paged(q, pool[:, :1].expand(4, 2, 16, 64), pool[:, :1].expand(4, 2, 16, 64), table, n)
+
+
+# ---------------------------------------------------------------------------- streams, graphs, a run of them
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+def test_attention_paged_in_two_graphs(K, t):
+    """Calls over a long cache, two captured and one eager on another stream, each with its own partial sums, at once."""
+    calls = [paged(name, TYPES[t], size, seed=seed) for name, size, seed in (("long", 64, 1), ("long of two heads", 64, 2), ("long window", 128, 3))]
+
+    def run(c):
+        return K.attention_paged(*c[:4], **c[7])
+
+    for c in calls:
+        run(c)
+    torch.cuda.synchronize()
+    graphs = []
+    for c in calls[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run(c)
+        graphs.append((graph, out))
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for turn in range(4):
+        for c in calls:
+            c[0].copy_(normal(gen(70 + turn), *c[0].shape))
+        torch.cuda.synchronize()
+        got = []
+        for s, (graph, _) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        with torch.cuda.stream(streams[2]):
+            eager = run(calls[2])
+        torch.cuda.synchronize()
+        got = [out.clone() for _, out in graphs] + [eager]
+        for out, c in zip(got, calls):
+            assert torch.equal(out, run(c))
+            within(out, *reference(c[0], c[4], c[5], visible(c[0], c[4], c[6], **c[7])), "turn %d" % turn)
+
+
+class Server(object):
+    """A layer's cache in pages and, next to it, the same rows as attention_window has them."""
+
+    heads, kv, size, page, width, pages, window, sinks = 4, 2, 64, 16, 12, 14, 60, 3
+
+    def __init__(self, K, t, batch, seed):
+        g = gen(seed)
+        self.K, self.t, self.batch = K, t, batch
+        self.k_pages, self.v_pages, _ = pool_of("heads", self.pages, self.kv, self.page, self.size, t, seed)
+        self.k, self.v = (normal(g, batch, self.width * self.page, self.kv, self.size).to(t) for _ in "kv")
+        self.table = torch.full((batch, self.width), -1, dtype=torch.int32, device="cuda")
+        self.free, self.free_count = torch.randperm(self.pages, generator=g, device="cuda").int(), ints([self.pages])
+        self.lengths, self.counts, self.keep = ints([0] * batch), ints([0] * batch), ints([0] * batch)
+
+    def step(self, qkv):
+        """`counts` new tokens of each sequence, and then a cut back to `keep`; everything is read on the device."""
+        K, rows = self.K, qkv.shape[1]
+        q, k, v = qkv[:, :, :self.heads], qkv[:, :, self.heads:self.heads + self.kv], qkv[:, :, self.heads + self.kv:]
+        slots, after, left = K.paged_extend(self.table, self.lengths, self.counts, self.free, self.free_count, self.page, rows)
+        K.paged_write(k, v, slots, self.k_pages, self.v_pages)
+        out = K.attention_paged(q, self.k_pages, self.v_pages, self.table, after, self.window, self.sinks, first=self.lengths)
+        kept, left = K.paged_cut(self.table, after, self.keep, self.free, left, self.page)
+        self.lengths.copy_(kept)
+        self.free_count.copy_(left)
+        return out, after, kept
+
+    def plain_step(self, qkv, before, after):
+        """The attention of the same step over rows that stand one behind the other."""
+        q, k, v = qkv[:, :, :self.heads], qkv[:, :, self.heads:self.heads + self.kv], qkv[:, :, self.heads + self.kv:]
+        for b, (n, m) in enumerate(zip(before, after)):
+            self.k[b, n:m], self.v[b, n:m] = k[b, :m - n], v[b, :m - n]
+        at = dict(left=self.window, sinks=self.sinks, lengths=ints(after), first=ints(before))
+        plain = self.K.attention_window(q, self.k, self.v, self.window, 0, self.sinks, first=at["first"], lengths=at["lengths"])
+        return plain, at
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+def test_a_server_step_by_step(K, t):
+    """Prompts, tokens, proposals that are taken back, sequences that end and others in their place, with too few pages at times."""
+    t, r = TYPES[t], random.Random(5)
+    server = Server(K, t, 6, 31)
+    refused = 0
+    for step in range(30):
+        rows = r.choice((1, 1, 1, 5, 40))
+        before = server.lengths.tolist()
+        counts = [r.choice((rows, rows, 0)) if n or rows > 1 else rows for n in before]
+        server.counts.copy_(ints(counts))
+        server.keep.copy_(ints([r.choice((1000, 1000, 1000, n + 1, 0)) for n in before]))
+        qkv = normal(gen(step), 6, rows, server.heads + 2 * server.kv, server.size).to(t)
+        got, after, kept = server.step(qkv)
+        refused += sum(1 for n, c, m in zip(before, counts, after.tolist()) if m != n + c)
+        plain, at = server.plain_step(qkv, before, after.tolist())
+        q = qkv[:, :, :server.heads]
+        want, bound = reference(q, server.k, server.v, visible(q, server.k, server.page, **at))
+        within(got, want, bound, "step %d" % step)
+        # (attention_window's probabilities have 22 bits in fp16, and both sides a rounding at the end)
+        within(got, plain.double(), 4 * bound + 2 * HALF[t] * want.abs(), "against rows in one piece, step %d" % step)
+        held = [p for row, n in zip(server.table.tolist(), kept.tolist()) for p in row[:up(n, server.page)]]
+        assert sorted(held + server.free.tolist()[:int(server.free_count)]) == list(range(server.pages))
+    assert 0 < refused < 60
+
+
+def test_a_captured_server(K):
+    """A step as a graph, replayed while lengths and tables change, with eager steps of another server in between, on another stream."""
+    t = torch.float16
+    servers = [Server(K, t, 3, 41), Server(K, t, 3, 41)]   # the same twice: one captured, one eager
+    other = Server(K, t, 5, 42)
+    qkv = normal(gen(1), 3, 1, 8, 64).to(t)
+    for s in servers:
+        s.counts.fill_(1)
+        s.keep.fill_(1000)
+    servers[0].step(qkv), servers[1].step(qkv)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, after, kept = servers[0].step(qkv)
+    stream = torch.cuda.Stream()
+    for turn in range(70):
+        qkv.copy_(normal(gen(100 + turn), *qkv.shape))
+        for s in servers:
+            s.keep.copy_(ints([0 if turn % 50 == 40 else 1000, 1000, turn % 9 * 8]))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        other.counts.fill_(2)
+        other.keep.fill_(100)
+        other.step(normal(gen(turn), 5, 3, 8, 64).to(t))
+        want = servers[1].step(qkv)
+        torch.cuda.synchronize()
+        for a, b in zip((out, after, kept, servers[0].table, servers[0].free, servers[0].k_pages),
+                        want + (servers[1].table, servers[1].free, servers[1].k_pages)):
+            assert torch.equal(a, b), turn
