@@ -7,6 +7,9 @@
 // A query that sees nothing, or that stands outside its sequence (p < 0 or p >= length[b]), gets zeros.  Heads share keys
 // and values in groups of heads / kv_heads.
 
+#include <atomic>
+#include <type_traits>
+
 #include "cubert_kernels.h"
 #include "device_common.h"
 #include "paged.h"
@@ -16,6 +19,8 @@ namespace {
 
 constexpr int kFar = (1 << 30) - 1;  // a bound or position that no sequence reaches
 constexpr float kNone = -3e38f;      // the maximum of no scores: finite, so that differences to it are numbers
+constexpr int kMaxGroups = 512;      // workgroups that a cache is cut for
+constexpr int kUncut = 8;            // units of a problem that one workgroup has
 
 struct PagedArgs {
     const void *q, *k, *v;
@@ -32,75 +37,611 @@ struct PagedArgs {
 
 __device__ __forceinline__ int clamp_to(int x, int low, int high) { return x < low ? low : x > high ? high : x; }
 
-// A workgroup per query and head, a thread per key for the scores and D / 4 threads to a key for the sums.
+template <typename T, typename V>
+__device__ __forceinline__ void store4(T *to, V x) {
+    store_vec<T, 4>(to, Vec<T, 4>{from_f32<T>(x[0]), from_f32<T>(x[1]), from_f32<T>(x[2]), from_f32<T>(x[3])});
+}
+
+typedef _Float16 v8f16 __attribute__((ext_vector_type(8)));
+typedef _Float16 v4f16 __attribute__((ext_vector_type(4)));
+typedef _Float16 v2f16 __attribute__((ext_vector_type(2)));
+typedef float v4f32 __attribute__((ext_vector_type(4)));
+typedef float v2f32 __attribute__((ext_vector_type(2)));
+typedef int v4i32 __attribute__((ext_vector_type(4)));
+typedef int v2i32 __attribute__((ext_vector_type(2)));
+
+// 16 rows (queries and heads of one key head) meet 16 keys in products of 16 x 16 with the keys as their rows: lane l has row l % 16 and
+// the keys 4 (l / 16) + i, i = 0..3, so that what belongs to a row, its maximum, its sum and its results, stays in four lanes.  Keys come from
+// memory as the products take them: lane l has of key l % 16 every fourth 16-byte piece.
+//
+// fp16: V passes through LDS, out of which it comes transposed, and the probabilities are the other factor as they are, as sums of two fp16
+// numbers, so that a result is rounded once, at the end.
+// fp32: a product with V takes a single number of one key from a lane.  Of the i-th key of its four a lane brings D / 16 columns of V, one after
+// the other, as they lie in memory, and nothing is transposed.
 template <typename T, int D>
-__global__ __launch_bounds__(kBlock) void attention_paged_kernel(PagedArgs a) {
-    constexpr int kQuads = D / 4, kAtOnce = kBlock / kQuads;
-    __shared__ float q[D], probs[kBlock], shared[kBlock / kWave], parts[kAtOnce][D];
-    __shared__ long long rows[kBlock];
-    const int head = blockIdx.x % a.heads, row = blockIdx.x / a.heads, b = row / a.q_rows, thread = threadIdx.x;
-    const int length = clamp_to(a.lengths[b], 0, a.width << a.shift);
-    const int p = (a.first != nullptr ? clamp_to(a.first[b], -kFar, kFar) : length - a.q_rows) + row - b * a.q_rows;
-    const bool there = p >= 0 && p < length;
-    const int begin = p > a.left ? p - a.left : 0, far = a.sinks < begin ? a.sinks : begin, count = there ? far + p + 1 - begin : 0;
-    const T *k = (const T *) a.k + head / (a.heads / a.kv_heads) * a.head_stride, *v = (const T *) a.v + head / (a.heads / a.kv_heads) * a.head_stride;
-    if (thread < D) {
-        const float x = to_f32(((const T *) a.q)[(size_t) row * a.ldq + head * D + thread]);
-        q[thread] = a.negate ? -x : x;
+struct Shape {
+    static constexpr bool kHalf = sizeof(T) == 2;
+    static constexpr int kRowBytes = D * (int) sizeof(T);
+    static constexpr int kKeyLoads = kRowBytes / 64;                                // 16-byte pieces of a key that a lane has
+    static constexpr int kSub = 8192 / (16 * kRowBytes) < 4 ? 8192 / (16 * kRowBytes) : 4;  // 16 keys each: what is on its way together
+    static constexpr int kKeys = 16 * kSub;
+    // V: requests for 16 keys, their size, and how many keys one has
+    static constexpr int kValueBytes = kHalf || kRowBytes >= 256 ? 16 : kRowBytes / 16;
+    static constexpr int kValueLoads = 16 * kRowBytes / (kWave * kValueBytes);
+    static constexpr int kColumns = kValueBytes / (int) sizeof(T);                  // neighbouring columns that a lane has
+    static constexpr int kValueLds = kHalf ? kKeys * kRowBytes : 0;                 // of a wavefront
+    static constexpr int kPitch = D + 4;                                            // floats between rows of sums
+    // How far a maximum may rise, in powers of two, before sums are scaled anew, and how much larger probabilities are, so that fp16's subnormals
+    // begin far below the maximum (2^-37 of it; 2^15 is still fp16).
+    static constexpr float kSlack = kHalf ? 3.f : 8.f, kRaise = kHalf ? 12.f : 0.f;
+};
+
+// (the same in every lane, which the compiler has to be told)
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// Registers of a request, and the numbers in them.
+template <int WORDS>
+using Words = int __attribute__((ext_vector_type(WORDS)));
+template <typename T, int N>
+using Numbers = T __attribute__((ext_vector_type(N)));
+
+__device__ __forceinline__ float quarters_max(float x) {
+    x = fmaxf(x, __shfl_xor(x, 16, kWave));
+    return fmaxf(x, __shfl_xor(x, 32, kWave));
+}
+
+__device__ __forceinline__ v4f16 read_transposed(const unsigned char *p) {
+    typedef short v4i16 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) v4i16 lds_v4i16;
+    return __builtin_bit_cast(v4f16, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16 *) p));
+}
+
+// Which of its 16-byte pieces a row of V keeps its piece `at` in: 32 lanes read 32 bytes of eight rows together, which lie on different banks.
+template <int ROW_BYTES>
+__device__ __forceinline__ int v_piece(int key, int at) {
+    return at ^ (key / (256 / ROW_BYTES) % (ROW_BYTES / 32) * 2);
+}
+
+// Probabilities as sums of two fp16 numbers, exact to 2^-21 of them: pairs of `high` and `low`.  Both are positive, the second one at least fp16's
+// smallest, 2^-36 of the largest probability, so that an infinite value of V stays infinite in either product.
+__device__ __forceinline__ void two_terms(float e0, float e1, v2f16 &high, v2f16 &low) {
+    high = __builtin_bit_cast(v2f16, __builtin_amdgcn_cvt_pkrtz(e0, e1));
+    float minus = -1.f;
+    asm("" : "+v"(minus));  // (as a constant it makes a conversion and a subtraction of one instruction)
+    low = __builtin_convertvector((v2f32{fmaf((float) high[0], minus, e0), fmaf((float) high[1], minus, e1)}), v2f16);
+    low = __builtin_elementwise_max(low, v2f16{(_Float16) 0x1p-24f, (_Float16) 0x1p-24f});
+}
+
+// What a launch is cut into: `groups` workgroups take runs of units, `least` of them at least, or (groups = 0) one workgroup has all of a problem.
+// A problem is a tile of rows of a sequence and a key head; sequences and tiles are numbered together, tile * batch + sequence.
+struct PagedPlan {
+    int rows, row_tiles, groups, least;  // rows of a tile
+    long long problems;
+    size_t floats;
+};
+
+// The keys that the queries of a tile of rows of a sequence see between them, in units of KEYS keys: those of the sinks, then those of the window.
+template <int KEYS>
+struct Reach {
+    int length, first, low, high;  // positions of the queries inside of the sequence
+    int of_sinks, begin, units;    // units of the sinks, the window's first, and all of them: one at least, so that somebody writes the zeros
+    bool any;
+
+    __device__ __forceinline__ Reach(const PagedArgs &a, const PagedPlan &plan, int length_, int first_, int tile) {
+        length = clamp_to(length_, 0, a.width << a.shift);
+        first = a.first != nullptr ? clamp_to(first_, -kFar, kFar) : length - a.q_rows;
+        low = first, high = first + a.q_rows - 1;
+        if (plan.row_tiles > 1) {
+            const int share = a.heads / a.kv_heads, rows = a.q_rows * share, row0 = tile * plan.rows;
+            low = first + row0 / share, high = first + ((row0 + plan.rows < rows ? row0 + plan.rows : rows) - 1) / share;
+        }
+        low = low < 0 ? 0 : low, high = high < length ? high : length - 1;
+        any = low <= high;
+        const int first_begin = low > a.left ? low - a.left : 0, end = high + 1, far = a.sinks < end ? a.sinks : end;
+        begin = first_begin / KEYS;
+        of_sinks = (far + KEYS - 1) / KEYS;
+        of_sinks = of_sinks < begin ? of_sinks : begin;
+        units = any ? of_sinks + (end + KEYS - 1) / KEYS - begin : 1;
+        if (!any) begin = of_sinks = 0;
     }
-    float top = kNone, sum = 0.f, x[4] = {};
-    const int group = thread / kQuads, d = thread % kQuads * 4;
-    for (int base = 0; base < count; base += kBlock) {
-        const int n = base + thread;
-        float score = -INFINITY;
-        long long at = -1;
-        __syncthreads();
-        if (n < count) {
-            const int j = n < far ? n : begin + n - far, page = a.table[(size_t) b * a.ld_table + (j >> a.shift)];
-            if (page >= 0 && page < a.pages) {
-                at = page * a.page_stride + (j & ((1 << a.shift) - 1)) * a.row_stride;
-                score = 0.f;
-                for (int e = 0; e < D; e += 4) {
-                    const Vec<T, 4> piece = load_vec<T, 4>(k + at + e);
+    __device__ __forceinline__ int key_of(int unit) const { return (unit < of_sinks ? unit : unit - of_sinks + begin) * KEYS; }
+};
+
+// The sum of x over this lane and those before it.
+__device__ __forceinline__ int sum_through(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
+    return x;
+}
+
+// Lengths and positions of 64 of the sequences and tiles, one to a lane.
+template <int KEYS>
+struct Sequences {
+    int first_one, length, first;
+
+    __device__ __forceinline__ int bring(const PagedArgs &a, const PagedPlan &plan, int from, int lane) {
+        const int i = from + lane, all = a.batch * plan.row_tiles, tile = plan.row_tiles > 1 ? i / a.batch : 0, b = i - tile * a.batch;
+        first_one = from, length = first = 0;
+        if (i < all) {
+            length = a.lengths[b];
+            if (a.first != nullptr) first = a.first[b];
+        }
+        return i < all ? Reach<KEYS>(a, plan, length, first, tile).units * a.kv_heads : 0;
+    }
+};
+
+template <typename T, int D, int TILES>
+struct Rows {
+    typedef Shape<T, D> S;
+    v4f32 q[TILES][S::kKeyLoads], ctx[TILES][D / 16];
+    float top[TILES], sum[TILES];
+};
+
+// Bound by reading K and V.
+template <typename T, int D, int TILES, bool CUT>
+__global__ __launch_bounds__(kBlock, 2) void attention_paged_kernel(PagedArgs a, PagedPlan plan) {
+    typedef Shape<T, D> S;
+    typedef Reach<S::kKeys> Reached;
+    constexpr int kWaves = kBlock / kWave, kRows = 16 * TILES, kSub = S::kSub, kKeys = S::kKeys;
+    extern __shared__ __align__(16) unsigned char smem[];
+    const int wave = wave_in_block(), lane = threadIdx.x & (kWave - 1), col = lane & 15, quarter = lane >> 4;
+    const int share = a.heads / a.kv_heads, rows = a.q_rows * share;
+    const int page_mask = (1 << a.shift) - 1;
+    const long long page_bytes = a.page_stride * (long long) sizeof(T);
+    const unsigned row_bytes = (unsigned) a.row_stride * (unsigned) sizeof(T);
+    const unsigned k_offset = (unsigned) col * row_bytes + (unsigned) quarter * 16;
+    constexpr int kPieces = S::kRowBytes / 16;  // of a row; fp16: the l / kPieces-th key of a request
+    const int v_key = S::kHalf ? lane / kPieces : quarter * 4;
+    const unsigned v_offset = (unsigned) v_key * row_bytes + (unsigned) (S::kHalf ? lane % kPieces * 16 : col * S::kValueBytes);
+    // of the j-th request for 16 keys: which of them it begins with, and which 256 bytes of a row it has
+    auto value_key = [](int j) { return S::kHalf ? j * (kWave / kPieces) : j * 4 / S::kValueLoads; };
+    auto value_part = [](int j) { return S::kHalf ? 0 : j % (S::kValueLoads / 4 > 0 ? S::kValueLoads / 4 : 1); };
+    unsigned char *const v_lds = smem + wave * S::kValueLds;
+
+    // which problem comes first, which of its units, and how many units this workgroup has
+    int entry, kv_head, unit, todo = 1 << 30, chunk = 1 << 30, base = 0;  // base: the entry's first unit among all
+    Sequences<kKeys> sequences;
+    if constexpr (CUT) {
+        const int all = a.batch * plan.row_tiles;
+        int units = sequences.bring(a, plan, 0, lane), sum = units;
+        for (int i = kWave; i < all; i += kWave) {
+            Sequences<kKeys> others;
+            sum += others.bring(a, plan, i, lane);
+        }
+        int through = sum_through(units);
+        const int total = all > kWave ? __builtin_amdgcn_readlane(sum_through(sum), kWave - 1) : __builtin_amdgcn_readlane(through, kWave - 1);
+        chunk = (total + plan.groups - 1) / plan.groups;
+        chunk = chunk > plan.least ? chunk : plan.least;
+        const int from = (int) blockIdx.x * chunk;  // (below 2^31 + 2^31 / groups: see plan_paged)
+        if (from >= total) return;
+        while (true) {
+            const unsigned long long after = __ballot(base + through > from);
+            if (after != 0) {
+                const int at = __builtin_ctzll(after);
+                entry = sequences.first_one + at;
+                units = __builtin_amdgcn_readlane(units, at);
+                base += __builtin_amdgcn_readlane(through, at) - units;
+                break;
+            }
+            base += __builtin_amdgcn_readlane(through, kWave - 1);
+            units = sequences.bring(a, plan, sequences.first_one + kWave, lane);
+            through = sum_through(units);
+        }
+        todo = total - from < chunk ? total - from : chunk;
+        const int each = units / a.kv_heads;
+        kv_head = (from - base) / each, unit = from - base - kv_head * each;
+    } else {
+        entry = blockIdx.x / a.kv_heads, kv_head = blockIdx.x - entry * a.kv_heads, unit = 0;
+    }
+    for (bool begun = true; todo > 0; begun = false) {
+        const int tile = plan.row_tiles > 1 ? entry / a.batch : 0, sequence = entry - tile * a.batch;
+        int length, first = 0;
+        if constexpr (CUT) {
+            if (entry - sequences.first_one >= kWave) sequences.bring(a, plan, entry, lane);
+            length = __builtin_amdgcn_readlane(sequences.length, entry - sequences.first_one);
+            first = __builtin_amdgcn_readlane(sequences.first, entry - sequences.first_one);
+        } else {
+            length = a.lengths[sequence];
+            if (a.first != nullptr) first = a.first[sequence];
+        }
+        const Reached reach(a, plan, length, first, tile);
+        const int count = reach.units - unit < todo ? reach.units - unit : todo;  // units of this problem that this workgroup has
+        const int row0 = tile * kRows;
+        const char *k_base = (const char *) a.k + kv_head * a.head_stride * (long long) sizeof(T);
+        const char *v_base = (const char *) a.v + kv_head * a.head_stride * (long long) sizeof(T);
+        const int *table = a.table + (size_t) sequence * a.ld_table;
+        const int seen_begin = reach.low > a.left ? reach.low - a.left : 0, all_begin = reach.high > a.left ? reach.high - a.left : 0;
+        const int seen_end = reach.any ? reach.high + 1 : 0, all_end = reach.any ? reach.low + 1 : 0;
+
+        // a wavefront's run among them; lane l has the page of the l-th 16 keys from unit x0 on
+        int x = unit + count * wave / kWaves;
+        const int until = unit + count * (wave + 1) / kWaves;
+        int x0 = x, pages = -1;
+        auto look_up = [&](int from_unit) {
+            x0 = from_unit;
+            const int key = reach.key_of(x0 + lane / kSub) + lane % kSub * 16;
+            pages = -1;
+            if (key < seen_end) {
+                const int page = table[key >> a.shift];
+                if (page >= 0 && page < a.pages) pages = page;
+            }
+        };
+        if (x < until) look_up(x);
+
+        Rows<T, D, TILES> r;
+        int begin[TILES], end[TILES];  // of what a lane's row sees, the sinks aside
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) score = fmaf(q[e + i], to_f32(piece.v[i]), score);
+        for (int m = 0; m < TILES; ++m) {
+            const int row = row0 + 16 * m + col, my_row = row < rows ? row : rows - 1, query = share == 1 ? my_row : my_row / share;
+            const char *q = (const char *) a.q + ((size_t) (sequence * a.q_rows + query) * a.ldq +
+                                                  (size_t) (kv_head * share + my_row - query * share) * D) * sizeof(T);
+#pragma unroll
+            for (int t = 0; t < S::kKeyLoads; ++t) {
+                r.q[m][t] = *reinterpret_cast<const v4f32 *>(q + 64 * t + 16 * quarter);
+                if (a.negate) {
+                    if constexpr (S::kHalf) r.q[m][t] = __builtin_bit_cast(v4f32, -__builtin_bit_cast(v8f16, r.q[m][t]));
+                    else r.q[m][t] = -r.q[m][t];
                 }
             }
-        }
-        rows[thread] = at;
-        float high = wave_max(score);
-        if ((thread & (kWave - 1)) == 0) shared[thread / kWave] = high;
-        __syncthreads();
-        high = top;
 #pragma unroll
-        for (int w = 0; w < kBlock / kWave; ++w) high = fmaxf(high, shared[w]);
-        const float shrink = __builtin_amdgcn_exp2f((top - high) * a.scale);
+            for (int d = 0; d < D / 16; ++d) r.ctx[m][d] = v4f32{};
+            r.top[m] = kNone, r.sum[m] = 0.f;
+            const int p = reach.first + query;
+            begin[m] = p > a.left ? p - a.left : 0, end[m] = p >= 0 && p < reach.length ? p + 1 : 0;
+        }
+
+        Words<4> k[kSub][S::kKeyLoads];
+        Words<S::kValueBytes / 4> v[kSub][S::kValueLoads];
+        unsigned there_next = 0;  // which 16 keys of a unit have a page
+        auto offset_of = [&](int unit_at, int n) -> long long {
+            const int page = __builtin_amdgcn_readlane(pages, (unit_at - x0) * kSub + n);
+            return (page < 0 ? 0 : page) * page_bytes + (long long) ((reach.key_of(unit_at) + 16 * n) & page_mask) * row_bytes;
+        };
+        auto bring_keys = [&](int unit_at) {
+            if (unit_at - x0 == kWave / kSub) look_up(unit_at);
+            there_next = 0;
+#pragma unroll
+            for (int n = 0; n < kSub; ++n) {
+                if (__builtin_amdgcn_readlane(pages, (unit_at - x0) * kSub + n) >= 0) there_next |= 1u << n;
+                const char *at = k_base + offset_of(unit_at, n);
+#pragma unroll
+                for (int t = 0; t < S::kKeyLoads; ++t) k[n][t] = *reinterpret_cast<const Words<4> *>(at + k_offset + 64 * t);
+            }
+        };
+        auto bring_values = [&](int unit_at) {
+#pragma unroll
+            for (int n = 0; n < kSub; ++n) {
+                const char *at = v_base + offset_of(unit_at, n);
+#pragma unroll
+                for (int j = 0; j < S::kValueLoads; ++j)
+                    v[n][j] = *reinterpret_cast<const Words<S::kValueBytes / 4> *>(at + value_key(j) * row_bytes + v_offset + 256 * value_part(j));
+            }
+        };
+        auto take = [&](int unit_at, auto more) {
+            const unsigned there = there_next;
+            const int key0 = reach.key_of(unit_at);
+            v4f32 s[TILES][kSub];
+#pragma unroll
+            for (int n = 0; n < kSub; ++n)
+#pragma unroll
+                for (int m = 0; m < TILES; ++m) s[m][n] = v4f32{};
+#pragma unroll
+            for (int t = 0; t < S::kKeyLoads; ++t)
+#pragma unroll
+                for (int n = 0; n < kSub; ++n)
+#pragma unroll
+                    for (int m = 0; m < TILES; ++m) {
+                        if constexpr (S::kHalf) {
+                            s[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8f16, k[n][t]), __builtin_bit_cast(v8f16, r.q[m][t]), s[m][n], 0, 0, 0);
+                        } else {
+                            const v4f32 piece = __builtin_bit_cast(v4f32, k[n][t]);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) s[m][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(piece[e], r.q[m][t][e], s[m][n], 0, 0, 0);
+                        }
+                    }
+            products_done();
+            if constexpr (decltype(more)::value) bring_keys(unit_at + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            const bool all = there == (1u << kSub) - 1 && key0 + kKeys <= all_end && (key0 >= all_begin || key0 + kKeys <= a.sinks);
+            if (!all) {
+#pragma unroll
+                for (int n = 0; n < kSub; ++n) {
+                    const bool is = there >> n & 1u;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = key0 + 16 * n + 4 * quarter + i;
+#pragma unroll
+                        for (int m = 0; m < TILES; ++m) s[m][n][i] = is && key < end[m] && (key >= begin[m] || key < a.sinks) ? s[m][n][i] : -INFINITY;
+                    }
+                    // (a key that nobody sees has probability 0, but 0 times what its row of V may hold need not be 0)
+#pragma unroll
+                    for (int j = 0; j < S::kValueLoads; ++j) {
+                        const int key = key0 + 16 * n + value_key(j) + v_key;
+                        const bool use = is && key < seen_end && (key >= seen_begin || key < a.sinks);
+#pragma unroll
+                        for (int w = 0; w < S::kValueBytes / 4; ++w) v[n][j][w] = use ? v[n][j][w] : 0;
+                    }
+                }
+            }
+            if constexpr (S::kHalf) {
+#pragma unroll
+                for (int n = 0; n < kSub; ++n)
+#pragma unroll
+                    for (int j = 0; j < S::kValueLoads; ++j) {
+                        const int key = 16 * n + value_key(j) + v_key;
+                        *reinterpret_cast<Words<4> *>(v_lds + key * S::kRowBytes + v_piece<S::kRowBytes>(key, lane % kPieces) * 16) = v[n][j];
+                    }
+                asm volatile("" ::: "memory");
+                __builtin_amdgcn_wave_barrier();
+                if constexpr (decltype(more)::value) bring_values(unit_at + 1);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int m = 0; m < TILES; ++m) {
+                float top = s[m][0][0];
+#pragma unroll
+                for (int n = 0; n < kSub; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) top = fmaxf(top, s[m][n][i]);
+                // sums are scaled anew only when some maximum has risen by more than they bear
+                if (__any((top - r.top[m]) * a.scale > S::kSlack)) {
+                    const float high = fmaxf(r.top[m], quarters_max(top)), shrink = __builtin_amdgcn_exp2f((r.top[m] - high) * a.scale);
+                    r.top[m] = high;
+                    r.sum[m] *= shrink;
+#pragma unroll
+                    for (int d = 0; d < D / 16; ++d) r.ctx[m][d] *= shrink;
+                }
+#pragma unroll
+                for (int n = 0; n < kSub; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        s[m][n][i] = __builtin_amdgcn_exp2f(fmaf(s[m][n][i] - r.top[m], a.scale, S::kRaise));
+                        r.sum[m] += s[m][n][i];
+                    }
+            }
+            if constexpr (S::kHalf) {
+#pragma unroll
+                for (int n = 0; n < kSub; n += 2) {
+                    v8f16 p[TILES], low[TILES];  // of the keys that the transposed V has in the same places
+#pragma unroll
+                    for (int m = 0; m < TILES; ++m)
+#pragma unroll
+                        for (int i = 0; i < 8; i += 2) {
+                            v2f16 x, y;
+                            two_terms(s[m][n + i / 4][i % 4], s[m][n + i / 4][i % 4 + 1], x, y);
+                            p[m][i] = x[0], p[m][i + 1] = x[1], low[m][i] = y[0], low[m][i + 1] = y[1];
+                        }
+#pragma unroll
+                    for (int d = 0; d < D / 16; ++d) {
+                        v4f16 part[2];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int key = 16 * (n + h) + 4 * quarter + col / 4, at = 2 * d + col % 4 / 2;
+                            part[h] = read_transposed(v_lds + key * S::kRowBytes + v_piece<S::kRowBytes>(key, at) * 16 + col % 2 * 8);
+                        }
+                        const v8f16 x = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+                        for (int m = 0; m < TILES; ++m) {
+                            r.ctx[m][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, low[m], r.ctx[m][d], 0, 0, 0);
+                            r.ctx[m][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, p[m], r.ctx[m][d], 0, 0, 0);
+                        }
+                    }
+                }
+                asm volatile("" ::: "memory");
+                __builtin_amdgcn_wave_barrier();
+            } else {
+#pragma unroll
+                for (int n = 0; n < kSub; ++n)
+#pragma unroll
+                    for (int j = 0; j < S::kValueLoads; ++j) {
+                        Words<S::kValueBytes / 4> words = v[n][j];
+                        pin_registers(words);  // (taken apart here, not where they arrive)
+                        const Numbers<T, S::kColumns> piece = __builtin_bit_cast(Numbers<T, S::kColumns>, words);
+#pragma unroll
+                        for (int e = 0; e < S::kColumns; ++e)
+#pragma unroll
+                            for (int m = 0; m < TILES; ++m) {
+                                v4f32 &to = r.ctx[m][value_part(j) * S::kColumns + e];
+                                to = __builtin_amdgcn_mfma_f32_16x16x4f32((float) piece[e], s[m][n][value_key(j)], to, 0, 0, 0);
+                            }
+                    }
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (decltype(more)::value) bring_values(unit_at + 1);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        if (x < until) {
+            bring_keys(x);
+            bring_values(x);
+            for (; x + 1 < until; ++x) take(x, std::true_type());
+            take(x, std::false_type());
+        }
+        products_done();
+
+        // the four wavefronts' sums: rows of D results, the maximum and the sum
+        const int present = rows - row0 < kRows ? rows - row0 : kRows;
+        float *merge = reinterpret_cast<float *>(smem);
+        __syncthreads();  // nobody reads V, or the sums of the problem before, any more
+#pragma unroll
+        for (int m = 0; m < TILES; ++m) {
+            float sum = r.sum[m] + __shfl_xor(r.sum[m], 16, kWave);
+            sum += __shfl_xor(sum, 32, kWave);
+            const int row = 16 * m + col;
+            if (row < present) {
+                float *to = merge + (wave * present + row) * S::kPitch;
+                if constexpr (S::kHalf) {
+#pragma unroll
+                    for (int d = 0; d < D / 16; ++d) *reinterpret_cast<v4f32 *>(to + 16 * d + 4 * quarter) = r.ctx[m][d];
+                } else {
+#pragma unroll
+                    for (int d = 0; d < D / 16; d += 2)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            *reinterpret_cast<v2f32 *>(to + d / S::kColumns * 64 + (4 * quarter + i) * S::kColumns + d % S::kColumns) =
+                                    v2f32{r.ctx[m][d][i], r.ctx[m][d + 1][i]};
+                }
+                if (quarter == 0) to[D] = r.top[m], to[D + 1] = sum;
+            }
+        }
+        __syncthreads();
+        const bool whole = !CUT || count == reach.units;
+        constexpr int kQuads = D / 4;  // a thread has four columns of a row
+        for (int i = threadIdx.x; i < present * kQuads; i += kBlock) {
+            const int row = i / kQuads, d = (i - row * kQuads) * 4;
+            float top = kNone;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) top = fmaxf(top, merge[(w * present + row) * S::kPitch + D]);
+            v4f32 x4 = v4f32{};
+            float total = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                const float *of = merge + (w * present + row) * S::kPitch;
+                const float f = __builtin_amdgcn_exp2f((of[D] - top) * a.scale);
+                total += of[D + 1] * f;
+                x4 += *reinterpret_cast<const v4f32 *>(of + d) * f;
+            }
+            const int out_row = row0 + row, query = share == 1 ? out_row : out_row / share, p = reach.first + query;
+            const bool there = p >= 0 && p < reach.length;
+            if (whole) {
+                T *ctx = (T *) a.ctx + (size_t) (sequence * a.q_rows + query) * a.ld_ctx + (size_t) (kv_head * share + out_row - query * share) * D + d;
+                const float by = there && total != 0.f ? 1.f / total : 0.f;  // (a sum that is no number stays none)
+                store4(ctx, by != 0.f ? x4 * by : v4f32{});
+            } else {
+                float *to = a.partials + ((size_t) (2 * blockIdx.x + (begun ? 0 : 1)) * kRows + row) * S::kPitch;
+                *reinterpret_cast<v4f32 *>(to + d) = there ? x4 : v4f32{};
+                if (d == 0) to[D] = there ? top : kNone, to[D + 1] = there ? total : 0.f;
+            }
+        }
+        if constexpr (!CUT) break;
+        todo -= count;
+        // Of a problem's first piece: where it stands, and how many more there are (each the first of its workgroup).
+        if (unit == 0 && threadIdx.x == 0) {
+            v2i32 *note = reinterpret_cast<v2i32 *>(a.partials + (size_t) 2 * plan.groups * kRows * S::kPitch);
+            const int last = base + (kv_head + 1) * reach.units - 1;
+            note[(size_t) entry * a.kv_heads + kv_head] = v2i32{2 * (int) blockIdx.x + (begun ? 0 : 1), last / chunk - (int) blockIdx.x};
+        }
+        unit = 0;
+        if (++kv_head == a.kv_heads) kv_head = 0, base += reach.units * a.kv_heads, ++entry;
+        __syncthreads();  // the sums have been read
+    }
+}
+
+// The pieces' sums of a row joined, by WAVES wavefronts: D / 4 lanes to a piece, their maxima and sums a lane each.
+template <typename T, int D, int WAVES>
+__global__ __launch_bounds__(kBlock) void attention_paged_join_kernel(PagedArgs a, PagedPlan plan) {
+    typedef Shape<T, D> S;
+    constexpr int kQuads = D / 4, kAtOnce = kWave / kQuads, kPer = kBlock / kWave / WAVES;
+    __shared__ float shared[WAVES > 1 ? WAVES * S::kPitch : 1];
+    const int wave = wave_in_block(), lane = threadIdx.x & (kWave - 1), share = a.heads / a.kv_heads, rows = a.q_rows * share;
+    const int i = blockIdx.x * kPer + wave / WAVES, part = wave % WAVES;
+    const int problem = i / plan.rows, row = i - problem * plan.rows;
+    if (problem >= plan.problems) return;
+    const int entry = problem / a.kv_heads, kv_head = problem - entry * a.kv_heads;
+    const int tile = plan.row_tiles > 1 ? entry / a.batch : 0, sequence = entry - tile * a.batch, out_row = tile * plan.rows + row;
+    if (out_row >= rows) return;
+    const v2i32 note = reinterpret_cast<const v2i32 *>(a.partials + (size_t) 2 * plan.groups * plan.rows * S::kPitch)[problem];
+    const int pieces = uniform(note[1]) + 1, slot = uniform(note[0]);
+    if (pieces == 1) return;  // its one workgroup has written it
+    const float *first = a.partials + ((size_t) slot * plan.rows + row) * S::kPitch;
+    const float *next = a.partials + ((size_t) (slot / 2 * 2) * plan.rows + row) * S::kPitch;
+    const size_t step = (size_t) 2 * plan.rows * S::kPitch;
+    auto piece_at = [&](int n) { return n == 0 ? first : next + n * step; };
+    const int until = pieces * (part + 1) / WAVES, at = lane / kQuads, d = lane % kQuads * 4;
+    float top = kNone, sum = 0.f;
+    v4f32 x = v4f32{};
+    for (int n0 = pieces * part / WAVES; n0 < until; n0 += kWave) {
+        const int here = until - n0 < kWave ? until - n0 : kWave;
+        const float *of = piece_at(n0 + (lane < here ? lane : 0));
+        const float my_top = of[D], my_sum = of[D + 1], high = fmaxf(top, wave_max(my_top));
+        const float weight = lane < here ? __builtin_amdgcn_exp2f((my_top - high) * a.scale) : 0.f, shrink = __builtin_amdgcn_exp2f((top - high) * a.scale);
         top = high;
-        probs[thread] = __builtin_amdgcn_exp2f((score - top) * a.scale);
-        __syncthreads();
-        const float part = wave_sum(probs[thread]);
-        if ((thread & (kWave - 1)) == 0) shared[thread / kWave] = part;
-        __syncthreads();
-        sum *= shrink;
+        sum = sum * shrink + wave_sum(weight * my_sum);
+        x *= shrink;
+        constexpr int kAhead = 8;
+        for (int n = 0; n < here; n += kAtOnce * kAhead) {
+            v4f32 y[kAhead];
 #pragma unroll
-        for (int w = 0; w < kBlock / kWave; ++w) sum += shared[w];
+            for (int u = 0; u < kAhead; ++u) {
+                const int m = n + u * kAtOnce + at;
+                y[u] = *reinterpret_cast<const v4f32 *>(piece_at(n0 + (m < here ? m : 0)) + d);
+            }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] *= shrink;
-        for (int m = group; m < kBlock; m += kAtOnce) {
-            if (rows[m] < 0) continue;
-            const Vec<T, 4> piece = load_vec<T, 4>(v + rows[m] + d);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = fmaf(probs[m], to_f32(piece.v[i]), x[i]);
+            for (int u = 0; u < kAhead; ++u) {
+                const int m = n + u * kAtOnce + at;
+                const float f = __shfl(weight, m < here ? m : 0, kWave);
+                if (m < here) x += y[u] * f;
+            }
         }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) parts[group][d + i] = x[i];
-    __syncthreads();
-    if (thread < D) {
-        float total = 0.f;
-        for (int g = 0; g < kAtOnce; ++g) total += parts[g][thread];
-        ((T *) a.ctx)[(size_t) row * a.ld_ctx + head * D + thread] = from_f32<T>(sum != 0.f ? total / sum : 0.f);
+    for (int m = kQuads; m < kWave; m *= 2)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] += __shfl_xor(x[e], m, kWave);
+    if constexpr (WAVES > 1) {
+        float *mine = shared + part * S::kPitch;
+        if (at == 0) *reinterpret_cast<v4f32 *>(mine + d) = x;
+        if (lane == 0) mine[D] = top, mine[D + 1] = sum;
+        __syncthreads();
+        if (part != 0) return;
+        float high = kNone;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) high = fmaxf(high, shared[w * S::kPitch + D]);
+        x = v4f32{}, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            const float f = __builtin_amdgcn_exp2f((shared[w * S::kPitch + D] - high) * a.scale);
+            sum += shared[w * S::kPitch + D + 1] * f;
+            x += *reinterpret_cast<const v4f32 *>(shared + w * S::kPitch + d) * f;
+        }
     }
+    if (at != 0) return;
+    const int query = out_row / share;
+    T *ctx = (T *) a.ctx + (size_t) (sequence * a.q_rows + query) * a.ld_ctx + (size_t) (kv_head * share + out_row - query * share) * D + d;
+    const float by = sum != 0.f ? 1.f / sum : 0.f;
+    store4(ctx, by != 0.f ? x * by : v4f32{});
+}
+
+PagedPlan plan_paged(bool half_precision, int batch, int heads, int kv_heads, int q_rows, long long limit, int head_size, int left, int sinks) {
+    PagedPlan plan;
+    const long long rows = (long long) q_rows * (heads / kv_heads);
+    plan.rows = rows <= 16 ? 16 : 32;
+    plan.row_tiles = (int) ((rows + plan.rows - 1) / plan.rows);
+    plan.problems = (long long) batch * kv_heads * plan.row_tiles;
+    const int row_bytes = head_size * (half_precision ? 2 : 4), keys = row_bytes >= 128 ? 8192 / row_bytes : 64;
+    long long reach = limit;  // the most keys that a tile of rows sees, and how many units of them
+    if (left >= 0 && (long long) left + plan.rows + sinks < reach) reach = (long long) left + plan.rows + sinks;
+    const long long units = (reach + keys - 1) / keys + (left >= 0 ? 2 : 0);
+    plan.least = 8, plan.groups = 0, plan.floats = 0;
+    if (units <= kUncut || plan.problems * units >= 1 << 30) return plan;  // (units are counted in 32 bits)
+    const long long most = (plan.problems * units + plan.least - 1) / plan.least;
+    plan.groups = (int) (most < kMaxGroups ? most : kMaxGroups);
+    plan.floats = (size_t) 2 * plan.groups * plan.rows * (head_size + 4) + 2 * (size_t) plan.problems;
+    return plan;
+}
+
+template <typename T, int D, int TILES, bool CUT>
+int run_paged(const PagedArgs &a, const PagedPlan &plan, hipStream_t stream) {
+    static std::atomic<unsigned long long> done{0};
+    typedef Shape<T, D> S;
+    const long long rows = (long long) a.q_rows * (a.heads / a.kv_heads);
+    const unsigned merge = (unsigned) (4 * (rows < plan.rows ? rows : plan.rows) * S::kPitch * 4), lds = merge > 4 * S::kValueLds ? merge : 4 * S::kValueLds;
+    if (lds > 48 * 1024 && !allow_large_lds(attention_paged_kernel<T, D, TILES, CUT>, done)) return CUBERT_UNSUPPORTED;
+    const dim3 grid(CUT ? (unsigned) plan.groups : (unsigned) plan.problems);
+    const int rc = launch_lds(attention_paged_kernel<T, D, TILES, CUT>, grid, dim3(kBlock), lds, stream, a, plan);
+    if (rc != 0 || !CUT) return rc;
+    const unsigned joins = (unsigned) (plan.problems * plan.rows);
+    if (joins >= 1024) return launch(attention_paged_join_kernel<T, D, 1>, dim3((joins + 3) / 4), dim3(kBlock), stream, a, plan);
+    return launch(attention_paged_join_kernel<T, D, 4>, dim3(joins), dim3(kBlock), stream, a, plan);
+}
+
+template <typename T, int D>
+int run_paged_size(const PagedArgs &a, const PagedPlan &plan, hipStream_t stream) {
+    if (plan.rows == 16) return plan.groups != 0 ? run_paged<T, D, 1, true>(a, plan, stream) : run_paged<T, D, 1, false>(a, plan, stream);
+    return plan.groups != 0 ? run_paged<T, D, 2, true>(a, plan, stream) : run_paged<T, D, 2, false>(a, plan, stream);
 }
 
 template <typename T>
@@ -133,13 +674,15 @@ int attention_paged(const T *q, int ldq, const T *k_pages, const T *v_pages, lon
     a.ldq = ldq, a.ld_ctx = ld_ctx, a.width = width, a.ld_table = ld_table;
     a.batch = batch, a.heads = heads, a.kv_heads = kv_heads, a.q_rows = q_rows, a.pages = pages, a.shift = __builtin_ctz((unsigned) page);
     a.left = left < 0 || left > kFar ? kFar : left, a.sinks = sinks < kFar ? sinks : kFar;
-    (void) partial_floats;
-    const unsigned long long blocks = (unsigned long long) batch * q_rows * heads;
-    if ((unsigned long long) batch * q_rows >= 1u << 24 || blocks >= 1u << 24) return CUBERT_UNSUPPORTED;
-    const dim3 grid((unsigned) blocks), block(kBlock);
-    if (head_size == 32) return launch(attention_paged_kernel<T, 32>, grid, block, (hipStream_t) stream, a);
-    if (head_size == 64) return launch(attention_paged_kernel<T, 64>, grid, block, (hipStream_t) stream, a);
-    return launch(attention_paged_kernel<T, 128>, grid, block, (hipStream_t) stream, a);
+    // (a launch holds less than 2^32 threads, and rows are counted in 32 bits)
+    if ((long long) batch * q_rows >= 1ll << 31 || (long long) batch * kv_heads >= 1 << 24 || (long long) q_rows * (heads / kv_heads) >= 1 << 30)
+        return CUBERT_UNSUPPORTED;
+    PagedPlan plan = plan_paged(sizeof(T) == 2, batch, heads, kv_heads, q_rows, (long long) width * page, head_size, a.left == kFar ? -1 : left, a.sinks);
+    if (plan.problems * plan.rows >= 1 << 24) return CUBERT_UNSUPPORTED;
+    if (plan.groups != 0 && (partials == nullptr || partial_floats < plan.floats || !is_aligned(partials, 16))) plan.groups = 0;
+    if (head_size == 32) return run_paged_size<T, 32>(a, plan, (hipStream_t) stream);
+    if (head_size == 64) return run_paged_size<T, 64>(a, plan, (hipStream_t) stream);
+    return run_paged_size<T, 128>(a, plan, (hipStream_t) stream);
 }
 
 }  // namespace
@@ -151,8 +694,10 @@ extern "C" {
 
 size_t cubert_attention_paged_partials(int half_precision, int batch, int heads, int kv_heads, int q_rows, int width, int page, int head_size, int left,
                                        int sinks) {
-    (void) half_precision, (void) batch, (void) heads, (void) kv_heads, (void) q_rows, (void) width, (void) page, (void) head_size, (void) left, (void) sinks;
-    return 0;
+    if (batch < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || q_rows < 1 || width < 1 || page < 1 || head_size < 1 || sinks < 0) return 0;
+    if ((long long) batch * kv_heads >= 1 << 24 || (long long) q_rows * (heads / kv_heads) >= 1 << 30 || (long long) width * page > cubert::kFar) return 0;  // refused
+    const cubert::PagedPlan plan = cubert::plan_paged(half_precision != 0, batch, heads, kv_heads, q_rows, (long long) width * page, head_size, left, sinks);
+    return plan.problems * plan.rows >= 1 << 24 ? 0 : plan.floats;
 }
 
 int cubert_attention_paged_f32(const float *q, int ldq, const float *k_pages, const float *v_pages, long long page_stride, long long head_stride,
