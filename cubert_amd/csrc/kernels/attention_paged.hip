@@ -19,8 +19,8 @@ namespace {
 
 constexpr int kFar = (1 << 30) - 1;  // a bound or position that no sequence reaches
 constexpr float kNone = -3e38f;      // the maximum of no scores: finite, so that differences to it are numbers
-constexpr int kMaxGroups = 512;      // workgroups that a cache is cut for
-constexpr int kUncut = 8;            // units of a problem that one workgroup has
+constexpr int kLeast = 8;            // units of a piece
+constexpr int kFewPieces = 16, kSomePieces = 64;  // of a problem, on average
 
 struct PagedArgs {
     const void *q, *k, *v;
@@ -112,10 +112,11 @@ __device__ __forceinline__ void two_terms(float e0, float e1, v2f16 &high, v2f16
     low = __builtin_elementwise_max(low, v2f16{(_Float16) 0x1p-24f, (_Float16) 0x1p-24f});
 }
 
-// What a launch is cut into: `groups` workgroups take runs of units, `least` of them at least, or (groups = 0) one workgroup has all of a problem.
-// A problem is a tile of rows of a sequence and a key head; sequences and tiles are numbered together, tile * batch + sequence.
+// A problem is a tile of rows of a sequence and a key head; sequences and tiles are numbered together, tile * batch + sequence.  A workgroup has one
+// (pieces = 0) or a piece of one: about `pieces` of all units, `least` units at least, so pieces + problems of them at most.
 struct PagedPlan {
-    int rows, row_tiles, groups, least;  // rows of a tile
+    int rows, row_tiles, pieces, least;  // rows of a tile
+    int slot_rows;                       // of which that many are there
     long long problems;
     size_t floats;
 };
@@ -158,21 +159,13 @@ __device__ __forceinline__ int sum_through(int x) {
     return x;
 }
 
-// Lengths and positions of 64 of the sequences and tiles, one to a lane.
+// The units of the sequence and tile `entry` (0 behind the last).
 template <int KEYS>
-struct Sequences {
-    int first_one, length, first;
-
-    __device__ __forceinline__ int bring(const PagedArgs &a, const PagedPlan &plan, int from, int lane) {
-        const int i = from + lane, all = a.batch * plan.row_tiles, tile = plan.row_tiles > 1 ? i / a.batch : 0, b = i - tile * a.batch;
-        first_one = from, length = first = 0;
-        if (i < all) {
-            length = a.lengths[b];
-            if (a.first != nullptr) first = a.first[b];
-        }
-        return i < all ? Reach<KEYS>(a, plan, length, first, tile).units * a.kv_heads : 0;
-    }
-};
+__device__ __forceinline__ int units_of(const PagedArgs &a, const PagedPlan &plan, int entry) {
+    if (entry >= a.batch * plan.row_tiles) return 0;
+    const int tile = plan.row_tiles > 1 ? entry / a.batch : 0, b = entry - tile * a.batch;
+    return Reach<KEYS>(a, plan, a.lengths[b], a.first != nullptr ? a.first[b] : 0, tile).units;
+}
 
 template <typename T, int D, int TILES>
 struct Rows {
@@ -182,14 +175,55 @@ struct Rows {
 };
 
 // Bound by reading K and V.
-template <typename T, int D, int TILES, bool CUT>
-__global__ __launch_bounds__(kBlock, 2) void attention_paged_kernel(PagedArgs a, PagedPlan plan) {
+template <typename T, int D, int TILES>
+__global__ __launch_bounds__(kBlock, TILES == 1 ? 3 : 2) void attention_paged_kernel(PagedArgs a, PagedPlan plan) {
     typedef Shape<T, D> S;
     typedef Reach<S::kKeys> Reached;
     constexpr int kWaves = kBlock / kWave, kRows = 16 * TILES, kSub = S::kSub, kKeys = S::kKeys;
     extern __shared__ __align__(16) unsigned char smem[];
     const int wave = wave_in_block(), lane = threadIdx.x & (kWave - 1), col = lane & 15, quarter = lane >> 4;
     const int share = a.heads / a.kv_heads, rows = a.q_rows * share;
+
+    // which problem, and which piece of it
+    int entry, kv_head, piece = 0, pieces = 1;
+    if (plan.pieces == 0) {
+        entry = blockIdx.x / a.kv_heads, kv_head = blockIdx.x - entry * a.kv_heads;
+    } else {
+        // (every wavefront looks through the sequences by itself, 64 at a time, the first of them out of registers)
+        constexpr int kKept = 4;
+        const int all = a.batch * plan.row_tiles;
+        int units[kKept], sum = 0;
+#pragma unroll
+        for (int n = 0; n < kKept; ++n) units[n] = n == 0 || n * kWave < all ? units_of<kKeys>(a, plan, n * kWave + lane) : 0;
+#pragma unroll
+        for (int n = 0; n < kKept; ++n) sum += units[n];
+        for (int i = kKept * kWave; i < all; i += kWave) sum += units_of<kKeys>(a, plan, i + lane);
+        const int total = __builtin_amdgcn_readlane(sum_through(sum), kWave - 1) * a.kv_heads;  // (below 2^30: see plan_paged)
+        const int least = (total + plan.pieces - 1) / plan.pieces, most = least > plan.least ? least : plan.least;  // units of a piece
+        int before = 0;
+        bool found = false;
+        auto look = [&](int from, int of_lane) {
+            const int own = (of_lane + most - 1) / most, through = sum_through(own * a.kv_heads);
+            const unsigned long long here = __ballot(before + through > (int) blockIdx.x);
+            if (here != 0) {
+                const int at = __builtin_ctzll(here);
+                found = true, entry = from + at, pieces = __builtin_amdgcn_readlane(own, at);
+                piece = (int) blockIdx.x - (before + __builtin_amdgcn_readlane(through, at) - pieces * a.kv_heads);
+                kv_head = piece / pieces, piece -= kv_head * pieces;
+            }
+            before += __builtin_amdgcn_readlane(through, kWave - 1);
+        };
+#pragma unroll
+        for (int n = 0; n < kKept; ++n)
+            if (!found && n * kWave < all) look(n * kWave, units[n]);
+        for (int i = kKept * kWave; !found && i < all; i += kWave) look(i, units_of<kKeys>(a, plan, i + lane));
+        if (!found) return;
+    }
+    const int tile = plan.row_tiles > 1 ? entry / a.batch : 0, sequence = entry - tile * a.batch, row0 = tile * kRows;
+    const Reached reach(a, plan, a.lengths[sequence], a.first != nullptr ? a.first[sequence] : 0, tile);
+    const int each = reach.units / pieces, rest = reach.units - each * pieces;
+    const int unit = each * piece + (piece < rest ? piece : rest), count = each + (piece < rest ? 1 : 0);  // units of this piece
+
     const int page_mask = (1 << a.shift) - 1;
     const long long page_bytes = a.page_stride * (long long) sizeof(T);
     const unsigned row_bytes = (unsigned) a.row_stride * (unsigned) sizeof(T);
@@ -201,380 +235,326 @@ __global__ __launch_bounds__(kBlock, 2) void attention_paged_kernel(PagedArgs a,
     auto value_key = [](int j) { return S::kHalf ? j * (kWave / kPieces) : j * 4 / S::kValueLoads; };
     auto value_part = [](int j) { return S::kHalf ? 0 : j % (S::kValueLoads / 4 > 0 ? S::kValueLoads / 4 : 1); };
     unsigned char *const v_lds = smem + wave * S::kValueLds;
+    const char *k_base = (const char *) a.k + kv_head * a.head_stride * (long long) sizeof(T);
+    const char *v_base = (const char *) a.v + kv_head * a.head_stride * (long long) sizeof(T);
+    const int *table = a.table + (size_t) sequence * a.ld_table;
+    const int seen_begin = reach.low > a.left ? reach.low - a.left : 0, all_begin = reach.high > a.left ? reach.high - a.left : 0;
+    const int seen_end = reach.any ? reach.high + 1 : 0, all_end = reach.any ? reach.low + 1 : 0;
 
-    // which problem comes first, which of its units, and how many units this workgroup has
-    int entry, kv_head, unit, todo = 1 << 30, chunk = 1 << 30, base = 0;  // base: the entry's first unit among all
-    Sequences<kKeys> sequences;
-    if constexpr (CUT) {
-        const int all = a.batch * plan.row_tiles;
-        int units = sequences.bring(a, plan, 0, lane), sum = units;
-        for (int i = kWave; i < all; i += kWave) {
-            Sequences<kKeys> others;
-            sum += others.bring(a, plan, i, lane);
+    // a wavefront's run among them; lane l has the page of the l-th 16 keys from unit x0 on
+    int x = unit + count * wave / kWaves;
+    const int until = unit + count * (wave + 1) / kWaves;
+    int x0 = x, pages = -1;
+    auto look_up = [&](int from_unit) {
+        x0 = from_unit;
+        const int key = reach.key_of(x0 + lane / kSub) + lane % kSub * 16;
+        pages = -1;
+        if (key < seen_end) {
+            const int page = table[key >> a.shift];
+            if (page >= 0 && page < a.pages) pages = page;
         }
-        int through = sum_through(units);
-        const int total = all > kWave ? __builtin_amdgcn_readlane(sum_through(sum), kWave - 1) : __builtin_amdgcn_readlane(through, kWave - 1);
-        chunk = (total + plan.groups - 1) / plan.groups;
-        chunk = chunk > plan.least ? chunk : plan.least;
-        const int from = (int) blockIdx.x * chunk;  // (below 2^31 + 2^31 / groups: see plan_paged)
-        if (from >= total) return;
-        while (true) {
-            const unsigned long long after = __ballot(base + through > from);
-            if (after != 0) {
-                const int at = __builtin_ctzll(after);
-                entry = sequences.first_one + at;
-                units = __builtin_amdgcn_readlane(units, at);
-                base += __builtin_amdgcn_readlane(through, at) - units;
-                break;
+    };
+    if (x < until) look_up(x);
+
+    Rows<T, D, TILES> r;
+    int begin[TILES], end[TILES];  // of what a lane's row sees, the sinks aside
+#pragma unroll
+    for (int m = 0; m < TILES; ++m) {
+        const int row = row0 + 16 * m + col, my_row = row < rows ? row : rows - 1, query = share == 1 ? my_row : my_row / share;
+        const char *q = (const char *) a.q + ((size_t) (sequence * a.q_rows + query) * a.ldq +
+                                              (size_t) (kv_head * share + my_row - query * share) * D) * sizeof(T);
+#pragma unroll
+        for (int t = 0; t < S::kKeyLoads; ++t) {
+            r.q[m][t] = *reinterpret_cast<const v4f32 *>(q + 64 * t + 16 * quarter);
+            if (a.negate) {
+                if constexpr (S::kHalf) r.q[m][t] = __builtin_bit_cast(v4f32, -__builtin_bit_cast(v8f16, r.q[m][t]));
+                else r.q[m][t] = -r.q[m][t];
             }
-            base += __builtin_amdgcn_readlane(through, kWave - 1);
-            units = sequences.bring(a, plan, sequences.first_one + kWave, lane);
-            through = sum_through(units);
         }
-        todo = total - from < chunk ? total - from : chunk;
-        const int each = units / a.kv_heads;
-        kv_head = (from - base) / each, unit = from - base - kv_head * each;
-    } else {
-        entry = blockIdx.x / a.kv_heads, kv_head = blockIdx.x - entry * a.kv_heads, unit = 0;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) r.ctx[m][d] = v4f32{};
+        r.top[m] = kNone, r.sum[m] = 0.f;
+        const int p = reach.first + query;
+        begin[m] = p > a.left ? p - a.left : 0, end[m] = p >= 0 && p < reach.length ? p + 1 : 0;
     }
-    for (bool begun = true; todo > 0; begun = false) {
-        const int tile = plan.row_tiles > 1 ? entry / a.batch : 0, sequence = entry - tile * a.batch;
-        int length, first = 0;
-        if constexpr (CUT) {
-            if (entry - sequences.first_one >= kWave) sequences.bring(a, plan, entry, lane);
-            length = __builtin_amdgcn_readlane(sequences.length, entry - sequences.first_one);
-            first = __builtin_amdgcn_readlane(sequences.first, entry - sequences.first_one);
-        } else {
-            length = a.lengths[sequence];
-            if (a.first != nullptr) first = a.first[sequence];
+
+    Words<4> k[kSub][S::kKeyLoads];
+    Words<S::kValueBytes / 4> v[kSub][S::kValueLoads];
+    unsigned there_next = 0;  // which 16 keys of a unit have a page
+    auto offset_of = [&](int unit_at, int n) -> long long {
+        const int page = __builtin_amdgcn_readlane(pages, (unit_at - x0) * kSub + n);
+        return (page < 0 ? 0 : page) * page_bytes + (long long) ((reach.key_of(unit_at) + 16 * n) & page_mask) * row_bytes;
+    };
+    auto bring_keys = [&](int unit_at) {
+        if (unit_at - x0 == kWave / kSub) look_up(unit_at);
+        there_next = 0;
+#pragma unroll
+        for (int n = 0; n < kSub; ++n) {
+            if (__builtin_amdgcn_readlane(pages, (unit_at - x0) * kSub + n) >= 0) there_next |= 1u << n;
+            const char *at = k_base + offset_of(unit_at, n);
+#pragma unroll
+            for (int t = 0; t < S::kKeyLoads; ++t) k[n][t] = *reinterpret_cast<const Words<4> *>(at + k_offset + 64 * t);
         }
-        const Reached reach(a, plan, length, first, tile);
-        const int count = reach.units - unit < todo ? reach.units - unit : todo;  // units of this problem that this workgroup has
-        const int row0 = tile * kRows;
-        const char *k_base = (const char *) a.k + kv_head * a.head_stride * (long long) sizeof(T);
-        const char *v_base = (const char *) a.v + kv_head * a.head_stride * (long long) sizeof(T);
-        const int *table = a.table + (size_t) sequence * a.ld_table;
-        const int seen_begin = reach.low > a.left ? reach.low - a.left : 0, all_begin = reach.high > a.left ? reach.high - a.left : 0;
-        const int seen_end = reach.any ? reach.high + 1 : 0, all_end = reach.any ? reach.low + 1 : 0;
-
-        // a wavefront's run among them; lane l has the page of the l-th 16 keys from unit x0 on
-        int x = unit + count * wave / kWaves;
-        const int until = unit + count * (wave + 1) / kWaves;
-        int x0 = x, pages = -1;
-        auto look_up = [&](int from_unit) {
-            x0 = from_unit;
-            const int key = reach.key_of(x0 + lane / kSub) + lane % kSub * 16;
-            pages = -1;
-            if (key < seen_end) {
-                const int page = table[key >> a.shift];
-                if (page >= 0 && page < a.pages) pages = page;
-            }
-        };
-        if (x < until) look_up(x);
-
-        Rows<T, D, TILES> r;
-        int begin[TILES], end[TILES];  // of what a lane's row sees, the sinks aside
+    };
+    auto bring_values = [&](int unit_at) {
 #pragma unroll
-        for (int m = 0; m < TILES; ++m) {
-            const int row = row0 + 16 * m + col, my_row = row < rows ? row : rows - 1, query = share == 1 ? my_row : my_row / share;
-            const char *q = (const char *) a.q + ((size_t) (sequence * a.q_rows + query) * a.ldq +
-                                                  (size_t) (kv_head * share + my_row - query * share) * D) * sizeof(T);
+        for (int n = 0; n < kSub; ++n) {
+            const char *at = v_base + offset_of(unit_at, n);
 #pragma unroll
-            for (int t = 0; t < S::kKeyLoads; ++t) {
-                r.q[m][t] = *reinterpret_cast<const v4f32 *>(q + 64 * t + 16 * quarter);
-                if (a.negate) {
-                    if constexpr (S::kHalf) r.q[m][t] = __builtin_bit_cast(v4f32, -__builtin_bit_cast(v8f16, r.q[m][t]));
-                    else r.q[m][t] = -r.q[m][t];
-                }
-            }
-#pragma unroll
-            for (int d = 0; d < D / 16; ++d) r.ctx[m][d] = v4f32{};
-            r.top[m] = kNone, r.sum[m] = 0.f;
-            const int p = reach.first + query;
-            begin[m] = p > a.left ? p - a.left : 0, end[m] = p >= 0 && p < reach.length ? p + 1 : 0;
+            for (int j = 0; j < S::kValueLoads; ++j)
+                v[n][j] = *reinterpret_cast<const Words<S::kValueBytes / 4> *>(at + value_key(j) * row_bytes + v_offset + 256 * value_part(j));
         }
-
-        Words<4> k[kSub][S::kKeyLoads];
-        Words<S::kValueBytes / 4> v[kSub][S::kValueLoads];
-        unsigned there_next = 0;  // which 16 keys of a unit have a page
-        auto offset_of = [&](int unit_at, int n) -> long long {
-            const int page = __builtin_amdgcn_readlane(pages, (unit_at - x0) * kSub + n);
-            return (page < 0 ? 0 : page) * page_bytes + (long long) ((reach.key_of(unit_at) + 16 * n) & page_mask) * row_bytes;
-        };
-        auto bring_keys = [&](int unit_at) {
-            if (unit_at - x0 == kWave / kSub) look_up(unit_at);
-            there_next = 0;
+    };
+    auto take = [&](int unit_at, auto more) {
+        const unsigned there = there_next;
+        const int key0 = reach.key_of(unit_at);
+        v4f32 s[TILES][kSub];
 #pragma unroll
-            for (int n = 0; n < kSub; ++n) {
-                if (__builtin_amdgcn_readlane(pages, (unit_at - x0) * kSub + n) >= 0) there_next |= 1u << n;
-                const char *at = k_base + offset_of(unit_at, n);
+        for (int n = 0; n < kSub; ++n)
 #pragma unroll
-                for (int t = 0; t < S::kKeyLoads; ++t) k[n][t] = *reinterpret_cast<const Words<4> *>(at + k_offset + 64 * t);
-            }
-        };
-        auto bring_values = [&](int unit_at) {
+            for (int m = 0; m < TILES; ++m) s[m][n] = v4f32{};
 #pragma unroll
-            for (int n = 0; n < kSub; ++n) {
-                const char *at = v_base + offset_of(unit_at, n);
-#pragma unroll
-                for (int j = 0; j < S::kValueLoads; ++j)
-                    v[n][j] = *reinterpret_cast<const Words<S::kValueBytes / 4> *>(at + value_key(j) * row_bytes + v_offset + 256 * value_part(j));
-            }
-        };
-        auto take = [&](int unit_at, auto more) {
-            const unsigned there = there_next;
-            const int key0 = reach.key_of(unit_at);
-            v4f32 s[TILES][kSub];
+        for (int t = 0; t < S::kKeyLoads; ++t)
 #pragma unroll
             for (int n = 0; n < kSub; ++n)
 #pragma unroll
-                for (int m = 0; m < TILES; ++m) s[m][n] = v4f32{};
+                for (int m = 0; m < TILES; ++m) {
+                    if constexpr (S::kHalf) {
+                        s[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8f16, k[n][t]), __builtin_bit_cast(v8f16, r.q[m][t]), s[m][n], 0, 0, 0);
+                    } else {
+                        const v4f32 piece = __builtin_bit_cast(v4f32, k[n][t]);
 #pragma unroll
-            for (int t = 0; t < S::kKeyLoads; ++t)
-#pragma unroll
-                for (int n = 0; n < kSub; ++n)
-#pragma unroll
-                    for (int m = 0; m < TILES; ++m) {
-                        if constexpr (S::kHalf) {
-                            s[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8f16, k[n][t]), __builtin_bit_cast(v8f16, r.q[m][t]), s[m][n], 0, 0, 0);
-                        } else {
-                            const v4f32 piece = __builtin_bit_cast(v4f32, k[n][t]);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) s[m][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(piece[e], r.q[m][t][e], s[m][n], 0, 0, 0);
-                        }
-                    }
-            products_done();
-            if constexpr (decltype(more)::value) bring_keys(unit_at + 1);
-            __builtin_amdgcn_sched_barrier(0);
-            const bool all = there == (1u << kSub) - 1 && key0 + kKeys <= all_end && (key0 >= all_begin || key0 + kKeys <= a.sinks);
-            if (!all) {
-#pragma unroll
-                for (int n = 0; n < kSub; ++n) {
-                    const bool is = there >> n & 1u;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int key = key0 + 16 * n + 4 * quarter + i;
-#pragma unroll
-                        for (int m = 0; m < TILES; ++m) s[m][n][i] = is && key < end[m] && (key >= begin[m] || key < a.sinks) ? s[m][n][i] : -INFINITY;
-                    }
-                    // (a key that nobody sees has probability 0, but 0 times what its row of V may hold need not be 0)
-#pragma unroll
-                    for (int j = 0; j < S::kValueLoads; ++j) {
-                        const int key = key0 + 16 * n + value_key(j) + v_key;
-                        const bool use = is && key < seen_end && (key >= seen_begin || key < a.sinks);
-#pragma unroll
-                        for (int w = 0; w < S::kValueBytes / 4; ++w) v[n][j][w] = use ? v[n][j][w] : 0;
+                        for (int e = 0; e < 4; ++e) s[m][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(piece[e], r.q[m][t][e], s[m][n], 0, 0, 0);
                     }
                 }
-            }
-            if constexpr (S::kHalf) {
-#pragma unroll
-                for (int n = 0; n < kSub; ++n)
-#pragma unroll
-                    for (int j = 0; j < S::kValueLoads; ++j) {
-                        const int key = 16 * n + value_key(j) + v_key;
-                        *reinterpret_cast<Words<4> *>(v_lds + key * S::kRowBytes + v_piece<S::kRowBytes>(key, lane % kPieces) * 16) = v[n][j];
-                    }
-                asm volatile("" ::: "memory");
-                __builtin_amdgcn_wave_barrier();
-                if constexpr (decltype(more)::value) bring_values(unit_at + 1);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-#pragma unroll
-            for (int m = 0; m < TILES; ++m) {
-                float top = s[m][0][0];
-#pragma unroll
-                for (int n = 0; n < kSub; ++n)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) top = fmaxf(top, s[m][n][i]);
-                // sums are scaled anew only when some maximum has risen by more than they bear
-                if (__any((top - r.top[m]) * a.scale > S::kSlack)) {
-                    const float high = fmaxf(r.top[m], quarters_max(top)), shrink = __builtin_amdgcn_exp2f((r.top[m] - high) * a.scale);
-                    r.top[m] = high;
-                    r.sum[m] *= shrink;
-#pragma unroll
-                    for (int d = 0; d < D / 16; ++d) r.ctx[m][d] *= shrink;
-                }
-#pragma unroll
-                for (int n = 0; n < kSub; ++n)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        s[m][n][i] = __builtin_amdgcn_exp2f(fmaf(s[m][n][i] - r.top[m], a.scale, S::kRaise));
-                        r.sum[m] += s[m][n][i];
-                    }
-            }
-            if constexpr (S::kHalf) {
-#pragma unroll
-                for (int n = 0; n < kSub; n += 2) {
-                    v8f16 p[TILES], low[TILES];  // of the keys that the transposed V has in the same places
-#pragma unroll
-                    for (int m = 0; m < TILES; ++m)
-#pragma unroll
-                        for (int i = 0; i < 8; i += 2) {
-                            v2f16 x, y;
-                            two_terms(s[m][n + i / 4][i % 4], s[m][n + i / 4][i % 4 + 1], x, y);
-                            p[m][i] = x[0], p[m][i + 1] = x[1], low[m][i] = y[0], low[m][i + 1] = y[1];
-                        }
-#pragma unroll
-                    for (int d = 0; d < D / 16; ++d) {
-                        v4f16 part[2];
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int key = 16 * (n + h) + 4 * quarter + col / 4, at = 2 * d + col % 4 / 2;
-                            part[h] = read_transposed(v_lds + key * S::kRowBytes + v_piece<S::kRowBytes>(key, at) * 16 + col % 2 * 8);
-                        }
-                        const v8f16 x = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-                        for (int m = 0; m < TILES; ++m) {
-                            r.ctx[m][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, low[m], r.ctx[m][d], 0, 0, 0);
-                            r.ctx[m][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, p[m], r.ctx[m][d], 0, 0, 0);
-                        }
-                    }
-                }
-                asm volatile("" ::: "memory");
-                __builtin_amdgcn_wave_barrier();
-            } else {
-#pragma unroll
-                for (int n = 0; n < kSub; ++n)
-#pragma unroll
-                    for (int j = 0; j < S::kValueLoads; ++j) {
-                        Words<S::kValueBytes / 4> words = v[n][j];
-                        pin_registers(words);  // (taken apart here, not where they arrive)
-                        const Numbers<T, S::kColumns> piece = __builtin_bit_cast(Numbers<T, S::kColumns>, words);
-#pragma unroll
-                        for (int e = 0; e < S::kColumns; ++e)
-#pragma unroll
-                            for (int m = 0; m < TILES; ++m) {
-                                v4f32 &to = r.ctx[m][value_part(j) * S::kColumns + e];
-                                to = __builtin_amdgcn_mfma_f32_16x16x4f32((float) piece[e], s[m][n][value_key(j)], to, 0, 0, 0);
-                            }
-                    }
-                __builtin_amdgcn_sched_barrier(0);
-                if constexpr (decltype(more)::value) bring_values(unit_at + 1);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        };
-        if (x < until) {
-            bring_keys(x);
-            bring_values(x);
-            for (; x + 1 < until; ++x) take(x, std::true_type());
-            take(x, std::false_type());
-        }
         products_done();
-
-        // the four wavefronts' sums: rows of D results, the maximum and the sum
-        const int present = rows - row0 < kRows ? rows - row0 : kRows;
-        float *merge = reinterpret_cast<float *>(smem);
-        __syncthreads();  // nobody reads V, or the sums of the problem before, any more
+        if constexpr (decltype(more)::value) bring_keys(unit_at + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        const bool all = there == (1u << kSub) - 1 && key0 + kKeys <= all_end && (key0 >= all_begin || key0 + kKeys <= a.sinks);
+        if (!all) {
+#pragma unroll
+            for (int n = 0; n < kSub; ++n) {
+                const bool is = there >> n & 1u;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int key = key0 + 16 * n + 4 * quarter + i;
+#pragma unroll
+                    for (int m = 0; m < TILES; ++m) s[m][n][i] = is && key < end[m] && (key >= begin[m] || key < a.sinks) ? s[m][n][i] : -INFINITY;
+                }
+                // (a key that nobody sees has probability 0, but 0 times what its row of V may hold need not be 0)
+#pragma unroll
+                for (int j = 0; j < S::kValueLoads; ++j) {
+                    const int key = key0 + 16 * n + value_key(j) + v_key;
+                    const bool use = is && key < seen_end && (key >= seen_begin || key < a.sinks);
+#pragma unroll
+                    for (int w = 0; w < S::kValueBytes / 4; ++w) v[n][j][w] = use ? v[n][j][w] : 0;
+                }
+            }
+        }
+        if constexpr (S::kHalf) {
+#pragma unroll
+            for (int n = 0; n < kSub; ++n)
+#pragma unroll
+                for (int j = 0; j < S::kValueLoads; ++j) {
+                    const int key = 16 * n + value_key(j) + v_key;
+                    *reinterpret_cast<Words<4> *>(v_lds + key * S::kRowBytes + v_piece<S::kRowBytes>(key, lane % kPieces) * 16) = v[n][j];
+                }
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_wave_barrier();
+            if constexpr (decltype(more)::value) bring_values(unit_at + 1);
+            __builtin_amdgcn_sched_barrier(0);
+        }
 #pragma unroll
         for (int m = 0; m < TILES; ++m) {
-            float sum = r.sum[m] + __shfl_xor(r.sum[m], 16, kWave);
-            sum += __shfl_xor(sum, 32, kWave);
-            const int row = 16 * m + col;
-            if (row < present) {
-                float *to = merge + (wave * present + row) * S::kPitch;
-                if constexpr (S::kHalf) {
+            float top = s[m][0][0];
 #pragma unroll
-                    for (int d = 0; d < D / 16; ++d) *reinterpret_cast<v4f32 *>(to + 16 * d + 4 * quarter) = r.ctx[m][d];
-                } else {
+            for (int n = 0; n < kSub; ++n)
 #pragma unroll
-                    for (int d = 0; d < D / 16; d += 2)
+                for (int i = 0; i < 4; ++i) top = fmaxf(top, s[m][n][i]);
+            // sums are scaled anew only when some maximum has risen by more than they bear
+            if (__any((top - r.top[m]) * a.scale > S::kSlack)) {
+                const float high = fmaxf(r.top[m], quarters_max(top)), shrink = __builtin_amdgcn_exp2f((r.top[m] - high) * a.scale);
+                r.top[m] = high;
+                r.sum[m] *= shrink;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            *reinterpret_cast<v2f32 *>(to + d / S::kColumns * 64 + (4 * quarter + i) * S::kColumns + d % S::kColumns) =
-                                    v2f32{r.ctx[m][d][i], r.ctx[m][d + 1][i]};
+                for (int d = 0; d < D / 16; ++d) r.ctx[m][d] *= shrink;
+            }
+#pragma unroll
+            for (int n = 0; n < kSub; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[m][n][i] = __builtin_amdgcn_exp2f(fmaf(s[m][n][i] - r.top[m], a.scale, S::kRaise));
+                    r.sum[m] += s[m][n][i];
                 }
-                if (quarter == 0) to[D] = r.top[m], to[D + 1] = sum;
-            }
         }
-        __syncthreads();
-        const bool whole = !CUT || count == reach.units;
-        constexpr int kQuads = D / 4;  // a thread has four columns of a row
-        for (int i = threadIdx.x; i < present * kQuads; i += kBlock) {
-            const int row = i / kQuads, d = (i - row * kQuads) * 4;
-            float top = kNone;
+        if constexpr (S::kHalf) {
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) top = fmaxf(top, merge[(w * present + row) * S::kPitch + D]);
-            v4f32 x4 = v4f32{};
-            float total = 0.f;
+            for (int n = 0; n < kSub; n += 2) {
+                v8f16 p[TILES], low[TILES];  // of the keys that the transposed V has in the same places
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
-                const float *of = merge + (w * present + row) * S::kPitch;
-                const float f = __builtin_amdgcn_exp2f((of[D] - top) * a.scale);
-                total += of[D + 1] * f;
-                x4 += *reinterpret_cast<const v4f32 *>(of + d) * f;
+                for (int m = 0; m < TILES; ++m)
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) {
+                        v2f16 x, y;
+                        two_terms(s[m][n + i / 4][i % 4], s[m][n + i / 4][i % 4 + 1], x, y);
+                        p[m][i] = x[0], p[m][i + 1] = x[1], low[m][i] = y[0], low[m][i + 1] = y[1];
+                    }
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d) {
+                    v4f16 part[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int key = 16 * (n + h) + 4 * quarter + col / 4, at = 2 * d + col % 4 / 2;
+                        part[h] = read_transposed(v_lds + key * S::kRowBytes + v_piece<S::kRowBytes>(key, at) * 16 + col % 2 * 8);
+                    }
+                    const v8f16 x = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+                    for (int m = 0; m < TILES; ++m) {
+                        r.ctx[m][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, low[m], r.ctx[m][d], 0, 0, 0);
+                        r.ctx[m][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, p[m], r.ctx[m][d], 0, 0, 0);
+                    }
+                }
             }
-            const int out_row = row0 + row, query = share == 1 ? out_row : out_row / share, p = reach.first + query;
-            const bool there = p >= 0 && p < reach.length;
-            if (whole) {
-                T *ctx = (T *) a.ctx + (size_t) (sequence * a.q_rows + query) * a.ld_ctx + (size_t) (kv_head * share + out_row - query * share) * D + d;
-                const float by = there && total != 0.f ? 1.f / total : 0.f;  // (a sum that is no number stays none)
-                store4(ctx, by != 0.f ? x4 * by : v4f32{});
-            } else {
-                float *to = a.partials + ((size_t) (2 * blockIdx.x + (begun ? 0 : 1)) * kRows + row) * S::kPitch;
-                *reinterpret_cast<v4f32 *>(to + d) = there ? x4 : v4f32{};
-                if (d == 0) to[D] = there ? top : kNone, to[D + 1] = there ? total : 0.f;
-            }
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_wave_barrier();
+        } else {
+#pragma unroll
+            for (int n = 0; n < kSub; ++n)
+#pragma unroll
+                for (int j = 0; j < S::kValueLoads; ++j) {
+                    Words<S::kValueBytes / 4> words = v[n][j];
+                    pin_registers(words);  // (taken apart here, not where they arrive)
+                    const Numbers<T, S::kColumns> piece = __builtin_bit_cast(Numbers<T, S::kColumns>, words);
+#pragma unroll
+                    for (int e = 0; e < S::kColumns; ++e)
+#pragma unroll
+                        for (int m = 0; m < TILES; ++m) {
+                            v4f32 &to = r.ctx[m][value_part(j) * S::kColumns + e];
+                            to = __builtin_amdgcn_mfma_f32_16x16x4f32((float) piece[e], s[m][n][value_key(j)], to, 0, 0, 0);
+                        }
+                }
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (decltype(more)::value) bring_values(unit_at + 1);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        if constexpr (!CUT) break;
-        todo -= count;
-        // Of a problem's first piece: where it stands, and how many more there are (each the first of its workgroup).
-        if (unit == 0 && threadIdx.x == 0) {
-            v2i32 *note = reinterpret_cast<v2i32 *>(a.partials + (size_t) 2 * plan.groups * kRows * S::kPitch);
-            const int last = base + (kv_head + 1) * reach.units - 1;
-            note[(size_t) entry * a.kv_heads + kv_head] = v2i32{2 * (int) blockIdx.x + (begun ? 0 : 1), last / chunk - (int) blockIdx.x};
-        }
-        unit = 0;
-        if (++kv_head == a.kv_heads) kv_head = 0, base += reach.units * a.kv_heads, ++entry;
-        __syncthreads();  // the sums have been read
+    };
+    if (x < until) {
+        bring_keys(x);
+        bring_values(x);
+        for (; x + 1 < until; ++x) take(x, std::true_type());
+        take(x, std::false_type());
     }
+    products_done();
+
+    // the four wavefronts' sums: rows of D results, the maximum and the sum
+    const int present = rows - row0 < kRows ? rows - row0 : kRows;
+    float *merge = reinterpret_cast<float *>(smem);
+    __syncthreads();  // nobody reads V any more
+#pragma unroll
+    for (int m = 0; m < TILES; ++m) {
+        float sum = r.sum[m] + __shfl_xor(r.sum[m], 16, kWave);
+        sum += __shfl_xor(sum, 32, kWave);
+        const int row = 16 * m + col;
+        if (row < present) {
+            float *to = merge + (wave * present + row) * S::kPitch;
+            if constexpr (S::kHalf) {
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d) *reinterpret_cast<v4f32 *>(to + 16 * d + 4 * quarter) = r.ctx[m][d];
+            } else {
+#pragma unroll
+                for (int d = 0; d < D / 16; d += 2)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        *reinterpret_cast<v2f32 *>(to + d / S::kColumns * 64 + (4 * quarter + i) * S::kColumns + d % S::kColumns) =
+                                v2f32{r.ctx[m][d][i], r.ctx[m][d + 1][i]};
+            }
+            if (quarter == 0) to[D] = r.top[m], to[D + 1] = sum;
+        }
+    }
+    __syncthreads();
+    constexpr int kQuads = D / 4;  // a thread has four columns of a row
+    for (int i = threadIdx.x; i < present * kQuads; i += kBlock) {
+        const int row = i / kQuads, d = (i - row * kQuads) * 4;
+        float top = kNone;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) top = fmaxf(top, merge[(w * present + row) * S::kPitch + D]);
+        v4f32 x4 = v4f32{};
+        float total = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float *of = merge + (w * present + row) * S::kPitch;
+            const float f = __builtin_amdgcn_exp2f((of[D] - top) * a.scale);
+            total += of[D + 1] * f;
+            x4 += *reinterpret_cast<const v4f32 *>(of + d) * f;
+        }
+        const int out_row = row0 + row, query = share == 1 ? out_row : out_row / share, p = reach.first + query;
+        const bool there = p >= 0 && p < reach.length;
+        if (pieces == 1) {
+            T *ctx = (T *) a.ctx + (size_t) (sequence * a.q_rows + query) * a.ld_ctx + (size_t) (kv_head * share + out_row - query * share) * D + d;
+            const float by = there && total != 0.f ? 1.f / total : 0.f;  // (a sum that is no number stays none)
+            store4(ctx, by != 0.f ? x4 * by : v4f32{});
+        } else {
+            float *to = a.partials + ((size_t) blockIdx.x * plan.slot_rows + row) * S::kPitch;
+            *reinterpret_cast<v4f32 *>(to + d) = there ? x4 : v4f32{};
+            if (d == 0) to[D] = there ? top : kNone, to[D + 1] = there ? total : 0.f;
+        }
+    }
+    // where a problem's pieces stand, for those who join them
+    if (plan.pieces != 0 && piece == 0 && threadIdx.x == 0)
+        reinterpret_cast<v2i32 *>(a.partials + (size_t) (plan.pieces + plan.problems) * plan.slot_rows * S::kPitch)[(size_t) entry * a.kv_heads + kv_head] =
+                v2i32{(int) blockIdx.x, pieces};
 }
 
-// The pieces' sums of a row joined, by WAVES wavefronts: D / 4 lanes to a piece, their maxima and sums a lane each.
-template <typename T, int D, int WAVES>
-__global__ __launch_bounds__(kBlock) void attention_paged_join_kernel(PagedArgs a, PagedPlan plan) {
+// The pieces' sums of a row joined, COLUMNS at a time, by WAVES wavefronts: COLUMNS / 4 lanes to a piece, their maxima and sums a lane each.
+template <typename T, int D, int COLUMNS, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave < kBlock ? kBlock : WAVES * kWave) void attention_paged_join_kernel(PagedArgs a, PagedPlan plan) {
     typedef Shape<T, D> S;
-    constexpr int kQuads = D / 4, kAtOnce = kWave / kQuads, kPer = kBlock / kWave / WAVES;
+    constexpr int kQuads = COLUMNS / 4, kAtOnce = kWave / kQuads, kPer = WAVES < 4 ? 4 / WAVES : 1, kAhead = kAtOnce >= 8 ? 4 : 8;
     __shared__ float shared[WAVES > 1 ? WAVES * S::kPitch : 1];
     const int wave = wave_in_block(), lane = threadIdx.x & (kWave - 1), share = a.heads / a.kv_heads, rows = a.q_rows * share;
     const int i = blockIdx.x * kPer + wave / WAVES, part = wave % WAVES;
-    const int problem = i / plan.rows, row = i - problem * plan.rows;
+    const int problem = i / plan.slot_rows, row = i - problem * plan.slot_rows;
     if (problem >= plan.problems) return;
+    const v2i32 note = reinterpret_cast<const v2i32 *>(a.partials + (size_t) (plan.pieces + plan.problems) * plan.slot_rows * S::kPitch)[problem];
+    const int pieces = uniform(note[1]);
+    if (pieces == 1) return;  // its one workgroup has written it
     const int entry = problem / a.kv_heads, kv_head = problem - entry * a.kv_heads;
     const int tile = plan.row_tiles > 1 ? entry / a.batch : 0, sequence = entry - tile * a.batch, out_row = tile * plan.rows + row;
     if (out_row >= rows) return;
-    const v2i32 note = reinterpret_cast<const v2i32 *>(a.partials + (size_t) 2 * plan.groups * plan.rows * S::kPitch)[problem];
-    const int pieces = uniform(note[1]) + 1, slot = uniform(note[0]);
-    if (pieces == 1) return;  // its one workgroup has written it
-    const float *first = a.partials + ((size_t) slot * plan.rows + row) * S::kPitch;
-    const float *next = a.partials + ((size_t) (slot / 2 * 2) * plan.rows + row) * S::kPitch;
-    const size_t step = (size_t) 2 * plan.rows * S::kPitch;
-    auto piece_at = [&](int n) { return n == 0 ? first : next + n * step; };
-    const int until = pieces * (part + 1) / WAVES, at = lane / kQuads, d = lane % kQuads * 4;
+    const size_t step = (size_t) plan.slot_rows * S::kPitch;
+    const float *first = a.partials + uniform(note[0]) * step + row * S::kPitch;
+    const int until = pieces * (part + 1) / WAVES, at = lane / kQuads, d = blockIdx.y * COLUMNS + lane % kQuads * 4;
     float top = kNone, sum = 0.f;
     v4f32 x = v4f32{};
     for (int n0 = pieces * part / WAVES; n0 < until; n0 += kWave) {
+        // all that there is to read at once, where that is little (past the last piece the first one again)
         const int here = until - n0 < kWave ? until - n0 : kWave;
-        const float *of = piece_at(n0 + (lane < here ? lane : 0));
-        const float my_top = of[D], my_sum = of[D + 1], high = fmaxf(top, wave_max(my_top));
-        const float weight = lane < here ? __builtin_amdgcn_exp2f((my_top - high) * a.scale) : 0.f, shrink = __builtin_amdgcn_exp2f((top - high) * a.scale);
-        top = high;
-        sum = sum * shrink + wave_sum(weight * my_sum);
-        x *= shrink;
-        constexpr int kAhead = 8;
-        for (int n = 0; n < here; n += kAtOnce * kAhead) {
-            v4f32 y[kAhead];
+        const float *of = first + (n0 + (lane < here ? lane : 0)) * step;
+        const v2f32 mine = *reinterpret_cast<const v2f32 *>(of + D);
+        v4f32 y[kAhead];
+        auto bring = [&](int n) {
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
                 const int m = n + u * kAtOnce + at;
-                y[u] = *reinterpret_cast<const v4f32 *>(piece_at(n0 + (m < here ? m : 0)) + d);
+                y[u] = *reinterpret_cast<const v4f32 *>(first + (n0 + (m < here ? m : 0)) * step + d);
             }
+        };
+        bring(0);
+        const float high = fmaxf(top, wave_max(mine[0])), shrink = __builtin_amdgcn_exp2f((top - high) * a.scale);
+        const float weight = lane < here ? __builtin_amdgcn_exp2f((mine[0] - high) * a.scale) : 0.f;
+        top = high;
+        sum = sum * shrink + wave_sum(weight * mine[1]);
+        x *= shrink;
+        for (int n = 0;;) {
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
                 const int m = n + u * kAtOnce + at;
                 const float f = __shfl(weight, m < here ? m : 0, kWave);
                 if (m < here) x += y[u] * f;
             }
+            n += kAtOnce * kAhead;
+            if (n >= here) break;
+            bring(n);
         }
     }
 #pragma unroll
@@ -615,33 +595,35 @@ PagedPlan plan_paged(bool half_precision, int batch, int heads, int kv_heads, in
     long long reach = limit;  // the most keys that a tile of rows sees, and how many units of them
     if (left >= 0 && (long long) left + plan.rows + sinks < reach) reach = (long long) left + plan.rows + sinks;
     const long long units = (reach + keys - 1) / keys + (left >= 0 ? 2 : 0);
-    plan.least = 8, plan.groups = 0, plan.floats = 0;
-    if (units <= kUncut || plan.problems * units >= 1 << 30) return plan;  // (units are counted in 32 bits)
+    plan.least = kLeast, plan.pieces = 0, plan.floats = 0;
+    plan.slot_rows = (int) (rows < plan.rows ? rows : plan.rows);
+    const long long uncut = plan.problems / 8 < 16 ? 16 : plan.problems / 8 < 128 ? plan.problems / 8 : 128;
+    if (units <= uncut || plan.problems * units >= 1 << 30) return plan;  // (units are counted in 32 bits)
     const long long most = (plan.problems * units + plan.least - 1) / plan.least;
-    plan.groups = (int) (most < kMaxGroups ? most : kMaxGroups);
-    plan.floats = (size_t) 2 * plan.groups * plan.rows * (head_size + 4) + 2 * (size_t) plan.problems;
+    plan.pieces = plan.problems <= 32 ? 256 - (int) plan.problems : plan.problems <= 160 ? 512 - (int) plan.problems : 1024;
+    if (most < plan.pieces) plan.pieces = (int) most;
+    plan.floats = (size_t) (plan.pieces + plan.problems) * plan.slot_rows * (head_size + 4) + 2 * (size_t) plan.problems;
     return plan;
 }
 
-template <typename T, int D, int TILES, bool CUT>
+template <typename T, int D, int TILES>
 int run_paged(const PagedArgs &a, const PagedPlan &plan, hipStream_t stream) {
     static std::atomic<unsigned long long> done{0};
     typedef Shape<T, D> S;
-    const long long rows = (long long) a.q_rows * (a.heads / a.kv_heads);
-    const unsigned merge = (unsigned) (4 * (rows < plan.rows ? rows : plan.rows) * S::kPitch * 4), lds = merge > 4 * S::kValueLds ? merge : 4 * S::kValueLds;
-    if (lds > 48 * 1024 && !allow_large_lds(attention_paged_kernel<T, D, TILES, CUT>, done)) return CUBERT_UNSUPPORTED;
-    const dim3 grid(CUT ? (unsigned) plan.groups : (unsigned) plan.problems);
-    const int rc = launch_lds(attention_paged_kernel<T, D, TILES, CUT>, grid, dim3(kBlock), lds, stream, a, plan);
-    if (rc != 0 || !CUT) return rc;
-    const unsigned joins = (unsigned) (plan.problems * plan.rows);
-    if (joins >= 1024) return launch(attention_paged_join_kernel<T, D, 1>, dim3((joins + 3) / 4), dim3(kBlock), stream, a, plan);
-    return launch(attention_paged_join_kernel<T, D, 4>, dim3(joins), dim3(kBlock), stream, a, plan);
+    const unsigned merge = (unsigned) (4 * plan.slot_rows * S::kPitch * 4), lds = merge > 4 * S::kValueLds ? merge : 4 * S::kValueLds;
+    if (lds > 48 * 1024 && !allow_large_lds(attention_paged_kernel<T, D, TILES>, done)) return CUBERT_UNSUPPORTED;
+    const int rc = launch_lds(attention_paged_kernel<T, D, TILES>, dim3((unsigned) (plan.pieces + plan.problems)), dim3(kBlock), lds, stream, a, plan);
+    if (rc != 0 || plan.pieces == 0) return rc;
+    const unsigned joins = (unsigned) (plan.problems * plan.slot_rows);
+    const int of_problem = plan.pieces / (int) plan.problems;  // pieces, on average
+    if (of_problem <= kFewPieces) return launch(attention_paged_join_kernel<T, D, D, 1>, dim3((joins + 3) / 4), dim3(kBlock), stream, a, plan);
+    if (of_problem <= kSomePieces) return launch(attention_paged_join_kernel<T, D, D, 4>, dim3(joins), dim3(kBlock), stream, a, plan);
+    return launch(attention_paged_join_kernel<T, D, 32, 16>, dim3(joins, D / 32), dim3(16 * kWave), stream, a, plan);
 }
 
 template <typename T, int D>
 int run_paged_size(const PagedArgs &a, const PagedPlan &plan, hipStream_t stream) {
-    if (plan.rows == 16) return plan.groups != 0 ? run_paged<T, D, 1, true>(a, plan, stream) : run_paged<T, D, 1, false>(a, plan, stream);
-    return plan.groups != 0 ? run_paged<T, D, 2, true>(a, plan, stream) : run_paged<T, D, 2, false>(a, plan, stream);
+    return plan.rows == 16 ? run_paged<T, D, 1>(a, plan, stream) : run_paged<T, D, 2>(a, plan, stream);
 }
 
 template <typename T>
@@ -679,7 +661,7 @@ int attention_paged(const T *q, int ldq, const T *k_pages, const T *v_pages, lon
         return CUBERT_UNSUPPORTED;
     PagedPlan plan = plan_paged(sizeof(T) == 2, batch, heads, kv_heads, q_rows, (long long) width * page, head_size, a.left == kFar ? -1 : left, a.sinks);
     if (plan.problems * plan.rows >= 1 << 24) return CUBERT_UNSUPPORTED;
-    if (plan.groups != 0 && (partials == nullptr || partial_floats < plan.floats || !is_aligned(partials, 16))) plan.groups = 0;
+    if (plan.pieces != 0 && (partials == nullptr || partial_floats < plan.floats || !is_aligned(partials, 16))) plan.pieces = 0;
     if (head_size == 32) return run_paged_size<T, 32>(a, plan, (hipStream_t) stream);
     if (head_size == 64) return run_paged_size<T, 64>(a, plan, (hipStream_t) stream);
     return run_paged_size<T, 128>(a, plan, (hipStream_t) stream);
