@@ -19,7 +19,6 @@ namespace {
 
 constexpr int kFar = (1 << 30) - 1;  // a bound or position that no sequence reaches
 constexpr float kNone = -3e38f;      // the maximum of no scores: finite, so that differences to it are numbers
-constexpr int kLeast = 8;            // units of a piece
 constexpr int kFewPieces = 16, kSomePieces = 64;  // of a problem, on average
 
 struct PagedArgs {
@@ -159,13 +158,20 @@ __device__ __forceinline__ int sum_through(int x) {
     return x;
 }
 
-// The units of the sequence and tile `entry` (0 behind the last).
+// Length, first position and units of the sequence and tile `entry` (0 units behind the last).
 template <int KEYS>
-__device__ __forceinline__ int units_of(const PagedArgs &a, const PagedPlan &plan, int entry) {
-    if (entry >= a.batch * plan.row_tiles) return 0;
-    const int tile = plan.row_tiles > 1 ? entry / a.batch : 0, b = entry - tile * a.batch;
-    return Reach<KEYS>(a, plan, a.lengths[b], a.first != nullptr ? a.first[b] : 0, tile).units;
-}
+struct Entry {
+    int length = 0, first = 0, units = 0;
+
+    __device__ __forceinline__ Entry() {}
+    __device__ __forceinline__ Entry(const PagedArgs &a, const PagedPlan &plan, int entry) {
+        if (entry >= a.batch * plan.row_tiles) return;
+        const int tile = plan.row_tiles > 1 ? entry / a.batch : 0, b = entry - tile * a.batch;
+        length = a.lengths[b];
+        if (a.first != nullptr) first = a.first[b];
+        units = Reach<KEYS>(a, plan, length, first, tile).units;
+    }
+};
 
 template <typename T, int D, int TILES>
 struct Rows {
@@ -185,29 +191,36 @@ __global__ __launch_bounds__(kBlock, TILES == 1 ? 3 : 2) void attention_paged_ke
     const int share = a.heads / a.kv_heads, rows = a.q_rows * share;
 
     // which problem, and which piece of it
-    int entry, kv_head, piece = 0, pieces = 1;
+    int entry, kv_head, piece = 0, pieces = 1, length, first = 0;
     if (plan.pieces == 0) {
         entry = blockIdx.x / a.kv_heads, kv_head = blockIdx.x - entry * a.kv_heads;
+        const int b = plan.row_tiles > 1 ? entry % a.batch : entry;
+        length = a.lengths[b];
+        if (a.first != nullptr) first = a.first[b];
     } else {
         // (every wavefront looks through the sequences by itself, 64 at a time, the first of them out of registers)
         constexpr int kKept = 4;
+        typedef Entry<kKeys> Found;
         const int all = a.batch * plan.row_tiles;
-        int units[kKept], sum = 0;
+        Found kept[kKept];
+        int sum = 0;
 #pragma unroll
-        for (int n = 0; n < kKept; ++n) units[n] = n == 0 || n * kWave < all ? units_of<kKeys>(a, plan, n * kWave + lane) : 0;
+        for (int n = 0; n < kKept; ++n)
+            if (n == 0 || n * kWave < all) kept[n] = Found(a, plan, n * kWave + lane);
 #pragma unroll
-        for (int n = 0; n < kKept; ++n) sum += units[n];
-        for (int i = kKept * kWave; i < all; i += kWave) sum += units_of<kKeys>(a, plan, i + lane);
+        for (int n = 0; n < kKept; ++n) sum += kept[n].units;
+        for (int i = kKept * kWave; i < all; i += kWave) sum += Found(a, plan, i + lane).units;
         const int total = __builtin_amdgcn_readlane(sum_through(sum), kWave - 1) * a.kv_heads;  // (below 2^30: see plan_paged)
         const int least = (total + plan.pieces - 1) / plan.pieces, most = least > plan.least ? least : plan.least;  // units of a piece
         int before = 0;
         bool found = false;
-        auto look = [&](int from, int of_lane) {
-            const int own = (of_lane + most - 1) / most, through = sum_through(own * a.kv_heads);
+        auto look = [&](int from, const Found &of) {
+            const int own = (of.units + most - 1) / most, through = sum_through(own * a.kv_heads);
             const unsigned long long here = __ballot(before + through > (int) blockIdx.x);
             if (here != 0) {
                 const int at = __builtin_ctzll(here);
                 found = true, entry = from + at, pieces = __builtin_amdgcn_readlane(own, at);
+                length = __builtin_amdgcn_readlane(of.length, at), first = __builtin_amdgcn_readlane(of.first, at);
                 piece = (int) blockIdx.x - (before + __builtin_amdgcn_readlane(through, at) - pieces * a.kv_heads);
                 kv_head = piece / pieces, piece -= kv_head * pieces;
             }
@@ -215,12 +228,12 @@ __global__ __launch_bounds__(kBlock, TILES == 1 ? 3 : 2) void attention_paged_ke
         };
 #pragma unroll
         for (int n = 0; n < kKept; ++n)
-            if (!found && n * kWave < all) look(n * kWave, units[n]);
-        for (int i = kKept * kWave; !found && i < all; i += kWave) look(i, units_of<kKeys>(a, plan, i + lane));
+            if (!found && n * kWave < all) look(n * kWave, kept[n]);
+        for (int i = kKept * kWave; !found && i < all; i += kWave) look(i, Found(a, plan, i + lane));
         if (!found) return;
     }
     const int tile = plan.row_tiles > 1 ? entry / a.batch : 0, sequence = entry - tile * a.batch, row0 = tile * kRows;
-    const Reached reach(a, plan, a.lengths[sequence], a.first != nullptr ? a.first[sequence] : 0, tile);
+    const Reached reach(a, plan, length, first, tile);
     const int each = reach.units / pieces, rest = reach.units - each * pieces;
     const int unit = each * piece + (piece < rest ? piece : rest), count = each + (piece < rest ? 1 : 0);  // units of this piece
 
@@ -595,7 +608,7 @@ PagedPlan plan_paged(bool half_precision, int batch, int heads, int kv_heads, in
     long long reach = limit;  // the most keys that a tile of rows sees, and how many units of them
     if (left >= 0 && (long long) left + plan.rows + sinks < reach) reach = (long long) left + plan.rows + sinks;
     const long long units = (reach + keys - 1) / keys + (left >= 0 ? 2 : 0);
-    plan.least = kLeast, plan.pieces = 0, plan.floats = 0;
+    plan.least = plan.problems * units <= 1536 ? 4 : 8, plan.pieces = 0, plan.floats = 0;
     plan.slot_rows = (int) (rows < plan.rows ? rows : plan.rows);
     const long long uncut = plan.problems / 8 < 16 ? 16 : plan.problems / 8 < 128 ? plan.problems / 8 : 128;
     if (units <= uncut || plan.problems * units >= 1 << 30) return plan;  // (units are counted in 32 bits)
