@@ -147,11 +147,9 @@ struct Shrink {
 
 constexpr int kAhead = 8;  // entries of a lane that are on their way together
 
-// How many pages a sequence gives back: entries that are no pages (a window has passed them, and they were taken out) do not count.
-__global__ __launch_bounds__(kBlock) void paged_cut_count_kernel(CutArgs a) {
-    const int b = blockIdx.x * (kBlock / kWave) + wave_in_block(), lane = threadIdx.x & (kWave - 1);
-    if (b >= a.batch) return;
-    const Shrink s(a, b);
+// How many pages a sequence gives back (to a wavefront): entries that are no pages (a window has passed them, and they were taken out) do not
+// count.
+__device__ __forceinline__ int pages_back(const CutArgs &a, int b, const Shrink &s, int lane) {
     const int *row = a.table + (size_t) b * a.ld_table;
     int count = 0;
     for (int i = s.begin + lane; i < s.end; i += kWave * kAhead) {
@@ -163,25 +161,11 @@ __global__ __launch_bounds__(kBlock) void paged_cut_count_kernel(CutArgs a) {
     }
 #pragma unroll
     for (int d = 1; d < kWave; d *= 2) count += __shfl_xor(count, d, kWave);
-    if (lane == 0) a.returned[b] = count, a.lengths_out[b] = s.keep;
+    return count;
 }
 
-// A wavefront per sequence puts them onto the stack, behind those of the sequences before it.
-__global__ __launch_bounds__(kBlock) void paged_cut_kernel(CutArgs a) {
-    const int b = blockIdx.x * (kBlock / kWave) + wave_in_block(), lane = threadIdx.x & (kWave - 1);
-    const int there = clamp_to(*a.free_count, 0, a.pages);
-    if (a.batch == 0 && blockIdx.x == 0 && threadIdx.x == 0) *a.free_out = there;
-    if (b >= a.batch) return;
-    const Shrink s(a, b);
-    long long before = 0;
-    for (int i = lane; i < b; i += kWave) before += a.returned[i];
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) before += __shfl_xor(before, d, kWave);
-    const long long height = there + before;
-    if (b == a.batch - 1 && lane == 0) {
-        const long long all = height + a.returned[b];
-        *a.free_out = (int) (all < a.pages ? all : a.pages);
-    }
+// They go onto the stack from `height` on, as far as it has room.
+__device__ __forceinline__ void put_back(const CutArgs &a, int b, const Shrink &s, long long height, int lane) {
     const int *row = a.table + (size_t) b * a.ld_table;
     const int free_places = height < a.pages ? a.pages - (int) height : 0;
     int *to = a.free + height;
@@ -203,6 +187,64 @@ __global__ __launch_bounds__(kBlock) void paged_cut_kernel(CutArgs a) {
         }
     }
 }
+
+__global__ __launch_bounds__(kBlock) void paged_cut_count_kernel(CutArgs a) {
+    const int b = blockIdx.x * (kBlock / kWave) + wave_in_block(), lane = threadIdx.x & (kWave - 1);
+    if (b >= a.batch) return;
+    const Shrink s(a, b);
+    const int count = pages_back(a, b, s, lane);
+    if (lane == 0) a.returned[b] = count, a.lengths_out[b] = s.keep;
+}
+
+// A wavefront per sequence puts its pages onto the stack, behind those of the sequences before it.
+__global__ __launch_bounds__(kBlock) void paged_cut_kernel(CutArgs a) {
+    const int b = blockIdx.x * (kBlock / kWave) + wave_in_block(), lane = threadIdx.x & (kWave - 1);
+    const int there = clamp_to(*a.free_count, 0, a.pages);
+    if (b >= a.batch) return;
+    const Shrink s(a, b);
+    long long before = 0;
+    for (int i = lane; i < b; i += kWave) before += a.returned[i];
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) before += __shfl_xor(before, d, kWave);
+    const long long height = there + before;
+    if (b == a.batch - 1 && lane == 0) {
+        const long long all = height + a.returned[b];
+        *a.free_out = (int) (all < a.pages ? all : a.pages);
+    }
+    put_back(a, b, s, height, lane);
+}
+
+// Few sequences with short tables: both in one workgroup of 16 wavefronts, which take the sequences in turn.
+constexpr int kFewSequences = 64, kFewWaves = 16;
+constexpr long long kFewEntries = 1 << 15;
+
+__global__ __launch_bounds__(kFewWaves * kWave) void paged_cut_few_kernel(CutArgs a) {
+    __shared__ int back[kFewSequences];
+    const int wave = wave_in_block(), lane = threadIdx.x & (kWave - 1);
+    const int there = clamp_to(*a.free_count, 0, a.pages);
+    for (int b = wave; b < a.batch; b += kFewWaves) {
+        const Shrink s(a, b);
+        const int count = pages_back(a, b, s, lane);
+        if (lane == 0) back[b] = count, a.lengths_out[b] = s.keep;
+    }
+    __syncthreads();
+    const int mine = lane < a.batch ? back[lane] : 0;
+    int through = mine;
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+        const int other = __shfl_up(through, d, kWave);
+        through += lane >= d ? other : 0;
+    }
+    if (wave == 0 && lane == kWave - 1) {
+        const long long all = (long long) there + through;
+        *a.free_out = (int) (all < a.pages ? all : a.pages);
+    }
+    for (int b = wave; b < a.batch; b += kFewWaves)
+        put_back(a, b, Shrink(a, b), there + __builtin_amdgcn_readlane(through - mine, b), lane);
+}
+
+// Measured, one launch / two, microseconds: see cubert_paged_cut.
+bool few_to_cut(int batch, int width) { return batch <= kFewSequences && (long long) batch * width <= kFewEntries; }
 
 // ---- rows into pages ----------------------------------------------------------
 
@@ -287,23 +329,27 @@ int cubert_paged_extend(int *table, int width, int ld_table, const int *lengths,
     return launch(paged_extend_kernel, dim3(blocks), dim3(kBlock), (hipStream_t) stream, a);
 }
 
+size_t cubert_paged_cut_work(int batch, int width) {
+    return batch < 1 || width < 1 || cubert::few_to_cut(batch, width) ? 0 : (size_t) batch;
+}
+
 int cubert_paged_cut(const int *table, int width, int ld_table, const int *lengths, const int *keep, int *free, const int *free_count, int pages,
                      int page, int batch, int *lengths_out, int *free_out, int *work, void *stream) {
     using namespace cubert;
     const int rc = check_tables(table, width, ld_table, lengths, free, free_count, pages, page, batch, lengths_out, free_out);
     if (rc != 0) return rc;
-    if (batch > 0 && work == nullptr) return CUBERT_BAD_ARGUMENT;
+    const bool few = few_to_cut(batch, width);
+    if (!few && work == nullptr) return CUBERT_BAD_ARGUMENT;
     if (batch > 1 << 25) return CUBERT_UNSUPPORTED;
     CutArgs a;
     a.table = table, a.lengths = lengths, a.keep = keep, a.free = free, a.free_count = free_count;
     a.lengths_out = lengths_out, a.free_out = free_out, a.returned = work;
     a.width = width, a.ld_table = ld_table, a.pages = pages, a.shift = __builtin_ctz((unsigned) page), a.batch = batch;
+    if (few) return launch(paged_cut_few_kernel, dim3(1), dim3(kFewWaves * kWave), (hipStream_t) stream, a);
     constexpr int kEach = kBlock / kWave;
-    const unsigned blocks = batch > 0 ? (unsigned) ((batch + kEach - 1) / kEach) : 1;
-    if (batch > 0) {
-        const int failed = launch(paged_cut_count_kernel, dim3(blocks), dim3(kBlock), (hipStream_t) stream, a);
-        if (failed != 0) return failed;
-    }
+    const unsigned blocks = (unsigned) ((batch + kEach - 1) / kEach);
+    const int failed = launch(paged_cut_count_kernel, dim3(blocks), dim3(kBlock), (hipStream_t) stream, a);
+    if (failed != 0) return failed;
     return launch(paged_cut_kernel, dim3(blocks), dim3(kBlock), (hipStream_t) stream, a);
 }
 

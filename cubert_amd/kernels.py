@@ -3,6 +3,7 @@ and stream here): thin wrappers over the C ABI of include/cubert_kernels.h.
 Tensors must be contiguous CUDA tensors of dtype float32 or float16; kernels run
 on torch's current stream."""
 import ctypes
+import functools
 
 import torch
 
@@ -395,6 +396,7 @@ def bias_res_ln_slices(partials, residual, bias, beta, gamma):
 _SUFFIXES = {torch.float32: "f32", torch.float16: "f16"}
 # a few tokens take a few microseconds, so the host's share of a call counts: the stream's handle without a Stream around it
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device  # (there are tensors on it: CUDA is initialised)
 
 
 def _device(t, *others):
@@ -411,7 +413,7 @@ def _device(t, *others):
 def _run_on(device, name, args, declines=True):
     """The entry point `name`, with `device` the current one; True, or False where it declines."""
     fn = getattr(lib(), name)
-    if device == torch.cuda.current_device():
+    if device == _current_device():
         rc = fn(*args)
     else:
         with torch.cuda.device(device):
@@ -610,33 +612,37 @@ def attention_window(q, k, v, left=-1, right=-1, sinks=0, first=None, lengths=No
 
 
 def _int32(t, shape, what):
-    if t.dtype != torch.int32 or t.shape != shape:
-        raise ValueError("%s: int32 %s expected, got %s %s" % (what, tuple(shape), t.dtype, tuple(t.shape)))
-    return _whole_ptr(t)
+    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
+        raise ValueError("%s: contiguous int32 %s expected, got %s %s" % (what, tuple(shape), t.dtype, tuple(t.shape)))
+    return t.data_ptr()
 
 
 def _table_args(table):
-    """Pointer, width and pitch of a table, int32 [batch, width], whose rows may stand apart."""
-    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[1] < 1:
-        raise ValueError("table: int32 [batch, width] expected, got %s %s" % (table.dtype, tuple(table.shape)))
-    batch, width = table.shape
-    pitch = table.stride(0) if batch > 1 else width
-    if (table.stride(1) != 1 and width > 1) or pitch < width:
-        raise ValueError("table: contiguous rows expected, got strides %s" % (table.stride(),))
-    _fits(max(batch, pitch))
-    return table.data_ptr(), width, pitch
+    """Batch, pointer, width and pitch of a table, int32 [batch, width], whose rows may stand apart."""
+    shape = table.shape
+    if table.dtype is not torch.int32 or len(shape) != 2 or shape[1] < 1:
+        raise ValueError("table: int32 [batch, width] expected, got %s %s" % (table.dtype, tuple(shape)))
+    batch, width = shape
+    pitch = width
+    if not table.is_contiguous():
+        pitch = table.stride(0) if batch > 1 else width
+        if (table.stride(1) != 1 and width > 1) or pitch < width:
+            raise ValueError("table: contiguous rows expected, got strides %s" % (table.stride(),))
+    return batch, table.data_ptr(), width, pitch
 
 
 def _stack_args(table, lengths, changes, what, free, free_count, page):
-    table_args = _table_args(table)
-    if free.dtype != torch.int32 or free.dim() != 1 or free.numel() < 1:
-        raise ValueError("free: int32 [pages] expected, got %s %s" % (free.dtype, tuple(free.shape)))
-    _fits(max(free.numel(), page))
+    batch, table_ptr, width, pitch = _table_args(table)
+    shape = free.shape
+    if len(shape) != 1 or shape[0] < 1:
+        raise ValueError("free: int32 [pages] expected, got %s %s" % (free.dtype, tuple(shape)))
+    pages = shape[0]
+    _fits(max(batch, pitch, pages, page))
     if page < 1 or page & (page - 1):
         raise ValueError("pages of a power of two of tokens expected, got %d" % page)
-    shape = table.shape[:1]
-    return table_args + (_int32(lengths, shape, "lengths"), None if changes is None else _int32(changes, shape, what), _whole_ptr(free),
-                         _int32(free_count, (1,), "free_count"), free.numel(), page, table.shape[0])
+    whole = (batch,)
+    return (table_ptr, width, pitch, _int32(lengths, whole, "lengths"), None if changes is None else _int32(changes, whole, what),
+            _int32(free, shape, "free"), _int32(free_count, (1,), "free_count"), pages, page, batch)
 
 
 def paged_extend(table, lengths, counts, free, free_count, page, rows):
@@ -647,8 +653,8 @@ def paged_extend(table, lengths, counts, free, free_count, page, rows):
     device = _device(table, lengths, counts, free, free_count)
     args = _stack_args(table, lengths, counts, "counts", free, free_count, page)
     _fits(rows)
-    slots = torch.empty((table.shape[0], rows), dtype=torch.int32, device=table.device)
-    after, left = torch.empty_like(lengths), torch.empty_like(free_count)
+    # (the kernel writes every element of the three; sizes as numbers of their own take the shorter way through torch)
+    slots, after, left = lengths.new_empty(args[-1], rows), torch.empty_like(lengths), torch.empty_like(free_count)
     _run_on(device, "cubert_paged_extend", args + (rows, slots.data_ptr(), after.data_ptr(), left.data_ptr(), _raw_stream(device)), declines=False)
     return slots, after, left
 
@@ -658,20 +664,32 @@ def paged_cut(table, lengths, keep, free, free_count, page):
     go onto the stack `free`, in place; `table` stays as it is, and entries of it that are no pages are passed over."""
     device = _device(table, lengths, keep, free, free_count)
     args = _stack_args(table, lengths, keep, "keep", free, free_count, page)
-    after, left, work = torch.empty_like(lengths), torch.empty_like(free_count), torch.empty_like(lengths)
-    _run_on(device, "cubert_paged_cut", args + (after.data_ptr(), left.data_ptr(), work.data_ptr(), _raw_stream(device)), declines=False)
+    after, left = torch.empty_like(lengths), torch.empty_like(free_count)
+    ints = _cut_work(args[-1], args[1])
+    work = lengths.new_empty(ints) if ints else None
+    _run_on(device, "cubert_paged_cut", args + (after.data_ptr(), left.data_ptr(), work.data_ptr() if ints else None, _raw_stream(device)),
+            declines=False)
     return after, left
 
 
+@functools.lru_cache(maxsize=4096)  # (sizes of a program's calls, over and over)
+def _cut_work(batch, width):
+    return lib().cubert_paged_cut_work(batch, width)
+
+
+@functools.lru_cache(maxsize=4096)
+def _paged_partials(*sizes):
+    return lib().cubert_attention_paged_partials(*sizes)
+
+
 def _pool_args(k_pages, v_pages):
-    shape = k_pages.shape
-    if len(shape) != 4 or v_pages.dtype != k_pages.dtype or v_pages.shape != shape:
+    """(pages, kv_heads, page, size) of two pools alike, and their pointers and strides."""
+    shape, strides = k_pages.shape, k_pages.stride()
+    if len(shape) != 4 or v_pages.dtype is not k_pages.dtype or v_pages.shape != shape:
         raise ValueError("pools [pages, kv_heads, page, size] alike expected, got %s and %s" % (tuple(shape), tuple(v_pages.shape)))
-    _fits(max(shape))
-    strides = k_pages.stride()
     if v_pages.stride() != strides or (strides[3] != 1 and shape[3] > 1):
         raise ValueError("pools at the same strides with contiguous rows expected, got %s and %s" % (strides, v_pages.stride()))
-    return (k_pages.data_ptr(), v_pages.data_ptr()) + strides[:3]
+    return shape, (k_pages.data_ptr(), v_pages.data_ptr()) + strides[:3]
 
 
 def paged_write(k, v, slots, k_pages, v_pages):
@@ -679,18 +697,17 @@ def paged_write(k, v, slots, k_pages, v_pages):
     [pages, kv_heads, page, size] (of any strides), in place; slots int32 [batch, rows] as paged_extend gives them, negative ones are left out.
     Returns the pools; None when the alignment does not fit."""
     device = _device(k, v, slots, k_pages, v_pages)
-    pools = _pool_args(k_pages, v_pages)
-    pages, kv_heads, page, size = k_pages.shape
-    if k.dim() != 4 or k.dtype != k_pages.dtype or v.dtype != k.dtype or v.shape != k.shape or k.shape[2:] != (kv_heads, size):
-        raise ValueError("k and v [batch, rows, %d, %d] like the pools expected, got %s and %s" % (kv_heads, size, tuple(k.shape), tuple(v.shape)))
-    tokens = k.shape[0] * k.shape[1]
-    _fits(max(*k.shape, tokens))
+    (pages, kv_heads, page, size), pools = _pool_args(k_pages, v_pages)
+    shape, t = k.shape, k.dtype
+    if len(shape) != 4 or t is not k_pages.dtype or v.dtype is not t or v.shape != shape or shape[2] != kv_heads or shape[3] != size:
+        raise ValueError("k and v [batch, rows, %d, %d] like the pools expected, got %s and %s" % (kv_heads, size, tuple(shape), tuple(v.shape)))
+    tokens = shape[0] * shape[1]
+    _fits(max(*shape, tokens, pages, page))
     ld = _heads_pitch(k, "k")
     if _heads_pitch(v, "v") != ld:
         raise ValueError("k and v at one row pitch expected, got strides %s and %s" % (k.stride(), v.stride()))
-    args = (k.data_ptr(), v.data_ptr(), ld, _int32(slots, k.shape[:2], "slots"), tokens) + pools + (pages, page, kv_heads, size, _raw_stream(device))
-    name = "cubert_paged_write_" + (_SUFFIXES.get(k.dtype) or _suffix(k))
-    return (k_pages, v_pages) if _run_on(device, name, args) else None
+    args = (k.data_ptr(), v.data_ptr(), ld, _int32(slots, shape[:2], "slots"), tokens) + pools + (pages, page, kv_heads, size, _raw_stream(device))
+    return (k_pages, v_pages) if _run_on(device, "cubert_paged_write_" + (_SUFFIXES.get(t) or _suffix(k)), args) else None
 
 
 def attention_paged(q, k_pages, v_pages, table, lengths, left=-1, sinks=0, first=None, alpha=None):
@@ -699,30 +716,30 @@ def attention_paged(q, k_pages, v_pages, table, lengths, left=-1, sinks=0, first
     sees key j < lengths with j <= p and (j >= p - left or j < sinks), where table[j / page] is a page; a negative left is no bound.
     q [batch, q_rows, heads, size], pools [pages, kv_heads, page, size] (of any strides), table int32 [batch, width], lengths int32 [batch].
     Queries that see nothing, or stand outside their sequence, give zeros.  None when the head size, the page or the alignment does not fit."""
-    t = q.dtype
     device = _device(q, k_pages, v_pages, table, lengths, first)
-    if q.dim() != 4 or k_pages.dtype != t:
-        raise ValueError("q [batch, q_rows, heads, size] of the pools' type expected, got %s %s" % (t, tuple(q.shape)))
-    pools = _pool_args(k_pages, v_pages)
-    batch, q_rows, heads, size = q.shape
-    pages, kv_heads, page, pool_size = k_pages.shape
-    _fits(max(q.shape))
+    t, shape = q.dtype, q.shape
+    if len(shape) != 4 or k_pages.dtype is not t:
+        raise ValueError("q [batch, q_rows, heads, size] of the pools' type expected, got %s %s" % (t, tuple(shape)))
+    (pages, kv_heads, page, pool_size), pools = _pool_args(k_pages, v_pages)
+    batch, q_rows, heads, size = shape
     if pool_size != size:
         raise ValueError("pools with rows of %d expected, got %s" % (size, tuple(k_pages.shape)))
     if kv_heads < 1 or heads % kv_heads:
         raise ValueError("%d heads cannot share %d" % (heads, kv_heads))
-    table_ptr, width, ld_table = _table_args(table)
-    if table.shape[0] != batch:
+    sequences, table_ptr, width, ld_table = _table_args(table)
+    if sequences != batch:
         raise ValueError("table: a row for each of %d sequences expected, got %s" % (batch, tuple(table.shape)))
+    _fits(max(batch, q_rows, heads, size, pages, page, ld_table))
     if not (-1 <= left <= 1 << 30 and 0 <= sinks <= 1 << 30):  # (the C interface has 32 bits)
         left, sinks = (max(min(n, 1 << 30), -1) for n in (left, sinks))
     suffix = _SUFFIXES.get(t) or _suffix(q)
     ldq = _heads_pitch(q, "q")
     ctx = torch.empty_like(q, memory_format=torch.contiguous_format)
-    floats = lib().cubert_attention_paged_partials(suffix == "f16", batch, heads, kv_heads, q_rows, width, page, size, left, sinks)
+    floats = _paged_partials(suffix == "f16", batch, heads, kv_heads, q_rows, width, page, size, left, sinks)
     partials = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
-    args = (q.data_ptr(), ldq) + pools + (table_ptr, width, ld_table, _int32(lengths, (batch,), "lengths"),
-                                          None if first is None else _int32(first, (batch,), "first"), ctx.data_ptr(), heads * size,
+    whole = (batch,)
+    args = (q.data_ptr(), ldq) + pools + (table_ptr, width, ld_table, _int32(lengths, whole, "lengths"),
+                                          None if first is None else _int32(first, whole, "first"), ctx.data_ptr(), heads * size,
                                           size ** -0.5 if alpha is None else float(alpha), batch, heads, kv_heads, q_rows, pages, page, size, left,
                                           sinks, partials.data_ptr() if floats else None, floats, _raw_stream(device))
     return ctx if _run_on(device, "cubert_attention_paged_" + suffix, args) else None

@@ -330,7 +330,9 @@ int cubert_paged_extend(int *table, int width, int ld_table, const int *lengths,
 /* Sequences keep their first keep[b] tokens (NULL: none; taken within 0..lengths[b]), and the pages behind these go back onto the stack in the
  * order of the sequences and their tables.  Entries that are no pages (outside 0..pages-1: whoever has taken a page out of a table has put something
  * else in its place) are passed over, and so is what the stack has no room for.  The table stays as it is: entries behind a length mean nothing.
- * A page belongs to one sequence.  lengths_out and free_out as above; `work` is batch ints that no other call uses before this one is done. */
+ * A page belongs to one sequence.  lengths_out and free_out as above; `work` is cubert_paged_cut_work ints of device memory that no other call
+ * uses before this one is done (none, and one launch, where that is 0). */
+size_t cubert_paged_cut_work(int batch, int width);
 int cubert_paged_cut(const int *table, int width, int ld_table, const int *lengths, const int *keep, int *free, const int *free_count,
                      int pages, int page, int batch, int *lengths_out, int *free_out, int *work, void *stream);
 

@@ -35,6 +35,15 @@ def test_tables_refuse(L, call):
         assert call(L, **other) == UNSUPPORTED, other
 
 
+def test_cut_work(L):
+    """An int per sequence, but for so few that one workgroup has them all."""
+    for batch, width in ((1, 1), (64, 512), (8, 4096), (1, 1 << 15)):
+        assert L.cubert_paged_cut_work(batch, width) == 0
+    for batch, width in ((65, 1), (64, 513), (1, (1 << 15) + 1), (5000, 7)):
+        assert L.cubert_paged_cut_work(batch, width) == batch
+    assert L.cubert_paged_cut_work(0, 1 << 20) == 0
+
+
 def test_extend_refuses(L):
     assert extend(L, rows=-1) == BAD_ARGUMENT
     assert extend(L, slots=None) == BAD_ARGUMENT
@@ -44,7 +53,8 @@ def test_extend_refuses(L):
 
 
 def test_cut_refuses(L):
-    assert cut(L, work=None) == BAD_ARGUMENT
+    assert cut(L, work=None, batch=65) == BAD_ARGUMENT
+    assert cut(L, work=None, width=1 << 15) == BAD_ARGUMENT
     assert cut(L, batch=(1 << 25) + 1) == UNSUPPORTED
 
 

@@ -199,6 +199,10 @@ CUT = {
     "many": (3000, 3, 16, 48, "any"),
     "pages of one": (20, 300, 1, 300, "any"),
     "wild": (200, 7, 16, 100, "wild"),
+    "as many as one workgroup takes": (64, 512, 1, 512, "any"),
+    "a sequence more": (65, 504, 1, 504, "any"),
+    "a page more": (64, 513, 1, 513, "any"),
+    "a few that are wild": (17, 40, 16, 640, "wild"),
 }
 
 
