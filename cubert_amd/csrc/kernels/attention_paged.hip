@@ -81,6 +81,11 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 // Registers of a request, and the numbers in them.
 template <int WORDS>
 using Words = int __attribute__((ext_vector_type(WORDS)));
+template <bool ONCE, typename W>
+__device__ __forceinline__ W read(const W *p) {
+    if constexpr (ONCE) return __builtin_nontemporal_load(p);
+    return *p;
+}
 template <typename T, int N>
 using Numbers = T __attribute__((ext_vector_type(N)));
 
@@ -116,6 +121,7 @@ __device__ __forceinline__ void two_terms(float e0, float e1, v2f16 &high, v2f16
 struct PagedPlan {
     int rows, row_tiles, pieces, least;  // rows of a tile
     int slot_rows;                       // of which that many are there
+    bool once;                           // K and V are read once, and are too large to be there still when they are read again
     long long problems;
     size_t floats;
 };
@@ -181,7 +187,7 @@ struct Rows {
 };
 
 // Bound by reading K and V.
-template <typename T, int D, int TILES>
+template <typename T, int D, int TILES, bool ONCE>
 __global__ __launch_bounds__(kBlock, TILES == 1 ? 3 : 2) void attention_paged_kernel(PagedArgs a, PagedPlan plan) {
     typedef Shape<T, D> S;
     typedef Reach<S::kKeys> Reached;
@@ -306,7 +312,7 @@ __global__ __launch_bounds__(kBlock, TILES == 1 ? 3 : 2) void attention_paged_ke
             if (__builtin_amdgcn_readlane(pages, (unit_at - x0) * kSub + n) >= 0) there_next |= 1u << n;
             const char *at = k_base + offset_of(unit_at, n);
 #pragma unroll
-            for (int t = 0; t < S::kKeyLoads; ++t) k[n][t] = *reinterpret_cast<const Words<4> *>(at + k_offset + 64 * t);
+            for (int t = 0; t < S::kKeyLoads; ++t) k[n][t] = read<ONCE>(reinterpret_cast<const Words<4> *>(at + k_offset + 64 * t));
         }
     };
     auto bring_values = [&](int unit_at) {
@@ -315,7 +321,7 @@ __global__ __launch_bounds__(kBlock, TILES == 1 ? 3 : 2) void attention_paged_ke
             const char *at = v_base + offset_of(unit_at, n);
 #pragma unroll
             for (int j = 0; j < S::kValueLoads; ++j)
-                v[n][j] = *reinterpret_cast<const Words<S::kValueBytes / 4> *>(at + value_key(j) * row_bytes + v_offset + 256 * value_part(j));
+                v[n][j] = read<ONCE>(reinterpret_cast<const Words<S::kValueBytes / 4> *>(at + value_key(j) * row_bytes + v_offset + 256 * value_part(j)));
         }
     };
     auto take = [&](int unit_at, auto more) {
@@ -610,22 +616,22 @@ PagedPlan plan_paged(bool half_precision, int batch, int heads, int kv_heads, in
     const long long units = (reach + keys - 1) / keys + (left >= 0 ? 2 : 0);
     plan.least = plan.problems * units <= 1536 ? 4 : 8, plan.pieces = 0, plan.floats = 0;
     plan.slot_rows = (int) (rows < plan.rows ? rows : plan.rows);
-    const long long uncut = plan.problems / 8 < 16 ? 16 : plan.problems / 8 < 128 ? plan.problems / 8 : 128;
+    const long long uncut = plan.problems / 8 < 16 ? 16 : plan.problems / 8 < 256 ? plan.problems / 8 : 256;
     if (units <= uncut || plan.problems * units >= 1 << 30) return plan;  // (units are counted in 32 bits)
     const long long most = (plan.problems * units + plan.least - 1) / plan.least;
-    plan.pieces = plan.problems <= 32 ? 256 - (int) plan.problems : plan.problems <= 160 ? 512 - (int) plan.problems : 1024;
+    plan.pieces = plan.problems <= 32 ? 256 - (int) plan.problems : plan.problems <= 100 ? 512 - (int) plan.problems : 2048;
     if (most < plan.pieces) plan.pieces = (int) most;
     plan.floats = (size_t) (plan.pieces + plan.problems) * plan.slot_rows * (head_size + 4) + 2 * (size_t) plan.problems;
     return plan;
 }
 
-template <typename T, int D, int TILES>
+template <typename T, int D, int TILES, bool ONCE>
 int run_paged(const PagedArgs &a, const PagedPlan &plan, hipStream_t stream) {
     static std::atomic<unsigned long long> done{0};
     typedef Shape<T, D> S;
     const unsigned merge = (unsigned) (4 * plan.slot_rows * S::kPitch * 4), lds = merge > 4 * S::kValueLds ? merge : 4 * S::kValueLds;
-    if (lds > 48 * 1024 && !allow_large_lds(attention_paged_kernel<T, D, TILES>, done)) return CUBERT_UNSUPPORTED;
-    const int rc = launch_lds(attention_paged_kernel<T, D, TILES>, dim3((unsigned) (plan.pieces + plan.problems)), dim3(kBlock), lds, stream, a, plan);
+    if (lds > 48 * 1024 && !allow_large_lds(attention_paged_kernel<T, D, TILES, ONCE>, done)) return CUBERT_UNSUPPORTED;
+    const int rc = launch_lds(attention_paged_kernel<T, D, TILES, ONCE>, dim3((unsigned) (plan.pieces + plan.problems)), dim3(kBlock), lds, stream, a, plan);
     if (rc != 0 || plan.pieces == 0) return rc;
     const unsigned joins = (unsigned) (plan.problems * plan.slot_rows);
     const int of_problem = plan.pieces / (int) plan.problems;  // pieces, on average
@@ -636,7 +642,8 @@ int run_paged(const PagedArgs &a, const PagedPlan &plan, hipStream_t stream) {
 
 template <typename T, int D>
 int run_paged_size(const PagedArgs &a, const PagedPlan &plan, hipStream_t stream) {
-    return plan.rows == 16 ? run_paged<T, D, 1>(a, plan, stream) : run_paged<T, D, 2>(a, plan, stream);
+    if (plan.once) return plan.rows == 16 ? run_paged<T, D, 1, true>(a, plan, stream) : run_paged<T, D, 2, true>(a, plan, stream);
+    return plan.rows == 16 ? run_paged<T, D, 1, false>(a, plan, stream) : run_paged<T, D, 2, false>(a, plan, stream);
 }
 
 template <typename T>
@@ -674,6 +681,7 @@ int attention_paged(const T *q, int ldq, const T *k_pages, const T *v_pages, lon
         return CUBERT_UNSUPPORTED;
     PagedPlan plan = plan_paged(sizeof(T) == 2, batch, heads, kv_heads, q_rows, (long long) width * page, head_size, a.left == kFar ? -1 : left, a.sinks);
     if (plan.problems * plan.rows >= 1 << 24) return CUBERT_UNSUPPORTED;
+    plan.once = plan.row_tiles == 1 && 2ll * pages * page * kv_heads * head_size * (long long) sizeof(T) >= 96ll << 20;
     if (plan.pieces != 0 && (partials == nullptr || partial_floats < plan.floats || !is_aligned(partials, 16))) plan.pieces = 0;
     if (head_size == 32) return run_paged_size<T, 32>(a, plan, (hipStream_t) stream);
     if (head_size == 64) return run_paged_size<T, 64>(a, plan, (hipStream_t) stream);
