@@ -18,7 +18,7 @@ namespace cubert {
 namespace {
 
 constexpr int kFar = (1 << 30) - 1;  // a bound or position that no sequence reaches
-constexpr float kNone = -3e38f;      // the maximum of no scores: finite, so that differences to it are numbers
+constexpr float kNone = -3.402823466e38f;  // the maximum of no scores: no finite score is less
 constexpr int kFewPieces = 16, kSomePieces = 64;  // of a problem, on average
 
 struct PagedArgs {
@@ -71,8 +71,8 @@ struct Shape {
     static constexpr int kValueLds = kHalf ? kKeys * kRowBytes : 0;                 // of a wavefront
     static constexpr int kPitch = D + 4;                                            // floats between rows of sums
     // How far a maximum may rise, in powers of two, before sums are scaled anew, and how much larger probabilities are, so that fp16's subnormals
-    // begin far below the maximum (2^-37 of it; 2^15 is still fp16).
-    static constexpr float kSlack = kHalf ? 3.f : 8.f, kRaise = kHalf ? 12.f : 0.f;
+    // begin far below the maximum (2^-37 of it; 2^15 is still fp16).  fp32: probabilities are 1 at most, as V may be as large as fp32 goes.
+    static constexpr float kSlack = kHalf ? 3.f : 0.f, kRaise = kHalf ? 12.f : 0.f;
 };
 
 // (the same in every lane, which the compiler has to be told)
@@ -106,14 +106,16 @@ __device__ __forceinline__ int v_piece(int key, int at) {
     return at ^ (key / (256 / ROW_BYTES) % (ROW_BYTES / 32) * 2);
 }
 
-// Probabilities as sums of two fp16 numbers, exact to 2^-21 of them: pairs of `high` and `low`.  Both are positive, the second one at least fp16's
-// smallest, 2^-36 of the largest probability, so that an infinite value of V stays infinite in either product.
+// Probabilities as sums of two fp16 numbers, exact to 2^-21 of them: pairs of `high` and `low`.  Neither is negative, and the second one is not 0
+// where the probability is more than 2^-37 of the largest, so that an infinite value of V stays infinite in either product.
 __device__ __forceinline__ void two_terms(float e0, float e1, v2f16 &high, v2f16 &low) {
+    constexpr float kLeast = 0x1p-24f;  // fp16's smallest
     high = __builtin_bit_cast(v2f16, __builtin_amdgcn_cvt_pkrtz(e0, e1));
     float minus = -1.f;
     asm("" : "+v"(minus));  // (as a constant it makes a conversion and a subtraction of one instruction)
-    low = __builtin_convertvector((v2f32{fmaf((float) high[0], minus, e0), fmaf((float) high[1], minus, e1)}), v2f16);
-    low = __builtin_elementwise_max(low, v2f16{(_Float16) 0x1p-24f, (_Float16) 0x1p-24f});
+    // (the middle one of the rest, the probability and the smallest: the rest, or as much of the smallest as there is)
+    low = __builtin_convertvector((v2f32{__builtin_amdgcn_fmed3f(fmaf((float) high[0], minus, e0), e0, kLeast),
+                                         __builtin_amdgcn_fmed3f(fmaf((float) high[1], minus, e1), e1, kLeast)}), v2f16);
 }
 
 // A problem is a tile of rows of a sequence and a key head; sequences and tiles are numbered together, tile * batch + sequence.  A workgroup has one

@@ -592,6 +592,50 @@ def test_attention_paged_of_large_scores(K, t, size):
 
 
 @pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("size", [32, 64, 128])
+def test_attention_paged_keeps_apart_what_rows_see(K, t, size):
+    """Values as large as there are in keys that only the last of a few queries sees, or only the first: the others have none of them."""
+    t, g = TYPES[t], gen(16)
+    largest = 65504.0 if t == torch.float16 else 1e30
+    k_pages, v_pages, _ = pool_of("heads", 40, 2, 16, size, t, 5)
+    v_pages *= 1e-4
+    table = torch.randperm(40, generator=g, device="cuda").int()[:33].view(1, -1).contiguous()
+    q = normal(g, 1, 5, 4, size).to(t)
+    at = dict(left=200, sinks=0, lengths=ints([520]), first=None)
+    for j in (519, 315):                                   # the last token, and the first one of the first query's window
+        v_pages[int(table[0, j // 16]), :, j % 16] = largest
+    k, v = (p.transpose(1, 2)[table.long()].reshape(1, 528, 2, size)[:, :520] for p in (k_pages, v_pages))
+    want, bound = reference(q, k, v, visible(q, k, 16, **at))
+    got = K.attention_paged(q, k_pages, v_pages, table, **at)
+    within(got, want, bound, "apart")
+    assert bool((got[0, 1:4].abs() < 1e-2).all()) and bool((got[0, [0, 4]].abs() > 1).any())
+
+
+@pytest.mark.parametrize("size", [32, 64, 128])
+def test_attention_paged_of_the_largest_numbers(K, size):
+    """Values near fp32's largest under scores that rise all the way, and scores near its least."""
+    g = gen(17)
+    k_pages, v_pages, _ = pool_of("heads", 40, 1, 16, size, torch.float32, 5)
+    table = torch.randperm(40, generator=g, device="cuda").int()[:32].view(1, -1).contiguous()
+    place = torch.arange(512, device="cuda")
+    for scores, values, alpha in ((place.float() / 2, 1e38, 1.0), (place.float() * 30, 3e38, 1.0), (-3.39e38 + place.float() * 1e32, 1.0, 1e-32),
+                                  (torch.full((512,), -3.35e38, device="cuda"), 1.0, 1.0)):
+        k_pages.zero_(), v_pages.zero_()
+        own = table[0, place // 16].long()
+        k_pages[own, 0, place % 16, 1] = scores
+        v_pages[own, 0, place % 16] = values * (torch.rand(512, size, generator=g, device="cuda") - 0.5)
+        q = torch.zeros(1, 1, 2, size, device="cuda")
+        q[..., 1] = 1
+        at = dict(left=-1, sinks=0, lengths=ints([512]), first=None)
+        k, v = (p.transpose(1, 2)[table.long()].reshape(1, 512, 1, size) for p in (k_pages, v_pages))
+        # (bounds go by the scores, so they are wide for some of these; that results are numbers is the point)
+        want, bound = reference(q, k, v, visible(q, k, 16, **at), alpha=alpha)
+        got = K.attention_paged(q, k_pages, v_pages, table, alpha=alpha, **at)
+        assert bool(torch.isfinite(got).all())
+        within(got, want, bound, "%g" % values)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
 def test_attention_paged_without_scores(K, t):
     """A scale of 0: the mean of what is seen."""
     for name in FEW:
