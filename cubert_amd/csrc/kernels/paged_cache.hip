@@ -243,7 +243,8 @@ __global__ __launch_bounds__(kFewWaves * kWave) void paged_cut_few_kernel(CutArg
         put_back(a, b, Shrink(a, b), there + __builtin_amdgcn_readlane(through - mine, b), lane);
 }
 
-// Measured, one launch / two, microseconds: see cubert_paged_cut.
+// One launch / two, microseconds on the GPU: 8 sequences of up to 4096 tokens in pages of 16 4.2 / 5.5, 64 of up to 8192 10.5 / 6.5; as a call, in
+// which a second launch and its memory are 4 of the host's, 7.9 / 12.2 and 10.5 / 12.
 bool few_to_cut(int batch, int width) { return batch <= kFewSequences && (long long) batch * width <= kFewEntries; }
 
 // ---- rows into pages ----------------------------------------------------------
@@ -257,6 +258,12 @@ struct WriteArgs {
     int shift, pieces_of_head, pieces;  // of 16 bytes, of a head and of all of a token's
 };
 
+typedef float v4f32 __attribute__((ext_vector_type(4)));
+
+// A 16-byte piece of a key and of a value to a thread.  Bound by memory: 16 prompts of up to 2048 tokens of 8 heads of 128, 134 MB, in 25 us (5.3
+// TB/s).  ONCE: past the caches, which large ones leave nothing in: that call 27.8 / 25.3 us, 65536 tokens 52.7 / 49.3; from 64 MB on (33 MB
+// in rows of 64 bytes 7.8 / 8.9).
+template <bool ONCE>
 __global__ __launch_bounds__(kBlock) void paged_write_kernel(WriteArgs a) {
     const unsigned long long i = (unsigned long long) blockIdx.x * kBlock + threadIdx.x;
     const unsigned token = (unsigned) (i / (unsigned) a.pieces);
@@ -267,9 +274,16 @@ __global__ __launch_bounds__(kBlock) void paged_write_kernel(WriteArgs a) {
     const long long from = token * a.from_bytes + (long long) piece * 16;
     const long long to = (long long) (slot >> a.shift) * a.page_bytes + (long long) (slot & ((1u << a.shift) - 1)) * a.row_bytes +
                          head * a.head_bytes + (piece - head * a.pieces_of_head) * 16;
-    const Vec<float, 4> x = load_vec<float, 4>((const float *) (a.k + from)), y = load_vec<float, 4>((const float *) (a.v + from));
-    store_vec<float, 4>((float *) (a.k_pages + to), x);
-    store_vec<float, 4>((float *) (a.v_pages + to), y);
+    const v4f32 *k = (const v4f32 *) (a.k + from), *v = (const v4f32 *) (a.v + from);
+    v4f32 *k_to = (v4f32 *) (a.k_pages + to), *v_to = (v4f32 *) (a.v_pages + to);
+    if constexpr (ONCE) {
+        const v4f32 x = __builtin_nontemporal_load(k), y = __builtin_nontemporal_load(v);
+        __builtin_nontemporal_store(x, k_to);
+        __builtin_nontemporal_store(y, v_to);
+    } else {
+        const v4f32 x = *k, y = *v;
+        *k_to = x, *v_to = y;
+    }
 }
 
 // What extend and cut have in common: sizes of tables and pages that 32 bits count.
@@ -304,7 +318,8 @@ int paged_write(const void *k, const void *v, int ld, const int *slots, int toke
     a.pieces_of_head = head_size / piece, a.pieces = kv_heads * a.pieces_of_head;
     const unsigned long long blocks = ((unsigned long long) tokens * a.pieces + kBlock - 1) / kBlock;
     if (blocks >= 1u << 24) return CUBERT_UNSUPPORTED;  // (a launch holds less than 2^32 threads)
-    return launch(paged_write_kernel, dim3((unsigned) blocks), dim3(kBlock), (hipStream_t) stream, a);
+    const bool once = (unsigned long long) tokens * a.pieces * 32 >= 64ull << 20;
+    return launch(once ? paged_write_kernel<true> : paged_write_kernel<false>, dim3((unsigned) blocks), dim3(kBlock), (hipStream_t) stream, a);
 }
 
 }  // namespace

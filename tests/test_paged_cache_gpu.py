@@ -312,6 +312,25 @@ def test_write(K, layout, t, batch, rows, heads, kv_heads, size, page):
     assert torch.equal(whole, want)                        # and nothing else has changed
 
 
+@pytest.mark.parametrize("t", ["f32", "f16"])
+def test_write_of_a_large_prompt(K, t):
+    """So much that it goes past the caches: 64 MB and more, all of it there for what reads it next."""
+    t, g = TYPES[t], gen(8)
+    batch, rows, kv, size, page = 3, 7001, 8, 128 if t == torch.float16 else 64, 64
+    pages = up(batch * rows, page) + 1
+    k_pages, v_pages, _ = pool_of("heads", pages, kv, page, size, t, 3)
+    packed = torch.randn(batch, rows, 3 * kv, size, generator=g, device="cuda").to(t)
+    slots = torch.randperm(pages * page, generator=g, device="cuda")[:batch * rows].int().view(batch, rows)
+    slots[1, 5000:] = -1
+    want_k, want_v = k_pages.clone(), v_pages.clone()
+    kept = slots >= 0
+    at = slots[kept].long()
+    for want, rows_of in ((want_k, packed[:, :, kv:2 * kv]), (want_v, packed[:, :, 2 * kv:])):
+        want.transpose(1, 2)[at // page, at % page] = rows_of[kept]
+    K.paged_write(packed[:, :, kv:2 * kv], packed[:, :, 2 * kv:], slots, k_pages, v_pages)
+    assert torch.equal(k_pages, want_k) and torch.equal(v_pages, want_v)
+
+
 def test_write_refuses(K):
     pool, q = torch.zeros(4, 2, 16, 64, device="cuda"), torch.zeros(2, 3, 4, 64, device="cuda")
     slots = torch.zeros(2, 3, dtype=torch.int32, device="cuda")
@@ -466,6 +485,23 @@ def test_attention_paged_in_any_layout(K, name, t, layout, size):
 
 FEW = ["one query", "no keys", "around a page", "around large pages", "a few tokens", "seven heads to one", "a window and sinks", "sinks alone",
        "before the sequence", "tokens in the middle", "long", "long window", "unlike lengths", "many short", "many rows"]
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("size", [32, 64, 128])
+@pytest.mark.parametrize("heads,q_rows", [(8, 1), (8, 4), (8, 9)])
+def test_attention_paged_of_a_large_pool(K, t, size, heads, q_rows):
+    """Pools of 96 MB and more, which are read past the caches, with sequences in a part of them."""
+    t, g = TYPES[t], gen(18)
+    page, kv = 64, 4
+    pages = (96 << 20) // (2 * page * kv * size * t.itemsize) + 1
+    k_pages, v_pages, _ = pool_of("heads", pages, kv, page, size, t, 7)
+    q, lengths = normal(g, 3, q_rows, heads, size).to(t), ints([1900, 77, 1])
+    table = torch.randperm(pages, generator=g, device="cuda").int()[:90].view(3, 30).contiguous()
+    k, v = (p.transpose(1, 2)[table.long()].reshape(3, 30 * page, kv, size) for p in (k_pages, v_pages))
+    at = dict(left=-1, sinks=0, lengths=lengths, first=None)
+    got = K.attention_paged(q, k_pages, v_pages, table, **at)
+    within(got, *reference(q, k, v, visible(q, k, page, **at)), "large pool")
 
 
 @pytest.mark.parametrize("name", FEW)
