@@ -19,7 +19,6 @@ namespace {
 
 constexpr int kFar = (1 << 30) - 1;  // a bound or position that no sequence reaches
 constexpr float kNone = -3.402823466e38f;  // the maximum of no scores: no finite score is less
-constexpr int kFewPieces = 16, kSomePieces = 64;  // of a problem, on average
 
 struct PagedArgs {
     const void *q, *k, *v;
@@ -46,17 +45,21 @@ typedef _Float16 v4f16 __attribute__((ext_vector_type(4)));
 typedef _Float16 v2f16 __attribute__((ext_vector_type(2)));
 typedef float v4f32 __attribute__((ext_vector_type(4)));
 typedef float v2f32 __attribute__((ext_vector_type(2)));
-typedef int v4i32 __attribute__((ext_vector_type(4)));
 typedef int v2i32 __attribute__((ext_vector_type(2)));
 
 // 16 rows (queries and heads of one key head) meet 16 keys in products of 16 x 16 with the keys as their rows: lane l has row l % 16 and
 // the keys 4 (l / 16) + i, i = 0..3, so that what belongs to a row, its maximum, its sum and its results, stays in four lanes.  Keys come from
-// memory as the products take them: lane l has of key l % 16 every fourth 16-byte piece.
+// memory as the products take them, lane l has of key l % 16 every fourth 16-byte piece, and do not pass through LDS.
 //
 // fp16: V passes through LDS, out of which it comes transposed, and the probabilities are the other factor as they are, as sums of two fp16
-// numbers, so that a result is rounded once, at the end.
+// numbers, so that a result is rounded once, at the end.  (With fp32's own products instead, which take V as it lies in memory, four times
+// the cycles: 1 x 1 over 64 keys of 12 heads 5.9 us for 4.5.)
 // fp32: a product with V takes a single number of one key from a lane.  Of the i-th key of its four a lane brings D / 16 columns of V, one after
 // the other, as they lie in memory, and nothing is transposed.
+//
+// What is on its way together, a unit, is 16 KB of K and V for a wavefront where rows have 128 bytes and more: while it works on one, K of the
+// next is requested as soon as this one's has been multiplied, and V as soon as this one's lies in LDS.  Twelve wavefronts to a compute unit have
+// 192 KB on their way.
 template <typename T, int D>
 struct Shape {
     static constexpr bool kHalf = sizeof(T) == 2;
@@ -81,13 +84,14 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 // Registers of a request, and the numbers in them.
 template <int WORDS>
 using Words = int __attribute__((ext_vector_type(WORDS)));
+template <typename T, int N>
+using Numbers = T __attribute__((ext_vector_type(N)));
+
 template <bool ONCE, typename W>
 __device__ __forceinline__ W read(const W *p) {
     if constexpr (ONCE) return __builtin_nontemporal_load(p);
     return *p;
 }
-template <typename T, int N>
-using Numbers = T __attribute__((ext_vector_type(N)));
 
 __device__ __forceinline__ float quarters_max(float x) {
     x = fmaxf(x, __shfl_xor(x, 16, kWave));
@@ -188,7 +192,11 @@ struct Rows {
     float top[TILES], sum[TILES];
 };
 
-// Bound by reading K and V.
+// Bound by reading K and V, and by what comes before and behind it: a chain of reads from the lengths over the table to the first keys takes 2.5
+// us, the join 4.  fp16, 64 x 1 over up to 4096 keys of 4 heads of 128, 272 MB in 53 us (5.1 TB/s); 256 x 1 over up to 512 of 12 heads of 64, 223
+// MB in 43 us (5.1 TB/s); 1 x 1 over 131072 of 2 heads of 128, 134 MB in 31 us; fp32, 32 x 1 over up to 4096 of 12 heads of 64, 443 MB in 78 us (5.7
+// TB/s).  One tile of rows: 168 registers, with which three workgroups fit a unit (two: the second of these calls 49 us, the first 57).
+// The four wavefronts have a run of the piece's units each; their sums meet in LDS, in wavefront order.
 template <typename T, int D, int TILES, bool ONCE>
 __global__ __launch_bounds__(kBlock, TILES == 1 ? 3 : 2) void attention_paged_kernel(PagedArgs a, PagedPlan plan) {
     typedef Shape<T, D> S;
@@ -606,25 +614,48 @@ __global__ __launch_bounds__(WAVES * kWave < kBlock ? kBlock : WAVES * kWave) vo
     store4(ctx, by != 0.f ? x * by : v4f32{});
 }
 
+// How a call is cut.  Microseconds of calls in a captured graph, over inputs in turn, fp16 where nothing is said:
+//
+// A workgroup to a problem / pieces and a join.  Few problems are cut where they have more than 16 units, many where they have more than an eighth
+// of their number: 1 x 1 over 2000 keys, 16 heads of 64 (16 problems of 32 units) 13.7 / 10.8; 8 x 1 over up to 1000, 4 of 128 (32 of 32) 13.7 /
+// 11.5; 128 x 1 over up to 1500, 2 of 64 (256 of 24) 14.1 / 19.9; 256 x 1 over up to 512, 12 of 64 (3072 of 8) 44 / 55; 128 x 1 over up
+// to 2048, 12 of 64 (1536 of 32, tables for 256) 85 / 81; 1 x 1 over 131072, 2 of 128 (2 of 4096) 1770 / 31.
+//
+// Pieces, 256 / 512 / 1024 / 2048 of all (less the number of problems where that is below the first number that fits).  A workgroup to a unit of
+// the card is enough where the pieces are alike, and leaves the join the least to do; many problems of unlike lengths want many pieces, which are
+// handed out as units come free: 4 x 1 over up to 30000, 4 of 128 (16 problems) 31.1 / 30.6 / 32.8 / 33.7; 1 x 8 over up to 16800, 96 heads to 12 of 128
+// (24) 34 / 45 / 52 / -; 48 x 1 over up to 4000, 2 of 128 (96) 31.4 / 27.6 / 29.3 / 30.0; 32 x 1, window 4096, 4 of 128 (128) 68.9 / 52.9 / 46.6 / 46.6;
+// 64 x 1 over up to 4096, 4 of 128 (256) 69.6 / 69.3 / 56.1 / 53.8.
+//
+// Units of a piece at least, 4 / 8: 8 x 1 over up to 1000, 4 of 128 (32 problems of 32) 11.3 / 12.6; fp32, 8 x 1 over up to 1000, 12 of 64 (96 of 32)
+// 15.2 / 13.8.
 PagedPlan plan_paged(bool half_precision, int batch, int heads, int kv_heads, int q_rows, long long limit, int head_size, int left, int sinks) {
     PagedPlan plan;
     const long long rows = (long long) q_rows * (heads / kv_heads);
     plan.rows = rows <= 16 ? 16 : 32;
     plan.row_tiles = (int) ((rows + plan.rows - 1) / plan.rows);
+    plan.slot_rows = (int) (rows < plan.rows ? rows : plan.rows);
     plan.problems = (long long) batch * kv_heads * plan.row_tiles;
+    plan.pieces = 0, plan.floats = 0, plan.once = false;
     const int row_bytes = head_size * (half_precision ? 2 : 4), keys = row_bytes >= 128 ? 8192 / row_bytes : 64;
     long long reach = limit;  // the most keys that a tile of rows sees, and how many units of them
     if (left >= 0 && (long long) left + plan.rows + sinks < reach) reach = (long long) left + plan.rows + sinks;
-    const long long units = (reach + keys - 1) / keys + (left >= 0 ? 2 : 0);
-    plan.least = plan.problems * units <= 1536 ? 4 : 8, plan.pieces = 0, plan.floats = 0;
-    plan.slot_rows = (int) (rows < plan.rows ? rows : plan.rows);
+    const long long units = (reach + keys - 1) / keys + (left >= 0 ? 2 : 0), all = plan.problems * units;
+    plan.least = all <= 1536 ? 4 : 8;
     const long long uncut = plan.problems / 8 < 16 ? 16 : plan.problems / 8 < 256 ? plan.problems / 8 : 256;
-    if (units <= uncut || plan.problems * units >= 1 << 30) return plan;  // (units are counted in 32 bits)
-    const long long most = (plan.problems * units + plan.least - 1) / plan.least;
+    if (units <= uncut || all >= 1 << 30) return plan;  // (units are counted in 32 bits)
     plan.pieces = plan.problems <= 32 ? 256 - (int) plan.problems : plan.problems <= 100 ? 512 - (int) plan.problems : 2048;
-    if (most < plan.pieces) plan.pieces = (int) most;
+    if ((all + plan.least - 1) / plan.least < plan.pieces) plan.pieces = (int) ((all + plan.least - 1) / plan.least);
     plan.floats = (size_t) (plan.pieces + plan.problems) * plan.slot_rows * (head_size + 4) + 2 * (size_t) plan.problems;
     return plan;
+}
+
+// Whether K and V are read past the caches: once, by one tile of rows, and out of pools that do not stay in the 256 MB behind the L2 caches until the next
+// call, from 96 MB on.  Microseconds without / with: 64 x 1 over up to 4096, 4 of 128 (272 MB) 60.2 / 53.5; 48 x 1 over up to 4000, 2 of 128 (108
+// MB) 29.3 / 27.2; 128 x 1 over up to 1500, 2 of 64 (55 MB, there still after four calls) 14.1 / 15.9; two tiles of rows, 1 x 8 over up to 16800, 96 heads to
+// 12 of 128, 34 / 41.
+bool read_once(const PagedPlan &plan, long long pages, int page, int kv_heads, int row_bytes) {
+    return plan.row_tiles == 1 && 2 * pages * page * kv_heads * row_bytes >= 96ll << 20;
 }
 
 template <typename T, int D, int TILES, bool ONCE>
@@ -636,9 +667,11 @@ int run_paged(const PagedArgs &a, const PagedPlan &plan, hipStream_t stream) {
     const int rc = launch_lds(attention_paged_kernel<T, D, TILES, ONCE>, dim3((unsigned) (plan.pieces + plan.problems)), dim3(kBlock), lds, stream, a, plan);
     if (rc != 0 || plan.pieces == 0) return rc;
     const unsigned joins = (unsigned) (plan.problems * plan.slot_rows);
-    const int of_problem = plan.pieces / (int) plan.problems;  // pieces, on average
-    if (of_problem <= kFewPieces) return launch(attention_paged_join_kernel<T, D, D, 1>, dim3((joins + 3) / 4), dim3(kBlock), stream, a, plan);
-    if (of_problem <= kSomePieces) return launch(attention_paged_join_kernel<T, D, D, 4>, dim3(joins), dim3(kBlock), stream, a, plan);
+    // Wavefronts to a row, by its pieces on average, 1 / 4 / 16 (which have 32 columns of it): fp32, 9 x 5 over up to 1000, 12 of 64 (8 pieces)
+    // 17.0 / 17.4 / 22.0 us the whole call; fp16, 64 x 1 over up to 4096 (8) 54.0 / 55.0 / 78.7; 1 x 1 over 60000, 1 of 128 (234) 27.1 / 17.1 / 15.0.
+    const int of_problem = plan.pieces / (int) plan.problems;
+    if (of_problem <= 16) return launch(attention_paged_join_kernel<T, D, D, 1>, dim3((joins + 3) / 4), dim3(kBlock), stream, a, plan);
+    if (of_problem <= 64) return launch(attention_paged_join_kernel<T, D, D, 4>, dim3(joins), dim3(kBlock), stream, a, plan);
     return launch(attention_paged_join_kernel<T, D, 32, 16>, dim3(joins, D / 32), dim3(16 * kWave), stream, a, plan);
 }
 
@@ -683,7 +716,7 @@ int attention_paged(const T *q, int ldq, const T *k_pages, const T *v_pages, lon
         return CUBERT_UNSUPPORTED;
     PagedPlan plan = plan_paged(sizeof(T) == 2, batch, heads, kv_heads, q_rows, (long long) width * page, head_size, a.left == kFar ? -1 : left, a.sinks);
     if (plan.problems * plan.rows >= 1 << 24) return CUBERT_UNSUPPORTED;
-    plan.once = plan.row_tiles == 1 && 2ll * pages * page * kv_heads * head_size * (long long) sizeof(T) >= 96ll << 20;
+    plan.once = read_once(plan, pages, page, kv_heads, head_size * (int) sizeof(T));
     if (plan.pieces != 0 && (partials == nullptr || partial_floats < plan.floats || !is_aligned(partials, 16))) plan.pieces = 0;
     if (head_size == 32) return run_paged_size<T, 32>(a, plan, (hipStream_t) stream);
     if (head_size == 64) return run_paged_size<T, 64>(a, plan, (hipStream_t) stream);
