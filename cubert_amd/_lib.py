@@ -124,8 +124,8 @@ SIGNATURES = {
     "cubert_w4_packed_bytes": (ctypes.c_size_t, [ci, ci, ci]),
     "cubert_w4_pack": (ci, [vp, vp, ci, ci, ci, vp, vp]),
     "cubert_attention_window_partials": (ctypes.c_size_t, [ci, ci, ci, ci, ci, ci, ci, ci, ci, ci]),
-    "cubert_paged_extend": (ci, [vp, ci, ci, vp, vp, vp, vp, ci, ci, ci, ci, vp, vp, vp, vp]),
-    "cubert_paged_cut": (ci, [vp, ci, ci, vp, vp, vp, vp, ci, ci, ci, vp, vp, vp, vp]),
+    "cubert_paged_extend": (ci, [vp, ci, ci, vp, vp, vp, vp, ci, ci, ci, ci, ci, vp, vp, vp, vp]),
+    "cubert_paged_cut": (ci, [vp, ci, ci, vp, vp, vp, vp, ci, ci, ci, ci, vp, vp, vp, vp]),
     "cubert_paged_cut_work": (ctypes.c_size_t, [ci, ci]),
     "cubert_attention_paged_partials": (ctypes.c_size_t, [ci, ci, ci, ci, ci, ci, ci, ci, ci, ci]),
     "cubert_blas_create": (vp, []),

@@ -2,7 +2,7 @@
 //
 //     page i of sequence b is table[b, i]; its token at position p has slot table[b, p / page] * page + p % page
 //
-// Pages of nobody stand on a stack, free[0 .. *free_count), and are taken from its top.
+// Pages of nobody stand on a stack of some places, free[0 .. *free_count), and are taken from its top.
 
 #include "cubert_kernels.h"
 #include "device_common.h"
@@ -20,7 +20,7 @@ struct ExtendArgs {
     int *table;
     const int *lengths, *counts, *free, *free_count;
     int *slots, *lengths_out, *free_out;
-    int width, ld_table, pages, shift, batch, rows;
+    int width, ld_table, places, pages, shift, batch, rows;  // places of the stack, pages that there are
 };
 
 // What a sequence has and asks for: `need` pages more for `count` tokens; none, and no tokens, where its table has no room for them.
@@ -57,7 +57,7 @@ __global__ __launch_bounds__(kBlock) void paged_extend_kernel(ExtendArgs a) {
     const int rows = a.rows > 0 ? a.rows : 1, total = a.batch * rows, thread = threadIdx.x, lane = thread & (kWave - 1);
     const int from = blockIdx.x * kSpan, until = total - from < kSpan ? total : from + kSpan;
     const int first = from / rows, last = (until - 1) / rows;  // the sequences that these slots belong to
-    const int there = clamp_to(*a.free_count, 0, a.pages);
+    const int there = clamp_to(*a.free_count, 0, a.places);
     if (total == 0) {
         if (thread == 0) *a.free_out = there;
         return;
@@ -132,7 +132,7 @@ struct CutArgs {
     int *free;
     const int *free_count;
     int *lengths_out, *free_out, *returned;
-    int width, ld_table, pages, shift, batch;
+    int width, ld_table, places, pages, shift, batch;
 };
 
 struct Shrink {
@@ -167,7 +167,7 @@ __device__ __forceinline__ int pages_back(const CutArgs &a, int b, const Shrink 
 // They go onto the stack from `height` on, as far as it has room.
 __device__ __forceinline__ void put_back(const CutArgs &a, int b, const Shrink &s, long long height, int lane) {
     const int *row = a.table + (size_t) b * a.ld_table;
-    const int free_places = height < a.pages ? a.pages - (int) height : 0;
+    const int free_places = height < a.places ? a.places - (int) height : 0;
     int *to = a.free + height;
     int at = 0;
     for (int base = s.begin; base < s.end && at < free_places; base += kWave * kAhead) {
@@ -199,7 +199,7 @@ __global__ __launch_bounds__(kBlock) void paged_cut_count_kernel(CutArgs a) {
 // A wavefront per sequence puts its pages onto the stack, behind those of the sequences before it.
 __global__ __launch_bounds__(kBlock) void paged_cut_kernel(CutArgs a) {
     const int b = blockIdx.x * (kBlock / kWave) + wave_in_block(), lane = threadIdx.x & (kWave - 1);
-    const int there = clamp_to(*a.free_count, 0, a.pages);
+    const int there = clamp_to(*a.free_count, 0, a.places);
     if (b >= a.batch) return;
     const Shrink s(a, b);
     long long before = 0;
@@ -209,7 +209,7 @@ __global__ __launch_bounds__(kBlock) void paged_cut_kernel(CutArgs a) {
     const long long height = there + before;
     if (b == a.batch - 1 && lane == 0) {
         const long long all = height + a.returned[b];
-        *a.free_out = (int) (all < a.pages ? all : a.pages);
+        *a.free_out = (int) (all < a.places ? all : a.places);
     }
     put_back(a, b, s, height, lane);
 }
@@ -221,7 +221,7 @@ constexpr long long kFewEntries = 1 << 15;
 __global__ __launch_bounds__(kFewWaves * kWave) void paged_cut_few_kernel(CutArgs a) {
     __shared__ int back[kFewSequences];
     const int wave = wave_in_block(), lane = threadIdx.x & (kWave - 1);
-    const int there = clamp_to(*a.free_count, 0, a.pages);
+    const int there = clamp_to(*a.free_count, 0, a.places);
     for (int b = wave; b < a.batch; b += kFewWaves) {
         const Shrink s(a, b);
         const int count = pages_back(a, b, s, lane);
@@ -237,7 +237,7 @@ __global__ __launch_bounds__(kFewWaves * kWave) void paged_cut_few_kernel(CutArg
     }
     if (wave == 0 && lane == kWave - 1) {
         const long long all = (long long) there + through;
-        *a.free_out = (int) (all < a.pages ? all : a.pages);
+        *a.free_out = (int) (all < a.places ? all : a.places);
     }
     for (int b = wave; b < a.batch; b += kFewWaves)
         put_back(a, b, Shrink(a, b), there + __builtin_amdgcn_readlane(through - mine, b), lane);
@@ -287,9 +287,9 @@ __global__ __launch_bounds__(kBlock) void paged_write_kernel(WriteArgs a) {
 }
 
 // What extend and cut have in common: sizes of tables and pages that 32 bits count.
-int check_tables(const void *table, int width, int ld_table, const void *lengths, const void *free, const void *free_count, int pages, int page, int batch,
-                 const void *lengths_out, const void *free_out) {
-    if (width < 1 || ld_table < width || pages < 1 || page < 1 || batch < 0) return CUBERT_BAD_ARGUMENT;
+int check_tables(const void *table, int width, int ld_table, const void *lengths, const void *free, const void *free_count, int places, int pages, int page,
+                 int batch, const void *lengths_out, const void *free_out) {
+    if (width < 1 || ld_table < width || places < 1 || pages < 1 || page < 1 || batch < 0) return CUBERT_BAD_ARGUMENT;
     if (free == nullptr || free_count == nullptr || free_out == nullptr || free_out == free_count) return CUBERT_BAD_ARGUMENT;
     if (batch > 0 && (table == nullptr || lengths == nullptr || lengths_out == nullptr || lengths_out == lengths)) return CUBERT_BAD_ARGUMENT;
     if ((page & (page - 1)) != 0) return CUBERT_UNSUPPORTED;
@@ -327,11 +327,11 @@ int paged_write(const void *k, const void *v, int ld, const int *slots, int toke
 
 extern "C" {
 
-int cubert_paged_extend(int *table, int width, int ld_table, const int *lengths, const int *counts, const int *free, const int *free_count, int pages,
-                        int page, int batch, int rows, int *slots, int *lengths_out, int *free_out, void *stream) {
+int cubert_paged_extend(int *table, int width, int ld_table, const int *lengths, const int *counts, const int *free, const int *free_count, int places,
+                        int pages, int page, int batch, int rows, int *slots, int *lengths_out, int *free_out, void *stream) {
     using namespace cubert;
     if (rows < 0) return CUBERT_BAD_ARGUMENT;
-    const int rc = check_tables(table, width, ld_table, lengths, free, free_count, pages, page, batch, lengths_out, free_out);
+    const int rc = check_tables(table, width, ld_table, lengths, free, free_count, places, pages, page, batch, lengths_out, free_out);
     if (rc != 0) return rc;
     if (batch > 0 && rows > 0 && slots == nullptr) return CUBERT_BAD_ARGUMENT;
     const long long total = (long long) batch * (rows > 0 ? rows : 1);
@@ -339,7 +339,7 @@ int cubert_paged_extend(int *table, int width, int ld_table, const int *lengths,
     ExtendArgs a;
     a.table = table, a.lengths = lengths, a.counts = counts, a.free = free, a.free_count = free_count;
     a.slots = slots, a.lengths_out = lengths_out, a.free_out = free_out;
-    a.width = width, a.ld_table = ld_table, a.pages = pages, a.shift = __builtin_ctz((unsigned) page), a.batch = batch, a.rows = rows;
+    a.width = width, a.ld_table = ld_table, a.places = places, a.pages = pages, a.shift = __builtin_ctz((unsigned) page), a.batch = batch, a.rows = rows;
     const unsigned blocks = total > 0 ? (unsigned) ((total + kSpan - 1) / kSpan) : 1;
     return launch(paged_extend_kernel, dim3(blocks), dim3(kBlock), (hipStream_t) stream, a);
 }
@@ -348,10 +348,10 @@ size_t cubert_paged_cut_work(int batch, int width) {
     return batch < 1 || width < 1 || cubert::few_to_cut(batch, width) ? 0 : (size_t) batch;
 }
 
-int cubert_paged_cut(const int *table, int width, int ld_table, const int *lengths, const int *keep, int *free, const int *free_count, int pages,
-                     int page, int batch, int *lengths_out, int *free_out, int *work, void *stream) {
+int cubert_paged_cut(const int *table, int width, int ld_table, const int *lengths, const int *keep, int *free, const int *free_count, int places,
+                     int pages, int page, int batch, int *lengths_out, int *free_out, int *work, void *stream) {
     using namespace cubert;
-    const int rc = check_tables(table, width, ld_table, lengths, free, free_count, pages, page, batch, lengths_out, free_out);
+    const int rc = check_tables(table, width, ld_table, lengths, free, free_count, places, pages, page, batch, lengths_out, free_out);
     if (rc != 0) return rc;
     const bool few = few_to_cut(batch, width);
     if (!few && work == nullptr) return CUBERT_BAD_ARGUMENT;
@@ -359,7 +359,7 @@ int cubert_paged_cut(const int *table, int width, int ld_table, const int *lengt
     CutArgs a;
     a.table = table, a.lengths = lengths, a.keep = keep, a.free = free, a.free_count = free_count;
     a.lengths_out = lengths_out, a.free_out = free_out, a.returned = work;
-    a.width = width, a.ld_table = ld_table, a.pages = pages, a.shift = __builtin_ctz((unsigned) page), a.batch = batch;
+    a.width = width, a.ld_table = ld_table, a.places = places, a.pages = pages, a.shift = __builtin_ctz((unsigned) page), a.batch = batch;
     if (few) return launch(paged_cut_few_kernel, dim3(1), dim3(kFewWaves * kWave), (hipStream_t) stream, a);
     constexpr int kEach = kBlock / kWave;
     const unsigned blocks = (unsigned) ((batch + kEach - 1) / kEach);

@@ -631,27 +631,29 @@ def _table_args(table):
     return batch, table.data_ptr(), width, pitch
 
 
-def _stack_args(table, lengths, changes, what, free, free_count, page):
+def _stack_args(table, lengths, changes, what, free, free_count, page, pages):
     batch, table_ptr, width, pitch = _table_args(table)
     shape = free.shape
     if len(shape) != 1 or shape[0] < 1:
-        raise ValueError("free: int32 [pages] expected, got %s %s" % (free.dtype, tuple(shape)))
-    pages = shape[0]
-    _fits(max(batch, pitch, pages, page))
+        raise ValueError("free: int32 [places] expected, got %s %s" % (free.dtype, tuple(shape)))
+    _fits(max(batch, pitch, shape[0], page, pages or 0))
     if page < 1 or page & (page - 1):
         raise ValueError("pages of a power of two of tokens expected, got %d" % page)
+    if pages is None:
+        pages = ((1 << 31) - 1) // page
     whole = (batch,)
     return (table_ptr, width, pitch, _int32(lengths, whole, "lengths"), None if changes is None else _int32(changes, whole, what),
-            _int32(free, shape, "free"), _int32(free_count, (1,), "free_count"), pages, page, batch)
+            _int32(free, shape, "free"), _int32(free_count, (1,), "free_count"), shape[0], pages, page, batch)
 
 
-def paged_extend(table, lengths, counts, free, free_count, page, rows):
+def paged_extend(table, lengths, counts, free, free_count, page, rows, pages=None):
     """Room for `counts` more tokens (int32 [batch], at most `rows`; None: `rows` each) of sequences that have `lengths` (int32 [batch]) in pages of
     `page` tokens, a power of two: (slots int32 [batch, rows], lengths afterwards, free_count afterwards).  New pages come from the top
-    of the stack free[:free_count] (int32 [pages] and [1]) and go into `table` (int32 [batch, width]), in place; slots are page * `page` +
-    place, -1 where there is no token.  A sequence whose table is too short, or for which the stack is, gets nothing and keeps its length."""
+    of the stack free[:free_count] (int32 [places] and [1]) and go into `table` (int32 [batch, width]), in place; slots are page * `page` +
+    place, -1 where there is no token.  A sequence whose table is too short, or for which the stack is, gets nothing and keeps its length.
+    pages: how many there are, numbers outside of which are none (None: as many as slots of 31 bits have)."""
     device = _device(table, lengths, counts, free, free_count)
-    args = _stack_args(table, lengths, counts, "counts", free, free_count, page)
+    args = _stack_args(table, lengths, counts, "counts", free, free_count, page, pages)
     _fits(rows)
     # (the kernel writes every element of the three; sizes as numbers of their own take the shorter way through torch)
     slots, after, left = lengths.new_empty(args[-1], rows), torch.empty_like(lengths), torch.empty_like(free_count)
@@ -659,11 +661,11 @@ def paged_extend(table, lengths, counts, free, free_count, page, rows):
     return slots, after, left
 
 
-def paged_cut(table, lengths, keep, free, free_count, page):
+def paged_cut(table, lengths, keep, free, free_count, page, pages=None):
     """Sequences cut back to their first `keep` tokens (int32 [batch]; None: none): (lengths afterwards, free_count afterwards).  The pages behind
-    go onto the stack `free`, in place; `table` stays as it is, and entries of it that are no pages are passed over."""
+    go onto the stack `free`, in place; `table` stays as it is, and entries of it that are no pages (outside 0..pages-1) are passed over."""
     device = _device(table, lengths, keep, free, free_count)
-    args = _stack_args(table, lengths, keep, "keep", free, free_count, page)
+    args = _stack_args(table, lengths, keep, "keep", free, free_count, page, pages)
     after, left = torch.empty_like(lengths), torch.empty_like(free_count)
     ints = _cut_work(args[-1], args[1])
     work = lengths.new_empty(ints) if ints else None

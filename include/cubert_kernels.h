@@ -313,9 +313,9 @@ int cubert_attention_window_f16(const cubert_half *q, int ldq, const cubert_half
  * The cache above has the rows of the longest sequence for every one; here keys and values of all sequences lie in pools of `pages` pages
  * of `page` tokens, a power of two, and a sequence has as many as its length takes.  Page i of sequence b is table[b * ld_table + i] (int32,
  * `width` entries per sequence, so width * page tokens at most), and its token at position p has slot table[b, p / page] * page + p % page.  Pages
- * of nobody stand on a stack, free[0 .. *free_count) with room for all `pages`, and are taken from its top.  Everything that changes from step
- * to step is read on the device, so one captured graph serves every step.  width * page and pages * page are below 2^31, otherwise
- * CUBERT_UNSUPPORTED, as for a page that is no power of two.  The reference keeps no cache. */
+ * of nobody stand on a stack of `places` places, free[0 .. *free_count), and are taken from its top.  Everything that changes from step to step is
+ * read on the device, so one captured graph serves every step.  width * page and pages * page are below 2^31, otherwise CUBERT_UNSUPPORTED, as
+ * for a page that is no power of two.  The reference keeps no cache. */
 
 /* Sequences of lengths[b] tokens grow by counts[b] (NULL: `rows` each; taken within 0..rows), in order:
  *   need = ceil((length + count) / page) - ceil(length / page);
@@ -325,7 +325,8 @@ int cubert_attention_window_f16(const cubert_half *q, int ldq, const cubert_half
  * is left of the stack.  The table's other entries and the stack stay as they are, so a call whose outputs are not taken over changes nothing that
  * counts.  lengths_out and free_out are other memory than lengths and free_count.  batch * rows below 2^31 - 1024.  One launch. */
 int cubert_paged_extend(int *table, int width, int ld_table, const int *lengths, const int *counts, const int *free, const int *free_count,
-                        int pages, int page, int batch, int rows, int *slots, int *lengths_out, int *free_out, void *stream);
+                        int places, int pages, int page, int batch, int rows, int *slots, int *lengths_out, int *free_out,
+                        void *stream);
 
 /* Sequences keep their first keep[b] tokens (NULL: none; taken within 0..lengths[b]), and the pages behind these go back onto the stack in the
  * order of the sequences and their tables.  Entries that are no pages (outside 0..pages-1: whoever has taken a page out of a table has put something
@@ -334,13 +335,13 @@ int cubert_paged_extend(int *table, int width, int ld_table, const int *lengths,
  * uses before this one is done (none, and one launch, where that is 0). */
 size_t cubert_paged_cut_work(int batch, int width);
 int cubert_paged_cut(const int *table, int width, int ld_table, const int *lengths, const int *keep, int *free, const int *free_count,
-                     int pages, int page, int batch, int *lengths_out, int *free_out, int *work, void *stream);
+                     int places, int pages, int page, int batch, int *lengths_out, int *free_out, int *work, void *stream);
 
 /* Keys and values of `tokens` tokens, [tokens, kv_heads * head_size] at ld elements per row (views of a packed projection), to their slots; a slot outside
  * 0..pages*page-1 is none, and its row stays out.  Pools are [pages, kv_heads, page, head_size] at any strides (in elements) that keep their
- * elements apart, the same for both: the tokens of a head together or the heads of a token, keys and values by turns.  Where a slot is given twice,
- * pieces of either row are kept.  Pointers, rows and strides are whole 16-byte pieces, and a launch holds 2^32 of them, otherwise
- * CUBERT_UNSUPPORTED. */
+ * elements apart, the same for both: the tokens of a head together or the heads of a token, keys and values by turns; k and v overlap nothing of
+ * them.  Where a slot is given twice, pieces of either row are kept.  Pointers, rows and strides are whole 16-byte pieces, and a launch holds
+ * 2^32 of them, otherwise CUBERT_UNSUPPORTED. */
 int cubert_paged_write_f32(const float *k, const float *v, int ld, const int *slots, int tokens, float *k_pages, float *v_pages,
                            long long page_stride, long long head_stride, long long row_stride, int pages, int page, int kv_heads,
                            int head_size, void *stream);
@@ -358,8 +359,9 @@ int cubert_paged_write_f16(const cubert_half *k, const cubert_half *v, int ld, c
  * what is no number holds here too.
  * q is [batch * q_rows, heads * head_size] at ldq elements per row, ctx like it at ld_ctx and apart from all that is read; pools as above, with pages
  * of 16 tokens at least that span less than 2^31 bytes from row to row.  Lengths are taken within 0..width*page, which is below 2^30.
- * head_size 32, 64 or 128, pointers and strides of whole 16-byte pieces; otherwise CUBERT_UNSUPPORTED.  One row to a few dozen of q_rows * heads /
- * kv_heads are what it is made for; more are right.
+ * head_size 32, 64 or 128, pointers and strides of whole 16-byte pieces, and batch * kv_heads times the rows of a key head, q_rows * heads /
+ * kv_heads in whole tiles of 16 (one) or 32, below 2^24; otherwise CUBERT_UNSUPPORTED.  One row to 32 are what it is made for; with more K and V are read
+ * once for every 32.
  * A long cache is cut along its length, into `partials`: cubert_attention_paged_partials floats of device memory, 16-byte aligned, that no
  * other call uses before this one is done.  With less (or NULL) the same call runs uncut. */
 size_t cubert_attention_paged_partials(int half_precision, int batch, int heads, int kv_heads, int q_rows, int width, int page,

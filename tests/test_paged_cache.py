@@ -15,20 +15,20 @@ def L():
     return lib()
 
 
-def extend(L, table=P, width=8, ld_table=None, lengths=P, counts=P, free=P, free_count=P, pages=100, page=16, batch=3, rows=2, slots=P, lengths_out=Q,
+def extend(L, table=P, width=8, ld_table=None, lengths=P, counts=P, free=P, free_count=P, places=100, pages=100, page=16, batch=3, rows=2, slots=P, lengths_out=Q,
            free_out=Q):
-    return L.cubert_paged_extend(table, width, width if ld_table is None else ld_table, lengths, counts, free, free_count, pages, page, batch, rows,
+    return L.cubert_paged_extend(table, width, width if ld_table is None else ld_table, lengths, counts, free, free_count, places, pages, page, batch, rows,
                                  slots, lengths_out, free_out, None)
 
 
-def cut(L, table=P, width=8, ld_table=None, lengths=P, keep=P, free=P, free_count=P, pages=100, page=16, batch=3, lengths_out=Q, free_out=Q, work=P):
-    return L.cubert_paged_cut(table, width, width if ld_table is None else ld_table, lengths, keep, free, free_count, pages, page, batch,
+def cut(L, table=P, width=8, ld_table=None, lengths=P, keep=P, free=P, free_count=P, places=100, pages=100, page=16, batch=3, lengths_out=Q, free_out=Q, work=P):
+    return L.cubert_paged_cut(table, width, width if ld_table is None else ld_table, lengths, keep, free, free_count, places, pages, page, batch,
                               lengths_out, free_out, work, None)
 
 
 @pytest.mark.parametrize("call", [extend, cut])
 def test_tables_refuse(L, call):
-    for wrong in (dict(table=None), dict(width=0), dict(ld_table=7), dict(lengths=None), dict(free=None), dict(free_count=None), dict(pages=0), dict(page=0),
+    for wrong in (dict(table=None), dict(width=0), dict(ld_table=7), dict(lengths=None), dict(free=None), dict(free_count=None), dict(places=0), dict(pages=0), dict(page=0),
                   dict(page=-16), dict(batch=-1), dict(lengths_out=None), dict(free_out=None), dict(lengths_out=P), dict(free_out=P)):
         assert call(L, **wrong) == BAD_ARGUMENT, wrong
     for other in (dict(page=12), dict(page=48), dict(width=1 << 27, page=16), dict(pages=1 << 27, page=16), dict(width=1, page=1 << 30, pages=2)):
@@ -192,6 +192,7 @@ def test_wrappers_refuse_what_32_bits_do_not_hold(monkeypatch):
                  lambda: kernels.paged_extend(whole(1, 3), whole(1), None, whole(large), whole(1), 16, 1),
                  lambda: kernels.paged_extend(whole(1, 3), whole(1), None, whole(9), whole(1), 1 << 32, 1),
                  lambda: kernels.paged_extend(whole(1, 3), whole(1), None, whole(9), whole(1), 16, large),
+                 lambda: kernels.paged_cut(whole(1, 3), whole(1), None, whole(9), whole(1), 16, large),
                  lambda: kernels.paged_cut(torch.empty_strided((2, 3), (large, 1), dtype=torch.int32, device="meta"), whole(2), None, whole(9), whole(1), 16),
                  lambda: kernels.paged_write(empty(1, large, 2, 64), empty(1, large, 2, 64), whole(1, large), pool, pool),
                  lambda: kernels.paged_write(empty(1, 1, 2, 64), empty(1, 1, 2, 64), whole(1, 1), empty(large, 2, 16, 64), empty(large, 2, 16, 64)),

@@ -45,11 +45,11 @@ def up(n, page):
 # ---------------------------------------------------------------------------- tables
 
 
-def extend_reference(table, lengths, counts, free, free_count, page, rows):
+def extend_reference(table, lengths, counts, free, free_count, page, rows, there=None):
     """What paged_extend gives, by a walk through the sequences: (slots, lengths, free_count, table)."""
-    width, pages = len(table[0]) if table else 1, len(free)
+    width, pages = len(table[0]) if table else 1, ((1 << 31) - 1) // page if there is None else there
     table, after = [list(r) for r in table], []
-    top, refused = min(max(free_count, 0), pages), False
+    top, refused = min(max(free_count, 0), len(free)), False
     slots = [[-1] * rows for _ in lengths]
     for b, n in enumerate(lengths):
         n = min(max(n, 0), width * page)
@@ -71,16 +71,16 @@ def extend_reference(table, lengths, counts, free, free_count, page, rows):
     return slots, after, top, table
 
 
-def cut_reference(table, lengths, keep, free, free_count, page):
+def cut_reference(table, lengths, keep, free, free_count, page, there=None):
     """(lengths, free_count, free) of paged_cut."""
-    width, pages = len(table[0]) if table else 1, len(free)
-    free, top, after = list(free), min(max(free_count, 0), pages), []
+    width, pages = len(table[0]) if table else 1, ((1 << 31) - 1) // page if there is None else there
+    free, top, after = list(free), min(max(free_count, 0), len(free)), []
     for b, n in enumerate(lengths):
         n = min(max(n, 0), width * page)
         left = min(max(keep[b], 0), n) if keep is not None else 0
         after.append(left)
         for i in range(up(left, page), up(n, page)):
-            if 0 <= table[b][i] < pages and top < pages:
+            if 0 <= table[b][i] < pages and top < len(free):
                 free[top] = table[b][i]
                 top += 1
     return after, top, free
@@ -159,10 +159,11 @@ def test_extend_of_what_no_program_hands_over(K):
     lengths, counts = [low, 20, high, 17, 30], [3, 40, 1, 4, 34]
     free = [6, -1, 11, high, low, 20, 0, 1, 2, 3, 4, 5]
     for there in (12, 6, 4, 0, -5, high):
-        got_table = ints(table)
-        slots, after, left = K.paged_extend(got_table, ints(lengths), ints(counts), ints(free), ints([there]), page, 40)
-        want = extend_reference(table, lengths, counts, free, there, page, 40)
-        assert (slots.tolist(), after.tolist(), left.tolist()[0], got_table.tolist()) == want
+        for pages in (12, None, 5, 1000):
+            got_table = ints(table)
+            slots, after, left = K.paged_extend(got_table, ints(lengths), ints(counts), ints(free), ints([there]), page, 40, pages)
+            want = extend_reference(table, lengths, counts, free, there, page, 40, pages)
+            assert (slots.tolist(), after.tolist(), left.tolist()[0], got_table.tolist()) == want
 
 
 def test_tables_with_rows_apart(K):
@@ -222,8 +223,9 @@ def test_cut(K, name, holes):
     if kind == "none" and holes:
         keep = None
     stack, on = ints(free), (ints(table), ints(lengths))
-    after, left = K.paged_cut(*on, None if keep is None else ints(keep), stack, ints([there]), page)
-    want = cut_reference(table, lengths, keep, free, there, page)
+    pages = len(free) if holes or len(name) % 2 else None
+    after, left = K.paged_cut(*on, None if keep is None else ints(keep), stack, ints([there]), page, pages)
+    want = cut_reference(table, lengths, keep, free, there, page, pages)
     assert after.tolist() == want[0] and left.tolist() == [want[1]] and stack.tolist() == want[2]
     assert on[0].tolist() == table and on[1].tolist() == lengths
 
@@ -239,6 +241,18 @@ def test_cut_of_more_than_the_stack_holds(K):
         want = cut_reference(table, lengths, None, [-8] * 10, there, 16)
         assert after.tolist() == want[0] and left.tolist() == [want[1]] and stack.tolist() == want[2]
         assert bool((room[:10] == -8).all()) and bool((room[20:] == -8).all())
+
+
+def test_a_stack_of_fewer_places_than_pages(K):
+    """Some of a pool's pages are not the stack's: their numbers are beyond its places."""
+    table, free = [[700, 3, -1, -1], [5, 900, 901, -1], [-1] * 4], [7, 999, 2, 0, 0]
+    on = ints(table)
+    slots, after, left = K.paged_extend(on, ints([20, 40, 0]), ints([13, 3, 2]), ints(free), ints([3]), 16, 13)
+    assert (slots.tolist(), after.tolist(), left.tolist()[0], on.tolist()) == extend_reference(table, [20, 40, 0], [13, 3, 2], free, 3, 16, 13)
+    assert slots[1, :3].tolist() == [901 * 16 + 8, 901 * 16 + 9, 901 * 16 + 10] and slots[2, 0] == 999 * 16
+    stack = ints(free)
+    after, left = K.paged_cut(on, after, ints([0, 16, 0]), stack, left, 16)
+    assert stack.tolist() == [7, 700, 3, 2, 900] and left.tolist() == [5]
 
 
 @pytest.mark.parametrize("page", [1, 16, 64])
