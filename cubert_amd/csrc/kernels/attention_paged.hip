@@ -618,7 +618,7 @@ __global__ __launch_bounds__(WAVES * kWave < kBlock ? kBlock : WAVES * kWave) vo
 //
 // A workgroup to a problem / pieces and a join.  Few problems are cut where they have more than 16 units, many where they have more than an eighth
 // of their number: 1 x 1 over 2000 keys, 16 heads of 64 (16 problems of 32 units) 13.7 / 10.8; 8 x 1 over up to 1000, 4 of 128 (32 of 32) 13.7 /
-// 11.5; 128 x 1 over up to 1500, 2 of 64 (256 of 24) 14.1 / 19.9; 256 x 1 over up to 512, 12 of 64 (3072 of 8) 44 / 55; 128 x 1 over up
+// 11.5; 128 x 1 over up to 1500, 2 of 64 (256 of 24) 14.1 / 19.9; 256 x 1 over up to 512, 12 of 64 (256 x 12 of 8) 44 / 55; 128 x 1 over up
 // to 2048, 12 of 64 (1536 of 32, tables for 256) 85 / 81; 1 x 1 over 131072, 2 of 128 (2 of 4096) 1770 / 31.
 //
 // Pieces, 256 / 512 / 1024 / 2048 of all (less the number of problems where that is below the first number that fits).  A workgroup to a unit of
@@ -631,6 +631,7 @@ __global__ __launch_bounds__(WAVES * kWave < kBlock ? kBlock : WAVES * kWave) vo
 // 15.2 / 13.8.
 PagedPlan plan_paged(bool half_precision, int batch, int heads, int kv_heads, int q_rows, long long limit, int head_size, int left, int sinks) {
     PagedPlan plan;
+    if (left >= kFar) left = -1;
     const long long rows = (long long) q_rows * (heads / kv_heads);
     plan.rows = rows <= 16 ? 16 : 32;
     plan.row_tiles = (int) ((rows + plan.rows - 1) / plan.rows);
@@ -714,7 +715,7 @@ int attention_paged(const T *q, int ldq, const T *k_pages, const T *v_pages, lon
     // (a launch holds less than 2^32 threads, and rows are counted in 32 bits)
     if ((long long) batch * q_rows >= 1ll << 31 || (long long) batch * kv_heads >= 1 << 24 || (long long) q_rows * (heads / kv_heads) >= 1 << 30)
         return CUBERT_UNSUPPORTED;
-    PagedPlan plan = plan_paged(sizeof(T) == 2, batch, heads, kv_heads, q_rows, (long long) width * page, head_size, a.left == kFar ? -1 : left, a.sinks);
+    PagedPlan plan = plan_paged(sizeof(T) == 2, batch, heads, kv_heads, q_rows, (long long) width * page, head_size, left, sinks);
     if (plan.problems * plan.rows >= 1 << 24) return CUBERT_UNSUPPORTED;
     plan.once = read_once(plan, pages, page, kv_heads, head_size * (int) sizeof(T));
     if (plan.pieces != 0 && (partials == nullptr || partial_floats < plan.floats || !is_aligned(partials, 16))) plan.pieces = 0;
