@@ -57,15 +57,16 @@ typedef int v2i32 __attribute__((ext_vector_type(2)));
 // fp32: a product with V takes a single number of one key from a lane.  Of the i-th key of its four a lane brings D / 16 columns of V, one after
 // the other, as they lie in memory, and nothing is transposed.
 //
-// What is on its way together, a unit, is 16 KB of K and V for a wavefront where rows have 128 bytes and more: while it works on one, K of the
-// next is requested as soon as this one's has been multiplied, and V as soon as this one's lies in LDS.  Twelve wavefronts to a compute unit have
-// 192 KB on their way.
+// What is on its way together, a unit, is 32 keys for a wavefront (16 where rows have 512 bytes): while it works on one, K of the next is requested as
+// soon as this one's has been multiplied, and V as soon as this one's lies in LDS.  Rows of 256 bytes: twelve wavefronts to a compute unit have 192
+// KB on their way.  (64 keys where rows have 128 bytes, and fewer wavefronts: 256 x 1 over up to 512 keys of 12 heads of 64 43.9 us for 42.1, 4 x 1
+// over up to 300 6.8 for 6.0.)
 template <typename T, int D>
 struct Shape {
     static constexpr bool kHalf = sizeof(T) == 2;
     static constexpr int kRowBytes = D * (int) sizeof(T);
     static constexpr int kKeyLoads = kRowBytes / 64;                                // 16-byte pieces of a key that a lane has
-    static constexpr int kSub = 8192 / (16 * kRowBytes) < 4 ? 8192 / (16 * kRowBytes) : 4;  // 16 keys each: what is on its way together
+    static constexpr int kSub = kRowBytes == 512 ? 1 : 2;                           // 16 keys each: what is on its way together
     static constexpr int kKeys = 16 * kSub;
     // V: requests for 16 keys, their size, and how many keys one has
     static constexpr int kValueBytes = kHalf || kRowBytes >= 256 ? 16 : kRowBytes / 16;
@@ -627,24 +628,31 @@ __global__ __launch_bounds__(WAVES * kWave < kBlock ? kBlock : WAVES * kWave) vo
 // (24) 34 / 45 / 52 / -; 48 x 1 over up to 4000, 2 of 128 (96) 31.4 / 27.6 / 29.3 / 30.0; 32 x 1, window 4096, 4 of 128 (128) 68.9 / 52.9 / 46.6 / 46.6;
 // 64 x 1 over up to 4096, 4 of 128 (256) 69.6 / 69.3 / 56.1 / 53.8.
 //
+// Rows of a tile, where there are more than 16, 16 / 32, by what K and V of a sequence and of all may come to: 8 x 1 over up to 4000, 32 heads to 1 of 64 (1
+// MB, 8) 11.1 / 12.2; 32 x 2 over up to 1000, 48 heads to 4 of 64 (0.25, 33) 10.2 / 13.0; 8 x 4 over up to 4000, 32 to 4 of 128 (2, 65) 20.9 / 18.4; 1 x
+// 8 over up to 16800, 96 to 12 of 128 (17, 206) 46.8 / 33.9; fp32, 8 x 1 over up to 8000, 32 to 1 of 128 (8, 65) 19.3 / 22.0; 4 x 4 over up to 16000,
+// 32 to 4 of 64 (8, 131) 30.3 / 26.3.
+//
 // Units of a piece at least, 4 / 8: 8 x 1 over up to 1000, 4 of 128 (32 problems of 32) 11.3 / 12.6; fp32, 8 x 1 over up to 1000, 12 of 64 (96 of 32)
 // 15.2 / 13.8.
 PagedPlan plan_paged(bool half_precision, int batch, int heads, int kv_heads, int q_rows, long long limit, int head_size, int left, int sinks) {
     PagedPlan plan;
     if (left >= kFar) left = -1;
     const long long rows = (long long) q_rows * (heads / kv_heads);
-    plan.rows = rows <= 16 ? 16 : 32;
+    const int row_bytes = head_size * (half_precision ? 2 : 4), keys = row_bytes == 512 ? 16 : 32;
+    const long long most = left >= 0 && (long long) left + q_rows + sinks < limit ? (long long) left + q_rows + sinks : limit;  // keys of a sequence
+    const long long bytes = most * 2 * row_bytes, all_bytes = (long long) batch * kv_heads * bytes;
+    plan.rows = rows > 16 && bytes > 1 << 20 && all_bytes >= (half_precision ? 24 << 20 : 96 << 20) ? 32 : 16;
     plan.row_tiles = (int) ((rows + plan.rows - 1) / plan.rows);
     plan.slot_rows = (int) (rows < plan.rows ? rows : plan.rows);
     plan.problems = (long long) batch * kv_heads * plan.row_tiles;
     plan.pieces = 0, plan.floats = 0, plan.once = false;
-    const int row_bytes = head_size * (half_precision ? 2 : 4), keys = row_bytes >= 128 ? 8192 / row_bytes : 64;
     long long reach = limit;  // the most keys that a tile of rows sees, and how many units of them
     if (left >= 0 && (long long) left + plan.rows + sinks < reach) reach = (long long) left + plan.rows + sinks;
     const long long units = (reach + keys - 1) / keys + (left >= 0 ? 2 : 0), all = plan.problems * units;
     plan.least = all <= 1536 ? 4 : 8;
-    const long long uncut = plan.problems / 8 < 16 ? 16 : plan.problems / 8 < 256 ? plan.problems / 8 : 256;
-    if (units <= uncut || all >= 1 << 30) return plan;  // (units are counted in 32 bits)
+    const long long uncut = plan.problems / 8 < 16 ? 16 : plan.problems / 8 < 256 ? plan.problems / 8 : 256;  // (16 KB each)
+    if (units * keys * row_bytes <= uncut * 8192 || all >= 1 << 30) return plan;  // (units are counted in 32 bits)
     plan.pieces = plan.problems <= 32 ? 256 - (int) plan.problems : plan.problems <= 100 ? 512 - (int) plan.problems : 2048;
     if ((all + plan.least - 1) / plan.least < plan.pieces) plan.pieces = (int) ((all + plan.least - 1) / plan.least);
     plan.floats = (size_t) (plan.pieces + plan.problems) * plan.slot_rows * (head_size + 4) + 2 * (size_t) plan.problems;

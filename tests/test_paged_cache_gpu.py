@@ -484,6 +484,25 @@ def test_attention_paged(K, name, t, size):
     assert torch.equal(got, K.attention_paged(q, k_pages, v_pages, table, **at))     # the same call gives the same bits
 
 
+@pytest.mark.parametrize("name", ["many rows", "many heads to one", "before the sequence", "padded tokens", "a prompt", "unlike lengths", "nobody", "long"])
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("size", [32, 64, 128])
+@pytest.mark.parametrize("filler", [None, math.nan])
+def test_attention_paged_with_wide_tables(K, name, t, size, filler):
+    """Tables with room for far longer sequences than there are: as calls on long ones are cut, and their rows."""
+    q, k_pages, v_pages, table, k, v, page, at = paged(name, TYPES[t], size, wide=20000)
+    seen = visible(q, k, page, **at)
+    want, bound = reference(q, k, v, seen)
+    if filler is not None:
+        keep = torch.zeros(k_pages.shape[0] * page, dtype=torch.bool, device="cuda")
+        b, j = seen.any(1).nonzero(as_tuple=True)
+        keep[table[b, j // page].long() * page + j % page] = True
+        k_pages, v_pages = (torch.where(keep.view(-1, 1, page, 1), p, filler) for p in (k_pages, v_pages))
+    got = K.attention_paged(q, k_pages, v_pages, table, **at)
+    within(got, want, bound, name)
+    assert bool((got[~seen.any(2)] == 0).all())
+
+
 @pytest.mark.parametrize("name", ["one query", "a few tokens", "a window and sinks", "long", "unlike lengths"])
 @pytest.mark.parametrize("t", ["f32", "f16"])
 @pytest.mark.parametrize("layout", LAYOUTS[1:])
