@@ -195,8 +195,8 @@ struct Rows {
 
 // Bound by reading K and V, and by what comes before and behind it: a chain of reads from the lengths over the table to the first keys takes 2.5
 // us, the join 4.  fp16, 64 x 1 over up to 4096 keys of 4 heads of 128, 272 MB in 53 us (5.1 TB/s); 256 x 1 over up to 512 of 12 heads of 64, 223
-// MB in 43 us (5.1 TB/s); 1 x 1 over 131072 of 2 heads of 128, 134 MB in 31 us; fp32, 32 x 1 over up to 4096 of 12 heads of 64, 443 MB in 78 us (5.7
-// TB/s).  One tile of rows: 168 registers, with which three workgroups fit a unit (two: the second of these calls 49 us, the first 57).
+// MB in 42 us (5.3 TB/s); 1 x 1 over 131072 of 2 heads of 128, 134 MB in 31 us; fp32, 32 x 1 over up to 4096 of 12 heads of 64, 443 MB in 78 us (5.7
+// TB/s).  One tile of rows: 168 registers at most, with which three workgroups and more fit a unit (two: the first of these calls 57 us).
 // The four wavefronts have a run of the piece's units each; their sums meet in LDS, in wavefront order.
 template <typename T, int D, int TILES, bool ONCE>
 __global__ __launch_bounds__(kBlock, TILES == 1 ? 3 : 2) void attention_paged_kernel(PagedArgs a, PagedPlan plan) {
@@ -617,24 +617,24 @@ __global__ __launch_bounds__(WAVES * kWave < kBlock ? kBlock : WAVES * kWave) vo
 
 // How a call is cut.  Microseconds of calls in a captured graph, over inputs in turn, fp16 where nothing is said:
 //
-// A workgroup to a problem / pieces and a join.  Few problems are cut where they have more than 16 units, many where they have more than an eighth
-// of their number: 1 x 1 over 2000 keys, 16 heads of 64 (16 problems of 32 units) 13.7 / 10.8; 8 x 1 over up to 1000, 4 of 128 (32 of 32) 13.7 /
-// 11.5; 128 x 1 over up to 1500, 2 of 64 (256 of 24) 14.1 / 19.9; 256 x 1 over up to 512, 12 of 64 (256 x 12 of 8) 44 / 55; 128 x 1 over up
-// to 2048, 12 of 64 (1536 of 32, tables for 256) 85 / 81; 1 x 1 over 131072, 2 of 128 (2 of 4096) 1770 / 31.
-//
-// Pieces, 256 / 512 / 1024 / 2048 of all (less the number of problems where that is below the first number that fits).  A workgroup to a unit of
-// the card is enough where the pieces are alike, and leaves the join the least to do; many problems of unlike lengths want many pieces, which are
-// handed out as units come free: 4 x 1 over up to 30000, 4 of 128 (16 problems) 31.1 / 30.6 / 32.8 / 33.7; 1 x 8 over up to 16800, 96 heads to 12 of 128
-// (24) 34 / 45 / 52 / -; 48 x 1 over up to 4000, 2 of 128 (96) 31.4 / 27.6 / 29.3 / 30.0; 32 x 1, window 4096, 4 of 128 (128) 68.9 / 52.9 / 46.6 / 46.6;
-// 64 x 1 over up to 4096, 4 of 128 (256) 69.6 / 69.3 / 56.1 / 53.8.
-//
 // Rows of a tile, where there are more than 16, 16 / 32, by what K and V of a sequence and of all may come to: 8 x 1 over up to 4000, 32 heads to 1 of 64 (1
 // MB, 8) 11.1 / 12.2; 32 x 2 over up to 1000, 48 heads to 4 of 64 (0.25, 33) 10.2 / 13.0; 8 x 4 over up to 4000, 32 to 4 of 128 (2, 65) 20.9 / 18.4; 1 x
 // 8 over up to 16800, 96 to 12 of 128 (17, 206) 46.8 / 33.9; fp32, 8 x 1 over up to 8000, 32 to 1 of 128 (8, 65) 19.3 / 22.0; 4 x 4 over up to 16000,
 // 32 to 4 of 64 (8, 131) 30.3 / 26.3.
 //
-// Units of a piece at least, 4 / 8: 8 x 1 over up to 1000, 4 of 128 (32 problems of 32) 11.3 / 12.6; fp32, 8 x 1 over up to 1000, 12 of 64 (96 of 32)
-// 15.2 / 13.8.
+// A workgroup to a problem / pieces and a join.  Few problems are cut where they have more than 256 KB, many where they have more than 2 KB for each of
+// their number: 1 x 1 over 2000 keys, 16 heads of 64 (16 problems of 0.5 MB) 14.3 / 10.4; 8 x 1 over up to 1000, 4 of 128 (32 of 0.5) 13.7 / 11.3;
+// 128 x 1 over up to 1500, 2 of 64 (256 of 0.4) 13.9 / 18.4; 256 x 1 over up to 512, 12 of 64 (256 x 12 of 0.1) 42 / 52; 128 x 1 over up to 2048, 12 of 64
+// (1536 of 0.5, tables for 4) 85 / 81; 1 x 1 over 131072, 2 of 128 (2 of 67) 1781 / 31.
+//
+// Pieces, 256 / 512 / 1024 / 2048 of all (less the number of problems where that is below the first number that fits).  A workgroup to a unit of
+// the card is enough where the pieces are alike, and leaves the join the least to do; many problems of unlike lengths want many pieces, which are
+// handed out as units come free: 4 x 1 over up to 30000, 4 of 128 (16 problems) 31.0 / 30.7 / 32.9 / 33.8; 1 x 8 over up to 16800, 96 heads to 12 of 128
+// (24) 34 / 44 / 50 / 76; 48 x 1 over up to 4000, 2 of 128 (96) 31.3 / 27.6 / 29.3 / 29.9; 32 x 1, window 4096, 4 of 128 (128) 68.8 / 53.0 / 46.5 / 46.4;
+// 64 x 1 over up to 4096, 4 of 128 (256) 70.3 / 70.1 / 55.7 / 54.1.
+//
+// Units of a piece at least, 4 / 8: 8 x 1 over up to 1000, 4 of 128 (32 problems of 32) 11.3 / 12.5; fp32, 8 x 1 over up to 1000, 12 of 64 (96 of 32)
+// 15.1 / 13.9.
 PagedPlan plan_paged(bool half_precision, int batch, int heads, int kv_heads, int q_rows, long long limit, int head_size, int left, int sinks) {
     PagedPlan plan;
     if (left >= kFar) left = -1;
@@ -659,10 +659,10 @@ PagedPlan plan_paged(bool half_precision, int batch, int heads, int kv_heads, in
     return plan;
 }
 
-// Whether K and V are read past the caches: once, by one tile of rows, and out of pools that do not stay in the 256 MB behind the L2 caches until the next
-// call, from 96 MB on.  Microseconds without / with: 64 x 1 over up to 4096, 4 of 128 (272 MB) 60.2 / 53.5; 48 x 1 over up to 4000, 2 of 128 (108
-// MB) 29.3 / 27.2; 128 x 1 over up to 1500, 2 of 64 (55 MB, there still after four calls) 14.1 / 15.9; two tiles of rows, 1 x 8 over up to 16800, 96 heads to
-// 12 of 128, 34 / 41.
+// Whether K and V are read past the caches: once, by one tile of rows, and out of pools that do not stay in the 256 MB behind the L2 caches until the
+// next call, from 96 MB on.  Microseconds without / with: 64 x 1 over up to 4096, 4 of 128 (272 MB) 60.0 / 53.6; 48 x 1 over up to 4000, 2 of 128 (108
+// MB) 29.4 / 27.5; 128 x 1 over up to 1500, 2 of 64 (55 MB, there still after four calls) 13.9 / 15.1; two tiles of 32 rows, 1 x 8 over up to 16800, 96 heads
+// to 12 of 128, 34 / 41.
 bool read_once(const PagedPlan &plan, long long pages, int page, int kv_heads, int row_bytes) {
     return plan.row_tiles == 1 && 2 * pages * page * kv_heads * row_bytes >= 96ll << 20;
 }
@@ -677,7 +677,7 @@ int run_paged(const PagedArgs &a, const PagedPlan &plan, hipStream_t stream) {
     if (rc != 0 || plan.pieces == 0) return rc;
     const unsigned joins = (unsigned) (plan.problems * plan.slot_rows);
     // Wavefronts to a row, by its pieces on average, 1 / 4 / 16 (which have 32 columns of it): fp32, 9 x 5 over up to 1000, 12 of 64 (8 pieces)
-    // 17.0 / 17.4 / 22.0 us the whole call; fp16, 64 x 1 over up to 4096 (8) 54.0 / 55.0 / 78.7; 1 x 1 over 60000, 1 of 128 (234) 27.1 / 17.1 / 15.0.
+    // 16.9 / 17.3 / 22.0 us the whole call; fp16, 64 x 1 over up to 4096 (8) 54.1 / 54.9 / 79.2; 1 x 1 over 60000, 1 of 128 (234) 27.1 / 17.0 / 15.1.
     const int of_problem = plan.pieces / (int) plan.problems;
     if (of_problem <= 16) return launch(attention_paged_join_kernel<T, D, D, 1>, dim3((joins + 3) / 4), dim3(kBlock), stream, a, plan);
     if (of_problem <= 64) return launch(attention_paged_join_kernel<T, D, D, 4>, dim3(joins), dim3(kBlock), stream, a, plan);

@@ -360,8 +360,8 @@ int cubert_paged_write_f16(const cubert_half *k, const cubert_half *v, int ld, c
  * q is [batch * q_rows, heads * head_size] at ldq elements per row, ctx like it at ld_ctx and apart from all that is read; pools as above, with pages
  * of 16 tokens at least that span less than 2^31 bytes from row to row.  Lengths are taken within 0..width*page, which is below 2^30.
  * head_size 32, 64 or 128, pointers and strides of whole 16-byte pieces, and batch * kv_heads times the rows of a key head, q_rows * heads /
- * kv_heads in whole tiles of 16 (one) or 32, below 2^24; otherwise CUBERT_UNSUPPORTED.  One row to 32 are what it is made for; with more K and V are read
- * once for every 32.
+ * kv_heads in whole tiles of 16 or 32, below 2^24; otherwise CUBERT_UNSUPPORTED.  One row to 32 are what it is made for; with more K and V are read
+ * once for every tile.
  * A long cache is cut along its length, into `partials`: cubert_attention_paged_partials floats of device memory, 16-byte aligned, that no
  * other call uses before this one is done.  With less (or NULL) the same call runs uncut. */
 size_t cubert_attention_paged_partials(int half_precision, int batch, int heads, int kv_heads, int q_rows, int width, int page,
