@@ -286,13 +286,15 @@ __global__ __launch_bounds__(kBlock) void paged_write_kernel(WriteArgs a) {
     }
 }
 
+constexpr int kMostSequences = 1 << 18;  // what a sequence asks for or returns is added up by all behind it
+
 // What extend and cut have in common: sizes of tables and pages that 32 bits count.
 int check_tables(const void *table, int width, int ld_table, const void *lengths, const void *free, const void *free_count, int places, int pages, int page,
                  int batch, const void *lengths_out, const void *free_out) {
     if (width < 1 || ld_table < width || places < 1 || pages < 1 || page < 1 || batch < 0) return CUBERT_BAD_ARGUMENT;
     if (free == nullptr || free_count == nullptr || free_out == nullptr || free_out == free_count) return CUBERT_BAD_ARGUMENT;
     if (batch > 0 && (table == nullptr || lengths == nullptr || lengths_out == nullptr || lengths_out == lengths)) return CUBERT_BAD_ARGUMENT;
-    if ((page & (page - 1)) != 0) return CUBERT_UNSUPPORTED;
+    if ((page & (page - 1)) != 0 || batch > kMostSequences) return CUBERT_UNSUPPORTED;
     const long long most = (1ll << 31) - 1;
     if ((long long) width * page > most || (long long) pages * page > most) return CUBERT_UNSUPPORTED;
     return 0;
@@ -355,7 +357,6 @@ int cubert_paged_cut(const int *table, int width, int ld_table, const int *lengt
     if (rc != 0) return rc;
     const bool few = few_to_cut(batch, width);
     if (!few && work == nullptr) return CUBERT_BAD_ARGUMENT;
-    if (batch > 1 << 25) return CUBERT_UNSUPPORTED;
     CutArgs a;
     a.table = table, a.lengths = lengths, a.keep = keep, a.free = free, a.free_count = free_count;
     a.lengths_out = lengths_out, a.free_out = free_out, a.returned = work;

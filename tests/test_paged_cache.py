@@ -48,6 +48,8 @@ def test_extend_refuses(L):
     assert extend(L, rows=-1) == BAD_ARGUMENT
     assert extend(L, slots=None) == BAD_ARGUMENT
     assert extend(L, batch=1 << 16, rows=1 << 15) == UNSUPPORTED
+    assert extend(L, batch=(1 << 18) + 1, rows=1) == UNSUPPORTED
+    assert cut(L, batch=(1 << 18) + 1) == UNSUPPORTED
     assert extend(L, batch=LARGE, rows=0) == UNSUPPORTED
     assert extend(L, batch=LARGE, rows=LARGE) == UNSUPPORTED
 
