@@ -20,6 +20,8 @@ namespace {
 constexpr int kFar = (1 << 30) - 1;  // a bound or position that no sequence reaches
 constexpr float kNone = -3.402823466e38f;  // the maximum of no scores: no finite score is less
 
+constexpr int kShared = 64;  // bytes of LDS in which wavefronts tell each other which piece theirs is
+
 struct PagedArgs {
     const void *q, *k, *v;
     void *ctx;
@@ -215,39 +217,79 @@ __global__ __launch_bounds__(kBlock, TILES == 1 ? 3 : 2) void attention_paged_ke
         length = a.lengths[b];
         if (a.first != nullptr) first = a.first[b];
     } else {
-        // (every wavefront looks through the sequences by itself, 64 at a time, the first of them out of registers)
-        constexpr int kKept = 4;
         typedef Entry<kKeys> Found;
-        const int all = a.batch * plan.row_tiles;
-        Found kept[kKept];
-        int sum = 0;
-#pragma unroll
-        for (int n = 0; n < kKept; ++n)
-            if (n == 0 || n * kWave < all) kept[n] = Found(a, plan, n * kWave + lane);
-#pragma unroll
-        for (int n = 0; n < kKept; ++n) sum += kept[n].units;
-        for (int i = kKept * kWave; i < all; i += kWave) sum += Found(a, plan, i + lane).units;
-        const int total = __builtin_amdgcn_readlane(sum_through(sum), kWave - 1) * a.kv_heads;  // (below 2^30: see plan_paged)
-        const int least = (total + plan.pieces - 1) / plan.pieces, most = least > plan.least ? least : plan.least;  // units of a piece
-        int before = 0;
+        const int all = a.batch * plan.row_tiles, block = (int) blockIdx.x;
+        int before = 0, most = 0;
         bool found = false;
+        auto units_of_piece = [&](int units) {  // (units of all sequences and tiles for a key head; of all of them below 2^30: see plan_paged)
+            const int least = (units * a.kv_heads + plan.pieces - 1) / plan.pieces;
+            most = least > plan.least ? least : plan.least;
+        };
+        auto own_pieces = [&](const Found &of) { return (of.units + most - 1) / most; };
         auto look = [&](int from, const Found &of) {
-            const int own = (of.units + most - 1) / most, through = sum_through(own * a.kv_heads);
-            const unsigned long long here = __ballot(before + through > (int) blockIdx.x);
+            const int own = own_pieces(of), through = sum_through(own * a.kv_heads);
+            const unsigned long long here = __ballot(before + through > block);
             if (here != 0) {
                 const int at = __builtin_ctzll(here);
                 found = true, entry = from + at, pieces = __builtin_amdgcn_readlane(own, at);
                 length = __builtin_amdgcn_readlane(of.length, at), first = __builtin_amdgcn_readlane(of.first, at);
-                piece = (int) blockIdx.x - (before + __builtin_amdgcn_readlane(through, at) - pieces * a.kv_heads);
+                piece = block - (before + __builtin_amdgcn_readlane(through, at) - pieces * a.kv_heads);
                 kv_head = piece / pieces, piece -= kv_head * pieces;
             }
             before += __builtin_amdgcn_readlane(through, kWave - 1);
         };
+        if (all <= kWave) {
+            // every wavefront looks through the sequences by itself, and none waits
+            const Found own(a, plan, lane);
+            units_of_piece(__builtin_amdgcn_readlane(sum_through(own.units), kWave - 1));
+            look(0, own);
+            if (!found) return;
+        } else {
+            // a quarter of them to a wavefront, the first 128 of it in registers (all of them to every one: 512 x 1 over up to 300, tables for 32768,
+            // 1 of 64 25 us for 15)
+            constexpr int kKept = 2;
+            int *shared = reinterpret_cast<int *>(smem);
+            const int chunks = (all + kBlock - 1) / kBlock, from = wave * chunks * kWave;
+            Found kept[kKept];
+            int units = 0, own = 0;
 #pragma unroll
-        for (int n = 0; n < kKept; ++n)
-            if (!found && n * kWave < all) look(n * kWave, kept[n]);
-        for (int i = kKept * kWave; !found && i < all; i += kWave) look(i, Found(a, plan, i + lane));
-        if (!found) return;
+            for (int n = 0; n < kKept; ++n)
+                if (n < chunks) kept[n] = Found(a, plan, from + n * kWave + lane);
+            for (int n = kKept; n < chunks; ++n) units += Found(a, plan, from + n * kWave + lane).units;
+#pragma unroll
+            for (int n = 0; n < kKept; ++n) units += kept[n].units;
+            units = __builtin_amdgcn_readlane(sum_through(units), kWave - 1);
+            if (lane == 0) shared[wave] = units;
+            __syncthreads();
+            units_of_piece(shared[0] + shared[1] + shared[2] + shared[3]);
+#pragma unroll
+            for (int n = 0; n < kKept; ++n) own += own_pieces(kept[n]);
+            for (int n = kKept; n < chunks; ++n) own += own_pieces(Found(a, plan, from + n * kWave + lane));
+            own = __builtin_amdgcn_readlane(sum_through(own), kWave - 1) * a.kv_heads;
+            if (lane == 0) shared[kWaves + wave] = own;
+            __syncthreads();
+            int through = 0;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                before += w < wave ? shared[kWaves + w] : 0;
+                through += shared[kWaves + w];
+            }
+            if (block >= uniform(through)) return;
+            before = uniform(before);
+            if (before <= block && block < before + own) {
+#pragma unroll
+                for (int n = 0; n < kKept; ++n)
+                    if (!found && n < chunks) look(from + n * kWave, kept[n]);
+                for (int n = kKept; !found && n < chunks; ++n) look(from + n * kWave, Found(a, plan, from + n * kWave + lane));
+                if (lane == 0) {
+                    int *to = shared + 2 * kWaves;
+                    to[0] = entry, to[1] = kv_head, to[2] = piece, to[3] = pieces, to[4] = length, to[5] = first;
+                }
+            }
+            __syncthreads();
+            const int *of = shared + 2 * kWaves;
+            entry = uniform(of[0]), kv_head = uniform(of[1]), piece = uniform(of[2]), pieces = uniform(of[3]), length = uniform(of[4]), first = uniform(of[5]);
+        }
     }
     const int tile = plan.row_tiles > 1 ? entry / a.batch : 0, sequence = entry - tile * a.batch, row0 = tile * kRows;
     const Reached reach(a, plan, length, first, tile);
@@ -264,7 +306,7 @@ __global__ __launch_bounds__(kBlock, TILES == 1 ? 3 : 2) void attention_paged_ke
     // of the j-th request for 16 keys: which of them it begins with, and which 256 bytes of a row it has
     auto value_key = [](int j) { return S::kHalf ? j * (kWave / kPieces) : j * 4 / S::kValueLoads; };
     auto value_part = [](int j) { return S::kHalf ? 0 : j % (S::kValueLoads / 4 > 0 ? S::kValueLoads / 4 : 1); };
-    unsigned char *const v_lds = smem + wave * S::kValueLds;
+    unsigned char *const v_lds = smem + kShared + wave * S::kValueLds;
     const char *k_base = (const char *) a.k + kv_head * a.head_stride * (long long) sizeof(T);
     const char *v_base = (const char *) a.v + kv_head * a.head_stride * (long long) sizeof(T);
     const int *table = a.table + (size_t) sequence * a.ld_table;
@@ -478,7 +520,7 @@ __global__ __launch_bounds__(kBlock, TILES == 1 ? 3 : 2) void attention_paged_ke
 
     // the four wavefronts' sums: rows of D results, the maximum and the sum
     const int present = rows - row0 < kRows ? rows - row0 : kRows;
-    float *merge = reinterpret_cast<float *>(smem);
+    float *merge = reinterpret_cast<float *>(smem + kShared);
     __syncthreads();  // nobody reads V any more
 #pragma unroll
     for (int m = 0; m < TILES; ++m) {
@@ -625,7 +667,9 @@ __global__ __launch_bounds__(WAVES * kWave < kBlock ? kBlock : WAVES * kWave) vo
 // A workgroup to a problem / pieces and a join.  Few problems are cut where they have more than 256 KB, many where they have more than 2 KB for each of
 // their number: 1 x 1 over 2000 keys, 16 heads of 64 (16 problems of 0.5 MB) 14.3 / 10.4; 8 x 1 over up to 1000, 4 of 128 (32 of 0.5) 13.7 / 11.3;
 // 128 x 1 over up to 1500, 2 of 64 (256 of 0.4) 13.9 / 18.4; 256 x 1 over up to 512, 12 of 64 (256 x 12 of 0.1) 42 / 52; 128 x 1 over up to 2048, 12 of 64
-// (1536 of 0.5, tables for 4) 85 / 81; 1 x 1 over 131072, 2 of 128 (2 of 67) 1781 / 31.
+// (1536 of 0.5, tables for 4) 85 / 81; 1 x 1 over 131072, 2 of 128 (2 of 67) 1781 / 31.  More than 2048 sequences and tiles never are, as every
+// workgroup looks through all of them: 1 of 64, tables for 32768 keys, 2048 x 1 over up to 6000 307 / 292, over up to 300 21 / 50; 4096 x 1 569 / 582 and
+// 36 / 110.
 //
 // Pieces, 256 / 512 / 1024 / 2048 of all (less the number of problems where that is below the first number that fits).  A workgroup to a unit of
 // the card is enough where the pieces are alike, and leaves the join the least to do; many problems of unlike lengths want many pieces, which are
@@ -652,7 +696,7 @@ PagedPlan plan_paged(bool half_precision, int batch, int heads, int kv_heads, in
     const long long units = (reach + keys - 1) / keys + (left >= 0 ? 2 : 0), all = plan.problems * units;
     plan.least = all <= 1536 ? 4 : 8;
     const long long uncut = plan.problems / 8 < 16 ? 16 : plan.problems / 8 < 256 ? plan.problems / 8 : 256;  // (16 KB each)
-    if (units * keys * row_bytes <= uncut * 8192 || all >= 1 << 30) return plan;  // (units are counted in 32 bits)
+    if (units * keys * row_bytes <= uncut * 8192 || (long long) batch * plan.row_tiles > 2048 || all >= 1 << 30) return plan;  // (units are counted in 32 bits)
     plan.pieces = plan.problems <= 32 ? 256 - (int) plan.problems : plan.problems <= 100 ? 512 - (int) plan.problems : 2048;
     if ((all + plan.least - 1) / plan.least < plan.pieces) plan.pieces = (int) ((all + plan.least - 1) / plan.least);
     plan.floats = (size_t) (plan.pieces + plan.problems) * plan.slot_rows * (head_size + 4) + 2 * (size_t) plan.problems;
@@ -671,7 +715,7 @@ template <typename T, int D, int TILES, bool ONCE>
 int run_paged(const PagedArgs &a, const PagedPlan &plan, hipStream_t stream) {
     static std::atomic<unsigned long long> done{0};
     typedef Shape<T, D> S;
-    const unsigned merge = (unsigned) (4 * plan.slot_rows * S::kPitch * 4), lds = merge > 4 * S::kValueLds ? merge : 4 * S::kValueLds;
+    const unsigned merge = (unsigned) (4 * plan.slot_rows * S::kPitch * 4), lds = kShared + (merge > 4 * S::kValueLds ? merge : 4 * S::kValueLds);
     if (lds > 48 * 1024 && !allow_large_lds(attention_paged_kernel<T, D, TILES, ONCE>, done)) return CUBERT_UNSUPPORTED;
     const int rc = launch_lds(attention_paged_kernel<T, D, TILES, ONCE>, dim3((unsigned) (plan.pieces + plan.problems)), dim3(kBlock), lds, stream, a, plan);
     if (rc != 0 || plan.pieces == 0) return rc;

@@ -393,8 +393,8 @@ ATTENTION = {
 
 
 def paged(name, t, size, layout="heads", seed=0, wide=3):
-    """Inputs of a case, and its keys and values as they would stand without pages."""
-    batch, q_rows, heads, kv_heads, page, left, sinks, lengths, first = ATTENTION[name]
+    """Inputs of a case (a name or the case itself), and its keys and values as they would stand without pages."""
+    batch, q_rows, heads, kv_heads, page, left, sinks, lengths, first = ATTENTION.get(name, name)
     g = gen(seed + size + len(name))
     longest = max(max(lengths), 1)
     width = up(longest, page) + wide
@@ -501,6 +501,21 @@ def test_attention_paged_with_wide_tables(K, name, t, size, filler):
     got = K.attention_paged(q, k_pages, v_pages, table, **at)
     within(got, want, bound, name)
     assert bool((got[~seen.any(2)] == 0).all())
+
+
+@pytest.mark.parametrize("batch,q_rows,left", [(64, 1, -1), (65, 1, -1), (128, 3, 40), (200, 20, -1), (256, 1, -1), (257, 1, -1), (300, 40, 100), (512, 1, -1),
+                                               (513, 2, -1), (700, 1, -1), (1025, 1, -1), (2048, 1, -1), (2049, 1, -1)])
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("at_end", [False, True])
+def test_attention_paged_of_many_sequences(K, batch, q_rows, left, t, at_end):
+    """Sequences among which a workgroup has to find its own, all but one in a few short."""
+    r = random.Random(batch)
+    lengths = [r.choice((0, 1, 9, 40, 70)) if r.random() < 0.97 else 600 for _ in range(batch)]
+    lengths[-1 if at_end else 0] = 640
+    case = (batch, q_rows, 2, 1, 16, left, 0, tuple(lengths), None)
+    q, k_pages, v_pages, table, k, v, page, at = paged(case, TYPES[t], 32, wide=4000)
+    want, bound = reference(q, k, v, visible(q, k, page, **at))
+    within(K.attention_paged(q, k_pages, v_pages, table, **at), want, bound, "many")
 
 
 @pytest.mark.parametrize("name", ["one query", "a few tokens", "a window and sinks", "long", "unlike lengths"])
