@@ -126,9 +126,11 @@ __device__ __forceinline__ void two_terms(float e0, float e1, v2f16 &high, v2f16
 }
 
 // A problem is a tile of rows of a sequence and a key head; sequences and tiles are numbered together, tile * batch + sequence.  A workgroup has one
-// (pieces = 0) or a piece of one: about `pieces` of all units, `least` units at least, so pieces + problems of them at most.
+// (pieces = 0) or a piece of one: about `pieces` of all units, kLeast units at least, so pieces + problems of them at most.
+constexpr int kLeast = 4;
+
 struct PagedPlan {
-    int rows, row_tiles, pieces, least;  // rows of a tile
+    int rows, row_tiles, pieces;  // rows of a tile
     int slot_rows;                       // of which that many are there
     bool once;                           // K and V are read once, and are too large to be there still when they are read again
     long long problems;
@@ -223,7 +225,7 @@ __global__ __launch_bounds__(kBlock, TILES == 1 ? 3 : 2) void attention_paged_ke
         bool found = false;
         auto units_of_piece = [&](int units) {  // (units of all sequences and tiles for a key head; of all of them below 2^30: see plan_paged)
             const int least = (units * a.kv_heads + plan.pieces - 1) / plan.pieces;
-            most = least > plan.least ? least : plan.least;
+            most = least > kLeast ? least : kLeast;
         };
         auto own_pieces = [&](const Found &of) { return (of.units + most - 1) / most; };
         auto look = [&](int from, const Found &of) {
@@ -677,8 +679,9 @@ __global__ __launch_bounds__(WAVES * kWave < kBlock ? kBlock : WAVES * kWave) vo
 // (24) 34 / 44 / 50 / 76; 48 x 1 over up to 4000, 2 of 128 (96) 31.3 / 27.6 / 29.3 / 29.9; 32 x 1, window 4096, 4 of 128 (128) 68.8 / 53.0 / 46.5 / 46.4;
 // 64 x 1 over up to 4096, 4 of 128 (256) 70.3 / 70.1 / 55.7 / 54.1.
 //
-// Units of a piece at least, 4 / 8: 8 x 1 over up to 1000, 4 of 128 (32 problems of 32) 11.3 / 12.5; fp32, 8 x 1 over up to 1000, 12 of 64 (96 of 32)
-// 15.1 / 13.9.
+// Units of a piece at least (a wavefront has one then), 4 / 8: 8 x 1 over up to 1000, 4 of 128 (32 problems of 32) 11.2 / 12.8; fp32, 9 x 5 over up to 1000,
+// 12 of 64 (108 of 32) 15.2 / 16.8, 8 x 1 (96) 15.0 / 13.6; 24 x 4 over up to 1000, 32 to 8 of 128 (192 of 32) 21.4 / 19.3; 16 x 1 over up to 500,
+// tables for 8192, 12 of 64 14.2 / 16.7.
 PagedPlan plan_paged(bool half_precision, int batch, int heads, int kv_heads, int q_rows, long long limit, int head_size, int left, int sinks) {
     PagedPlan plan;
     if (left >= kFar) left = -1;
@@ -694,11 +697,10 @@ PagedPlan plan_paged(bool half_precision, int batch, int heads, int kv_heads, in
     long long reach = limit;  // the most keys that a tile of rows sees, and how many units of them
     if (left >= 0 && (long long) left + plan.rows + sinks < reach) reach = (long long) left + plan.rows + sinks;
     const long long units = (reach + keys - 1) / keys + (left >= 0 ? 2 : 0), all = plan.problems * units;
-    plan.least = all <= 1536 ? 4 : 8;
     const long long uncut = plan.problems / 8 < 16 ? 16 : plan.problems / 8 < 256 ? plan.problems / 8 : 256;  // (16 KB each)
     if (units * keys * row_bytes <= uncut * 8192 || (long long) batch * plan.row_tiles > 2048 || all >= 1 << 30) return plan;  // (units are counted in 32 bits)
     plan.pieces = plan.problems <= 32 ? 256 - (int) plan.problems : plan.problems <= 100 ? 512 - (int) plan.problems : 2048;
-    if ((all + plan.least - 1) / plan.least < plan.pieces) plan.pieces = (int) ((all + plan.least - 1) / plan.least);
+    if ((all + kLeast - 1) / kLeast < plan.pieces) plan.pieces = (int) ((all + kLeast - 1) / kLeast);
     plan.floats = (size_t) (plan.pieces + plan.problems) * plan.slot_rows * (head_size + 4) + 2 * (size_t) plan.problems;
     return plan;
 }
@@ -721,7 +723,7 @@ int run_paged(const PagedArgs &a, const PagedPlan &plan, hipStream_t stream) {
     if (rc != 0 || plan.pieces == 0) return rc;
     const unsigned joins = (unsigned) (plan.problems * plan.slot_rows);
     // Wavefronts to a row, by its pieces on average, 1 / 4 / 16 (which have 32 columns of it): fp32, 9 x 5 over up to 1000, 12 of 64 (8 pieces)
-    // 16.9 / 17.3 / 22.0 us the whole call; fp16, 64 x 1 over up to 4096 (8) 54.1 / 54.9 / 79.2; 1 x 1 over 60000, 1 of 128 (234) 27.1 / 17.0 / 15.1.
+    // 15.2 / 15.6 / 20.6 us the whole call; fp16, 64 x 1 over up to 4096 (8) 54.1 / 54.9 / 79.2; 1 x 1 over 60000, 1 of 128 (234) 27.1 / 17.0 / 15.1.
     const int of_problem = plan.pieces / (int) plan.problems;
     if (of_problem <= 16) return launch(attention_paged_join_kernel<T, D, D, 1>, dim3((joins + 3) / 4), dim3(kBlock), stream, a, plan);
     if (of_problem <= 64) return launch(attention_paged_join_kernel<T, D, D, 4>, dim3(joins), dim3(kBlock), stream, a, plan);
