@@ -662,9 +662,9 @@ __global__ __launch_bounds__(WAVES * kWave < kBlock ? kBlock : WAVES * kWave) vo
 // How a call is cut.  Microseconds of calls in a captured graph, over inputs in turn, fp16 where nothing is said:
 //
 // Rows of a tile, where there are more than 16, 16 / 32, by what K and V of a sequence and of all may come to: 8 x 1 over up to 4000, 32 heads to 1 of 64 (1
-// MB, 8) 11.1 / 12.2; 32 x 2 over up to 1000, 48 heads to 4 of 64 (0.25, 33) 10.2 / 13.0; 8 x 4 over up to 4000, 32 to 4 of 128 (2, 65) 20.9 / 18.4; 1 x
-// 8 over up to 16800, 96 to 12 of 128 (17, 206) 46.8 / 33.9; fp32, 8 x 1 over up to 8000, 32 to 1 of 128 (8, 65) 19.3 / 22.0; 4 x 4 over up to 16000,
-// 32 to 4 of 64 (8, 131) 30.3 / 26.3.
+// MB, 8) 11.2 / 11.9; 32 x 2 over up to 1000, 48 heads to 4 of 64 (0.25, 33) 10.3 / 12.9; 8 x 32 over up to 2000, 16 of 64 (0.5, 65) 15.2 / 18.3; 16 x
+// 4 over up to 4000, 64 to 4 of 64 (1, 65) 24.6 / 21.2; 8 x 4 over up to 4000, 32 to 4 of 128 (2, 65) 20.6 / 18.1; 1 x 8 over up to 16800, 96 to 12 of 128
+// (17, 206) 47 / 34; fp32, 8 x 1 over up to 8000, 32 to 1 of 128 (8, 65) 19.1 / 21.8; 4 x 4 over up to 16000, 32 to 4 of 64 (8, 131) 30.1 / 25.5.
 //
 // A workgroup to a problem / pieces and a join.  Few problems are cut where they have more than 256 KB, many where they have more than 2 KB for each of
 // their number: 1 x 1 over 2000 keys, 16 heads of 64 (16 problems of 0.5 MB) 14.3 / 10.4; 8 x 1 over up to 1000, 4 of 128 (32 of 0.5) 13.7 / 11.3;
@@ -673,11 +673,14 @@ __global__ __launch_bounds__(WAVES * kWave < kBlock ? kBlock : WAVES * kWave) vo
 // workgroup looks through all of them: 1 of 64, tables for 32768 keys, 2048 x 1 over up to 6000 307 / 292, over up to 300 21 / 50; 4096 x 1 569 / 582 and
 // 36 / 110.
 //
-// Pieces, 256 / 512 / 1024 / 2048 of all (less the number of problems where that is below the first number that fits).  A workgroup to a unit of
-// the card is enough where the pieces are alike, and leaves the join the least to do; many problems of unlike lengths want many pieces, which are
-// handed out as units come free: 4 x 1 over up to 30000, 4 of 128 (16 problems) 31.0 / 30.7 / 32.9 / 33.8; 1 x 8 over up to 16800, 96 heads to 12 of 128
-// (24) 34 / 44 / 50 / 76; 48 x 1 over up to 4000, 2 of 128 (96) 31.3 / 27.6 / 29.3 / 29.9; 32 x 1, window 4096, 4 of 128 (128) 68.8 / 53.0 / 46.5 / 46.4;
-// 64 x 1 over up to 4096, 4 of 128 (256) 70.3 / 70.1 / 55.7 / 54.1.
+// Pieces of all.  With few problems as many as fit the card together, a workgroup or two to a unit of it, which leaves the join the least to do; 256 /
+// 512 / 1024 / 2048: 4 x 1 over up to 30000, 4 of 128 (16 problems) 31.0 / 30.7 / 32.9 / 33.8; 1 x 8 over up to 16800, 96 heads to 12 of 128 (24) 34 / 44
+// / 50 / 76; 48 x 1 over up to 4000, 2 of 128 (96) 31.3 / 27.6 / 29.3 / 29.9.  Many problems of unlike lengths want more, which are handed out as
+// units come free, up to 2048, but what the pieces write and the join reads should be little next to K and V: 1/64 of them, or three pieces to a
+// problem; and a last round of workgroups that has few of them costs as much as a full one, so they are whole rounds of 256 where a problem
+// ends with half a piece.  2048 / this: 64 x 1 over up to 4096, 4 of 128 (256) 53.1 / 53.2; 32 x 1, window 4096, 4 of 128 (128) 46.0 / 46.9; 32 x 1 over
+// up to 4096, 16 to 4 of 128 (128) 35.9 / 32.6, 64 to 4 (16 rows) 43.1 / 34.8, 32 x 5 over up to 4000, 16 to 4 (20 rows) 52 / 36.5; 16 x 8 over up to
+// 4000, 64 to 8 (256, 32 rows) 75 / 63; 512 x 1 over up to 6000, 1 of 64 78.3 / 79.0.
 //
 // Units of a piece at least (a wavefront has one then), 4 / 8: 8 x 1 over up to 1000, 4 of 128 (32 problems of 32) 11.2 / 12.8; fp32, 9 x 5 over up to 1000,
 // 12 of 64 (108 of 32) 15.2 / 16.8, 8 x 1 (96) 15.0 / 13.6; 24 x 4 over up to 1000, 32 to 8 of 128 (192 of 32) 21.4 / 19.3; 16 x 1 over up to 500,
@@ -688,8 +691,8 @@ PagedPlan plan_paged(bool half_precision, int batch, int heads, int kv_heads, in
     const long long rows = (long long) q_rows * (heads / kv_heads);
     const int row_bytes = head_size * (half_precision ? 2 : 4), keys = row_bytes == 512 ? 16 : 32;
     const long long most = left >= 0 && (long long) left + q_rows + sinks < limit ? (long long) left + q_rows + sinks : limit;  // keys of a sequence
-    const long long bytes = most * 2 * row_bytes, all_bytes = (long long) batch * kv_heads * bytes;
-    plan.rows = rows > 16 && bytes > 1 << 20 && all_bytes >= (half_precision ? 24 << 20 : 96 << 20) ? 32 : 16;
+    const long long bytes = most * 2 * row_bytes, of = (long long) batch * kv_heads, all_bytes = of < (1ll << 62) / bytes ? of * bytes : 1ll << 62;
+    plan.rows = rows > 16 && bytes >= 768 << 10 && all_bytes >= (half_precision ? 24 << 20 : 96 << 20) ? 32 : 16;
     plan.row_tiles = (int) ((rows + plan.rows - 1) / plan.rows);
     plan.slot_rows = (int) (rows < plan.rows ? rows : plan.rows);
     plan.problems = (long long) batch * kv_heads * plan.row_tiles;
@@ -699,7 +702,13 @@ PagedPlan plan_paged(bool half_precision, int batch, int heads, int kv_heads, in
     const long long units = (reach + keys - 1) / keys + (left >= 0 ? 2 : 0), all = plan.problems * units;
     const long long uncut = plan.problems / 8 < 16 ? 16 : plan.problems / 8 < 256 ? plan.problems / 8 : 256;  // (16 KB each)
     if (units * keys * row_bytes <= uncut * 8192 || (long long) batch * plan.row_tiles > 2048 || all >= 1 << 30) return plan;  // (units are counted in 32 bits)
-    plan.pieces = plan.problems <= 32 ? 256 - (int) plan.problems : plan.problems <= 100 ? 512 - (int) plan.problems : 2048;
+    if (plan.problems <= 100) {
+        plan.pieces = (plan.problems <= 32 ? 256 : 512) - (int) plan.problems;
+    } else {
+        const long long worth = all_bytes / 64 / (plan.slot_rows * (head_size + 4) * 8), few = 3 * plan.problems;
+        const long long rounds = ((worth > few ? worth : few) + 255) / 256;
+        plan.pieces = rounds < 8 ? (int) (256 * rounds - plan.problems / 2) : 2048;
+    }
     if ((all + kLeast - 1) / kLeast < plan.pieces) plan.pieces = (int) ((all + kLeast - 1) / kLeast);
     plan.floats = (size_t) (plan.pieces + plan.problems) * plan.slot_rows * (head_size + 4) + 2 * (size_t) plan.problems;
     return plan;
