@@ -675,16 +675,18 @@ __global__ __launch_bounds__(WAVES * kWave < kBlock ? kBlock : WAVES * kWave) vo
 //
 // Pieces of all.  With few problems as many as fit the card together, a workgroup or two to a unit of it, which leaves the join the least to do; 256 /
 // 512 / 1024 / 2048: 4 x 1 over up to 30000, 4 of 128 (16 problems) 31.0 / 30.7 / 32.9 / 33.8; 1 x 8 over up to 16800, 96 heads to 12 of 128 (24) 34 / 44
-// / 50 / 76; 48 x 1 over up to 4000, 2 of 128 (96) 31.3 / 27.6 / 29.3 / 29.9.  Many problems of unlike lengths want more, which are handed out as
+// / 50 / 76; 48 x 1 over up to 4000, 2 of 128 (96) 31.3 / 26.3 / 29.3 / 29.9.  (Less one / half a one for each problem, as a problem ends with half a piece
+// where lengths differ: fp32, 4 x 8 over up to 8000, 32 to 4 of 64 (32 problems of two tiles) 28.0 / 25.0; 1 x 8 over up to 16800, of one length, 34 / 55, so not
+// where one round of workgroups is all.)  Many problems of unlike lengths want more, which are handed out as
 // units come free, up to 2048, but what the pieces write and the join reads should be little next to K and V: 1/64 of them, or three pieces to a
-// problem; and a last round of workgroups that has few of them costs as much as a full one, so they are whole rounds of 256 where a problem
-// ends with half a piece.  2048 / this: 64 x 1 over up to 4096, 4 of 128 (256) 53.1 / 53.2; 32 x 1, window 4096, 4 of 128 (128) 46.0 / 46.9; 32 x 1 over
+// problem; and a last round of workgroups that has few of them costs as much as a full one, so they are whole rounds of 256.
+// 2048 / this: 64 x 1 over up to 4096, 4 of 128 (256) 53.1 / 53.2; 32 x 1, window 4096, 4 of 128 (128) 46.0 / 46.9; 32 x 1 over
 // up to 4096, 16 to 4 of 128 (128) 35.9 / 32.6, 64 to 4 (16 rows) 43.1 / 34.8, 32 x 5 over up to 4000, 16 to 4 (20 rows) 52 / 36.5; 16 x 8 over up to
 // 4000, 64 to 8 (256, 32 rows) 75 / 63; 512 x 1 over up to 6000, 1 of 64 78.3 / 79.0.
 //
-// Units of a piece at least (a wavefront has one then), 4 / 8: 8 x 1 over up to 1000, 4 of 128 (32 problems of 32) 11.2 / 12.8; fp32, 9 x 5 over up to 1000,
-// 12 of 64 (108 of 32) 15.2 / 16.8, 8 x 1 (96) 15.0 / 13.6; 24 x 4 over up to 1000, 32 to 8 of 128 (192 of 32) 21.4 / 19.3; 16 x 1 over up to 500,
-// tables for 8192, 12 of 64 14.2 / 16.7.
+// Units of a piece at least (a wavefront has one then), 4 / 8: 8 x 1 over up to 1000, 4 of 128 (32 problems of 32) 11.1 / 12.2; fp32, 9 x 5 over up to 1000,
+// 12 of 64 (108 of 32) 15.0 / 16.7, 8 x 1 (96) 13.9 / 13.5; 24 x 4 over up to 1000, 32 to 8 of 128 (192 of 32) 20.3 / 19.0; 16 x 1 over up to 500,
+// tables for 8192, 12 of 64 14.3 / 16.8.
 PagedPlan plan_paged(bool half_precision, int batch, int heads, int kv_heads, int q_rows, long long limit, int head_size, int left, int sinks) {
     PagedPlan plan;
     if (left >= kFar) left = -1;
@@ -702,8 +704,10 @@ PagedPlan plan_paged(bool half_precision, int batch, int heads, int kv_heads, in
     const long long units = (reach + keys - 1) / keys + (left >= 0 ? 2 : 0), all = plan.problems * units;
     const long long uncut = plan.problems / 8 < 16 ? 16 : plan.problems / 8 < 256 ? plan.problems / 8 : 256;  // (16 KB each)
     if (units * keys * row_bytes <= uncut * 8192 || (long long) batch * plan.row_tiles > 2048 || all >= 1 << 30) return plan;  // (units are counted in 32 bits)
-    if (plan.problems <= 100) {
-        plan.pieces = (plan.problems <= 32 ? 256 : 512) - (int) plan.problems;
+    if (plan.problems <= 32) {
+        plan.pieces = 256 - (int) plan.problems;
+    } else if (plan.problems <= 100) {
+        plan.pieces = 512 - (int) plan.problems / 2;
     } else {
         const long long worth = all_bytes / 64 / (plan.slot_rows * (head_size + 4) * 8), few = 3 * plan.problems;
         const long long rounds = ((worth > few ? worth : few) + 255) / 256;
