@@ -113,8 +113,9 @@ __device__ __forceinline__ int v_piece(int key, int at) {
     return at ^ (key / (256 / ROW_BYTES) % (ROW_BYTES / 32) * 2);
 }
 
-// Probabilities as sums of two fp16 numbers, exact to 2^-21 of them: pairs of `high` and `low`.  Neither is negative, and the second one is not 0
-// where the probability is more than 2^-37 of the largest, so that an infinite value of V stays infinite in either product.
+// Probabilities as sums of two fp16 numbers: pairs of `high` and `low`, off by 2^-21 of those from kSmall on, and by 2^-24 below it.  Neither is
+// negative, and the second one is not 0 where the probability is more than 2^-37 of the largest, so that an infinite value of V stays infinite in
+// either product.
 __device__ __forceinline__ void two_terms(float e0, float e1, v2f16 &high, v2f16 &low) {
     constexpr float kLeast = 0x1p-24f;  // fp16's smallest
     high = __builtin_bit_cast(v2f16, __builtin_amdgcn_cvt_pkrtz(e0, e1));
@@ -123,6 +124,28 @@ __device__ __forceinline__ void two_terms(float e0, float e1, v2f16 &high, v2f16
     // (the middle one of the rest, the probability and the smallest: the rest, or as much of the smallest as there is)
     low = __builtin_convertvector((v2f32{__builtin_amdgcn_fmed3f(fmaf((float) high[0], minus, e0), e0, kLeast),
                                          __builtin_amdgcn_fmed3f(fmaf((float) high[1], minus, e1), e1, kLeast)}), v2f16);
+}
+
+// What the two terms of a probability below kSmall (2^-15 to 2^-18 of the largest) leave out, kLeftOverBy times: 2^-24 at most in either direction, which
+// is exact in fp32, as two fp16 numbers.  With them probabilities down to 2^-54 of the largest are exact to 2^-21 of themselves, each.  (A first
+// token often has nearly all of the weight and a value near 0, and a result is what the small ones leave.)  Only units that have such
+// probabilities take these products; microseconds without any / with them in every unit / of the two terms alone: 64 x 1 over up to 4096 keys of 4 heads
+// of 128 53.8 / 56.8 / 53.4, 1 x 1 over 131072 of 2 heads 30.1 / 35.4 / 30.0, over 64 of 12 heads of 64 4.3 / 4.7 / 4.2.
+constexpr float kSmall = 0x1p-3f, kLeftOverBy = 0x1p38f;
+
+__device__ __forceinline__ void left_over(float e0, float e1, v2f16 &high, v2f16 &low) {
+    v2f16 x, y;
+    two_terms(e0, e1, x, y);
+    const float r0 = e0 < kSmall ? (e0 - (float) x[0] - (float) y[0]) * kLeftOverBy : 0.f;
+    const float r1 = e1 < kSmall ? (e1 - (float) x[1] - (float) y[1]) * kLeftOverBy : 0.f;
+    high = __builtin_bit_cast(v2f16, __builtin_amdgcn_cvt_pkrtz(r0, r1));
+    low = __builtin_convertvector((v2f32{r0 - (float) high[0], r1 - (float) high[1]}), v2f16);
+}
+
+// Infinities as the largest numbers: they reach a result with the two terms, and what those leave out may be negative, or nothing.
+__device__ __forceinline__ v8f16 finite(v8f16 x) {
+    constexpr _Float16 kMost = 65504;
+    return __builtin_elementwise_maximum(__builtin_elementwise_minimum(x, (v8f16) kMost), (v8f16) -kMost);
 }
 
 // A problem is a tile of rows of a sequence and a key head; sequences and tiles are numbered together, tile * batch + sequence.  A workgroup has one
@@ -379,6 +402,15 @@ __global__ __launch_bounds__(kBlock, TILES == 1 ? 3 : 2) void attention_paged_ke
                 v[n][j] = read<ONCE>(reinterpret_cast<const Words<S::kValueBytes / 4> *>(at + value_key(j) * row_bytes + v_offset + 256 * value_part(j)));
         }
     };
+    auto transposed_values = [&](int n, int d) {  // columns 16 d.. of keys 16 n.. of the unit in LDS
+        v4f16 part[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int key = 16 * (n + h) + 4 * quarter + col / 4, at = 2 * d + col % 4 / 2;
+            part[h] = read_transposed(v_lds + key * S::kRowBytes + v_piece<S::kRowBytes>(key, at) * 16 + col % 2 * 8);
+        }
+        return __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
+    };
     auto take = [&](int unit_at, auto more) {
         const unsigned there = there_next;
         const int key0 = reach.key_of(unit_at);
@@ -438,6 +470,7 @@ __global__ __launch_bounds__(kBlock, TILES == 1 ? 3 : 2) void attention_paged_ke
             if constexpr (decltype(more)::value) bring_values(unit_at + 1);
             __builtin_amdgcn_sched_barrier(0);
         }
+        unsigned least = ~0u;  // of the probabilities that are not 0, as bits and less 1
 #pragma unroll
         for (int m = 0; m < TILES; ++m) {
             float top = s[m][0][0];
@@ -459,9 +492,60 @@ __global__ __launch_bounds__(kBlock, TILES == 1 ? 3 : 2) void attention_paged_ke
                 for (int i = 0; i < 4; ++i) {
                     s[m][n][i] = __builtin_amdgcn_exp2f(fmaf(s[m][n][i] - r.top[m], a.scale, S::kRaise));
                     r.sum[m] += s[m][n][i];
+                    if constexpr (S::kHalf) {
+                        const unsigned bits = __builtin_bit_cast(unsigned, s[m][n][i]) - 1;
+                        least = bits < least ? bits : least;
+                    }
                 }
         }
+        [[maybe_unused]] const bool some_small = S::kHalf && __any(least < __builtin_bit_cast(unsigned, kSmall) - 1);
         if constexpr (S::kHalf) {
+            // (Sums are scaled by a power of two in place, which keeps them as they are, 2^99 at most: sums of their own would be 32 registers more.
+            // So would all of V, which is read anew for each product, and copies of sums and probabilities, which the pins prevent.)
+            if (some_small) {
+#pragma unroll
+                for (int m = 0; m < TILES; ++m)
+#pragma unroll
+                    for (int d = 0; d < D / 16; ++d) {
+                        pin_registers(r.ctx[m][d]);
+                        r.ctx[m][d] *= kLeftOverBy;
+                    }
+#pragma unroll
+                for (int n = 0; n < kSub; n += 2) {
+                    v8f16 p[TILES], low[TILES];
+#pragma unroll
+                    for (int m = 0; m < TILES; ++m)
+#pragma unroll
+                        for (int i = 0; i < 8; i += 2) {
+                            v2f16 x, y;
+                            left_over(s[m][n + i / 4][i % 4], s[m][n + i / 4][i % 4 + 1], x, y);
+                            p[m][i] = x[0], p[m][i + 1] = x[1], low[m][i] = y[0], low[m][i + 1] = y[1];
+                        }
+#pragma unroll
+                    for (int d = 0; d < D / 16; ++d) {
+                        asm volatile("" ::: "memory");
+                        const v8f16 x = finite(transposed_values(n, d));
+#pragma unroll
+                        for (int m = 0; m < TILES; ++m) {
+                            r.ctx[m][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, low[m], r.ctx[m][d], 0, 0, 0);
+                            r.ctx[m][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, p[m], r.ctx[m][d], 0, 0, 0);
+                        }
+                    }
+                }
+                products_done();
+#pragma unroll
+                for (int m = 0; m < TILES; ++m)
+#pragma unroll
+                    for (int d = 0; d < D / 16; ++d) {
+                        r.ctx[m][d] *= 1 / kLeftOverBy;
+                        pin_registers(r.ctx[m][d]);
+                    }
+                asm volatile("" ::: "memory");
+            }
+#pragma unroll
+            for (int m = 0; m < TILES; ++m)
+#pragma unroll
+                for (int n = 0; n < kSub; ++n) pin_registers(s[m][n]);
 #pragma unroll
             for (int n = 0; n < kSub; n += 2) {
                 v8f16 p[TILES], low[TILES];  // of the keys that the transposed V has in the same places
@@ -475,13 +559,7 @@ __global__ __launch_bounds__(kBlock, TILES == 1 ? 3 : 2) void attention_paged_ke
                     }
 #pragma unroll
                 for (int d = 0; d < D / 16; ++d) {
-                    v4f16 part[2];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int key = 16 * (n + h) + 4 * quarter + col / 4, at = 2 * d + col % 4 / 2;
-                        part[h] = read_transposed(v_lds + key * S::kRowBytes + v_piece<S::kRowBytes>(key, at) * 16 + col % 2 * 8);
-                    }
-                    const v8f16 x = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
+                    const v8f16 x = transposed_values(n, d);
 #pragma unroll
                     for (int m = 0; m < TILES; ++m) {
                         r.ctx[m][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, low[m], r.ctx[m][d], 0, 0, 0);

@@ -946,3 +946,65 @@ def test_a_captured_server(K):
         for a, b in zip((out, after, kept, servers[0].table, servers[0].free, servers[0].k_pages),
                         want + (servers[1].table, servers[1].free, servers[1].k_pages)):
             assert torch.equal(a, b), turn
+
+
+# ---------------------------------------------------------------------------- probabilities far below the largest
+
+# heads, kv_heads, q_rows, entries of the table behind the last page (with very many of them 20 rows share a tile)
+SHARED = {"one row": (1, 1, 1, 3), "a few rows": (4, 2, 3, 3), "twenty rows": (20, 1, 1, 20000), "twenty rows of five": (8, 2, 5, 20000)}
+
+
+def next_to_one_key(heads, kv_heads, q_rows, wide, t, size, gap, where, n=600, seed=21):
+    """One sequence in which a key stands `gap` above all others and has nothing in its value; scores are exact in fp32 and all values positive."""
+    g = gen(seed)
+    page, width = 16, up(n, 16) + wide
+    table = torch.full((1, width), -1, dtype=torch.int32, device="cuda")
+    table[0, :up(n, page)] = torch.randperm(up(n, page), generator=g, device="cuda").int()
+    k_pages, v_pages, _ = pool_of("heads", up(n, page), kv_heads, page, size, t, seed)
+    k, v = torch.zeros(1, n, kv_heads, size, dtype=t, device="cuda"), (1 + torch.rand(1, n, kv_heads, size, generator=g, device="cuda")).mul(2.0 ** 14).to(t)
+    k[0, :, :, 0] = -(torch.arange(n, device="cuda") % 8 / 8)[:, None].to(t)
+    k[0, where, :, 0], v[0, where] = gap, 0
+    at = torch.arange(n, device="cuda")
+    own = table[0].long()[at // page]
+    k_pages[own, :, at % page], v_pages[own, :, at % page] = k[0], v[0]
+    q = torch.zeros(1, q_rows, heads, size, dtype=t, device="cuda")
+    q[..., 0] = 1
+    return q, k_pages, v_pages, table, k, v, page, dict(left=-1, sinks=0, lengths=ints([n]), first=None)
+
+
+@pytest.mark.parametrize("rows", list(SHARED))
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("size", [32, 64, 128])
+@pytest.mark.parametrize("where", [0, 21, 599])
+def test_attention_paged_next_to_a_key_without_value(K, rows, t, size, where):
+    """A key that has nearly all of the weight and nothing to give, as a first token often has: the result is made of probabilities that are a
+    2^12th to a 2^50th of the largest, and these are as exact, each by itself."""
+    for gap in (8.0, 12.0, 17.0, 19.5, 21.5, 24.0, 28.0, 34.0):
+        q, k_pages, v_pages, table, k, v, page, at = next_to_one_key(*SHARED[rows], TYPES[t], size, gap, where)
+        seen = visible(q, k, page, **at)
+        want, _ = reference(q, k, v, seen, alpha=1.0)
+        got = K.attention_paged(q, k_pages, v_pages, table, alpha=1.0, **at)
+        # Scores and their differences are exact.  The factor log2(e) has 2 roundings, the product with it and 12 added to it one: of x = 1.45 gap
+        # + 14 as a power of two, so an exponential is off by log(2) 3 x u, and by 2^-22; fp16's terms leave out 2^-21.  Sums have n terms,
+        # products, and are scaled anew as often as in `reference`.  All terms are positive, so a sum is off by no more than they are.
+        n = 600
+        each = 3 * (1.45 * gap + 14) * U + 3 * 2.0 ** -22 + 2.0 ** -21 + (2 * n + 16) * U + (n / 16 + 2) * 2.0 ** -22
+        bound = want.abs() * (each + (1 + each) * (HALF[TYPES[t]] + 4 * U)) + SMALL[TYPES[t]]
+        within(got, want, bound, "gap %g" % gap)
+
+
+@pytest.mark.parametrize("rows", list(SHARED))
+@pytest.mark.parametrize("size", [32, 64, 128])
+def test_attention_paged_of_infinite_values_among_small_probabilities(K, rows, size):
+    """An infinite value of the key that has nearly all of the weight stays infinite, what is no number stays none, in their columns alone."""
+    for gap in (17.0, 24.0):
+        q, k_pages, v_pages, table, k, v, page, at = next_to_one_key(*SHARED[rows], torch.float16, size, gap, 21)
+        clean = K.attention_paged(q, k_pages, v_pages, table, alpha=1.0, **at)
+        own = int(table[0, 21 // page])
+        v_pages[own, :, 21 % page, 3], v_pages[own, :, 21 % page, 4], v_pages[own, :, 21 % page, 9] = math.inf, -math.inf, math.nan
+        v_pages[int(table[0, 590 // page]), :, 590 % page, 11] = math.nan
+        got = K.attention_paged(q, k_pages, v_pages, table, alpha=1.0, **at)
+        assert bool((got[..., 3] == math.inf).all()) and bool((got[..., 4] == -math.inf).all())
+        assert bool(torch.isnan(got[..., [9, 11]]).all())
+        got[..., [3, 4, 9, 11]] = clean[..., [3, 4, 9, 11]]
+        assert torch.equal(got, clean)
