@@ -300,6 +300,30 @@ int check_tables(const void *table, int width, int ld_table, const void *lengths
     return 0;
 }
 
+// `count` ints that a call reads or writes.
+struct Ints {
+    const int *at;
+    long long count;
+
+    bool meets(const Ints &other) const {
+        if (at == nullptr || other.at == nullptr) return false;
+        const uintptr_t a = (uintptr_t) at, b = (uintptr_t) other.at;
+        return a < b + 4 * (unsigned long long) other.count && b < a + 4 * (unsigned long long) count;
+    }
+};
+
+// Whether what a call writes shares memory with what it reads (workgroups read it that have not begun when others write) or with its other results.
+template <int OUT, int IN>
+bool results_apart(const Ints (&out)[OUT], const Ints (&in)[IN]) {
+    for (int i = 0; i < OUT; ++i) {
+        for (int j = 0; j < i; ++j)
+            if (out[i].meets(out[j])) return false;
+        for (int j = 0; j < IN; ++j)
+            if (out[i].meets(in[j])) return false;
+    }
+    return true;
+}
+
 int paged_write(const void *k, const void *v, int ld, const int *slots, int tokens, void *k_pages, void *v_pages, long long page_stride,
                 long long head_stride, long long row_stride, int pages, int page, int kv_heads, int head_size, int element, void *stream) {
     if (tokens < 0 || pages < 1 || page < 1 || kv_heads < 1 || head_size < 1 || ld < (long long) kv_heads * head_size) return CUBERT_BAD_ARGUMENT;
@@ -338,6 +362,8 @@ int cubert_paged_extend(int *table, int width, int ld_table, const int *lengths,
     if (batch > 0 && rows > 0 && slots == nullptr) return CUBERT_BAD_ARGUMENT;
     const long long total = (long long) batch * (rows > 0 ? rows : 1);
     if (total > (1ll << 31) - 1 - kSpan) return CUBERT_UNSUPPORTED;
+    if (!results_apart({{slots, (long long) batch * rows}, {lengths_out, batch}, {free_out, 1}}, {{lengths, batch}, {counts, batch}, {free, places}, {free_count, 1}}))
+        return CUBERT_BAD_ARGUMENT;
     ExtendArgs a;
     a.table = table, a.lengths = lengths, a.counts = counts, a.free = free, a.free_count = free_count;
     a.slots = slots, a.lengths_out = lengths_out, a.free_out = free_out;
@@ -357,6 +383,10 @@ int cubert_paged_cut(const int *table, int width, int ld_table, const int *lengt
     if (rc != 0) return rc;
     const bool few = few_to_cut(batch, width);
     if (!few && work == nullptr) return CUBERT_BAD_ARGUMENT;
+    // (what is written over keep[b] is keep[b] within its range, which another look at it does not change)
+    if (!results_apart({{lengths_out, batch}, {free_out, 1}, {few ? nullptr : work, batch}},
+                       {{lengths, batch}, {keep != lengths_out ? keep : nullptr, batch}, {free, places}, {free_count, 1}}))
+        return CUBERT_BAD_ARGUMENT;
     CutArgs a;
     a.table = table, a.lengths = lengths, a.keep = keep, a.free = free, a.free_count = free_count;
     a.lengths_out = lengths_out, a.free_out = free_out, a.returned = work;

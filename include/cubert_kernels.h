@@ -323,7 +323,7 @@ int cubert_attention_window_f16(const cubert_half *q, int ldq, const cubert_half
  * New pages go into the table, the one from the top of the stack first; slots[b * rows + t] becomes the slot of new token t, -1 where
  * there is none (or where table or stack hold something that is no page); lengths_out[b] the length afterwards and *free_out what
  * is left of the stack.  The table's other entries and the stack stay as they are, so a call whose outputs are not taken over changes nothing that
- * counts.  lengths_out and free_out are other memory than lengths and free_count.  2^18 sequences at most, and batch * rows below 2^31 - 1024, otherwise
+ * counts.  slots, lengths_out and free_out overlap nothing that is read, nor one another (CUBERT_BAD_ARGUMENT).  2^18 sequences at most, and batch * rows below 2^31 - 1024, otherwise
  * CUBERT_UNSUPPORTED.  One launch. */
 int cubert_paged_extend(int *table, int width, int ld_table, const int *lengths, const int *counts, const int *free, const int *free_count,
                         int places, int pages, int page, int batch, int rows, int *slots, int *lengths_out, int *free_out,
@@ -332,7 +332,7 @@ int cubert_paged_extend(int *table, int width, int ld_table, const int *lengths,
 /* Sequences keep their first keep[b] tokens (NULL: none; taken within 0..lengths[b]), and the pages behind these go back onto the stack in the
  * order of the sequences and their tables.  Entries that are no pages (outside 0..pages-1: whoever has taken a page out of a table has put something
  * else in its place) are passed over, and so is what the stack has no room for.  The table stays as it is: entries behind a length mean nothing.
- * A page belongs to one sequence.  lengths_out, free_out and the number of sequences as above; `work` is cubert_paged_cut_work ints of device memory that no other call
+ * A page belongs to one sequence.  lengths_out, free_out and the number of sequences as above, but lengths_out may be keep; `work` is cubert_paged_cut_work ints of device memory that no other call
  * uses before this one is done (none, and one launch, where that is 0). */
 size_t cubert_paged_cut_work(int batch, int width);
 int cubert_paged_cut(const int *table, int width, int ld_table, const int *lengths, const int *keep, int *free, const int *free_count,

@@ -215,3 +215,30 @@ def test_bounds_of_any_size_reach_the_library(monkeypatch):
                               (5, 3 - (1 << 32), (5, -1))):
         kernels.attention_paged(q, pool, pool, ints(2, 3), n, left, sinks)
         assert calls[-1][-5:-3] == sent                    # left, sinks, partials, their number, stream
+
+
+def test_tables_refuse_results_over_what_they_read(L):
+    """Workgroups read lengths, counts and the stack when others write already."""
+    ints = 4
+    there = dict(table=1 << 20, lengths=2 << 20, counts=3 << 20, free=4 << 20, free_count=5 << 20, slots=6 << 20, lengths_out=7 << 20, free_out=8 << 20)
+    count = dict(lengths=300, counts=300, free=100, free_count=1, slots=600, lengths_out=300, free_out=1)
+    for out in ("slots", "lengths_out", "free_out"):
+        for other in ("lengths", "counts", "free", "free_count", "slots", "lengths_out", "free_out"):
+            if out == other:
+                continue
+            for at in {0, count[other] - 1, 1 - count[out]}:   # the same memory, the last of one the first of the other
+                changed = dict(there)
+                changed[out] = there[other] + ints * at
+                assert extend(L, batch=300, rows=2, **changed) == BAD_ARGUMENT, (out, other, at)
+    there["keep"], there["work"] = there.pop("counts"), there.pop("slots")
+    count.update(keep=300, work=300)
+    for out in ("work", "lengths_out", "free_out"):
+        for other in ("lengths", "keep", "free", "free_count", "work", "lengths_out", "free_out"):
+            if out == other:
+                continue
+            for at in {0, count[other] - 1, 1 - count[out]}:
+                if (out, other, at) == ("lengths_out", "keep", 0):  # (which works: what is written is what was read, within its range)
+                    continue
+                changed = dict(there)
+                changed[out] = there[other] + ints * at
+                assert cut(L, batch=300, **changed) == BAD_ARGUMENT, (out, other, at)

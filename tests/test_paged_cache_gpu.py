@@ -1008,3 +1008,18 @@ def test_attention_paged_of_infinite_values_among_small_probabilities(K, rows, s
         assert bool(torch.isnan(got[..., [9, 11]]).all())
         got[..., [3, 4, 9, 11]] = clean[..., [3, 4, 9, 11]]
         assert torch.equal(got, clean)
+
+
+@pytest.mark.parametrize("batch", [5, 400])
+def test_cut_over_what_is_kept(K, batch):
+    """The lengths afterwards may go over `keep`, in one launch and in two."""
+    from cubert_amd._lib import lib
+    table, lengths, free, there = tables(3, batch, 9, 16, batch * 9 + 4, 140)
+    r = random.Random(batch)
+    keep = [r.choice((0, n, n + 5, -3, r.randint(0, n))) for n in lengths]
+    on, stack, count, left = [ints(x) for x in (table, lengths, keep)], ints(free), ints([there]), ints([0])
+    work = torch.zeros(batch, dtype=torch.int32, device="cuda")
+    rc = lib().cubert_paged_cut(on[0].data_ptr(), 9, 9, on[1].data_ptr(), on[2].data_ptr(), stack.data_ptr(), count.data_ptr(), len(free), len(free), 16, batch,
+                                on[2].data_ptr(), left.data_ptr(), work.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    assert (on[2].tolist(), left.tolist()[0], stack.tolist()) == cut_reference(table, lengths, keep, free, there, 16)
