@@ -344,6 +344,7 @@ int paged_write(const void *k, const void *v, int ld, const int *slots, int toke
     a.pieces_of_head = head_size / piece, a.pieces = kv_heads * a.pieces_of_head;
     const unsigned long long blocks = ((unsigned long long) tokens * a.pieces + kBlock - 1) / kBlock;
     if (blocks >= 1u << 24) return CUBERT_UNSUPPORTED;  // (a launch holds less than 2^32 threads)
+    if (k_pages == v_pages) return CUBERT_BAD_ARGUMENT;  // (keys and values would be written over each other)
     const bool once = (unsigned long long) tokens * a.pieces * 32 >= 64ull << 20;
     return launch(once ? paged_write_kernel<true> : paged_write_kernel<false>, dim3((unsigned) blocks), dim3(kBlock), (hipStream_t) stream, a);
 }

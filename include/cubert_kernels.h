@@ -340,9 +340,9 @@ int cubert_paged_cut(const int *table, int width, int ld_table, const int *lengt
 
 /* Keys and values of `tokens` tokens, [tokens, kv_heads * head_size] at ld elements per row (views of a packed projection), to their slots; a slot outside
  * 0..pages*page-1 is none, and its row stays out.  Pools are [pages, kv_heads, page, head_size] at any strides (in elements) that keep their
- * elements apart, the same for both: the tokens of a head together or the heads of a token, keys and values by turns; k and v overlap nothing of
- * them.  Where a slot is given twice, pieces of either row are kept.  Pointers, rows and strides are whole 16-byte pieces, and a launch holds
- * 2^32 of them, otherwise CUBERT_UNSUPPORTED. */
+ * elements apart, the same for both: the tokens of a head together or the heads of a token, keys and values by turns.  No element of one pool is one
+ * of the other (the same pointer twice is CUBERT_BAD_ARGUMENT), and k and v overlap nothing of them.  Where a slot is given twice, pieces of
+ * either row are kept.  Pointers, rows and strides are whole 16-byte pieces, and a launch holds 2^32 of them, otherwise CUBERT_UNSUPPORTED. */
 int cubert_paged_write_f32(const float *k, const float *v, int ld, const int *slots, int tokens, float *k_pages, float *v_pages,
                            long long page_stride, long long head_stride, long long row_stride, int pages, int page, int kv_heads,
                            int head_size, void *stream);

@@ -242,3 +242,8 @@ def test_tables_refuse_results_over_what_they_read(L):
                 changed = dict(there)
                 changed[out] = there[other] + ints * at
                 assert cut(L, batch=300, **changed) == BAD_ARGUMENT, (out, other, at)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+def test_write_refuses_one_pool_for_both(L, t):
+    assert write(L, t, k_pages=Q, v_pages=Q) == BAD_ARGUMENT
