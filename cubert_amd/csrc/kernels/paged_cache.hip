@@ -21,6 +21,7 @@ struct ExtendArgs {
     const int *lengths, *counts, *free, *free_count;
     int *slots, *lengths_out, *free_out;
     int width, ld_table, places, pages, shift, batch, rows;  // places of the stack, pages that there are
+    int spans;  // of kSpan slots, of a workgroup
 };
 
 // What a sequence has and asks for: `need` pages more for `count` tokens; none, and no tokens, where its table has no room for them.
@@ -50,78 +51,84 @@ __device__ __forceinline__ int block_sum(int x, int *shared) {
     return sum;
 }
 
-// A sequence is served if it needs no page, or if all that is asked for up to it is there.  A workgroup has kSpan slots; it adds up what the
-// sequences before them ask for (a few bytes per sequence, which the cache has), so that none waits for another.
+// A sequence is served if it needs no page, or if all that is asked for up to it is there.  A workgroup has kSpan slots, or several times as many, one
+// after the other; it adds up what the sequences before them ask for (a few bytes per sequence, which the cache has), so that none waits for another.
 __global__ __launch_bounds__(kBlock) void paged_extend_kernel(ExtendArgs a) {
     __shared__ int shared[kBlock / kWave], starts[kSpan], lengths[kSpan], counts[kSpan];
     const int rows = a.rows > 0 ? a.rows : 1, total = a.batch * rows, thread = threadIdx.x, lane = thread & (kWave - 1);
-    const int from = blockIdx.x * kSpan, until = total - from < kSpan ? total : from + kSpan;
-    const int first = from / rows, last = (until - 1) / rows;  // the sequences that these slots belong to
     const int there = clamp_to(*a.free_count, 0, a.places);
     if (total == 0) {
         if (thread == 0) *a.free_out = there;
         return;
     }
-    int before = 0;
-    for (int b = thread; b < first; b += kBlock) before += Growth(a, b).need;
-    before = block_sum(before, shared);
-    // sequences in runs of kSpan / kBlock to a thread
-    constexpr int kRun = kSpan / kBlock;
-    int need[kRun], sum = 0;
+    const int spans = (total - 1) / kSpan + 1, begin = blockIdx.x * a.spans, end = begin + a.spans < spans ? begin + a.spans : spans;
+    int before = 0, first = 0;  // what the sequences before `first` ask for
+    for (int span = begin; span < end; ++span) {
+        const int from = span * kSpan, until = total - from < kSpan ? total : from + kSpan;
+        const int next = from / rows, last = (until - 1) / rows;  // the sequences that these slots belong to
+        int passed = 0;
+        for (int b = first + thread; b < next; b += kBlock) passed += Growth(a, b).need;
+        before += block_sum(passed, shared);
+        first = next;
+        // sequences in runs of kSpan / kBlock to a thread
+        constexpr int kRun = kSpan / kBlock;
+        int need[kRun], sum = 0;
 #pragma unroll
-    for (int n = 0; n < kRun; ++n) {
-        const int at = thread * kRun + n;
-        need[n] = 0;
-        if (first + at <= last) {
-            const Growth g(a, first + at);
-            need[n] = g.need, lengths[at] = g.length, counts[at] = g.fits ? g.count : 0;
-        }
-        sum += need[n];
-    }
-    int through = sum;
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) {
-        const int other = __shfl_up(through, d, kWave);
-        through += lane >= d ? other : 0;
-    }
-    if (lane == kWave - 1) shared[thread / kWave] = through;
-    __syncthreads();
-    int start = before + through - sum;
-#pragma unroll
-    for (int w = 0; w < kBlock / kWave; ++w)
-        if (w < thread / kWave) start += shared[w];
-#pragma unroll
-    for (int n = 0; n < kRun; ++n) {
-        const int at = thread * kRun + n, b = first + at;
-        if (b <= last) {
-            starts[at] = start;
-            const bool granted = need[n] == 0 || start + need[n] <= there;
-            if (!granted) counts[at] = 0;
-            // what stays on the stack is what the first one left that did not get its pages, or else the last one (several workgroups may
-            // have its slots, and all write this)
-            if (start <= there && (start + need[n] > there || b == a.batch - 1)) *a.free_out = there - start - (granted ? need[n] : 0);
-        }
-        start += need[n];
-    }
-    __syncthreads();
-    for (int i = from + thread; i < until; i += kBlock) {
-        const int b = i / rows, t = i - b * rows, at = b - first, length = lengths[at], count = counts[at];
-        if (t == 0) a.lengths_out[b] = length + count;
-        if (a.rows == 0) continue;
-        int slot = -1;
-        if (t < count) {
-            const int p = length + t, index = p >> a.shift, held = pages_of(length, a.shift);
-            int *entry = a.table + (size_t) b * a.ld_table + index;
-            int page;
-            if (index < held) {
-                page = *entry;
-            } else {
-                page = a.free[there - 1 - (starts[at] + index - held)];
-                if ((p & ((1 << a.shift) - 1)) == 0) *entry = page;
+        for (int n = 0; n < kRun; ++n) {
+            const int at = thread * kRun + n;
+            need[n] = 0;
+            if (first + at <= last) {
+                const Growth g(a, first + at);
+                need[n] = g.need, lengths[at] = g.length, counts[at] = g.fits ? g.count : 0;
             }
-            if (page >= 0 && page < a.pages) slot = (page << a.shift) + (p & ((1 << a.shift) - 1));
+            sum += need[n];
         }
-        a.slots[i] = slot;
+        int through = sum;
+#pragma unroll
+        for (int d = 1; d < kWave; d *= 2) {
+            const int other = __shfl_up(through, d, kWave);
+            through += lane >= d ? other : 0;
+        }
+        if (lane == kWave - 1) shared[thread / kWave] = through;
+        __syncthreads();
+        int start = before + through - sum;
+#pragma unroll
+        for (int w = 0; w < kBlock / kWave; ++w)
+            if (w < thread / kWave) start += shared[w];
+#pragma unroll
+        for (int n = 0; n < kRun; ++n) {
+            const int at = thread * kRun + n, b = first + at;
+            if (b <= last) {
+                starts[at] = start;
+                const bool granted = need[n] == 0 || start + need[n] <= there;
+                if (!granted) counts[at] = 0;
+                // what stays on the stack is what the first one left that did not get its pages, or else the last one (several workgroups may
+                // have its slots, and all write this)
+                if (start <= there && (start + need[n] > there || b == a.batch - 1)) *a.free_out = there - start - (granted ? need[n] : 0);
+            }
+            start += need[n];
+        }
+        __syncthreads();
+        for (int i = from + thread; i < until; i += kBlock) {
+            const int b = i / rows, t = i - b * rows, at = b - first, length = lengths[at], count = counts[at];
+            if (t == 0) a.lengths_out[b] = length + count;
+            if (a.rows == 0) continue;
+            int slot = -1;
+            if (t < count) {
+                const int p = length + t, index = p >> a.shift, held = pages_of(length, a.shift);
+                int *entry = a.table + (size_t) b * a.ld_table + index;
+                int page;
+                if (index < held) {
+                    page = *entry;
+                } else {
+                    page = a.free[there - 1 - (starts[at] + index - held)];
+                    if ((p & ((1 << a.shift) - 1)) == 0) *entry = page;
+                }
+                if (page >= 0 && page < a.pages) slot = (page << a.shift) + (p & ((1 << a.shift) - 1));
+            }
+            a.slots[i] = slot;
+        }
+        __syncthreads();  // (the next span's sequences take their places)
     }
 }
 
@@ -286,7 +293,9 @@ __global__ __launch_bounds__(kBlock) void paged_write_kernel(WriteArgs a) {
     }
 }
 
-constexpr int kMostSequences = 1 << 18;  // what a sequence asks for or returns is added up by all behind it
+// What a sequence asks for or returns is added up by all behind it: by a wavefront for each, when they are cut, by 2048 workgroups at most (eight to a
+// unit of the card) when they grow.
+constexpr int kMostSequences = 1 << 18, kExtendGroups = 2048;
 
 // What extend and cut have in common: sizes of tables and pages that 32 bits count.
 int check_tables(const void *table, int width, int ld_table, const void *lengths, const void *free, const void *free_count, int places, int pages, int page,
@@ -369,7 +378,9 @@ int cubert_paged_extend(int *table, int width, int ld_table, const int *lengths,
     a.table = table, a.lengths = lengths, a.counts = counts, a.free = free, a.free_count = free_count;
     a.slots = slots, a.lengths_out = lengths_out, a.free_out = free_out;
     a.width = width, a.ld_table = ld_table, a.places = places, a.pages = pages, a.shift = __builtin_ctz((unsigned) page), a.batch = batch, a.rows = rows;
-    const unsigned blocks = total > 0 ? (unsigned) ((total + kSpan - 1) / kSpan) : 1;
+    const int spans = total > 0 ? (int) ((total + kSpan - 1) / kSpan) : 1;
+    a.spans = (spans + kExtendGroups - 1) / kExtendGroups;
+    const unsigned blocks = (unsigned) ((spans + a.spans - 1) / a.spans);
     return launch(paged_extend_kernel, dim3(blocks), dim3(kBlock), (hipStream_t) stream, a);
 }
 

@@ -1023,3 +1023,50 @@ def test_cut_over_what_is_kept(K, batch):
                                 on[2].data_ptr(), left.data_ptr(), work.data_ptr(), torch.cuda.current_stream().cuda_stream)
     assert rc == 0
     assert (on[2].tolist(), left.tolist()[0], stack.tolist()) == cut_reference(table, lengths, keep, free, there, 16)
+
+
+# batch, rows, page, pages to spare: more slots than 2048 workgroups of 1024 have
+LARGE_EXTEND = {"long prompts": (5, 700000, 64, 60000), "many prompts": (3001, 900, 16, 200000), "many prompts and a short stack": (3001, 900, 16, 90000),
+                "as many sequences as there may be": (1 << 18, 9, 4, 700000)}
+
+
+@pytest.mark.parametrize("name", list(LARGE_EXTEND))
+def test_extend_of_very_many_slots(K, name):
+    """A workgroup takes several times its 1024 slots, and carries on what it has added up."""
+    batch, rows, page, spare = LARGE_EXTEND[name]
+    r = random.Random(batch)
+    lengths, counts = [r.randint(0, 3 * page) for _ in range(batch)], [r.choice((0, rows, r.randint(0, rows))) for _ in range(batch)]
+    width = up(rows, page) + 3
+    table, held = [], 0
+    for n in lengths:
+        table.append(list(range(held, held + up(n, page))) + [-1] * (width - up(n, page)))
+        held += up(n, page)
+    free = list(range(held, held + spare))
+    r.shuffle(free)
+    on = ints(table)
+    slots, after, left = K.paged_extend(on, ints(lengths), ints(counts), ints(free), ints([spare]), page, rows)
+    want = extend_reference(table, lengths, counts, free, spare, page, rows)
+    assert torch.equal(slots.cpu(), torch.tensor(want[0], dtype=torch.int32)) and after.tolist() == want[1] and left.tolist() == [want[2]]
+    assert torch.equal(on.cpu(), torch.tensor(want[3], dtype=torch.int32))
+
+
+def test_extend_of_very_many_slots_in_time(K):
+    """As many workgroups as there are thousands of slots would add up all sequences each: fifty times as long as it takes to write the slots (2048
+    workgroups: six times)."""
+    batch, rows = 1 << 17, 2048
+    table, lengths, free = torch.zeros(batch, 2, dtype=torch.int32, device="cuda"), ints(list(range(2048))).repeat(batch // 2048), ints(list(range(2 * batch)))
+
+    def least(call):
+        times = []
+        for _ in range(6):
+            a, b = torch.cuda.Event(True), torch.cuda.Event(True)
+            a.record()
+            call()
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+
+    slots = torch.empty(batch, rows, dtype=torch.int32, device="cuda")
+    count = ints([2 * batch])
+    assert least(lambda: K.paged_extend(table, lengths, None, free, count, rows, rows)) < 20 * least(lambda: slots.fill_(-1))
