@@ -157,6 +157,7 @@ struct PagedPlan {
     int slot_rows;                       // of which that many are there
     bool once;                           // K and V are read once, and are too large to be there still when they are read again
     long long problems;
+    long long bytes;  // of K and V, of all sequences, if they are as long as their tables and the window let them be
     size_t floats;
 };
 
@@ -775,7 +776,7 @@ PagedPlan plan_paged(bool half_precision, int batch, int heads, int kv_heads, in
     plan.rows = rows > 16 && bytes >= 768 << 10 && all_bytes >= (half_precision ? 24 << 20 : 96 << 20) ? 32 : 16;
     plan.row_tiles = (int) ((rows + plan.rows - 1) / plan.rows);
     plan.slot_rows = (int) (rows < plan.rows ? rows : plan.rows);
-    plan.problems = (long long) batch * kv_heads * plan.row_tiles;
+    plan.problems = (long long) batch * kv_heads * plan.row_tiles, plan.bytes = all_bytes;
     plan.pieces = 0, plan.floats = 0, plan.once = false;
     long long reach = limit;  // the most keys that a tile of rows sees, and how many units of them
     if (left >= 0 && (long long) left + plan.rows + sinks < reach) reach = (long long) left + plan.rows + sinks;
@@ -796,12 +797,16 @@ PagedPlan plan_paged(bool half_precision, int batch, int heads, int kv_heads, in
     return plan;
 }
 
-// Whether K and V are read past the caches: once, by one tile of rows, and out of pools that do not stay in the 256 MB behind the L2 caches until the
-// next call, from 96 MB on.  Microseconds without / with: 64 x 1 over up to 4096, 4 of 128 (272 MB) 60.0 / 53.6; 48 x 1 over up to 4000, 2 of 128 (108
-// MB) 29.4 / 27.5; 128 x 1 over up to 1500, 2 of 64 (55 MB, there still after four calls) 13.9 / 15.1; two tiles of 32 rows, 1 x 8 over up to 16800, 96 heads
-// to 12 of 128, 34 / 41.
+// Whether K and V are read past the caches: once, by one tile of rows, and where neither the pools nor what the tables have room for stays in the 256 MB
+// behind the L2 caches until the next call, from 101 MB on.  Microseconds without / with, four sets of inputs in turn / sixteen, of which little is there
+// still, in pools of 1 GB: 64 x 1 over up to 4096, 4 of 128 (322 MB read, tables for 537) 67.2 / 60.9, 65.4 / 58.5; 48 x 1 over up to 4000, 2 of 128 (116,
+// 201) 29.7 / 27.6, 29.4 / 27.4; 64 x 1 over up to 1000, 4 of 128 (80, 134) 20.2 / 23.6, 22.7 / 23.4; below 101 MB of tables 128 x 1 over up to 1500, 2 of 64
+// (58, 98) 15.5 / 18.6, 18.7 / 18.3; 16 x 1 over up to 500, 12 of 64 (15, 25) 7.8 / 8.2, 7.6 / 8.0; fp32, 9 x 5 over up to 1000, 12 of 64 (33, 57) 15.7 /
+// 16.5, 16.7 / 16.3.  Tables that are far wider than sequences are long take the same side as long sequences: 64 x 1 over up to 500 in tables for 8192, 4 of 128
+// (40) 16.0 / 16.7, 18.3 / 17.8.  Two tiles of 32 rows, 1 x 8 over up to 16800, 96 heads to 12 of 128, 34 / 41.
 bool read_once(const PagedPlan &plan, long long pages, int page, int kv_heads, int row_bytes) {
-    return plan.row_tiles == 1 && 2 * pages * page * kv_heads * row_bytes >= 96ll << 20;
+    constexpr long long kLarge = 96ll << 20;
+    return plan.row_tiles == 1 && plan.bytes >= kLarge && 2 * pages * page * kv_heads * row_bytes >= kLarge;
 }
 
 template <typename T, int D, int TILES, bool ONCE>

@@ -1070,3 +1070,17 @@ def test_extend_of_very_many_slots_in_time(K):
     slots = torch.empty(batch, rows, dtype=torch.int32, device="cuda")
     count = ints([2 * batch])
     assert least(lambda: K.paged_extend(table, lengths, None, free, count, rows, rows)) < 20 * least(lambda: slots.fill_(-1))
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("size", [32, 64, 128])
+@pytest.mark.parametrize("name", ["long", "a few tokens", "many heads to one", "many rows", "a window and sinks"])
+@pytest.mark.parametrize("wide", [3, 20000])
+def test_attention_paged_is_the_same_in_a_larger_pool(K, name, t, size, wide):
+    """Pages of nobody, 96 MB and more of them, change how pools are read, where tables have room for as much, and no bit of the results."""
+    q, k_pages, v_pages, table, k, v, page, at = paged(name, TYPES[t], size, wide=wide)
+    got = K.attention_paged(q, k_pages, v_pages, table, **at)
+    more = (100 << 20) // (2 * page * k_pages.shape[1] * size * q.element_size())
+    k_large, v_large = (torch.cat([p, torch.full((more,) + p.shape[1:], math.nan, dtype=p.dtype, device="cuda")]) for p in (k_pages, v_pages))
+    assert torch.equal(got, K.attention_paged(q, k_large, v_large, table, **at))
+    within(got, *reference(q, k, v, visible(q, k, page, **at)), name)
