@@ -748,9 +748,11 @@ __global__ __launch_bounds__(WAVES * kWave < kBlock ? kBlock : WAVES * kWave) vo
 // A workgroup to a problem / pieces and a join.  Few problems are cut where they have more than 256 KB, many where they have more than 2 KB for each of
 // their number: 1 x 1 over 2000 keys, 16 heads of 64 (16 problems of 0.5 MB) 14.3 / 10.4; 8 x 1 over up to 1000, 4 of 128 (32 of 0.5) 13.7 / 11.3;
 // 128 x 1 over up to 1500, 2 of 64 (256 of 0.4) 13.9 / 18.4; 256 x 1 over up to 512, 12 of 64 (256 x 12 of 0.1) 42 / 52; 128 x 1 over up to 2048, 12 of 64
-// (1536 of 0.5, tables for 4) 85 / 81; 1 x 1 over 131072, 2 of 128 (2 of 67) 1781 / 31.  More than 2048 sequences and tiles never are, as every
-// workgroup looks through all of them: 1 of 64, tables for 32768 keys, 2048 x 1 over up to 6000 307 / 292, over up to 300 21 / 50; 4096 x 1 569 / 582 and
-// 36 / 110.
+// (1536 of 0.5, tables for 4) 85 / 81; 1 x 1 over 131072, 2 of 128 (2 of 67) 1781 / 31.  More than 1280 sequences and tiles never are, as every
+// workgroup looks through all of them, which short sequences in wide tables have nothing to set against: 1 of 64, tables for 32768 keys, over up to 300 / 1500
+// / 6000 each, 512 x 1 9.0 / 15.5, 27 / 31, 95 / 80; 1024 x 1 12.6 / 25.9, 48 / 52, 179 / 152; 1280 x 1 14.2 / 32.4, 58 / 63, 217 / 189; 1536 x 1 16.7 / 39.1,
+// 66 / 73, 254 / 226; 2048 x 1 22 / 53, 85 / 97, 319 / 299; 4096 x 1 37 / 108, 153 / 193, 585 / 600; 2 of 128, tables for 8192, over up to 300 / 2000 / 8000,
+// 768 x 1 30 / 47, 166 / 161, 648 / 581; 1024 x 1 39 / 43, 208 / 208, 805 / 811.
 //
 // Pieces of all.  With few problems as many as fit the card together, a workgroup or two to a unit of it, which leaves the join the least to do; 256 /
 // 512 / 1024 / 2048: 4 x 1 over up to 30000, 4 of 128 (16 problems) 31.0 / 30.7 / 32.9 / 33.8; 1 x 8 over up to 16800, 96 heads to 12 of 128 (24) 34 / 44
@@ -782,7 +784,7 @@ PagedPlan plan_paged(bool half_precision, int batch, int heads, int kv_heads, in
     if (left >= 0 && (long long) left + plan.rows + sinks < reach) reach = (long long) left + plan.rows + sinks;
     const long long units = (reach + keys - 1) / keys + (left >= 0 ? 2 : 0), all = plan.problems * units;
     const long long uncut = plan.problems / 8 < 16 ? 16 : plan.problems / 8 < 256 ? plan.problems / 8 : 256;  // (16 KB each)
-    if (units * keys * row_bytes <= uncut * 8192 || (long long) batch * plan.row_tiles > 2048 || all >= 1 << 30) return plan;  // (units are counted in 32 bits)
+    if (units * keys * row_bytes <= uncut * 8192 || (long long) batch * plan.row_tiles > 1280 || all >= 1 << 30) return plan;  // (units are counted in 32 bits)
     if (plan.problems <= 32) {
         plan.pieces = 256 - (int) plan.problems;
     } else if (plan.problems <= 100) {

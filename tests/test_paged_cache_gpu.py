@@ -1084,3 +1084,15 @@ def test_attention_paged_is_the_same_in_a_larger_pool(K, name, t, size, wide):
     k_large, v_large = (torch.cat([p, torch.full((more,) + p.shape[1:], math.nan, dtype=p.dtype, device="cuda")]) for p in (k_pages, v_pages))
     assert torch.equal(got, K.attention_paged(q, k_large, v_large, table, **at))
     within(got, *reference(q, k, v, visible(q, k, page, **at)), name)
+
+
+@pytest.mark.parametrize("batch,q_rows", [(600, 1), (767, 2), (768, 1), (769, 1), (1280, 1), (1281, 1)])
+@pytest.mark.parametrize("t", ["f32", "f16"])
+def test_attention_paged_of_as_many_sequences_as_are_cut(K, batch, q_rows, t):
+    """1280 sequences are the most that are cut into pieces: five chunks of 64 for each of a workgroup's wavefronts to look through."""
+    r = random.Random(batch)
+    lengths = [r.choice((0, 1, 9, 40, 70)) if r.random() < 0.97 else 1600 for _ in range(batch)]
+    lengths[0], lengths[-1] = 900, 1700
+    q, k_pages, v_pages, table, k, v, page, at = paged((batch, q_rows, 2, 1, 16, -1, 0, tuple(lengths), None), TYPES[t], 32, wide=4000)
+    want, bound = reference(q, k, v, visible(q, k, page, **at))
+    within(K.attention_paged(q, k_pages, v_pages, table, **at), want, bound, "many")
