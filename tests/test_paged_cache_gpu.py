@@ -1096,3 +1096,133 @@ def test_attention_paged_of_as_many_sequences_as_are_cut(K, batch, q_rows, t):
     q, k_pages, v_pages, table, k, v, page, at = paged((batch, q_rows, 2, 1, 16, -1, 0, tuple(lengths), None), TYPES[t], 32, wide=4000)
     want, bound = reference(q, k, v, visible(q, k, page, **at))
     within(K.attention_paged(q, k_pages, v_pages, table, **at), want, bound, "many")
+
+
+# ---------------------------------------------------------------------------- tiles of 32 rows
+
+# More than 16 rows share a tile of 32 where tables and window have room for 768 KB of K and V for a sequence and key head, and 24 MB (fp16) or
+# 96 MB (fp32) of all.  Cases as above; those without a window have tables for 320000 keys, which is as much for two key heads of the smallest size.
+TILES = {
+    "seventeen rows": (2, 1, 17, 1, 16, -1, 0, (500, 40), None),
+    "twenty rows": (2, 5, 8, 2, 16, -1, 0, (1000, 333), None),
+    "thirty-two rows": (3, 8, 8, 2, 64, -1, 0, (700, 0, 130), None),
+    "padded": (4, 5, 8, 2, 16, -1, 0, (50, 51, 52, 53), (44, 50, 52, 60)),
+    "before the sequence": (3, 20, 2, 2, 16, -1, 0, (64, 7, 0), None),
+    "tokens in the middle": (2, 3, 16, 2, 16, -1, 0, (600, 1000), (90, 20)),
+    "three tiles": (2, 9, 18, 2, 16, -1, 0, (700, 45), None),
+    "unlike lengths": (33, 3, 8, 1, 16, -1, 0, tuple((37 * i * i) % 1500 for i in range(33)), None),
+    "long": (1, 8, 8, 2, 16, -1, 0, (9000,), None),
+}
+# key heads and window by type and size, so that the window's keys are as many bytes
+WINDOWS = {("f16", 32): (36, 6200), ("f16", 64): (30, 3500), ("f16", 128): (26, 2100), ("f32", 32): (128, 3300), ("f32", 64): (104, 2100),
+           ("f32", 128): (100, 1100)}
+
+
+def tiles_case(name, t, size, layout="heads"):
+    if name != "window":
+        return paged(TILES[name], TYPES[t], size, layout, wide=20000)
+    kv, left = WINDOWS[t, size]                            # (in two sequences, one of them within the window)
+    return paged((2, 5, 2 * kv, kv // 2, 16, left, 3, (left + 700, 40), None), TYPES[t], size, layout, wide=0)
+
+
+def in_pool(pool, *pages):
+    """Pools as they are, or behind so many pages of nobody that the pool is read past the caches."""
+    if pool == "own":
+        return pages
+    more = (100 << 20) // (2 * pages[0][0].numel() * pages[0].element_size()) + 1
+    return tuple(torch.cat([p, torch.full((more,) + p.shape[1:], math.nan, dtype=p.dtype, device="cuda")]) for p in pages)
+
+
+def attention_uncut(q, k_pages, v_pages, table, left, sinks, lengths, first, alpha=None):
+    """attention_paged without memory for partial sums."""
+    from cubert_amd._lib import lib
+    batch, q_rows, heads, size = q.shape
+    out = torch.full_like(q, math.nan, memory_format=torch.contiguous_format)
+    rc = getattr(lib(), "cubert_attention_paged_" + ("f32" if q.dtype == torch.float32 else "f16"))(
+        q.data_ptr(), q.stride(1) if q_rows > 1 else heads * size, k_pages.data_ptr(), v_pages.data_ptr(), *k_pages.stride()[:3], table.data_ptr(),
+        table.shape[1], table.shape[1], lengths.data_ptr(), None if first is None else first.data_ptr(), out.data_ptr(), heads * size,
+        size ** -0.5 if alpha is None else alpha, batch, heads, k_pages.shape[1], q_rows, k_pages.shape[0], k_pages.shape[2], size, left, sinks, None, 0,
+        torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    return out
+
+
+@pytest.mark.parametrize("name", list(TILES) + ["window"])
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("size", [32, 64, 128])
+@pytest.mark.parametrize("pool", ["own", "large"])
+def test_attention_paged_in_tiles_of_32_rows(K, name, t, size, pool):
+    """Cut and uncut, with the same bits each time."""
+    q, k_pages, v_pages, table, k, v, page, at = tiles_case(name, t, size)
+    k_pages, v_pages = in_pool(pool, k_pages, v_pages)
+    seen = visible(q, k, page, **at)
+    want, bound = reference(q, k, v, seen)
+    got = K.attention_paged(q, k_pages, v_pages, table, **at)
+    within(got, want, bound, name)
+    assert bool((got[~seen.any(2)] == 0).all())
+    assert torch.equal(got, K.attention_paged(q, k_pages, v_pages, table, **at))
+    got = attention_uncut(q, k_pages, v_pages, table, **at)
+    within(got, want, bound, name + " uncut")
+    assert bool((got[~seen.any(2)] == 0).all())
+
+
+@pytest.mark.parametrize("name", ["seventeen rows", "padded", "tokens in the middle", "three tiles", "unlike lengths", "window"])
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("size", [32, 64, 128])
+@pytest.mark.parametrize("pool", ["own", "large"])
+def test_attention_paged_in_tiles_of_32_rows_without_some_pages(K, name, t, size, pool):
+    """Entries that are no pages, and no numbers in all that no query sees."""
+    q, k_pages, v_pages, table, k, v, page, at = tiles_case(name, t, size)
+    gone = torch.rand(table.shape, generator=gen(4), device="cuda") < 0.3
+    wild = ints([-1, 1 << 30, (1 << 31) - 1, -(1 << 31)]).repeat(table.numel() // 4 + 1)[:table.numel()].view(table.shape)
+    table = torch.where(gone, wild, table)
+    seen = visible(q, k, page, table=table, pages=k_pages.shape[0], **at)
+    keep = torch.zeros(k_pages.shape[0] * page, dtype=torch.bool, device="cuda")
+    b, j = seen.any(1).nonzero(as_tuple=True)
+    keep[table[b, j // page].long() * page + j % page] = True
+    k_pages, v_pages = in_pool(pool, *(torch.where(keep.view(-1, 1, page, 1), p, math.nan) for p in (k_pages, v_pages)))
+    want, bound = reference(q, k, v, seen)
+    for got in (K.attention_paged(q, k_pages, v_pages, table, **at), attention_uncut(q, k_pages, v_pages, table, **at)):
+        within(got, want, bound, name)
+        assert bool((got[~seen.any(2)] == 0).all())
+
+
+@pytest.mark.parametrize("name", ["twenty rows", "three tiles", "window"])
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("size", [32, 64, 128])
+@pytest.mark.parametrize("layout", LAYOUTS[1:])
+def test_attention_paged_in_tiles_of_32_rows_in_any_layout(K, name, t, size, layout):
+    """Pools of other strides, queries out of a packed projection, a scale below 0."""
+    q, k_pages, v_pages, table, k, v, page, at = tiles_case(name, t, size, layout)
+    packed = torch.zeros(q.shape[0], q.shape[1], q.shape[2] + 3, size, dtype=q.dtype, device="cuda")
+    packed[:, :, 1:-2] = q
+    want, bound = reference(q, k, v, visible(q, k, page, **at), alpha=-0.03)
+    within(K.attention_paged(packed[:, :, 1:-2], k_pages, v_pages, table, alpha=-0.03, **at), want, bound, name)
+
+
+@pytest.mark.parametrize("name", ["twenty rows", "thirty-two rows", "window"])
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("size", [32, 64, 128])
+@pytest.mark.parametrize("pool", ["own", "large"])
+def test_attention_paged_in_tiles_of_32_rows_of_no_number(K, name, t, size, pool):
+    """What is no number in a query, and an infinite key: the results that take it, and no others."""
+    q, k_pages, v_pages, table, k, v, page, at = tiles_case(name, t, size)
+    q[..., 5] = torch.where(q[..., 5] < 0, -0.5, 0.5).to(q.dtype)
+    seen, share = visible(q, k, page, **at), q.shape[2] // k.shape[2]
+    b, i = (int(x) for x in seen.any(2).nonzero()[seen.any(2).sum() // 2])
+    j = int(seen[b, i].nonzero()[0])
+    without = seen.clone()
+    without[b, :, j] = False
+    want, bound = reference(q, k, v, seen)
+    want_without, bound_without = reference(q, k, v, without)
+    meets = torch.zeros(q.shape[:3], dtype=torch.bool, device="cuda")
+    meets[b, :, :share] = seen[b, :, j, None]
+    none = meets & (q[..., 5] > 0)
+    want, bound = torch.where(meets[..., None], want_without, want), torch.where(meets[..., None], bound_without, bound)
+    k_pages[int(table[b, j // page]), 0, j % page, 5] = math.inf
+    q[b, i, -1, 2] = math.nan
+    none[b, i, -1] = True
+    k_pages, v_pages = in_pool(pool, k_pages, v_pages)
+    for got in (K.attention_paged(q, k_pages, v_pages, table, **at), attention_uncut(q, k_pages, v_pages, table, **at)):
+        assert bool(torch.isnan(got[none]).all())
+        within(torch.where(none[..., None], 0, got), torch.where(none[..., None], 0.0, want), bound, name)
