@@ -1226,3 +1226,70 @@ def test_attention_paged_in_tiles_of_32_rows_of_no_number(K, name, t, size, pool
     for got in (K.attention_paged(q, k_pages, v_pages, table, **at), attention_uncut(q, k_pages, v_pages, table, **at)):
         assert bool(torch.isnan(got[none]).all())
         within(torch.where(none[..., None], 0, got), torch.where(none[..., None], 0.0, want), bound, name)
+
+
+# ---------------------------------------------------------------------------- every key of a long axis, once
+
+LONG_ROWS = {"one row": (1, 1, 1, 3), "heads of two": (8, 2, 1, 3), "sixteen rows": (4, 1, 4, 3), "twenty rows": (20, 1, 1, 20000), "two tiles": (20, 1, 2, 20000)}
+
+
+def alike(heads, kv_heads, q_rows, wide, t, size, n, page, seed=23):
+    """A sequence of n keys with the same score, of which the last q_rows queries see n - q_rows + 1 to n, and pools of zeros for its values."""
+    width = up(n, page) + wide * 16 // page
+    table = torch.full((1, width), -1, dtype=torch.int32, device="cuda")
+    table[0, :up(n, page)] = torch.randperm(up(n, page), generator=gen(seed), device="cuda").int()
+    k_pages = torch.zeros(up(n, page), kv_heads, page, size, dtype=t, device="cuda")
+    q = torch.zeros(1, q_rows, heads, size, dtype=t, device="cuda")
+    return q, k_pages, torch.zeros_like(k_pages), table, ints([n])
+
+
+def exactly(got, want, t, what):
+    """Probabilities are powers of two and values too, or nothing: their sums are exact in fp32.  What is left is fp32's reciprocal of the number of keys, the
+    product with it, and the storage type's rounding; in fp16 the second terms of the probabilities, 2^-36 of them."""
+    within(got, want, want.abs() * (HALF[t] + 5 * U) + SMALL[t], what)
+
+
+@pytest.mark.parametrize("rows", list(LONG_ROWS))
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("size", [32, 64, 128])
+@pytest.mark.parametrize("cut", [True, False])
+def test_attention_paged_counts_every_key_once(K, rows, t, size, cut):
+    """Column d counts the keys j with j % size = d, about 300 each, so a key more or less is 7 roundings of fp16; and then those of the d-th stretch."""
+    t, (heads, kv, q_rows, wide), page, n = TYPES[t], LONG_ROWS[rows], 16, 300 * size + 77
+    q, k_pages, v_pages, table, lengths = alike(heads, kv, q_rows, wide, t, size, n, page)
+    at, seen = torch.arange(n, device="cuda"), n - q_rows + 1 + torch.arange(q_rows, device="cuda")
+    for of in (at % size, at // up(n, size)):
+        column = torch.zeros(n, size, dtype=torch.float64, device="cuda")
+        column[at, of] = 1
+        v_pages[table[0].long()[at // page], :, at % page] = column.to(t)[:, None]
+        want = (column.cumsum(0)[seen - 1] / seen[:, None])[None, :, None].expand(1, q_rows, heads, size)
+        call = dict(left=-1, sinks=0, lengths=lengths, first=None)
+        exactly(K.attention_paged(q, k_pages, v_pages, table, **call) if cut else attention_uncut(q, k_pages, v_pages, table, **call), want, t, rows)
+
+
+@pytest.mark.parametrize("rows", list(LONG_ROWS))
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("size", [32, 64, 128])
+@pytest.mark.parametrize("n,page", [(60000, 16), (131072, 256)])
+def test_attention_paged_takes_each_key_of_a_long_axis(K, rows, t, size, n, page):
+    """A column for each of some keys: on either side of what a wavefront has on its way together (16 or 32), of the pages it looks up at once (512 or
+    1024 keys), of pages, and of pieces wherever these may begin; and the first and the last."""
+    t, (heads, kv, q_rows, wide) = TYPES[t], LONG_ROWS[rows]
+    q, k_pages, v_pages, table, lengths = alike(heads, kv, q_rows, wide, t, size, n, page)
+    r = random.Random(n)
+    keys = [0, 15, 16, 31, 32, 511, 512, 1023, 1024, 2047, 2048, n // 2 - 1, n // 2, n - 1025, n - 33, n - 32, n - 17, n - 16, n - q_rows - 1]
+    for pieces in (226, 232, 240, 254, 255, 448, 512):      # (whole units to each)
+        for i in (1, pieces // 2, pieces - 1):
+            edge = n // 32 * i // pieces * 32
+            keys += [edge - 32, edge - 1, edge, edge + 31]
+    keys += [r.randrange(n - q_rows) for _ in range(-len(keys) % size)]
+    seen = n - q_rows + 1 + torch.arange(q_rows, device="cuda")
+    for i in range(0, len(keys), size):
+        v_pages.zero_()
+        column = torch.arange(size, device="cuda")
+        key = torch.tensor(keys[i:i + size], device="cuda")
+        v_pages[table[0].long()[key // page], :, key % page, column] = 2.0 ** 15
+        want = torch.zeros(n, size, dtype=torch.float64, device="cuda")
+        want[key, column] = 2.0 ** 15
+        want = (want.cumsum(0)[seen - 1] / seen[:, None])[None, :, None].expand(1, q_rows, heads, size)
+        exactly(K.attention_paged(q, k_pages, v_pages, table, lengths), want, t, "keys %d" % i)
