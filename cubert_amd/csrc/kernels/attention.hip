@@ -574,15 +574,6 @@ __global__ __launch_bounds__(KT * kWave) void attention_fused_kernel(const T *__
 //    ones).
 // Needs the mask (if any) readable as words (RAGGED: as bytes) and ctx rows 16-byte aligned; the launcher falls back
 // otherwise.
-typedef _Float16 v4f16 __attribute__((ext_vector_type(4)));
-
-// ds_read_b64_tr_b16: see the comment above for what arrives in which lane.
-__device__ __forceinline__ v4f16 lds_read_transposed(const half_t *p) {
-    typedef short v4i16 __attribute__((ext_vector_type(4)));
-    typedef __attribute__((address_space(3))) v4i16 lds_v4i16;
-    return __builtin_bit_cast(v4f16, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16 *) p));
-}
-
 // Halves per row of V in LDS: the 32 lanes of a lane half read 4 rows x 64 bytes at once, which fall on different
 // banks when the pitch is an odd multiple of 64 bytes (64 banks of 4 bytes).
 template <int D>
@@ -780,7 +771,7 @@ __global__ __launch_bounds__(KT * kWave) void attention_fused_half_kernel(const 
             for (int jt = 0; jt < kColTiles; ++jt) {
                 const T *at = tr_base + (kt * 32 + run * 16) * kPitchV + jt * 32;
                 Vec<T, V> bv;
-                const v4f16 lo = lds_read_transposed(at), hi = lds_read_transposed(at + 8 * kPitchV);
+                const v4f16 lo = read_transposed(at), hi = read_transposed(at + 8 * kPitchV);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     bv.v[e] = lo[e];
@@ -1303,7 +1294,7 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void attention_spread_half_kernel
     Operand ones;
 #pragma unroll
     for (int e = 0; e < V; ++e) ones.v[e] = (half_t) 1.f;
-    // (lds_read_transposed: lane i of a group of 16 names row i / 4 and column block i % 4 of a patch)
+    // (read_transposed: lane i of a group of 16 names row i / 4 and column block i % 4 of a patch)
     const int tr_group = lane >> 4, tr_i = lane & 15;
     const int tr_row = (tr_group >> 1) * 4 + (tr_i >> 2), tr_column = (tr_group & 1) * 16 + (tr_i & 3) * 4;
 #pragma unroll
@@ -1347,7 +1338,7 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void attention_spread_half_kernel
             for (int jt = 0; jt < kColTiles; ++jt) {
                 const int column = jt * 32 + tr_column;
                 auto patch = [&](int row) {
-                    return lds_read_transposed(reinterpret_cast<const half_t *>(values + row * D * 2 + value_unit(row, column / V) * 16) +
+                    return read_transposed(reinterpret_cast<const half_t *>(values + row * D * 2 + value_unit(row, column / V) * 16) +
                                                column % V);
                 };
                 const v4f16 lo = patch(run * 16 + tr_row), hi = patch(run * 16 + 8 + tr_row);

@@ -35,15 +35,12 @@ struct PagedArgs {
     bool negate;  // alpha is negative: q changes its sign, so that the largest score is that of the largest product
 };
 
-__device__ __forceinline__ int clamp_to(int x, int low, int high) { return x < low ? low : x > high ? high : x; }
-
 template <typename T, typename V>
 __device__ __forceinline__ void store4(T *to, V x) {
     store_vec<T, 4>(to, Vec<T, 4>{from_f32<T>(x[0]), from_f32<T>(x[1]), from_f32<T>(x[2]), from_f32<T>(x[3])});
 }
 
 typedef _Float16 v8f16 __attribute__((ext_vector_type(8)));
-typedef _Float16 v4f16 __attribute__((ext_vector_type(4)));
 typedef _Float16 v2f16 __attribute__((ext_vector_type(2)));
 typedef float v4f32 __attribute__((ext_vector_type(4)));
 typedef float v2f32 __attribute__((ext_vector_type(2)));
@@ -94,17 +91,6 @@ template <bool ONCE, typename W>
 __device__ __forceinline__ W read(const W *p) {
     if constexpr (ONCE) return __builtin_nontemporal_load(p);
     return *p;
-}
-
-__device__ __forceinline__ float quarters_max(float x) {
-    x = fmaxf(x, __shfl_xor(x, 16, kWave));
-    return fmaxf(x, __shfl_xor(x, 32, kWave));
-}
-
-__device__ __forceinline__ v4f16 read_transposed(const unsigned char *p) {
-    typedef short v4i16 __attribute__((ext_vector_type(4)));
-    typedef __attribute__((address_space(3))) v4i16 lds_v4i16;
-    return __builtin_bit_cast(v4f16, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16 *) p));
 }
 
 // Which of its 16-byte pieces a row of V keeps its piece `at` in: 32 lanes read 32 bytes of eight rows together, which lie on different banks.

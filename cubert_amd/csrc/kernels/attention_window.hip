@@ -32,10 +32,7 @@ struct WindowArgs {
     bool negate;  // alpha is negative: q changes its sign, so that the largest score is that of the largest product
 };
 
-__device__ __forceinline__ int clamp_to(int x, int low, int high) { return x < low ? low : x > high ? high : x; }
-
 typedef _Float16 v8f16 __attribute__((ext_vector_type(8)));
-typedef _Float16 v4f16 __attribute__((ext_vector_type(4)));
 typedef _Float16 v2f16 __attribute__((ext_vector_type(2)));
 typedef float v4f32 __attribute__((ext_vector_type(4)));
 typedef float v2f32 __attribute__((ext_vector_type(2)));
@@ -103,12 +100,6 @@ template <typename T, int ROW_BYTES>
 __device__ __forceinline__ int v_piece(int key, int at) {
     if constexpr (sizeof(T) == 2) return ROW_BYTES == 256 ? at ^ ((key & 3) << 2) : ROW_BYTES == 128 ? at ^ ((key & 2) << 1) : at;
     return ROW_BYTES >= 256 ? at ^ ((key & 4) << 1) : at;
-}
-
-__device__ __forceinline__ v4f16 read_transposed(const unsigned char *p) {
-    typedef short v4i16 __attribute__((ext_vector_type(4)));
-    typedef __attribute__((address_space(3))) v4i16 lds_v4i16;
-    return __builtin_bit_cast(v4f16, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16 *) p));
 }
 
 // e as a sum of two fp16 numbers, exact to 22 bits: pairs of `high` and `low`
@@ -264,11 +255,6 @@ struct FewRows {
         top = kNone, sum = 0.f;
     }
 };
-
-__device__ __forceinline__ float quarters_max(float x) {
-    x = fmaxf(x, __shfl_xor(x, 16, kWave));
-    return fmaxf(x, __shfl_xor(x, 32, kWave));
-}
 
 // 32 keys, those with bits 0 in `visible` left out unless all of them are seen
 template <int D>

@@ -52,6 +52,18 @@ __device__ __forceinline__ float from_f32<float>(float x) { return x; }
 template <>
 __device__ __forceinline__ half_t from_f32<half_t>(float x) { return (half_t) x; }  // round to nearest even
 
+__device__ __forceinline__ int clamp_to(int x, int low, int high) { return x < low ? low : x > high ? high : x; }
+
+// ds_read_b64_tr_b16 at an address in LDS: lane i of a group of 16 names row i / 4 and columns 4 (i % 4).. of a patch of 4 rows and 16 columns,
+// and gets column i of its rows.
+typedef _Float16 v4f16 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ v4f16 read_transposed(const void *p) {
+    typedef short v4i16 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) v4i16 lds_v4i16;
+    return __builtin_bit_cast(v4f16, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16 *) p));
+}
+
 // An fp32 value as the sum of two fp16 numbers, hi = fp16(x) and lo = fp16(x - hi) (x - hi is exact in fp32), both
 // clamped to the fp16 range: the operand form of the fp32 Dense layers that run on the fp16 matrix cores.
 __device__ __forceinline__ void split_two_terms(float x, half_t &hi, half_t &lo) {
@@ -132,6 +144,12 @@ __device__ __forceinline__ float group_reduce(float v, Op op) {
     if (LANES >= 32) v = op(v, __shfl_xor(v, 16, kWave));
     if (LANES >= 64) v = op(v, __shfl_xor(v, 32, kWave));
     return v;
+}
+
+// Over the four lanes that are 16 apart, which a product of 16 x 16 leaves a row's results in.
+__device__ __forceinline__ float quarters_max(float x) {
+    x = fmaxf(x, __shfl_xor(x, 16, kWave));
+    return fmaxf(x, __shfl_xor(x, 32, kWave));
 }
 
 __device__ __forceinline__ float wave_sum(float v) { return group_reduce<kWave>(v, SumOp()); }

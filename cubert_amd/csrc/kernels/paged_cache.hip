@@ -11,7 +11,6 @@
 namespace cubert {
 namespace {
 
-__device__ __forceinline__ int clamp_to(int x, int low, int high) { return x < low ? low : x > high ? high : x; }
 __device__ __forceinline__ int pages_of(int tokens, int shift) { return tokens == 0 ? 0 : ((tokens - 1) >> shift) + 1; }
 
 constexpr int kSpan = 1024;  // slots of a workgroup
