@@ -743,8 +743,8 @@ __global__ __launch_bounds__(WAVES * kWave < kBlock ? kBlock : WAVES * kWave) vo
 // Pieces of all.  With few problems as many as fit the card together, a workgroup or two to a unit of it, which leaves the join the least to do; 256 /
 // 512 / 1024 / 2048: 4 x 1 over up to 30000, 4 of 128 (16 problems) 31.0 / 30.7 / 32.9 / 33.8; 1 x 8 over up to 16800, 96 heads to 12 of 128 (24) 34 / 44
 // / 50 / 76; 48 x 1 over up to 4000, 2 of 128 (96) 31.3 / 26.3 / 29.3 / 29.9.  (Less one / half a one for each problem, as a problem ends with half a piece
-// where lengths differ: fp32, 4 x 8 over up to 8000, 32 to 4 of 64 (32 problems of two tiles) 28.0 / 25.0; 1 x 8 over up to 16800, of one length, 34 / 55, so not
-// where one round of workgroups is all.)  Many problems of unlike lengths want more, which are handed out as
+// where lengths differ: fp32, 4 x 8 over up to 8000, 32 heads to 4 of 64 (64 problems: four tiles of 16) 35.4 / 29.4, 48 x 1 31.3 / 27.3; 1 x 8 over up to
+// 16800, of one length, 34 / 55, so not where one round of workgroups is all.)  Many problems of unlike lengths want more, which are handed out as
 // units come free, up to 2048, but what the pieces write and the join reads should be little next to K and V: 1/64 of them, or three pieces to a
 // problem; and a last round of workgroups that has few of them costs as much as a full one, so they are whole rounds of 256.
 // 2048 / this: 64 x 1 over up to 4096, 4 of 128 (256) 53.1 / 53.2; 32 x 1, window 4096, 4 of 128 (128) 46.0 / 46.9; 32 x 1 over
