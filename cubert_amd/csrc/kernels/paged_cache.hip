@@ -314,7 +314,7 @@ struct Ints {
     long long count;
 
     bool meets(const Ints &other) const {
-        if (at == nullptr || other.at == nullptr) return false;
+        if (at == nullptr || other.at == nullptr || count == 0 || other.count == 0) return false;
         const uintptr_t a = (uintptr_t) at, b = (uintptr_t) other.at;
         return a < b + 4 * (unsigned long long) other.count && b < a + 4 * (unsigned long long) count;
     }

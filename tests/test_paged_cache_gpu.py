@@ -1293,3 +1293,72 @@ def test_attention_paged_takes_each_key_of_a_long_axis(K, rows, t, size, n, page
         want[key, column] = 2.0 ** 15
         want = (want.cumsum(0)[seen - 1] / seen[:, None])[None, :, None].expand(1, q_rows, heads, size)
         exactly(K.attention_paged(q, k_pages, v_pages, table, lengths), want, t, "keys %d" % i)
+
+
+# ---------------------------------------------------------------------------- calls at the edges of what is allowed
+
+
+def test_results_of_nothing_overlap_nothing(K):
+    """No rows, or no sequences: pointers that nothing is written to may be any."""
+    from cubert_amd._lib import lib
+    table, lengths, free, count, after, left = ints([[3, -1], [4, -1]]), ints([5, 9]), ints([1, 2, 0, 0]), ints([2]), ints([7, 7]), ints([7])
+    stream = torch.cuda.current_stream().cuda_stream
+    rc = lib().cubert_paged_extend(table.data_ptr(), 2, 2, lengths.data_ptr(), None, free.data_ptr(), count.data_ptr(), 4, 5, 16, 2, 0, lengths.data_ptr() + 4,
+                                   after.data_ptr(), left.data_ptr(), stream)
+    assert rc == 0 and after.tolist() == [5, 9] and left.tolist() == [2]
+    left.fill_(7)
+    for call in (lambda: lib().cubert_paged_extend(table.data_ptr(), 2, 2, lengths.data_ptr(), None, free.data_ptr(), count.data_ptr(), 4, 5, 16, 0, 3,
+                                                   lengths.data_ptr(), lengths.data_ptr(), left.data_ptr(), stream),
+                 lambda: lib().cubert_paged_cut(table.data_ptr(), 2, 2, lengths.data_ptr(), None, free.data_ptr(), count.data_ptr(), 4, 5, 16, 0,
+                                                lengths.data_ptr(), left.data_ptr(), None, stream)):
+        assert call() == 0 and left.tolist() == [2] and lengths.tolist() == [5, 9]
+        left.fill_(7)
+
+
+@pytest.mark.parametrize("name", ["one query", "a few tokens", "long", "nobody", "many rows"])
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("wide", [3, 20000])
+@pytest.mark.parametrize("cut", [True, False])
+def test_attention_paged_between_other_columns(K, name, t, wide, cut):
+    """Results in the middle of wider rows: what is beside them stays, and so do the bits."""
+    from cubert_amd._lib import lib
+    q, k_pages, v_pages, table, _, _, page, at = paged(name, TYPES[t], 64, wide=wide)
+    batch, q_rows, heads, size = q.shape
+    floats = lib().cubert_attention_paged_partials(int(t == "f16"), batch, heads, k_pages.shape[1], q_rows, table.shape[1], page, size, at["left"], at["sinks"])
+    partials = torch.full((floats,), math.nan, device="cuda") if cut else None
+    whole = torch.full((batch * q_rows + 2, heads * size + 24), -7.0, dtype=q.dtype, device="cuda")
+    out = whole[1:-1, 8:-16]
+    rc = getattr(lib(), "cubert_attention_paged_" + t)(
+        q.data_ptr(), heads * size, k_pages.data_ptr(), v_pages.data_ptr(), *k_pages.stride()[:3], table.data_ptr(), table.shape[1], table.shape[1],
+        at["lengths"].data_ptr(), None, out.data_ptr(), heads * size + 24, size ** -0.5, batch, heads, k_pages.shape[1], q_rows, k_pages.shape[0], page, size,
+        at["left"], at["sinks"], partials.data_ptr() if floats and cut else None, floats if cut else 0, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    want = K.attention_paged(q, k_pages, v_pages, table, **at) if cut else attention_uncut(q, k_pages, v_pages, table, **at)
+    assert torch.equal(out.reshape(q.shape), want)
+    out.fill_(-7.0)
+    assert bool((whole == -7.0).all())
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("size", [32, 64, 128])
+@pytest.mark.parametrize("page,lengths", [(4096, (5000, 1, 4096, 8191)), (65536, (70000, 65535, 30)), (1 << 20, (3000,))])
+def test_attention_paged_of_very_large_pages(K, t, size, page, lengths):
+    q, k_pages, v_pages, table, k, v, page, at = paged((len(lengths), 2, 4, 2, page, 1500, 5, lengths, None), TYPES[t], size, wide=1)
+    want, bound = reference(q, k, v, visible(q, k, page, **at))
+    within(K.attention_paged(q, k_pages, v_pages, table, **at), want, bound, "large pages")
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("cut", [True, False])
+def test_attention_paged_of_sixteen_million_keys(K, t, cut):
+    """A table that has a few pages over and over (reading allows it), up to the last of 2^24 keys; sums of powers of two are exact in fp32."""
+    t, n, page, size, pages = TYPES[t], 1 << 24, 16, 32, 9
+    g = gen(29)
+    table = torch.randint(pages, (1, n // page), generator=g, device="cuda").int()
+    k_pages = torch.zeros(pages, 1, page, size, dtype=t, device="cuda")
+    v_pages = (torch.rand(pages, 1, page, size, generator=g, device="cuda") < 0.3).to(t)
+    q = torch.zeros(1, 1, 2, size, dtype=t, device="cuda")
+    call = dict(left=-1, sinks=0, lengths=ints([n]), first=None)
+    count = torch.bincount(table[0].long(), minlength=pages).double()
+    want = ((v_pages[:, 0].double().sum(1) * count[:, None]).sum(0) / n).expand(1, 1, 2, size)
+    exactly(K.attention_paged(q, k_pages, v_pages, table, **call) if cut else attention_uncut(q, k_pages, v_pages, table, **call), want, t, "all of them")
