@@ -266,9 +266,9 @@ struct WriteArgs {
 
 typedef float v4f32 __attribute__((ext_vector_type(4)));
 
-// A 16-byte piece of a key and of a value to a thread.  Bound by memory: 16 prompts of up to 2048 tokens of 8 heads of 128, 134 MB, in 25 us (5.3
-// TB/s).  ONCE: past the caches, which large ones leave nothing in: that call 27.8 / 25.3 us, 65536 tokens 52.7 / 49.3; from 64 MB on (33 MB
-// in rows of 64 bytes 7.8 / 8.9).
+// A 16-byte piece of a key and of a value to a thread.  Bound by memory: 16 prompts of up to 2048 tokens of 8 heads of 128, 134 MB, in 26.5 us (5.1
+// TB/s).  ONCE: past the caches, which large ones leave nothing in, from 64 MB on; microseconds without / with: 16384 tokens of 8 heads of 128 (134 MB) 29.6
+// / 25.1, 32768 53.8 / 46.1, 65536 of 2 of 64 (67 MB) 15.1 / 14.5; 131072 of 1 of 32 (33 MB) 8.4 / 9.4.
 template <bool ONCE>
 __global__ __launch_bounds__(kBlock) void paged_write_kernel(WriteArgs a) {
     const unsigned long long i = (unsigned long long) blockIdx.x * kBlock + threadIdx.x;

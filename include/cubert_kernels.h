@@ -285,7 +285,8 @@ int cubert_dense_w4_i8_f16(void *stream, int tokens, int features, int in, const
  * over the keys it sees.  A query that sees none, or that stands outside its sequence (p < 0 or p >= lengths[b]), gets
  * zeros; unlike in cubert_attention_fused_* a masked key is no key at all.  Scores, probabilities and sums are held in fp32, or in
  * two or three terms of 16 bits where a matrix product takes them: a result is rounded to the storage type once, however many rows
- * are asked for.
+ * are asked for.  (The terms of fp16 leave out up to 2^-35 of the largest probability: where that key's value is next to nothing and the others
+ * have less than 2^-25 of it, what they leave is off by more than a rounding.)
  * q is [batch * q_rows, heads * head_size] at ldq elements per row, k and v [batch * kv_rows, kv_heads * head_size] at ldkv
  * (kv_rows: the rows a sequence has in the cache, whatever its length), ctx like q at ld_ctx.  `first` (NULL: 0) and
  * `lengths` (NULL: kv_rows; larger ones count as kv_rows) are device arrays of `batch` ints, `mask` (NULL: all kept) is
@@ -356,7 +357,8 @@ int cubert_paged_write_f16(const cubert_half *k, const cubert_half *v, int ld, c
  *   ctx[b, i, a, :] = sum_j softmax_j(alpha Q[b, i, a, :] . K[j, a', :]) V[j, a', :],  a' = a / (heads / kv_heads)
  * over the keys it sees.  A query that sees none, or that stands outside its sequence, gets zeros.  A negative left is no bound.  Any
  * entry of a table is safe: what is outside 0..pages-1 is no page (a window may leave pages behind and have them used again).
- * Scores, probabilities and sums are in fp32, and results are rounded once.  What is said above of K and V that nobody sees, of infinities and of
+ * Scores, probabilities and sums are in fp32, and results are rounded once (probabilities of fp16 are exact to 2^-21 of themselves down to 2^-54 of the
+ * largest).  What is said above of K and V that nobody sees, of infinities and of
  * what is no number holds here too.
  * q is [batch * q_rows, heads * head_size] at ldq elements per row, ctx like it at ld_ctx and apart from all that is read; pools as above, with pages
  * of 16 tokens at least that span less than 2^31 bytes from row to row.  Lengths are taken within 0..width*page, which is below 2^30.
