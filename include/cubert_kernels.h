@@ -357,9 +357,9 @@ int cubert_paged_write_f16(const cubert_half *k, const cubert_half *v, int ld, c
  *   ctx[b, i, a, :] = sum_j softmax_j(alpha Q[b, i, a, :] . K[j, a', :]) V[j, a', :],  a' = a / (heads / kv_heads)
  * over the keys it sees.  A query that sees none, or that stands outside its sequence, gets zeros.  A negative left is no bound.  Any
  * entry of a table is safe: what is outside 0..pages-1 is no page (a window may leave pages behind and have them used again).
- * Scores, probabilities and sums are in fp32, and results are rounded once (probabilities of fp16 are exact to 2^-21 of themselves down to 2^-54 of the
- * largest).  What is said above of K and V that nobody sees, of infinities and of
- * what is no number holds here too.
+ * Scores, probabilities and sums are in fp32, and results are rounded once (probabilities are exact to 2^-21 of themselves in fp16 down to 2^-54 of
+ * the largest; in fp32 what is below 2^-126 of it is 0).  What is said above of K and V that nobody sees, of infinities and of what is no number holds
+ * here too.
  * q is [batch * q_rows, heads * head_size] at ldq elements per row, ctx like it at ld_ctx and apart from all that is read; pools as above, with pages
  * of 16 tokens at least that span less than 2^31 bytes from row to row.  Lengths are taken within 0..width*page, which is below 2^30.
  * head_size 32, 64 or 128, pointers and strides of whole 16-byte pieces, and batch * kv_heads times the rows of a key head, q_rows * heads /
